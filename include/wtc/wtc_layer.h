@@ -1,0 +1,124 @@
+/*
+ * wtc_layer.h -- C-ABI of the operators around the fused Matmul->row-Softmax
+ * chain that a transformer layer needs, on device pointers and a HIP stream:
+ *
+ *   wtc_matmul_epilogue            out = round(act(A . B + bias) + residual)
+ *   wtc_matmul_epilogue_backward   dA, dB, dbias of it
+ *   wtc_window_attention           causal attention with a sliding window and
+ *                                  a few first tokens that stay visible
+ *   wtc_window_attention_backward  dQ, dK, dV of it
+ *   wtc_window_attention_decode    the same for one token a sequence against
+ *                                  a cache, which it also appends to
+ *
+ * Status codes, wtc_last_error() and element type codes are wtc_hip.h's.
+ * Every call is asynchronous on `stream` (a hipStream_t, or NULL) and may be
+ * captured into a graph: nothing is allocated, synchronised or kept.  All
+ * buffers are the caller's.  Where a *_workspace_size function says that a
+ * call needs scratch memory, the caller passes it (256-byte aligned,
+ * uninitialised; calls that may overlap must not share one); too little of it
+ * is WTC_ERR_WORKSPACE.  Calls may come from any host thread.  Results do not
+ * depend on timing: nothing is summed by atomics.
+ */
+#ifndef WTC_LAYER_H
+#define WTC_LAYER_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define WTC_ACT_NONE 0
+#define WTC_ACT_RELU 1
+#define WTC_ACT_GELU 2      /* z * Phi(z) */
+#define WTC_ACT_GELU_TANH 3 /* its tanh form */
+#define WTC_ACT_SILU 4
+
+/*
+ * A matrix product with an epilogue.  A [m][k] row-major; B [k][n] row-major,
+ * or with b_trans its transpose stored as [n][k]; out, residual and pre [m][n].
+ * The ld* are row strides in elements.  dtype (WTC_DTYPE_F16 / BF16): A, B and
+ * pre; out_dtype (dtype or WTC_DTYPE_F32): out and residual; bias_dtype
+ * (dtype or WTC_DTYPE_F32): bias.  A, B, dout, pre and out start 16-byte
+ * aligned and their rows are 16-byte aligned; n and k are multiples of 8 (k
+ * may be 0: then A . B is 0).  m and n may be 0.  No operand spans 2 GiB.
+ */
+typedef struct wtc_matmul_args {
+  int64_t m, n, k;
+  int64_t lda, ldb, ldr, ldo;
+  int64_t b_trans;
+  int64_t dtype, out_dtype, bias_dtype;
+  int64_t activation;
+  int64_t ldd; /* dout (backward) */
+} wtc_matmul_args;
+
+int64_t wtc_matmul_epilogue_workspace_size(const wtc_matmul_args* p);
+/* bias, residual and pre may be NULL.  pre: z = A . B + bias rounded to dtype
+ * (dense [m][n]), what the backward pass of an activation needs. */
+int wtc_matmul_epilogue(const wtc_matmul_args* p, const void* a, const void* b, const void* bias,
+                        const void* residual, void* out, void* pre, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+int64_t wtc_matmul_epilogue_backward_workspace_size(const wtc_matmul_args* p);
+/* dz = dout * act'(pre); da = dz . B^T (dense [m][k]), db = A^T . dz (dense, in
+ * B's layout), both of `dtype`, and dbias = the column sums of dz in f32.  Each
+ * of the three may be NULL (not computed).  dout is of `dtype`.  pre may be
+ * NULL with WTC_ACT_NONE.  The residual's gradient is dout itself. */
+int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, const void* a, const void* b,
+                                 const void* pre, void* da, void* db, float* dbias, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/*
+ * Attention.  q, out and dout [batch][lq][heads][dim]; k and v
+ * [batch][lk][kv_heads][dim]; heads a multiple of kv_heads, query head h
+ * reads key head h / (heads / kv_heads).  Strides (elements) of sequence,
+ * token and head; dim is contiguous, a multiple of 8 up to 128.  All starts
+ * and strides are 16-byte aligned.  dtype: WTC_DTYPE_F16 or BF16.
+ *
+ * q_lens / k_lens: int32 [batch] on the device, the tokens of each sequence
+ * (clamped to lq / lk), or NULL (all).  The queries are the last tokens: query
+ * i of a sequence stands at position p = i + k_len - q_len and sees the keys
+ * j <= p with p - j < window or j < sinks (window 0: no limit).  A query that
+ * sees no key, or stands behind its sequence's end, gives zeros (log-sum-exp
+ * -inf, gradient 0); keys behind the end are not read (gradient 0).
+ */
+typedef struct wtc_attention_args {
+  int64_t batch, heads, kv_heads, lq, lk, dim;
+  int64_t window, sinks;
+  int64_t dtype;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+  int64_t do_stride[3];            /* backward: dout */
+  int64_t kn_stride[2], vn_stride[2]; /* decode: sequence and head of k_new, v_new */
+  const int32_t* q_lens;
+  const int32_t* k_lens;
+  double scale;
+} wtc_attention_args;
+
+/* lse: f32 [batch][heads][lq], the rows' log-sum-exp of scale * q . k (NULL: not written) */
+int wtc_window_attention(const wtc_attention_args* p, const void* q, const void* k, const void* v, void* out,
+                         float* lse, void* stream);
+
+int64_t wtc_window_attention_backward_workspace_size(const wtc_attention_args* p);
+/* out and lse: of the forward call.  dq, dk, dv: dense, in the layouts of q, k, v. */
+int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout, const void* q, const void* k,
+                                  const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p);
+/* One token a sequence (lq = 1).  k and v are caches of lk rows a sequence, lk
+ * > sinks: token j stands in row j if j < sinks, else in row sinks + (j -
+ * sinks) % (lk - sinks), so that a cache that is full keeps the first `sinks`
+ * and the newest lk - sinks tokens (the window is at most that).  k_lens:
+ * tokens of each sequence with the new one, any number (0: an idle sequence;
+ * its out is 0 and its cache is left alone).  k_new, v_new
+ * [batch][kv_heads][dim]: the new token's key and value, written to the
+ * caches and attended to; both NULL: the caches hold them already. */
+int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void* k, void* v, const void* k_new,
+                                const void* v_new, void* out, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* WTC_LAYER_H */

@@ -80,6 +80,16 @@ SIGNATURES = {
     "wtc_check_status": (ctypes.c_int, [_c_p]),
     "wtc_set_exchange_wait_limit": (ctypes.c_int, [ctypes.c_uint64]),
     "wtc_release_stream": (ctypes.c_int, [_c_p]),
+    # wtc_layer.h: the argument structs go as packed bytes
+    "wtc_matmul_epilogue_workspace_size": (_c_i64, [ctypes.c_char_p]),
+    "wtc_matmul_epilogue": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 7 + [ctypes.c_size_t, _c_p]),
+    "wtc_matmul_epilogue_backward_workspace_size": (_c_i64, [ctypes.c_char_p]),
+    "wtc_matmul_epilogue_backward": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 8 + [ctypes.c_size_t, _c_p]),
+    "wtc_window_attention": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 6),
+    "wtc_window_attention_backward_workspace_size": (_c_i64, [ctypes.c_char_p]),
+    "wtc_window_attention_backward": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 10 + [ctypes.c_size_t, _c_p]),
+    "wtc_window_attention_decode_workspace_size": (_c_i64, [ctypes.c_char_p]),
+    "wtc_window_attention_decode": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 7 + [ctypes.c_size_t, _c_p]),
     "wtc_last_error": (ctypes.c_char_p, []),
     "wtc_version": (ctypes.c_char_p, []),
     "welder_compile_typical_chain_to_nvvm": (ctypes.c_int, [

@@ -52,7 +52,9 @@ ARCH = "gfx950"
 
 HIP_SOURCES = ["fused_matmul_softmax.hip", "wide_tile.hip", "rowblock_softmax.hip", "fewrows_softmax.hip",
                "unfused_chain.hip",
-               "launch.hip"]
+               "matmul_epilogue.hip", "window_attention.hip", "window_decode.hip",
+               "launch.hip", "layer_launch.hip"]
+HOST_SOURCES = ["launch.hip", "layer_launch.hip"]  # no kernels to report on
 CXX_SOURCES = ["chain_recognizer.cpp", "variants.cpp", "tile_solver.cpp", "compile_capi.cpp"]
 
 HIP_FLAGS = [
@@ -201,7 +203,7 @@ def build(verbose: bool = False) -> Path:
 
     OBJ.mkdir(exist_ok=True)
     sources = HIP_SOURCES + [s for s in CXX_SOURCES if (CSRC / s).exists()]
-    device_only = [s for s in HIP_SOURCES if s != "launch.hip"]
+    device_only = [s for s in HIP_SOURCES if s not in HOST_SOURCES]
     with cf.ThreadPoolExecutor(max_workers=8) as ex:
         co_jobs = [ex.submit(_code_object, s) for s in device_only]
         stamps_job = ex.submit(_compile_stamps)

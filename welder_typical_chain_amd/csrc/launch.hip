@@ -621,6 +621,10 @@ __global__ void fill_random_kernel(uint8_t* p, int64_t count, int dtype, uint64_
 
 }  // namespace
 
+namespace wtc {
+int report(int code, const std::string& msg) { return fail(code, msg); }
+}  // namespace wtc
+
 extern "C" {
 
 const char* wtc_last_error(void) { return g_last_error.c_str(); }

@@ -1,0 +1,343 @@
+// layer_launch.hip -- host side of include/wtc/wtc_layer.h: argument checks,
+// workspace layouts and the launches.
+#include <algorithm>
+#include <cmath>
+#include <exception>
+
+#include "layer_common.h"
+#include "layer_kernels.h"
+#include "wtc/wtc_hip.h"
+
+namespace {
+
+using namespace wtc;
+
+constexpr int64_t kMost = 1ll << 30;          // rows, tokens, heads, ...
+constexpr int64_t kSpan = 0x7FFFFFFFll;       // bytes of an operand of a product
+constexpr int64_t kTokenStride = 1ll << 23;   // elements: a tile's rows stay within 32-bit offsets
+constexpr int64_t kMaxDim = 128;
+
+int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int bad(const std::string& msg) { return report(WTC_ERR_ARG, msg); }
+
+// No C++ exception leaves a C entry point.
+template <typename F> int guarded(F f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    return report(WTC_ERR_HIP, e.what());
+  }
+}
+int launched(hipError_t e, const char* what) {
+  return e == hipSuccess ? WTC_OK : report(WTC_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+int check_workspace(const void* ws, size_t bytes, int64_t need) {
+  if (need == 0) return WTC_OK;
+  if (!ws || (int64_t)bytes < need)
+    return report(WTC_ERR_WORKSPACE, "workspace of " + std::to_string(need) + " bytes needed");
+  if (reinterpret_cast<uintptr_t>(ws) & 255) return bad("the workspace must be 256-byte aligned");
+  return WTC_OK;
+}
+
+// ---- matrix products ---------------------------------------------------------
+int check_matmul(const wtc_matmul_args& p, bool backward) {
+  if (p.dtype != WTC_DTYPE_F16 && p.dtype != WTC_DTYPE_BF16) return bad("dtype must be f16 or bf16");
+  if (p.out_dtype != p.dtype && p.out_dtype != WTC_DTYPE_F32) return bad("out_dtype must be the input type or f32");
+  if (p.bias_dtype != p.dtype && p.bias_dtype != WTC_DTYPE_F32) return bad("bias_dtype must be the input type or f32");
+  if (p.activation < WTC_ACT_NONE || p.activation > WTC_ACT_SILU) return bad("unknown activation");
+  if (p.m < 0 || p.n < 0 || p.k < 0) return bad("negative extent");
+  if (p.m > kMost || p.n > kMost || p.k > kMost) return report(WTC_ERR_UNSUPPORTED, "extent above 2^30");
+  if (p.n % 8 || p.k % 8) return bad("n and k must be multiples of 8");
+  const int64_t b_cols = p.b_trans ? p.k : p.n, b_rows = p.b_trans ? p.n : p.k;
+  if (p.lda < p.k || p.ldb < b_cols || p.lda % 8 || p.ldb % 8)
+    return bad("lda and ldb must be multiples of 8 that hold a row");
+  if (p.lda > kMost || p.ldb > kMost || p.m * p.lda * 2 > kSpan || b_rows * p.ldb * 2 > kSpan)
+    return report(WTC_ERR_UNSUPPORTED, "an operand spans more than 2 GiB");
+  if (backward) {
+    if (p.ldd < p.n || p.ldd % 8) return bad("ldd must be a multiple of 8 that holds a row");
+    if (p.ldd > kMost || p.m * p.ldd * 2 > kSpan || p.m * p.n * 2 > kSpan)
+      return report(WTC_ERR_UNSUPPORTED, "dout spans more than 2 GiB");
+  } else if (p.ldo < p.n || p.ldr < p.n || p.ldo % 8 || p.ldr % 8 || p.ldo > kMost || p.ldr > kMost) {
+    return bad("ldo and ldr must be multiples of 8 that hold a row");
+  }
+  return WTC_OK;
+}
+
+int matmul_forward(const wtc_matmul_args& p, const void* a, const void* b, const void* bias, const void* residual,
+                   void* out, void* pre, hipStream_t stream) {
+  MatmulParams q{};
+  q.a = static_cast<const uint8_t*>(a);
+  q.b = static_cast<const uint8_t*>(b);
+  q.bias = bias;
+  q.residual = residual;
+  q.out = out;
+  q.pre = pre;
+  q.a_row = p.lda;
+  q.a_col = 1;
+  q.b_row = p.b_trans ? 1 : p.ldb;
+  q.b_col = p.b_trans ? p.ldb : 1;
+  q.ldr = p.ldr;
+  q.ldo = p.ldo;
+  q.ldp = p.n;
+  q.m = (int)p.m;
+  q.n = (int)p.n;
+  q.k = (int)p.k;
+  q.bias_f32 = p.bias_dtype == WTC_DTYPE_F32;
+  q.act = (int)p.activation;
+  return launched(launch_matmul(q, (int)p.dtype, (int)p.out_dtype, stream), "matmul_epilogue");
+}
+
+// ---- attention ----------------------------------------------------------------
+int check_strides(const int64_t* s, int count, int64_t tokens, const char* what) {
+  for (int i = 0; i < count; ++i)
+    if (s[i] < 0 || s[i] % 8) return bad(std::string(what) + ": strides must be multiples of 8");
+  if (count == 3 && tokens > 1 && s[1] > kTokenStride)
+    return report(WTC_ERR_UNSUPPORTED, std::string(what) + ": token stride above 2^23 elements");
+  return WTC_OK;
+}
+// Rows of a tensor that is written may not overlap.
+int check_distinct(const int64_t* s, int64_t n0, int64_t n1, int64_t n2, int64_t dim, const char* what) {
+  std::pair<int64_t, int64_t> d[3] = {{s[0], n0}, {s[1], n1}, {s[2], n2}};
+  std::sort(d, d + 3);
+  int64_t span = dim;
+  for (auto& x : d) {
+    if (x.second <= 1) continue;
+    if (x.first < span) return bad(std::string(what) + ": rows overlap");
+    span += x.first * (x.second - 1);
+  }
+  return WTC_OK;
+}
+
+int check_attention(const wtc_attention_args& p, bool decode) {
+  if (p.dtype != WTC_DTYPE_F16 && p.dtype != WTC_DTYPE_BF16) return bad("dtype must be f16 or bf16");
+  if (p.batch < 0 || p.lq < 0 || p.lk < 0 || p.window < 0 || p.sinks < 0) return bad("negative extent");
+  if (p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads) return bad("heads must be a multiple of kv_heads");
+  if (p.dim < 8 || p.dim > kMaxDim || p.dim % 8) return bad("dim must be a multiple of 8 up to 128");
+  if (p.batch > kMost || p.lq > kMost || p.lk > kMost || p.heads > (1 << 16) ||
+      p.batch * p.heads > kMost || p.batch * p.heads * p.lq > kMost || p.batch * p.kv_heads > kMost / std::max<int64_t>(p.lk, 1))
+    return report(WTC_ERR_UNSUPPORTED, "extent above 2^30");
+  if (!std::isfinite(p.scale)) return bad("scale must be finite");
+  int rc;
+  if ((rc = check_strides(p.q_stride, 3, p.lq, "q"))) return rc;
+  if ((rc = check_strides(p.k_stride, 3, p.lk, "k"))) return rc;
+  if ((rc = check_strides(p.v_stride, 3, p.lk, "v"))) return rc;
+  if ((rc = check_strides(p.o_stride, 3, p.lq, "out"))) return rc;
+  if (decode) {
+    if (p.lq != 1) return bad("decode takes one token a sequence");
+    if (p.lk <= p.sinks) return bad("the cache must have more rows than sinks");
+    if (!p.k_lens && p.batch) return bad("decode needs k_lens");
+    if ((rc = check_strides(p.kn_stride, 2, 0, "k_new"))) return rc;
+    if ((rc = check_strides(p.vn_stride, 2, 0, "v_new"))) return rc;
+  }
+  return WTC_OK;
+}
+
+AttnParams attention_params(const wtc_attention_args& p) {
+  AttnParams q{};
+  for (int i = 0; i < 3; ++i) {
+    q.q_stride[i] = p.q_stride[i];
+    q.k_stride[i] = p.k_stride[i];
+    q.v_stride[i] = p.v_stride[i];
+    q.o_stride[i] = p.o_stride[i];
+    q.do_stride[i] = p.do_stride[i];
+  }
+  for (int i = 0; i < 2; ++i) {
+    q.kn_stride[i] = p.kn_stride[i];
+    q.vn_stride[i] = p.vn_stride[i];
+  }
+  q.q_lens = p.q_lens;
+  q.k_lens = p.k_lens;
+  q.window = p.window == 0 ? INT32_MAX : std::min<int64_t>(p.window, INT32_MAX);
+  q.batch = (int)p.batch;
+  q.heads = (int)p.heads;
+  q.kv_heads = (int)p.kv_heads;
+  q.group = (int)(p.heads / p.kv_heads);
+  q.lq = (int)p.lq;
+  q.lk = (int)p.lk;
+  q.dim = (int)p.dim;
+  q.sinks = (int)std::min<int64_t>(p.sinks, p.lk);
+  q.scale = (float)p.scale;
+  return q;
+}
+
+int64_t backward_workspace(const wtc_attention_args& p) { return align256(p.batch * p.heads * p.lq * 4); }
+int64_t matmul_backward_workspace(const wtc_matmul_args& p) {
+  return p.activation == WTC_ACT_NONE ? 0 : align256(p.m * p.n * 2);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t wtc_matmul_epilogue_workspace_size(const wtc_matmul_args* p) {
+  if (!p) return bad("NULL arguments"), -1;
+  if (guarded([&] { return check_matmul(*p, false); })) return -1;
+  return 0;
+}
+
+int wtc_matmul_epilogue(const wtc_matmul_args* p, const void* a, const void* b, const void* bias,
+                        const void* residual, void* out, void* pre, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  return guarded([&]() -> int {
+    if (!p) return bad("NULL arguments");
+    if (int rc = check_matmul(*p, false)) return rc;
+    if (p->m == 0 || p->n == 0) return WTC_OK;
+    if (!out || (p->k && (!a || !b))) return bad("NULL operand");
+    if (!aligned16(a) || !aligned16(b) || !aligned16(out) || !aligned16(pre) || !aligned16(residual) || !aligned16(bias))
+      return bad("pointers must be 16-byte aligned");
+    return matmul_forward(*p, a, b, bias, residual, out, pre, static_cast<hipStream_t>(stream));
+  });
+}
+
+int64_t wtc_matmul_epilogue_backward_workspace_size(const wtc_matmul_args* p) {
+  if (!p) return bad("NULL arguments"), -1;
+  if (guarded([&] { return check_matmul(*p, true); })) return -1;
+  return matmul_backward_workspace(*p);
+}
+
+int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, const void* a, const void* b,
+                                 const void* pre, void* da, void* db, float* dbias, void* workspace,
+                                 size_t workspace_bytes, void* stream_) {
+  return guarded([&]() -> int {
+    if (!p) return bad("NULL arguments");
+    if (int rc = check_matmul(*p, true)) return rc;
+    const hipStream_t stream = static_cast<hipStream_t>(stream_);
+    const bool act = p->activation != WTC_ACT_NONE;
+    if ((p->m && p->n) && (!dout || (act && !pre) || (db && p->k && !a) || (da && p->k && !b)))
+      return bad("NULL operand");
+    if (!aligned16(dout) || !aligned16(a) || !aligned16(b) || !aligned16(pre) || !aligned16(da) || !aligned16(db) ||
+        !aligned16(dbias))
+      return bad("pointers must be 16-byte aligned");
+    if (int rc = check_workspace(workspace, workspace_bytes, matmul_backward_workspace(*p))) return rc;
+    void* dz = act ? workspace : const_cast<void*>(dout);
+    const int64_t ldz = act ? p->n : p->ldd;
+    if (p->n && (act || dbias)) {
+      ActBackwardParams q{dout, pre, act && (da || db) ? dz : nullptr, dbias, p->m, p->n, p->ldd, (int)p->activation};
+      if (int rc = launched(launch_act_backward(q, (int)p->dtype, stream), "activation gradient")) return rc;
+    }
+    MatmulParams q{};
+    if (da && p->m && p->k) {  // dz [m][n] . B^T
+      q.a = static_cast<const uint8_t*>(dz);
+      q.b = static_cast<const uint8_t*>(b);
+      q.a_row = ldz;
+      q.a_col = 1;
+      q.b_row = p->b_trans ? p->ldb : 1;
+      q.b_col = p->b_trans ? 1 : p->ldb;
+      q.out = da;
+      q.ldo = p->k;
+      q.m = (int)p->m;
+      q.n = (int)p->k;
+      q.k = (int)p->n;
+      if (int rc = launched(launch_matmul(q, (int)p->dtype, (int)p->dtype, stream), "da")) return rc;
+    }
+    if (db && p->n && p->k) {  // A^T . dz, or its transpose
+      const uint8_t *x = static_cast<const uint8_t*>(a), *y = static_cast<const uint8_t*>(dz);
+      q.a = p->b_trans ? y : x;
+      q.b = p->b_trans ? x : y;
+      q.a_row = 1;
+      q.a_col = p->b_trans ? ldz : p->lda;
+      q.b_row = p->b_trans ? p->lda : ldz;
+      q.b_col = 1;
+      q.out = db;
+      q.m = (int)(p->b_trans ? p->n : p->k);
+      q.n = (int)(p->b_trans ? p->k : p->n);
+      q.ldo = q.n;
+      q.k = (int)p->m;
+      if (int rc = launched(launch_matmul(q, (int)p->dtype, (int)p->dtype, stream), "db")) return rc;
+    }
+    return WTC_OK;
+  });
+}
+
+int wtc_window_attention(const wtc_attention_args* p, const void* q, const void* k, const void* v, void* out,
+                         float* lse, void* stream) {
+  return guarded([&]() -> int {
+    if (!p) return bad("NULL arguments");
+    if (int rc = check_attention(*p, false)) return rc;
+    if (int rc = check_distinct(p->o_stride, p->batch, p->lq, p->heads, p->dim, "out")) return rc;
+    if (p->batch == 0 || p->lq == 0) return WTC_OK;
+    if (!q || !out || (p->lk && (!k || !v))) return bad("NULL operand");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return bad("pointers must be 16-byte aligned");
+    AttnParams a = attention_params(*p);
+    a.q = static_cast<const uint8_t*>(q);
+    a.k = static_cast<const uint8_t*>(k);
+    a.v = static_cast<const uint8_t*>(v);
+    a.out = static_cast<uint8_t*>(out);
+    a.lse = lse;
+    return launched(launch_attention(a, (int)p->dtype, static_cast<hipStream_t>(stream)), "window_attention");
+  });
+}
+
+int64_t wtc_window_attention_backward_workspace_size(const wtc_attention_args* p) {
+  if (!p) return bad("NULL arguments"), -1;
+  if (guarded([&] { return check_attention(*p, false); })) return -1;
+  return backward_workspace(*p);
+}
+
+int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout, const void* q, const void* k,
+                                  const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int {
+    if (!p) return bad("NULL arguments");
+    if (int rc = check_attention(*p, false)) return rc;
+    if (int rc = check_strides(p->do_stride, 3, p->lq, "dout")) return rc;
+    if (p->batch == 0) return WTC_OK;
+    if ((p->lq && (!dout || !q || !out || !lse || !dq)) || (p->lk && (!k || !v || !dk || !dv)))
+      return bad("NULL operand");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(dout) || !aligned16(dq) ||
+        !aligned16(dk) || !aligned16(dv))
+      return bad("pointers must be 16-byte aligned");
+    if (int rc = check_workspace(workspace, workspace_bytes, backward_workspace(*p))) return rc;
+    AttnParams a = attention_params(*p);
+    a.q = static_cast<const uint8_t*>(q);
+    a.k = static_cast<const uint8_t*>(k);
+    a.v = static_cast<const uint8_t*>(v);
+    a.o = static_cast<const uint8_t*>(out);
+    a.dout = static_cast<const uint8_t*>(dout);
+    a.lse_in = lse;
+    a.delta = static_cast<float*>(workspace);
+    a.dq = static_cast<uint8_t*>(dq);
+    a.dk = static_cast<uint8_t*>(dk);
+    a.dv = static_cast<uint8_t*>(dv);
+    return launched(launch_attention_backward(a, (int)p->dtype, static_cast<hipStream_t>(stream)),
+                    "window_attention_backward");
+  });
+}
+
+int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p) {
+  if (!p) return bad("NULL arguments"), -1;
+  if (guarded([&] { return check_attention(*p, true); })) return -1;
+  return 0;
+}
+
+int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void* k, void* v, const void* k_new,
+                                const void* v_new, void* out, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  return guarded([&]() -> int {
+    if (!p) return bad("NULL arguments");
+    if (int rc = check_attention(*p, true)) return rc;
+    if (int rc = check_distinct(p->o_stride, p->batch, 1, p->heads, p->dim, "out")) return rc;
+    if (!k_new != !v_new) return bad("k_new and v_new go together");
+    if (k_new) {
+      if (int rc = check_distinct(p->k_stride, p->batch, p->lk, p->kv_heads, p->dim, "k")) return rc;
+      if (int rc = check_distinct(p->v_stride, p->batch, p->lk, p->kv_heads, p->dim, "v")) return rc;
+    }
+    if (p->batch == 0) return WTC_OK;
+    if (!q || !k || !v || !out) return bad("NULL operand");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(k_new) || !aligned16(v_new))
+      return bad("pointers must be 16-byte aligned");
+    AttnParams a = attention_params(*p);
+    a.window = std::min<int64_t>(a.window, p->lk - p->sinks);
+    a.q = static_cast<const uint8_t*>(q);
+    a.k = static_cast<const uint8_t*>(k);
+    a.v = static_cast<const uint8_t*>(v);
+    a.k_new = static_cast<const uint8_t*>(k_new);
+    a.v_new = static_cast<const uint8_t*>(v_new);
+    a.out = static_cast<uint8_t*>(out);
+    return launched(launch_attention_decode(a, (int)p->dtype, static_cast<hipStream_t>(stream)),
+                    "window_attention_decode");
+  });
+}
+
+}  // extern "C"
