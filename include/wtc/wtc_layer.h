@@ -38,8 +38,8 @@ extern "C" {
 /*
  * A matrix product with an epilogue.  A [m][k] row-major; B [k][n] row-major,
  * or with b_trans its transpose stored as [n][k]; out, residual and pre [m][n].
- * The ld* are row strides in elements.  dtype (WTC_DTYPE_F16 / BF16): A, B and
- * pre; out_dtype (dtype or WTC_DTYPE_F32): out and residual; bias_dtype
+ * The ld* are row strides in elements.  dtype (WTC_DTYPE_F16 / BF16): A and B;
+ * out_dtype (dtype or WTC_DTYPE_F32): out and residual; bias_dtype
  * (dtype or WTC_DTYPE_F32): bias.  A, B, dout, pre and out start 16-byte
  * aligned and their rows are 16-byte aligned; n and k are multiples of 8 (k
  * may be 0: then A . B is 0).  m and n may be 0.  No operand spans 2 GiB.
@@ -54,10 +54,10 @@ typedef struct wtc_matmul_args {
 } wtc_matmul_args;
 
 int64_t wtc_matmul_epilogue_workspace_size(const wtc_matmul_args* p);
-/* bias, residual and pre may be NULL.  pre: z = A . B + bias rounded to dtype
- * (dense [m][n]), what the backward pass of an activation needs. */
+/* bias, residual and pre may be NULL.  pre: z = A . B + bias in f32 (dense
+ * [m][n]), what the backward pass of an activation needs. */
 int wtc_matmul_epilogue(const wtc_matmul_args* p, const void* a, const void* b, const void* bias,
-                        const void* residual, void* out, void* pre, void* workspace, size_t workspace_bytes,
+                        const void* residual, void* out, float* pre, void* workspace, size_t workspace_bytes,
                         void* stream);
 
 int64_t wtc_matmul_epilogue_backward_workspace_size(const wtc_matmul_args* p);
@@ -66,7 +66,7 @@ int64_t wtc_matmul_epilogue_backward_workspace_size(const wtc_matmul_args* p);
  * of the three may be NULL (not computed).  dout is of `dtype`.  pre may be
  * NULL with WTC_ACT_NONE.  The residual's gradient is dout itself. */
 int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, const void* a, const void* b,
-                                 const void* pre, void* da, void* db, float* dbias, void* workspace,
+                                 const float* pre, void* da, void* db, float* dbias, void* workspace,
                                  size_t workspace_bytes, void* stream);
 
 /*

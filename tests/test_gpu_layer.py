@@ -35,9 +35,9 @@ def check_matmul(W, m, n, k, dtype, out_dtype, kind, bias, residual, trans, a=No
     r = rand(seed + 3, m, n, dtype=out_dtype) if residual else None
     out, pre = W.matmul_epilogue(a, b, bias=bv, residual=r, activation=kind, out_dtype=out_dtype, return_pre=True)
     y, z, dz, dy = U.matmul_reference(a, b, bv, r, kind)
-    assert out.dtype == out_dtype and pre.dtype == dtype
+    assert out.dtype == out_dtype and pre.dtype == F32
     U.assert_within(out, y, U.rounded(y, dy, out_dtype), "out")
-    U.assert_within(pre, z, U.rounded(z, dz, dtype), "pre")
+    U.assert_within(pre, z, U.rounded(z, dz, F32), "pre")
     again = W.matmul_epilogue(a, b, bias=bv, residual=r, activation=kind, out_dtype=out_dtype)
     assert torch.equal(out, again), "two calls differ"
 
@@ -113,7 +113,7 @@ def test_matmul_extreme_values(W):
 def test_matmul_backward(W, m, n, k, dtype, trans, kind):
     a = rand(1, m, k, dtype=dtype)
     b = rand(2, n, k, dtype=dtype, by=0.1).t() if trans else rand(2, k, n, dtype=dtype, by=0.1)
-    dout, pre = rand(3, m, n, dtype=dtype), rand(4, m, n, dtype=dtype)
+    dout, pre = rand(3, m, n, dtype=dtype), rand(4, m, n)
     da, db, dbias = W.matmul_epilogue_backward(dout, a, b, pre=None if kind == "none" else pre, activation=kind)
     assert db.stride() == b.stride() or min(n, k) == 1
     dz = dout.double() * U.act_slope(pre.double(), kind)

@@ -60,46 +60,46 @@ __device__ inline float sigmoid(float z) {
 constexpr float kTanhC = 1.5957691216057308f;   // 2 sqrt(2 / pi): tanh(u) = 2 sigmoid(2u) - 1
 constexpr float kTanhC3 = 0.044715f;
 
-__device__ inline float act_value(float z, int act) {
-  switch (act) {
-    case WTC_ACT_RELU: return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-    // z of -inf: Phi and the sigmoid are 0 there, and so is the product's limit
-    case WTC_ACT_GELU: return z == -INFINITY ? 0.0f : z * normal_cdf(z);
-    case WTC_ACT_GELU_TANH: return z == -INFINITY ? 0.0f : z * sigmoid(kTanhC * z * __builtin_fmaf(kTanhC3 * z, z, 1.0f));
-    case WTC_ACT_SILU: return z == -INFINITY ? 0.0f : z * sigmoid(z);
-  }
+template <int ACT> __device__ inline float act_value(float z) {
+  if constexpr (ACT == WTC_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays NaN
+  // z of -inf: Phi and the sigmoid are 0 there, and so is the product's limit
+  if constexpr (ACT == WTC_ACT_GELU) return z == -INFINITY ? 0.0f : z * normal_cdf(z);
+  if constexpr (ACT == WTC_ACT_GELU_TANH)
+    return z == -INFINITY ? 0.0f : z * sigmoid(kTanhC * z * __builtin_fmaf(kTanhC3 * z, z, 1.0f));
+  if constexpr (ACT == WTC_ACT_SILU) return z == -INFINITY ? 0.0f : z * sigmoid(z);
   return z;
 }
-__device__ inline float act_slope(float z, int act) {
-  switch (act) {
-    case WTC_ACT_RELU: return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
-    case WTC_ACT_GELU: {
-      if (fabsf(z) > 16.0f) return z < 0.0f ? 0.0f : 1.0f;  // z * density(z) is 0 in f32 (and no inf * 0)
-      return __builtin_fmaf(z * 0.3989422804014327f, __builtin_amdgcn_exp2f(-0.7213475204444817f * z * z), normal_cdf(z));
-    }
-    case WTC_ACT_GELU_TANH: {
-      if (fabsf(z) > 16.0f) return z < 0.0f ? 0.0f : 1.0f;
-      const float y = sigmoid(kTanhC * z * __builtin_fmaf(kTanhC3 * z, z, 1.0f));
-      return __builtin_fmaf(z * y * (1.0f - y) * kTanhC, __builtin_fmaf(3.0f * kTanhC3 * z, z, 1.0f), y);
-    }
-    case WTC_ACT_SILU: {
-      if (fabsf(z) > 128.0f) return z < 0.0f ? 0.0f : 1.0f;
-      const float y = sigmoid(z);
-      return y * __builtin_fmaf(z, 1.0f - y, 1.0f);
-    }
+// Far out the slopes are 0 or 1 to the last bit of f32 (and the formulas would meet inf * 0).
+template <int ACT> __device__ inline float act_slope(float z) {
+  if constexpr (ACT == WTC_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
+  if constexpr (ACT == WTC_ACT_GELU) {
+    if (fabsf(z) > 16.0f) return z < 0.0f ? 0.0f : 1.0f;
+    return __builtin_fmaf(z * 0.3989422804014327f, __builtin_amdgcn_exp2f(-0.7213475204444817f * z * z), normal_cdf(z));
+  }
+  if constexpr (ACT == WTC_ACT_GELU_TANH) {
+    if (fabsf(z) > 16.0f) return z < 0.0f ? 0.0f : 1.0f;
+    const float y = sigmoid(kTanhC * z * __builtin_fmaf(kTanhC3 * z, z, 1.0f));
+    return __builtin_fmaf(z * y * (1.0f - y) * kTanhC, __builtin_fmaf(3.0f * kTanhC3 * z, z, 1.0f), y);
+  }
+  if constexpr (ACT == WTC_ACT_SILU) {
+    if (fabsf(z) > 128.0f) return z < 0.0f ? 0.0f : 1.0f;
+    const float y = sigmoid(z);
+    return y * __builtin_fmaf(z, 1.0f - y, 1.0f);
   }
   return 1.0f;
 }
 
 // ---- kernel arguments --------------------------------------------------------
 struct MatmulParams {
-  const uint8_t *a, *b;        // operands, element (i, kk) at i * a_row + kk * a_col (b: kk * b_row + j * b_col)
+  const uint8_t *a, *b;
   const void *bias, *residual;
   void *out, *pre;
-  int64_t a_row, a_col, b_row, b_col;
+  float* partial;        // [splits][m][n], if splits > 1
+  int64_t lda, ldb;      // elements between rows (KC) or between k (KS)
   int64_t ldr, ldo, ldp;
   int32_t m, n, k;
   int32_t bias_f32, act;
+  int32_t splits, slabs;  // k-slabs per split
 };
 
 struct AttnParams {

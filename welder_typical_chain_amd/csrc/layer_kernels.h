@@ -6,15 +6,26 @@
 
 namespace wtc {
 
-struct ActBackwardParams {
-  const void *dout, *pre;
-  void* dz;      // dense [m][n]; NULL: not written
-  float* dbias;  // [n]; NULL: not computed
-  int64_t m, n, ldd;
-  int32_t act;
+struct MatmulPlan {
+  int tile, splits, slabs;
 };
+MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, int cu_count);
+int64_t matmul_workspace(const MatmulPlan& plan, int64_t m, int64_t n);
+// aks / bks: the operand is strided along k (element (row, k) at k * ld + row) instead
+// of contiguous (row * ld + k); aks only with bks and out_dt == dt.
+hipError_t launch_matmul(const MatmulParams& p, const MatmulPlan& plan, int dt, int out_dt, bool aks, bool bks,
+                         hipStream_t stream);
 
-hipError_t launch_matmul(const MatmulParams& p, int dt, int out_dt, hipStream_t stream);
+struct ActBackwardParams {
+  const void* dout;
+  const float* pre;  // dense [m][n]
+  void* dz;          // dense [m][n]; NULL: not written
+  float* dbias;      // [n]; NULL: not computed
+  float* partial;    // [chunks][n], if chunks > 1
+  int64_t m, n, ldd, chunk_rows;
+  int32_t chunks, act;
+};
+int64_t act_backward_chunk_rows(int64_t m, int64_t n, int cu_count);
 hipError_t launch_act_backward(const ActBackwardParams& p, int dt, hipStream_t stream);
 
 hipError_t launch_attention(const AttnParams& p, int dt, hipStream_t stream);

@@ -49,6 +49,9 @@ int check_matmul(const wtc_matmul_args& p, bool backward) {
   if (p.m < 0 || p.n < 0 || p.k < 0) return bad("negative extent");
   if (p.m > kMost || p.n > kMost || p.k > kMost) return report(WTC_ERR_UNSUPPORTED, "extent above 2^30");
   if (p.n % 8 || p.k % 8) return bad("n and k must be multiples of 8");
+  // workgroups of the smallest tile with the most splits, of the forward product and of the gradients
+  const int64_t mt = (p.m + 127) / 128, nt = (p.n + 127) / 128, kt = (p.k + 127) / 128;
+  if (std::max({mt * nt, mt * kt, kt * nt}) > kMost / 16) return report(WTC_ERR_UNSUPPORTED, "too many tiles");
   const int64_t b_cols = p.b_trans ? p.k : p.n, b_rows = p.b_trans ? p.n : p.k;
   if (p.lda < p.k || p.ldb < b_cols || p.lda % 8 || p.ldb % 8)
     return bad("lda and ldb must be multiples of 8 that hold a row");
@@ -64,28 +67,39 @@ int check_matmul(const wtc_matmul_args& p, bool backward) {
   return WTC_OK;
 }
 
-int matmul_forward(const wtc_matmul_args& p, const void* a, const void* b, const void* bias, const void* residual,
-                   void* out, void* pre, hipStream_t stream) {
-  MatmulParams q{};
-  q.a = static_cast<const uint8_t*>(a);
-  q.b = static_cast<const uint8_t*>(b);
-  q.bias = bias;
-  q.residual = residual;
-  q.out = out;
-  q.pre = pre;
-  q.a_row = p.lda;
-  q.a_col = 1;
-  q.b_row = p.b_trans ? 1 : p.ldb;
-  q.b_col = p.b_trans ? p.ldb : 1;
-  q.ldr = p.ldr;
-  q.ldo = p.ldo;
-  q.ldp = p.n;
-  q.m = (int)p.m;
-  q.n = (int)p.n;
-  q.k = (int)p.k;
-  q.bias_f32 = p.bias_dtype == WTC_DTYPE_F32;
-  q.act = (int)p.activation;
-  return launched(launch_matmul(q, (int)p.dtype, (int)p.out_dtype, stream), "matmul_epilogue");
+// Compute units of the current device (256 where none is visible).
+int cu_count() {
+  static thread_local int dev = -1, count = 256;
+  int now = -1;
+  if (hipGetDevice(&now) != hipSuccess) return 256;
+  if (now != dev) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, now) != hipSuccess || n <= 0) n = 256;
+    dev = now;
+    count = n;
+  }
+  return count;
+}
+
+// Scratch of a backward call: dz (where an activation makes one), the columns'
+// sums of row chunks, the partial products of da, then of db (one after the
+// other in the same place).
+struct MatmulBackwardPlan {
+  int64_t chunk_rows, chunks;
+  MatmulPlan da, db;
+  int64_t sums_at, partial_at, total;
+};
+MatmulBackwardPlan plan_backward(const wtc_matmul_args& p) {
+  MatmulBackwardPlan q{};
+  const int cus = cu_count();
+  q.chunk_rows = act_backward_chunk_rows(p.m, p.n, cus);
+  q.chunks = std::max<int64_t>(1, (p.m + q.chunk_rows - 1) / q.chunk_rows);
+  q.da = plan_matmul(p.m, p.k, p.n, cus);
+  q.db = p.b_trans ? plan_matmul(p.n, p.k, p.m, cus) : plan_matmul(p.k, p.n, p.m, cus);
+  q.sums_at = p.activation == WTC_ACT_NONE ? 0 : align256(p.m * p.n * 2);
+  q.partial_at = q.sums_at + (q.chunks > 1 ? align256(q.chunks * p.n * 4) : 0);
+  q.total = q.partial_at + align256(std::max(matmul_workspace(q.da, p.m, p.k), matmul_workspace(q.db, p.k, p.n)));
+  return q;
 }
 
 // ---- attention ----------------------------------------------------------------
@@ -162,9 +176,6 @@ AttnParams attention_params(const wtc_attention_args& p) {
 }
 
 int64_t backward_workspace(const wtc_attention_args& p) { return align256(p.batch * p.heads * p.lq * 4); }
-int64_t matmul_backward_workspace(const wtc_matmul_args& p) {
-  return p.activation == WTC_ACT_NONE ? 0 : align256(p.m * p.n * 2);
-}
 
 }  // namespace
 
@@ -173,11 +184,11 @@ extern "C" {
 int64_t wtc_matmul_epilogue_workspace_size(const wtc_matmul_args* p) {
   if (!p) return bad("NULL arguments"), -1;
   if (guarded([&] { return check_matmul(*p, false); })) return -1;
-  return 0;
+  return align256(matmul_workspace(plan_matmul(p->m, p->n, p->k, cu_count()), p->m, p->n));
 }
 
 int wtc_matmul_epilogue(const wtc_matmul_args* p, const void* a, const void* b, const void* bias,
-                        const void* residual, void* out, void* pre, void* workspace, size_t workspace_bytes,
+                        const void* residual, void* out, float* pre, void* workspace, size_t workspace_bytes,
                         void* stream) {
   return guarded([&]() -> int {
     if (!p) return bad("NULL arguments");
@@ -186,18 +197,40 @@ int wtc_matmul_epilogue(const wtc_matmul_args* p, const void* a, const void* b, 
     if (!out || (p->k && (!a || !b))) return bad("NULL operand");
     if (!aligned16(a) || !aligned16(b) || !aligned16(out) || !aligned16(pre) || !aligned16(residual) || !aligned16(bias))
       return bad("pointers must be 16-byte aligned");
-    return matmul_forward(*p, a, b, bias, residual, out, pre, static_cast<hipStream_t>(stream));
+    const MatmulPlan plan = plan_matmul(p->m, p->n, p->k, cu_count());
+    if (int rc = check_workspace(workspace, workspace_bytes, align256(matmul_workspace(plan, p->m, p->n)))) return rc;
+    MatmulParams q{};
+    q.a = static_cast<const uint8_t*>(a);
+    q.b = static_cast<const uint8_t*>(b);
+    q.bias = bias;
+    q.residual = residual;
+    q.out = out;
+    q.pre = pre;
+    q.partial = static_cast<float*>(workspace);
+    q.lda = p->lda;
+    q.ldb = p->ldb;
+    q.ldr = p->ldr;
+    q.ldo = p->ldo;
+    q.ldp = p->n;
+    q.m = (int)p->m;
+    q.n = (int)p->n;
+    q.k = (int)p->k;
+    q.bias_f32 = p->bias_dtype == WTC_DTYPE_F32;
+    q.act = (int)p->activation;
+    return launched(launch_matmul(q, plan, (int)p->dtype, (int)p->out_dtype, false, !p->b_trans,
+                                  static_cast<hipStream_t>(stream)),
+                    "matmul_epilogue");
   });
 }
 
 int64_t wtc_matmul_epilogue_backward_workspace_size(const wtc_matmul_args* p) {
   if (!p) return bad("NULL arguments"), -1;
   if (guarded([&] { return check_matmul(*p, true); })) return -1;
-  return matmul_backward_workspace(*p);
+  return plan_backward(*p).total;
 }
 
 int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, const void* a, const void* b,
-                                 const void* pre, void* da, void* db, float* dbias, void* workspace,
+                                 const float* pre, void* da, void* db, float* dbias, void* workspace,
                                  size_t workspace_bytes, void* stream_) {
   return guarded([&]() -> int {
     if (!p) return bad("NULL arguments");
@@ -209,42 +242,53 @@ int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, con
     if (!aligned16(dout) || !aligned16(a) || !aligned16(b) || !aligned16(pre) || !aligned16(da) || !aligned16(db) ||
         !aligned16(dbias))
       return bad("pointers must be 16-byte aligned");
-    if (int rc = check_workspace(workspace, workspace_bytes, matmul_backward_workspace(*p))) return rc;
-    void* dz = act ? workspace : const_cast<void*>(dout);
+    const MatmulBackwardPlan plan = plan_backward(*p);
+    if (int rc = check_workspace(workspace, workspace_bytes, plan.total)) return rc;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    uint8_t* dz = act ? ws : static_cast<uint8_t*>(const_cast<void*>(dout));
     const int64_t ldz = act ? p->n : p->ldd;
-    if (p->n && (act || dbias)) {
-      ActBackwardParams q{dout, pre, act && (da || db) ? dz : nullptr, dbias, p->m, p->n, p->ldd, (int)p->activation};
-      if (int rc = launched(launch_act_backward(q, (int)p->dtype, stream), "activation gradient")) return rc;
+    const int dt = (int)p->dtype;
+    if (p->n && ((act && (da || db)) || dbias)) {
+      ActBackwardParams q{};
+      q.dout = dout;
+      q.pre = pre;
+      q.dz = act && (da || db) ? dz : nullptr;
+      q.dbias = dbias;
+      q.partial = reinterpret_cast<float*>(ws + plan.sums_at);
+      q.m = p->m;
+      q.n = p->n;
+      q.ldd = p->ldd;
+      q.chunk_rows = plan.chunk_rows;
+      q.chunks = (int)plan.chunks;
+      q.act = (int)p->activation;
+      if (int rc = launched(launch_act_backward(q, dt, stream), "activation gradient")) return rc;
     }
     MatmulParams q{};
-    if (da && p->m && p->k) {  // dz [m][n] . B^T
-      q.a = static_cast<const uint8_t*>(dz);
+    q.partial = reinterpret_cast<float*>(ws + plan.partial_at);
+    if (da && p->m && p->k) {  // dz [m][n] . B^T: B stored by rows is contiguous along n
+      q.a = dz;
       q.b = static_cast<const uint8_t*>(b);
-      q.a_row = ldz;
-      q.a_col = 1;
-      q.b_row = p->b_trans ? p->ldb : 1;
-      q.b_col = p->b_trans ? 1 : p->ldb;
+      q.lda = ldz;
+      q.ldb = p->ldb;
       q.out = da;
       q.ldo = p->k;
       q.m = (int)p->m;
       q.n = (int)p->k;
       q.k = (int)p->n;
-      if (int rc = launched(launch_matmul(q, (int)p->dtype, (int)p->dtype, stream), "da")) return rc;
+      if (int rc = launched(launch_matmul(q, plan.da, dt, dt, false, p->b_trans, stream), "da")) return rc;
     }
-    if (db && p->n && p->k) {  // A^T . dz, or its transpose
-      const uint8_t *x = static_cast<const uint8_t*>(a), *y = static_cast<const uint8_t*>(dz);
-      q.a = p->b_trans ? y : x;
-      q.b = p->b_trans ? x : y;
-      q.a_row = 1;
-      q.a_col = p->b_trans ? ldz : p->lda;
-      q.b_row = p->b_trans ? p->lda : ldz;
-      q.b_col = 1;
+    if (db && p->n && p->k) {  // A^T . dz, or its transpose dz^T . A: both strided along m
+      const uint8_t* x = static_cast<const uint8_t*>(a);
+      q.a = p->b_trans ? dz : x;
+      q.b = p->b_trans ? x : dz;
+      q.lda = p->b_trans ? ldz : p->lda;
+      q.ldb = p->b_trans ? p->lda : ldz;
       q.out = db;
       q.m = (int)(p->b_trans ? p->n : p->k);
       q.n = (int)(p->b_trans ? p->k : p->n);
       q.ldo = q.n;
       q.k = (int)p->m;
-      if (int rc = launched(launch_matmul(q, (int)p->dtype, (int)p->dtype, stream), "db")) return rc;
+      if (int rc = launched(launch_matmul(q, plan.db, dt, dt, true, true, stream), "db")) return rc;
     }
     return WTC_OK;
   });

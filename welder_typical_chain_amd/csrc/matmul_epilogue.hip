@@ -1,79 +1,444 @@
-// matmul_epilogue.hip -- kernels of wtc_matmul_epilogue and its gradients.
+// matmul_epilogue.hip -- kernels of wtc_matmul_epilogue and its gradients:
+//   out = round(act(A . B + bias) + residual), da = dz . B^T, db = A^T . dz
+//
+// One tile kernel for the three products.  An operand is either contiguous
+// along the contraction (KC: A of the product, both operands of da) or strided
+// along it (KS: B of the product, both operands of db); with B stored as its
+// transpose the two kinds change places.  A tile's k-slab of 32 elements takes
+// 64 bytes per row of the operand either way:
+//   KC  [rows][4 chunks of 16 bytes], read with ds_read_b128 (a64_lds_offset)
+//   KS  [32 k][128 columns] per 128 rows of the operand, read with the
+//       transposing ds_read_b64_tr_b16 (btr_offset)
+// 4 waves in a 2 x 2 grid, each a quarter of the tile in 32 x 32 MFMA subtiles
+// (v_mfma_f32_32x32x16, D = B^T . A^T: a lane's accumulators belong to one
+// output row).  Slabs go through a ring of 4 stages filled by direct-to-LDS
+// loads, three ahead of the one whose MFMAs run; the fragments of a slab's
+// second half are read while the MFMAs of the first issue, and the next
+// slab's first half under those of the second.
 #include "layer_common.h"
 #include "layer_kernels.h"
 
 namespace wtc {
 namespace {
 
+constexpr int kSlab = 64;    // bytes of k per ring stage and operand row
+constexpr int kSlabK = 32;   // elements
+constexpr int kStages = 4;
+constexpr int kThreads = 256;
+
 __device__ inline float load_elem(const void* p, int64_t i, int dt) {
   if (dt == DT_F32) return static_cast<const float*>(p)[i];
   if (dt == DT_F16) return (float)static_cast<const _Float16*>(p)[i];
   return (float)static_cast<const __bf16*>(p)[i];
 }
-template <int DT> __device__ inline void store_elem(void* p, int64_t i, float x) {
-  static_cast<typename Elem<DT>::type*>(p)[i] = (typename Elem<DT>::type)x;
-}
 
-constexpr int kT = 16;
-
-// One output element a thread, operands staged 16 x 16 at a time.
-template <int DT, int OUT_DT>
-__global__ void __launch_bounds__(kT* kT) matmul_simple_kernel(const MatmulParams p) {
-  __shared__ float sa[kT][kT + 1], sb[kT][kT + 1];
-  const int tx = threadIdx.x % kT, ty = threadIdx.x / kT;
-  const int nt = (p.n + kT - 1) / kT;
-  const int64_t i = (int64_t)(blockIdx.x / nt) * kT + ty, j = (int64_t)(blockIdx.x % nt) * kT + tx;
-  const int64_t i_b = j - tx + ty;  // column of b this thread stages
-  float acc = 0.0f;
-  for (int k0 = 0; k0 < p.k; k0 += kT) {
-    const int ka = k0 + tx;
-    sa[ty][tx] = i < p.m && ka < p.k ? load_elem(p.a, i * p.a_row + ka * p.a_col, DT) : 0.0f;
-    sb[tx][ty] = i_b < p.n && ka < p.k ? load_elem(p.b, ka * p.b_row + i_b * p.b_col, DT) : 0.0f;
-    __syncthreads();
-    for (int kk = 0; kk < kT; ++kk) acc = __builtin_fmaf(sa[ty][kk], sb[kk][tx], acc);
-    __syncthreads();
+// Eight consecutive values, 16-byte aligned.
+template <int DT> __device__ inline void load8(const void* p, int64_t i, float (&x)[8]) {
+  if constexpr (DT == DT_F32) {
+    const f32x4 *q = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i), lo = q[0], hi = q[1];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = lo[u], x[4 + u] = hi[u];
+  } else {
+    const auto v = *reinterpret_cast<const typename Elem<DT>::vec8*>(static_cast<const typename Elem<DT>::type*>(p) + i);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = (float)v[u];
   }
-  if (i >= p.m || j >= p.n) return;
-  if (p.bias) acc += load_elem(p.bias, j, p.bias_f32 ? DT_F32 : DT);
-  if (p.pre) store_elem<DT>(p.pre, i * p.ldp + j, acc);
-  acc = act_value(acc, p.act);
-  if (p.residual) acc += load_elem(p.residual, i * p.ldr + j, OUT_DT);
-  store_elem<OUT_DT>(p.out, i * p.ldo + j, acc);
+}
+template <int DT> __device__ inline void store8(void* p, int64_t i, const float (&x)[8]) {
+  if constexpr (DT == DT_F32) {
+    f32x4* q = reinterpret_cast<f32x4*>(static_cast<float*>(p) + i);
+    q[0] = f32x4{x[0], x[1], x[2], x[3]};
+    q[1] = f32x4{x[4], x[5], x[6], x[7]};
+  } else {
+    uint32_t w[4];
+    pack4<DT>(f32x4{x[0], x[1], x[2], x[3]}, &w[0], &w[1]);
+    pack4<DT>(f32x4{x[4], x[5], x[6], x[7]}, &w[2], &w[3]);
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + i) = u32x4{w[0], w[1], w[2], w[3]};
+  }
 }
 
-// dz = dout * act'(pre), rounded for the products; a column's sum in f32 of the
-// values before rounding.  One thread a column, rows in their order.
+// The epilogue of eight columns n .. n+7 of row m; z: the products.
+template <int DT, int OUT_DT, int ACT>
+__device__ inline void finish8(const MatmulParams& p, int64_t m, int64_t n, float (&z)[8]) {
+  float y[8];
+  if (p.bias) {
+    if (p.bias_f32) load8<DT_F32>(p.bias, n, y);
+    else load8<DT>(p.bias, n, y);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) z[u] += y[u];
+  }
+  if (p.pre) store8<DT_F32>(p.pre, m * p.ldp + n, z);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) z[u] = act_value<ACT>(z[u]);
+  if (p.residual) {
+    load8<OUT_DT>(p.residual, m * p.ldr + n, y);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) z[u] += y[u];
+  }
+  store8<OUT_DT>(p.out, m * p.ldo + n, z);
+}
+
+// Direct-to-LDS loads of one operand: wave w fills blocks nb*w .. of 1 KiB.
+// Rows (KC) and columns (KS) past the operand's end are parked at kOutOfRange,
+// whose loads give zeros; so are slabs from k_end on.
+template <bool KS, int ROWS> struct Loader {
+  static constexpr int NB = ROWS * kSlab / 1024 / 4;  // blocks per wave: 4 or 2
+  i32x4 rsrc;
+  uint32_t off[NB];
+  uint32_t ld, kpos, lds;
+  __device__ inline void init(const uint8_t* base, uint32_t rows, uint32_t row0, uint32_t k_total, uint32_t ld_bytes,
+                              int wave, int lane) {
+    const uint32_t bytes = KS ? (k_total ? (k_total - 1) * ld_bytes + rows * 2 : 0) : (rows - 1) * ld_bytes + k_total * 2;
+    const i32x4 r = raw_rsrc(base, bytes);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(r[i]);
+    ld = ld_bytes;
+    if constexpr (KS) {
+      // blocks of 4 k-rows x 128 columns, 8 a 128-column half
+      const int half = wave * NB / 8, blk = wave * NB % 8;
+      const uint32_t col = row0 + 128u * half + 8u * (uint32_t)dma_b_chunk(blk, lane);
+      kpos = (uint32_t)dma_b_row(blk, lane);
+#pragma unroll
+      for (int q = 0; q < NB; ++q) off[q] = col < rows ? (kpos + 4u * q) * ld + col * 2u : kOutOfRange;
+      lds = (uint32_t)(half * 8192 + blk * 1024);
+    } else {
+      kpos = 8u * (uint32_t)dma64_a_chunk(0, lane);
+#pragma unroll
+      for (int q = 0; q < NB; ++q) {
+        const uint32_t row = row0 + (uint32_t)dma64_a_row(wave * NB + q, lane);
+        off[q] = row < rows ? row * ld + kpos * 2u : kOutOfRange;
+      }
+      lds = (uint32_t)(wave * NB * 1024);
+    }
+  }
+  // block q of slab kt (k from 32 kt), elements from k_end on read as zeros
+  __device__ inline void issue(uint32_t stage, int kt, uint32_t k_end, int q) const {
+    const uint32_t k = (uint32_t)kt * kSlabK + kpos + (KS ? 4u * q : 0u);
+    const uint32_t step = KS ? (uint32_t)kt * kSlabK * ld : (uint32_t)kt * kSlab;
+    dma16(rsrc, k < k_end && off[q] != kOutOfRange ? off[q] + step : kOutOfRange, stage + lds + q * 1024);
+  }
+};
+
+// Fragment reads of one operand for a wave's W subtiles of 32 rows.
+template <bool KS, int W> struct Frags {
+  uint32_t base[KS ? W : 2];
+  __device__ inline void init(uint32_t at, int row0, int lane) {
+    if constexpr (KS) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const int c = row0 + 32 * i;
+        base[i] = at + (uint32_t)((c >> 7) * 8192 + btr_offset(btr_k(0, 0, lane), btr_n(c & 127, lane)));
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) base[s] = at + (uint32_t)a64_lds_offset(row0 + frag_row(lane), frag64_chunk16(lane, s));
+    }
+  }
+  static constexpr int READS = KS ? 2 * W : W;
+  __device__ inline void read(const uint8_t* st, int s, int u, u32x4 (&f)[W]) const {
+    if constexpr (KS) {
+      const int i = u >> 1, h = u & 1;
+      const u32x2 v = tr_read(st + base[i] + (16 * s + 4 * h) * 256);
+      f[i][2 * h] = v[0];
+      f[i][2 * h + 1] = v[1];
+    } else {
+      f[u] = *reinterpret_cast<const u32x4*>(st + base[s] + u * 2048);
+    }
+  }
+};
+
+template <int TM, int TN> struct TileLds {
+  static constexpr int A_STAGE = TM * kSlab, STAGE = (TM + TN) * kSlab;
+  static constexpr int RING = kStages * STAGE;
+  // epilogue: a wave stages 32 rows of its quarter in f32
+  static constexpr int PITCH = TN / 2 * 4 + 16;
+  static constexpr int TOTAL = RING > 4 * 32 * PITCH ? RING : 4 * 32 * PITCH;
+  static_assert(TOTAL <= 160 * 1024, "LDS");
+};
+
+// Grid: tiles * splits; split s takes k-slabs [s * slabs, (s + 1) * slabs) and, where
+// there are several, writes f32 partial products [split][m][n] to p.partial.
+template <int DT, int OUT_DT, bool AKS, bool BKS, int TM, int TN>
+__global__ void __launch_bounds__(kThreads, TM == 256 ? 1 : 2) matmul_tile_kernel(const MatmulParams p) {
+  using L = TileLds<TM, TN>;
+  constexpr int WM = TM / 64, WN = TN / 64;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const uint32_t rows = (uint32_t)(p.m + TM - 1) / TM, cols = (uint32_t)(p.n + TN - 1) / TN;
+  uint32_t rt, ct;  // all splits of a tile row are rows of the map
+  tile_of_block(blockIdx.x, gridDim.x, rows * p.splits, cols, &rt, &ct);
+  const uint32_t split = rt / rows;
+  rt -= split * rows;
+  const uint32_t row0 = rt * TM, n0 = ct * TN;
+  const int kt0 = (int)split * p.slabs;
+  const int nk = min(p.slabs, (p.k + kSlabK - 1) / kSlabK - kt0);
+  const uint32_t k_end = (uint32_t)min((int64_t)p.k, (int64_t)(kt0 + p.slabs) * kSlabK);
+
+  f32x16 acc[WM][WN];
+#pragma unroll
+  for (int i = 0; i < WM; ++i)
+#pragma unroll
+    for (int j = 0; j < WN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+
+  Loader<AKS, TM> la;
+  Loader<BKS, TN> lb;
+  la.init(p.a, (uint32_t)p.m, row0, (uint32_t)p.k, (uint32_t)p.lda * 2u, wave, lane);
+  lb.init(p.b, (uint32_t)p.n, n0, (uint32_t)p.k, (uint32_t)p.ldb * 2u, wave, lane);
+  Frags<AKS, WM> fa;
+  Frags<BKS, WN> fb;
+  fa.init(0, wm * (TM / 2), lane);
+  fb.init(L::A_STAGE, wn * (TN / 2), lane);
+  constexpr int NA = Loader<AKS, TM>::NB, LOADS = NA + Loader<BKS, TN>::NB;
+  constexpr int RA = Frags<AKS, WM>::READS, R = RA + Frags<BKS, WN>::READS;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
+  auto load = [&](uint32_t stage, int kt, int j) {
+    // A and B blocks alternate
+    if (j & 1) lb.issue(stage + L::A_STAGE, kt0 + kt, k_end, j >> 1);
+    else la.issue(stage, kt0 + kt, k_end, j >> 1);
+  };
+  static_assert(NA * 2 == LOADS, "square tiles");
+  auto read = [&](const uint8_t* st, int s, int u, u32x4 (&a)[WM], u32x4 (&b)[WN]) {
+    if (u < RA) fa.read(st, s, u, a);
+    else if (u < R) fb.read(st, s, u - RA, b);
+  };
+  constexpr int RG = (R + WM - 1) / WM, LG = LOADS / WM;  // reads and loads per group of MFMAs
+  if (nk > 0) {
+#pragma unroll
+    for (int q = 0; q < kStages; ++q)
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) load(lds0 + q * L::STAGE, q, j);
+    wait_loads_barrier<LOADS*(kStages - 1)>();
+    u32x4 a0[WM], b0[WN], a1[WM], b1[WN];
+#pragma unroll
+    for (int u = 0; u < R; ++u) read(smem, 0, u, a0, b0);
+    for (int kt = 0; kt < nk; ++kt) {
+      const uint8_t* cur = smem + (kt % kStages) * L::STAGE;
+      const uint8_t* nxt = smem + ((kt + 1) % kStages) * L::STAGE;
+      const uint32_t fill = lds0 + (kt % kStages) * L::STAGE;
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int g = 0; g < WM; ++g) {
+#pragma unroll
+        for (int u = 0; u < RG; ++u) read(cur, 1, RG * g + u, a1, b1);
+#pragma unroll
+        for (int j = 0; j < WN; ++j) acc[g][j] = mfma32<DT>(b0[j], a0[g], acc[g][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wait_loads_barrier<LOADS*(kStages - 2)>();  // slab kt+1 landed; slab kt read
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int g = 0; g < WM; ++g) {
+#pragma unroll
+        for (int j = 0; j < WN; ++j) {
+          acc[g][j] = mfma32<DT>(b1[j], a1[g], acc[g][j]);
+          if (j < LG) {  // each load right behind an MFMA
+            __builtin_amdgcn_sched_barrier(0);
+            load(fill, kt + kStages, LG * g + j);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (j == LG - 1) {
+#pragma unroll
+            for (int u = 0; u < RG; ++u) read(nxt, 0, RG * g + u, a0, b0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    wait_loads_barrier<0>();
+  }
+
+  // ---- epilogue: each wave by itself, 32 rows at a time through its part of LDS,
+  // from a row a lane to eight columns a lane
+  constexpr int CW = TN / 2, LPR = CW / 8, RPI = 64 / LPR;
+  uint8_t* stg = smem + wave * 32 * L::PITCH;
+  auto epilogue = [&](auto finish) {
+#pragma unroll
+    for (int mt = 0; mt < WM; ++mt) {
+#pragma unroll
+      for (int j = 0; j < WN; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(stg + acc_j(lane) * L::PITCH + (j * 32 + acc_i(lane, 4 * g)) * 4) =
+              f32x4{acc[mt][j][4 * g], acc[mt][j][4 * g + 1], acc[mt][j][4 * g + 2], acc[mt][j][4 * g + 3]};
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 2
+      for (int it = 0; it < 32 / RPI; ++it) {
+        const int r = it * RPI + lane / LPR, c = lane % LPR * 8;
+        const int64_t m = (int64_t)row0 + wm * (TM / 2) + mt * 32 + r, n = (int64_t)n0 + wn * CW + c;
+        float z[8];
+        const f32x4* src = reinterpret_cast<const f32x4*>(stg + r * L::PITCH + c * 4);
+        const f32x4 lo = src[0], hi = src[1];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) z[u] = lo[u], z[4 + u] = hi[u];
+        if (m < p.m && n < p.n) finish(m, n, z);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  };
+  if (p.splits > 1) {
+    float* part = p.partial + (int64_t)split * p.m * p.n;
+    epilogue([&](int64_t m, int64_t n, float (&z)[8]) { store8<DT_F32>(part, m * p.n + n, z); });
+    return;
+  }
+  switch (p.act) {
+    case WTC_ACT_NONE: return epilogue([&](int64_t m, int64_t n, float (&z)[8]) { finish8<DT, OUT_DT, WTC_ACT_NONE>(p, m, n, z); });
+    case WTC_ACT_RELU: return epilogue([&](int64_t m, int64_t n, float (&z)[8]) { finish8<DT, OUT_DT, WTC_ACT_RELU>(p, m, n, z); });
+    case WTC_ACT_GELU: return epilogue([&](int64_t m, int64_t n, float (&z)[8]) { finish8<DT, OUT_DT, WTC_ACT_GELU>(p, m, n, z); });
+    case WTC_ACT_GELU_TANH: return epilogue([&](int64_t m, int64_t n, float (&z)[8]) { finish8<DT, OUT_DT, WTC_ACT_GELU_TANH>(p, m, n, z); });
+    case WTC_ACT_SILU: return epilogue([&](int64_t m, int64_t n, float (&z)[8]) { finish8<DT, OUT_DT, WTC_ACT_SILU>(p, m, n, z); });
+  }
+}
+
+// The partial products of all splits, summed in their order, and the epilogue.
+template <int DT, int OUT_DT>
+__global__ void __launch_bounds__(256) matmul_join_kernel(const MatmulParams p) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8, total = (int64_t)p.m * p.n;
+  if (at >= total) return;
+  float z[8], y[8];
+  load8<DT_F32>(p.partial, at, z);
+  for (int s = 1; s < p.splits; ++s) {
+    load8<DT_F32>(p.partial, s * total + at, y);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) z[u] += y[u];
+  }
+  const int64_t m = at / p.n, n = at - m * p.n;
+  switch (p.act) {
+    case WTC_ACT_NONE: return finish8<DT, OUT_DT, WTC_ACT_NONE>(p, m, n, z);
+    case WTC_ACT_RELU: return finish8<DT, OUT_DT, WTC_ACT_RELU>(p, m, n, z);
+    case WTC_ACT_GELU: return finish8<DT, OUT_DT, WTC_ACT_GELU>(p, m, n, z);
+    case WTC_ACT_GELU_TANH: return finish8<DT, OUT_DT, WTC_ACT_GELU_TANH>(p, m, n, z);
+    case WTC_ACT_SILU: return finish8<DT, OUT_DT, WTC_ACT_SILU>(p, m, n, z);
+  }
+}
+
+// dz = dout * act'(pre), rounded for the products; the columns' sums in f32 of
+// the values before rounding.  A workgroup takes 128 columns (16 threads of
+// eight) of `chunk` rows, 16 rows at a time; with several row chunks the sums
+// go to p.partial [chunk][n], which sum_chunks_kernel adds in order.
 template <int DT>
 __global__ void __launch_bounds__(256) act_backward_kernel(const ActBackwardParams p) {
+  __shared__ float red[16][128 + 4];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int cols = (int)((p.n + 127) / 128);
+  const int chunk = blockIdx.x / cols;
+  const int64_t n = (int64_t)(blockIdx.x % cols) * 128 + tx * 8;
+  const int64_t m1 = min(p.m, (int64_t)(chunk + 1) * p.chunk_rows);
+  float sum[8] = {};
+  if (n < p.n)
+    for (int64_t m = (int64_t)chunk * p.chunk_rows + ty; m < m1; m += 16) {
+      float g[8], z[8];
+      load8<DT>(p.dout, m * p.ldd + n, g);
+      if (p.act != WTC_ACT_NONE) {
+        load8<DT_F32>(p.pre, m * p.n + n, z);
+        switch (p.act) {
+          case WTC_ACT_RELU: for (int u = 0; u < 8; ++u) g[u] *= act_slope<WTC_ACT_RELU>(z[u]); break;
+          case WTC_ACT_GELU: for (int u = 0; u < 8; ++u) g[u] *= act_slope<WTC_ACT_GELU>(z[u]); break;
+          case WTC_ACT_GELU_TANH: for (int u = 0; u < 8; ++u) g[u] *= act_slope<WTC_ACT_GELU_TANH>(z[u]); break;
+          case WTC_ACT_SILU: for (int u = 0; u < 8; ++u) g[u] *= act_slope<WTC_ACT_SILU>(z[u]); break;
+        }
+        if (p.dz) store8<DT>(p.dz, m * p.n + n, g);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum[u] += g[u];
+    }
+  if (!p.dbias) return;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) red[ty][tx * 8 + u] = sum[u];
+  __syncthreads();
+  const int64_t j = (int64_t)(blockIdx.x % cols) * 128 + threadIdx.x;
+  if (threadIdx.x < 128 && j < p.n) {
+    float s = 0.0f;
+    for (int r = 0; r < 16; ++r) s += red[r][threadIdx.x];
+    (p.chunks > 1 ? p.partial + chunk * p.n : p.dbias)[j] = s;
+  }
+}
+__global__ void __launch_bounds__(256) sum_chunks_kernel(const ActBackwardParams p) {
   const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (j >= p.n) return;
-  float sum = 0.0f;
-  for (int64_t i = 0; i < p.m; ++i) {
-    float g = load_elem(p.dout, i * p.ldd + j, DT);
-    if (p.act != WTC_ACT_NONE) g *= act_slope(load_elem(p.pre, i * p.n + j, DT), p.act);
-    sum += g;
-    if (p.dz) store_elem<DT>(p.dz, i * p.n + j, g);
-  }
-  if (p.dbias) p.dbias[j] = sum;
+  float s = 0.0f;
+  for (int c = 0; c < p.chunks; ++c) s += p.partial[c * p.n + j];
+  p.dbias[j] = s;
+}
+
+template <typename P> hipError_t run(const void* fn, int64_t grid, int threads, const P& p, hipStream_t stream) {
+  P q = p;
+  void* args[] = {&q};
+  return hipLaunchKernel(fn, dim3((unsigned)grid), dim3(threads), args, 0, stream);
+}
+
+template <int DT, int OUT_DT, int T> const void* tile_by_kind(bool aks, bool bks) {
+  if (aks) return (const void*)&matmul_tile_kernel<DT, DT, true, true, T, T>;  // db: out is of the input type
+  return bks ? (const void*)&matmul_tile_kernel<DT, OUT_DT, false, true, T, T>
+             : (const void*)&matmul_tile_kernel<DT, OUT_DT, false, false, T, T>;
+}
+template <int DT, int OUT_DT> const void* tile_by_size(int tile, bool aks, bool bks) {
+  return tile == 256 ? tile_by_kind<DT, OUT_DT, 256>(aks, bks) : tile_by_kind<DT, OUT_DT, 128>(aks, bks);
 }
 
 }  // namespace
 
-hipError_t launch_matmul(const MatmulParams& p, int dt, int out_dt, hipStream_t stream) {
-  const int64_t grid = ((int64_t)(p.m + kT - 1) / kT) * ((p.n + kT - 1) / kT);
-  const void* fn =
-      dt == DT_F16 ? (out_dt == DT_F32 ? (const void*)&matmul_simple_kernel<DT_F16, DT_F32> : (const void*)&matmul_simple_kernel<DT_F16, DT_F16>)
-                   : (out_dt == DT_F32 ? (const void*)&matmul_simple_kernel<DT_BF16, DT_F32> : (const void*)&matmul_simple_kernel<DT_BF16, DT_BF16>);
-  MatmulParams q = p;
-  void* args[] = {&q};
-  return hipLaunchKernel(fn, dim3((unsigned)grid), dim3(kT * kT), args, 0, stream);
+// The tile and the number of k-splits: as many workgroups as the chip holds at
+// once (256 of the large tile, 512 of the small one), each with at least 8 slabs.
+MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, int cu_count) {
+  MatmulPlan best{};
+  double best_us = 0;
+  const int64_t slabs = (k + kSlabK - 1) / kSlabK;
+  for (int tile : {256, 128}) {
+    const int64_t tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
+    const int64_t slots = tile == 256 ? cu_count : 2 * cu_count;
+    for (int64_t s = 1; s <= 16 && (s == 1 || slabs / s >= 4); s *= 2) {
+      const int64_t per = (slabs + s - 1) / s;
+      const int64_t splits = per ? (slabs + per - 1) / per : 1;
+      const int64_t waves = (tiles * splits + slots - 1) / slots;
+      const double slab_us = tile == 256 ? 0.62 : 0.40;
+      double us = waves * (per * slab_us + (tile == 256 ? 6.0 : 3.0));
+      if (splits > 1) us += 4.0 + (double)m * n * 4 * (splits + 1) * 2 / 4.0e6;
+      if (best_us == 0 || us < best_us) {
+        best_us = us;
+        best = MatmulPlan{tile, (int)splits, (int)per};
+      }
+    }
+  }
+  return best;
+}
+int64_t matmul_workspace(const MatmulPlan& plan, int64_t m, int64_t n) {
+  return plan.splits > 1 ? plan.splits * m * n * 4 : 0;
+}
+
+hipError_t launch_matmul(const MatmulParams& params, const MatmulPlan& plan, int dt, int out_dt, bool aks, bool bks,
+                         hipStream_t stream) {
+  MatmulParams p = params;
+  p.splits = plan.splits;
+  p.slabs = plan.slabs;
+  const int64_t grid = ((int64_t)(p.m + plan.tile - 1) / plan.tile) * ((p.n + plan.tile - 1) / plan.tile) * p.splits;
+  const bool f32 = out_dt == DT_F32;
+  const void* fn = dt == DT_F16 ? (f32 ? tile_by_size<DT_F16, DT_F32>(plan.tile, aks, bks) : tile_by_size<DT_F16, DT_F16>(plan.tile, aks, bks))
+                                : (f32 ? tile_by_size<DT_BF16, DT_F32>(plan.tile, aks, bks) : tile_by_size<DT_BF16, DT_BF16>(plan.tile, aks, bks));
+  const hipError_t e = run(fn, grid, kThreads, p, stream);
+  if (e != hipSuccess || p.splits == 1) return e;
+  fn = dt == DT_F16 ? (f32 ? (const void*)&matmul_join_kernel<DT_F16, DT_F32> : (const void*)&matmul_join_kernel<DT_F16, DT_F16>)
+                    : (f32 ? (const void*)&matmul_join_kernel<DT_BF16, DT_F32> : (const void*)&matmul_join_kernel<DT_BF16, DT_BF16>);
+  return run(fn, ((int64_t)p.m * p.n / 8 + 255) / 256, 256, p, stream);
+}
+
+// Row chunks of the activation's gradient: enough workgroups to fill the chip, of at least 32 rows.
+int64_t act_backward_chunk_rows(int64_t m, int64_t n, int cu_count) {
+  const int64_t cols = (n + 127) / 128;
+  const int64_t chunks = cols ? (4 * cu_count + cols - 1) / cols : 1;
+  const int64_t rows = (m + chunks - 1) / chunks;
+  return rows < 32 ? 32 : (rows + 15) / 16 * 16;
 }
 
 hipError_t launch_act_backward(const ActBackwardParams& p, int dt, hipStream_t stream) {
-  const void* fn = dt == DT_F16 ? (const void*)&act_backward_kernel<DT_F16> : (const void*)&act_backward_kernel<DT_BF16>;
-  ActBackwardParams q = p;
-  void* args[] = {&q};
-  return hipLaunchKernel(fn, dim3((unsigned)((p.n + 255) / 256)), dim3(256), args, 0, stream);
+  const int64_t cols = (p.n + 127) / 128;
+  const hipError_t e = run(dt == DT_F16 ? (const void*)&act_backward_kernel<DT_F16> : (const void*)&act_backward_kernel<DT_BF16>,
+                           cols * p.chunks, 256, p, stream);
+  if (e != hipSuccess || p.chunks == 1 || !p.dbias) return e;
+  return run((const void*)&sum_chunks_kernel, (p.n + 255) / 256, 256, p, stream);
 }
 
 }  // namespace wtc

@@ -125,8 +125,8 @@ def matmul_epilogue(a: torch.Tensor, b: torch.Tensor, *, bias: torch.Tensor | No
     "gelu" (z Phi(z)), "gelu_tanh" or "silu".  Products and epilogue are
     float32, rounded once to `out_dtype` (a's type, or float32).  `out` may be
     `residual` itself, and no other input.  With return_pre=True the result is
-    (out, pre), pre = a @ b + bias rounded to a's type, which
-    matmul_epilogue_backward needs for an activation.
+    (out, pre), pre = a @ b + bias in float32, which matmul_epilogue_backward
+    needs for an activation (rounded to 16 bits it would move dbias by 5e-4).
     """
     code = _code_of(a, "a")
     k = a.shape[-1] if a.dim() else 0
@@ -164,7 +164,7 @@ def matmul_epilogue(a: torch.Tensor, b: torch.Tensor, *, bias: torch.Tensor | No
         r2 = residual if residual.dim() == 2 else residual.reshape(-1, n) if residual.numel() else out2
         ldr = _row_stride(r2, "residual")
         residual = r2
-    pre = torch.empty(shape, dtype=a.dtype, device=a.device) if return_pre else None
+    pre = torch.empty(shape, dtype=torch.float32, device=a.device) if return_pre else None
     lib = _lib.lib()
     args = _pack_matmul(m, n, k, _row_stride(a2, "a"), ldb, ldr, ldo, trans, code, _FLOATS[out_dtype], bias_code,
                         act, n)
@@ -192,14 +192,15 @@ def matmul_epilogue_backward(dout: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     a2 = a if a.dim() == 2 else a.reshape(-1, k) if a.numel() else a.new_empty((lead.numel(), k))
     m = a2.shape[0]
     n, ldb, trans = _weights(b, k)
-    device = _check_inputs(a.dtype, ("dout", dout), ("a", a), ("b", b), ("pre", pre))
+    device = _check_inputs(a.dtype, ("dout", dout), ("a", a), ("b", b))
+    _check_inputs(torch.float32, ("pre", pre))
     act = _activation(activation)
     if dout.shape != lead + (n,):
         raise ValueError(f"dout must be {tuple(lead + (n,))}")
     if act and pre is None:
         raise ValueError("the gradient of an activation needs pre")
-    if pre is not None and (pre.shape != dout.shape or not pre.is_contiguous()):
-        raise ValueError("pre must be contiguous and of dout's shape")
+    if pre is not None and (pre.shape != dout.shape or not pre.is_contiguous() or pre.get_device() != device):
+        raise ValueError("pre must be contiguous, of dout's shape and on its device")
     d2 = dout if dout.dim() == 2 else dout.reshape(-1, n) if dout.numel() else dout.new_empty((m, n))
     da = torch.empty(a.shape, dtype=a.dtype, device=a.device) if need_a else None
     db = None
