@@ -95,9 +95,10 @@ typedef struct wtc_attention_args {
   double scale;
 } wtc_attention_args;
 
+int64_t wtc_window_attention_workspace_size(const wtc_attention_args* p);
 /* lse: f32 [batch][heads][lq], the rows' log-sum-exp of scale * q . k (NULL: not written) */
 int wtc_window_attention(const wtc_attention_args* p, const void* q, const void* k, const void* v, void* out,
-                         float* lse, void* stream);
+                         float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 int64_t wtc_window_attention_backward_workspace_size(const wtc_attention_args* p);
 /* out and lse: of the forward call.  dq, dk, dv: dense, in the layouts of q, k, v. */

@@ -92,7 +92,7 @@ BAD_ATTENTION = [
     (dict(o=(2048, 0, 64)), ERR_ARG), (dict(o=(2048, 256, 32)), ERR_ARG), (dict(o=(0, 256, 64)), ERR_ARG),
     (dict(lq=1 << 31), ERR_UNSUPPORTED)])
 def test_attention_refusals(L, kw, code):
-    assert L.wtc_window_attention(attention_args(**kw), A, A, A, A, None, None) == code
+    assert L.wtc_window_attention(attention_args(**kw), A, A, A, A, None, A, 1 << 40, None) == code
     assert L.wtc_last_error()
 
 
@@ -101,10 +101,10 @@ def test_attention_pointer_refusals(L):
     for k in range(4):
         ptrs = [A, A, A, A]
         ptrs[k] += 2
-        assert L.wtc_window_attention(ok, *ptrs, None, None) == ERR_ARG
+        assert L.wtc_window_attention(ok, *ptrs, None, A, 1 << 40, None) == ERR_ARG
         ptrs[k] = None
-        assert L.wtc_window_attention(ok, *ptrs, None, None) == ERR_ARG
-    assert L.wtc_window_attention(attention_args(batch=0), None, None, None, None, None, None) == 0
+        assert L.wtc_window_attention(ok, *ptrs, None, A, 1 << 40, None) == ERR_ARG
+    assert L.wtc_window_attention(attention_args(batch=0), None, None, None, None, None, None, 0, None) == 0
 
 
 @pytest.mark.parametrize("kw,code", BAD_ATTENTION + [(dict(do=(2048, 250, 64)), ERR_ARG)])

@@ -112,6 +112,8 @@ struct AttnParams {
   int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3], do_stride[3];  // elements
   int64_t kn_stride[2], vn_stride[2];
   int64_t window;  // INT32_MAX at most (no limit)
+  float *part_out, *part_lse;  // of a row's splits: normalised results and log-sum-exp
+  int32_t splits, row_blocks;
   int32_t batch, heads, kv_heads, group, lq, lk, dim, sinks;
   float scale;
 };

@@ -28,7 +28,13 @@ struct ActBackwardParams {
 int64_t act_backward_chunk_rows(int64_t m, int64_t n, int cu_count);
 hipError_t launch_act_backward(const ActBackwardParams& p, int dt, hipStream_t stream);
 
-hipError_t launch_attention(const AttnParams& p, int dt, hipStream_t stream);
+struct AttnPlan {
+  int waves, splits;
+};
+AttnPlan plan_attention(const AttnParams& p, int cu_count);
+int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);
+// p.part_out: attention_workspace() bytes
+hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, hipStream_t stream);
 hipError_t launch_attention_backward(const AttnParams& p, int dt, hipStream_t stream);
 hipError_t launch_attention_decode(const AttnParams& p, int dt, hipStream_t stream);
 

@@ -156,6 +156,9 @@ AttnParams attention_params(const wtc_attention_args& p) {
     q.o_stride[i] = p.o_stride[i];
     q.do_stride[i] = p.do_stride[i];
   }
+  // the stride of a single token counts for nothing
+  if (p.lq <= 1) q.q_stride[1] = q.o_stride[1] = q.do_stride[1] = 0;
+  if (p.lk <= 1) q.k_stride[1] = q.v_stride[1] = 0;
   for (int i = 0; i < 2; ++i) {
     q.kn_stride[i] = p.kn_stride[i];
     q.vn_stride[i] = p.vn_stride[i];
@@ -294,8 +297,15 @@ int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, con
   });
 }
 
+int64_t wtc_window_attention_workspace_size(const wtc_attention_args* p) {
+  if (!p) return bad("NULL arguments"), -1;
+  if (guarded([&] { return check_attention(*p, false); })) return -1;
+  const AttnParams a = attention_params(*p);
+  return align256(attention_workspace(a, plan_attention(a, cu_count())));
+}
+
 int wtc_window_attention(const wtc_attention_args* p, const void* q, const void* k, const void* v, void* out,
-                         float* lse, void* stream) {
+                         float* lse, void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&]() -> int {
     if (!p) return bad("NULL arguments");
     if (int rc = check_attention(*p, false)) return rc;
@@ -309,7 +319,10 @@ int wtc_window_attention(const wtc_attention_args* p, const void* q, const void*
     a.v = static_cast<const uint8_t*>(v);
     a.out = static_cast<uint8_t*>(out);
     a.lse = lse;
-    return launched(launch_attention(a, (int)p->dtype, static_cast<hipStream_t>(stream)), "window_attention");
+    const AttnPlan plan = plan_attention(a, cu_count());
+    if (int rc = check_workspace(workspace, workspace_bytes, align256(attention_workspace(a, plan)))) return rc;
+    a.part_out = static_cast<float*>(workspace);
+    return launched(launch_attention(a, plan, (int)p->dtype, static_cast<hipStream_t>(stream)), "window_attention");
   });
 }
 

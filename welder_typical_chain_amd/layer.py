@@ -282,8 +282,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     b, lq, h, _ = q.shape
     lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if return_lse else None
     args = _pack_attention(*head, *_strides(out, "out"), 0, 0, 0, 0, 0, 0, 0, *tail)
-    _launch(device, _lib.lib().wtc_window_attention, args, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-            out.data_ptr(), _ptr(lse))
+    lib = _lib.lib()
+    ws, ws_ptr, ws_bytes = _scratch(lib.wtc_window_attention_workspace_size(args), device)
+    _launch(device, lib.wtc_window_attention, args, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+            _ptr(lse), ws_ptr, ws_bytes)
     return (out, lse) if return_lse else out
 
 
