@@ -106,14 +106,17 @@ struct AttnParams {
   const uint8_t *q, *k, *v, *dout, *o;
   uint8_t *out, *dq, *dk, *dv;
   const float* lse_in;
-  float *lse, *delta;
+  float* lse;
+  float2* stats;  // backward: a row's (lse in the log2 domain, sum of dout * out)
   const int32_t *q_lens, *k_lens;
   const uint8_t *k_new, *v_new;
   int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3], do_stride[3];  // elements
   int64_t kn_stride[2], vn_stride[2];
   int64_t window;  // INT32_MAX at most (no limit)
   float *part_out, *part_lse;  // of a row's splits: normalised results and log-sum-exp
+  float* part_far;
   int32_t splits, row_blocks;
+  int32_t key_blocks, far_blocks, far_chunks, far_rows;
   int32_t batch, heads, kv_heads, group, lq, lk, dim, sinks;
   float scale;
 };

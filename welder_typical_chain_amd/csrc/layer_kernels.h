@@ -35,7 +35,13 @@ AttnPlan plan_attention(const AttnParams& p, int cu_count);
 int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);
 // p.part_out: attention_workspace() bytes
 hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, hipStream_t stream);
-hipError_t launch_attention_backward(const AttnParams& p, int dt, hipStream_t stream);
+struct AttnBackwardPlan {
+  int key_blocks, far_blocks, far_chunks, far_rows;
+  int64_t part_at, workspace;  // bytes
+};
+AttnBackwardPlan plan_attention_backward(const AttnParams& p);
+// p.stats: plan.workspace bytes
+hipError_t launch_attention_backward(const AttnParams& p, const AttnBackwardPlan& plan, int dt, hipStream_t stream);
 hipError_t launch_attention_decode(const AttnParams& p, int dt, hipStream_t stream);
 
 }  // namespace wtc

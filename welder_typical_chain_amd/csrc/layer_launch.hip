@@ -178,7 +178,21 @@ AttnParams attention_params(const wtc_attention_args& p) {
   return q;
 }
 
-int64_t backward_workspace(const wtc_attention_args& p) { return align256(p.batch * p.heads * p.lq * 4); }
+// The gradient addresses a tile's query rows (64 positions or one group of query
+// heads) with 32-bit offsets.
+int check_group_span(const wtc_attention_args& p, const int64_t* s, const char* what) {
+  const int64_t heads = std::min<int64_t>(p.heads / p.kv_heads, 64), most = kSpan / 2;
+  if (p.heads > 1 && s[2] > most / heads) return report(WTC_ERR_UNSUPPORTED, std::string(what) + ": a key head's query heads span more than 2 GiB");
+  if (p.lq > 1 && (heads - 1) * s[2] + 64 / heads * s[1] + p.dim > most)
+    return report(WTC_ERR_UNSUPPORTED, std::string(what) + ": a tile of query rows spans more than 2 GiB");
+  return WTC_OK;
+}
+int check_attention_backward(const wtc_attention_args& p) {
+  if (int rc = check_attention(p, false)) return rc;
+  if (int rc = check_strides(p.do_stride, 3, p.lq, "dout")) return rc;
+  if (int rc = check_group_span(p, p.q_stride, "q")) return rc;
+  return check_group_span(p, p.do_stride, "dout");
+}
 
 }  // namespace
 
@@ -328,8 +342,8 @@ int wtc_window_attention(const wtc_attention_args* p, const void* q, const void*
 
 int64_t wtc_window_attention_backward_workspace_size(const wtc_attention_args* p) {
   if (!p) return bad("NULL arguments"), -1;
-  if (guarded([&] { return check_attention(*p, false); })) return -1;
-  return backward_workspace(*p);
+  if (guarded([&] { return check_attention_backward(*p); })) return -1;
+  return plan_attention_backward(attention_params(*p)).workspace;
 }
 
 int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout, const void* q, const void* k,
@@ -337,27 +351,27 @@ int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout,
                                   void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&]() -> int {
     if (!p) return bad("NULL arguments");
-    if (int rc = check_attention(*p, false)) return rc;
-    if (int rc = check_strides(p->do_stride, 3, p->lq, "dout")) return rc;
+    if (int rc = check_attention_backward(*p)) return rc;
     if (p->batch == 0) return WTC_OK;
     if ((p->lq && (!dout || !q || !out || !lse || !dq)) || (p->lk && (!k || !v || !dk || !dv)))
       return bad("NULL operand");
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(dout) || !aligned16(dq) ||
         !aligned16(dk) || !aligned16(dv))
       return bad("pointers must be 16-byte aligned");
-    if (int rc = check_workspace(workspace, workspace_bytes, backward_workspace(*p))) return rc;
     AttnParams a = attention_params(*p);
+    const AttnBackwardPlan plan = plan_attention_backward(a);
+    if (int rc = check_workspace(workspace, workspace_bytes, plan.workspace)) return rc;
     a.q = static_cast<const uint8_t*>(q);
     a.k = static_cast<const uint8_t*>(k);
     a.v = static_cast<const uint8_t*>(v);
     a.o = static_cast<const uint8_t*>(out);
     a.dout = static_cast<const uint8_t*>(dout);
     a.lse_in = lse;
-    a.delta = static_cast<float*>(workspace);
+    a.stats = static_cast<float2*>(workspace);
     a.dq = static_cast<uint8_t*>(dq);
     a.dk = static_cast<uint8_t*>(dk);
     a.dv = static_cast<uint8_t*>(dv);
-    return launched(launch_attention_backward(a, (int)p->dtype, static_cast<hipStream_t>(stream)),
+    return launched(launch_attention_backward(a, plan, (int)p->dtype, static_cast<hipStream_t>(stream)),
                     "window_attention_backward");
   });
 }

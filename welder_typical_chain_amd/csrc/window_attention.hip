@@ -305,29 +305,32 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 }
 
 // ---- gradients ------------------------------------------------------------------
-// delta = sum_d dout * out of a row, and the row's dq.  One wave a row.
-template <int DT>
-__global__ void __launch_bounds__(64) attention_dq_rows_kernel(const AttnParams p) {
+// With P = exp(S - lse), D = sum_d dout out and dS = P (dP - D), dP = dout . V^T:
+//   dq = scale dS . K      per row block, keys streamed   (attention_dq_kernel)
+//   dv = P^T . dout, dk = scale dS^T . Q
+//                          per key block, queries streamed (attention_dkv_kernel)
+// Two kernels, each recomputing S and dP (7 products instead of 5): no dq sums
+// through atomics, whose order would change the result, and no f32 dq in memory.
+// The first writes each row's (lse in the log2 domain, D) as p.stats, rows packed
+// as the tiles are: [batch][kv_heads][lq][G].
+__device__ inline int64_t stats_row(const AttnParams& p, int b, int hk, int i) {
+  return (((int64_t)b * p.kv_heads + hk) * p.lq + i) * p.group;
+}
+
+// dq of one row by a whole wave, for the rows that come out as NaN (see attention_row).
+template <int DT> __device__ inline void dq_row(const AttnParams& p, int b, int h, int i) {
   using T = typename Elem<DT>::type;
-  const int lane = threadIdx.x;
-  const int h = blockIdx.x % p.heads;
-  const int i = blockIdx.x / p.heads % p.lq, b = blockIdx.x / p.heads / p.lq;
-  const int nq = seq_queries(p, b), pos = i + seq_keys(p, b) - nq;
+  const int lane = threadIdx.x & 63;
+  const int pos = i + seq_keys(p, b) - seq_queries(p, b);
   const T* q = (const T*)p.q + b * p.q_stride[0] + i * p.q_stride[1] + h * p.q_stride[2];
   const T* k = (const T*)p.k + b * p.k_stride[0] + h / p.group * p.k_stride[2];
   const T* v = (const T*)p.v + b * p.v_stride[0] + h / p.group * p.v_stride[2];
   const T* g = (const T*)p.dout + b * p.do_stride[0] + i * p.do_stride[1] + h * p.do_stride[2];
   const T* o = (const T*)p.o + b * p.o_stride[0] + i * p.o_stride[1] + h * p.o_stride[2];
-  const int64_t row_id = ((int64_t)b * p.heads + h) * p.lq + i;
-  Seen seen(p.window, p.sinks, pos);
-  if (i >= nq) seen.count = 0;
-  float acc[2] = {0.0f, 0.0f}, delta = 0.0f;
-  if (seen.count) {
-    for (int d = lane; d < p.dim; d += 64) delta = __builtin_fmaf((float)g[d], (float)o[d], delta);
-    delta = wave_sum(delta);
-  }
-  if (lane == 0) p.delta[row_id] = delta;
-  const float lse = p.lse_in[row_id];
+  const float delta = dot_rows<DT>(g, o, p.dim);
+  const float lse = p.lse_in[((int64_t)b * p.heads + h) * p.lq + i];
+  const Seen seen(p.window, p.sinks, pos);
+  float acc[2] = {0.0f, 0.0f};
   for (int t0 = 0; t0 < seen.count; t0 += 64) {
     float ds = 0.0f;
     if (t0 + lane < seen.count) {
@@ -347,31 +350,29 @@ __global__ void __launch_bounds__(64) attention_dq_rows_kernel(const AttnParams 
     if (lane + 64 * c < p.dim) dq[lane + 64 * c] = (T)acc[c];
 }
 
-// dk and dv of one key row: over the query heads that share it, 64 queries at a time.
-template <int DT>
-__global__ void __launch_bounds__(64) attention_dkv_rows_kernel(const AttnParams p) {
+// dk and dv of one key by a whole wave, 64 queries at a time, likewise.
+template <int DT> __device__ inline void dkv_row(const AttnParams& p, int b, int hk, int j) {
   using T = typename Elem<DT>::type;
-  const int lane = threadIdx.x;
-  const int hk = blockIdx.x % p.kv_heads;
-  const int j = blockIdx.x / p.kv_heads % p.lk, b = blockIdx.x / p.kv_heads / p.lk;
-  const int nq = seq_queries(p, b), nk = seq_keys(p, b), shift = nk - nq;
+  const int lane = threadIdx.x & 63;
+  const int nq = seq_queries(p, b), shift = seq_keys(p, b) - nq;
   const T* k = (const T*)p.k + b * p.k_stride[0] + j * p.k_stride[1] + hk * p.k_stride[2];
   const T* v = (const T*)p.v + b * p.v_stride[0] + j * p.v_stride[1] + hk * p.v_stride[2];
   // queries of positions j .. j + window - 1 (a first token: all from j on)
   const int i0 = max(0, j - shift);
-  int i1 = j < nk ? nq : 0;
-  if (j >= p.sinks) i1 = (int)min((int64_t)i1, j + p.window - shift);
+  const int i1 = j < p.sinks ? nq : (int)min((int64_t)nq, j + p.window - shift);
+  const float c2 = p.scale * kLog2e;
   float ak[2] = {0.0f, 0.0f}, av[2] = {0.0f, 0.0f};
-  for (int h = hk * p.group; h < (hk + 1) * p.group; ++h) {
+  for (int x = 0; x < p.group; ++x) {
+    const int h = hk * p.group + x;
     const T* q = (const T*)p.q + b * p.q_stride[0] + h * p.q_stride[2];
     const T* g = (const T*)p.dout + b * p.do_stride[0] + h * p.do_stride[2];
-    const int64_t row0 = ((int64_t)b * p.heads + h) * p.lq;
     for (int t0 = i0; t0 < i1; t0 += 64) {
       float w = 0.0f, ds = 0.0f;
       const int i = t0 + lane;
       if (i < i1) {
-        w = __expf(p.scale * dot_rows<DT>(q + i * p.q_stride[1], k, p.dim) - p.lse_in[row0 + i]);
-        ds = p.scale * w * (dot_rows<DT>(g + i * p.do_stride[1], v, p.dim) - p.delta[row0 + i]);
+        const float2 st = p.stats[stats_row(p, b, hk, i) + x];
+        w = __builtin_amdgcn_exp2f(c2 * dot_rows<DT>(q + i * p.q_stride[1], k, p.dim) - st.x);
+        ds = p.scale * w * (dot_rows<DT>(g + i * p.do_stride[1], v, p.dim) - st.y);
       }
       for (int t = 0; t < min(64, i1 - t0); ++t) {
         const float wt = __shfl(w, t), dt = __shfl(ds, t);
@@ -389,6 +390,400 @@ __global__ void __launch_bounds__(64) attention_dkv_rows_kernel(const AttnParams
       ((T*)p.dk)[at + lane + 64 * c] = (T)ak[c];
       ((T*)p.dv)[at + lane + 64 * c] = (T)av[c];
     }
+}
+
+// Row blocks and key tiles as in attention_tile_kernel; keys in subtiles of 32:
+//   S^T = K . Q^T, dP^T = V . dout^T, dq^T += K^T . dS^T
+template <int DT, int ND, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnParams p) {
+  using L = FwdLds<ND, NW>;
+  constexpr int RB = L::RB, NS = 2 * ND;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
+  const int blk = p.row_blocks - 1 - (int)(id % p.row_blocks);
+  const int hk = (int)(id / p.row_blocks % p.kv_heads), b = (int)(id / p.row_blocks / p.kv_heads);
+  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
+  const int r0 = blk * NW * 32;
+  const int r = r0 + wave * 32 + (lane & 31), i = r / p.group, x = r - i * p.group, h = hk * p.group + x;
+  const bool valid = i < nq;
+  const int pos = valid ? i + shift : -1;
+  const int i_last = min((r0 + NW * 32 - 1) / p.group, nq - 1);
+  const int p_lo = r0 / p.group + shift, p_hi = i_last + shift;
+  const int lo = (int)max((int64_t)0, (int64_t)p_lo - p.window + 1);
+  const int end = r0 / p.group < nq ? max(p_hi + 1, 0) : 0;
+  const int s_end = end ? min(p.sinks, lo) : 0;
+  const int t_sink = (s_end + kKeys - 1) / kKeys, t_all = end > lo ? t_sink + (end - lo + kKeys - 1) / kKeys : 0;
+  const int w_lo = (r0 + wave * 32) / p.group + shift;
+  const int w_hi = min((r0 + wave * 32 + 31) / p.group, nq - 1) + shift;
+  const bool w_any = (r0 + wave * 32) / p.group < nq && w_hi >= 0;
+
+  u32x4 qf[NS], gf[NS];
+  load_row<NS>(p.q + 2 * (b * p.q_stride[0] + (int64_t)i * p.q_stride[1] + h * p.q_stride[2]), valid, p.dim, half, qf);
+  load_row<NS>(p.dout + 2 * (b * p.do_stride[0] + (int64_t)i * p.do_stride[1] + h * p.do_stride[2]), valid, p.dim, half, gf);
+  float delta = 0.0f, lse2 = INFINITY;  // no keys: every weight 0
+  {
+    const uint8_t* orow = p.o + 2 * (b * p.o_stride[0] + (int64_t)i * p.o_stride[1] + h * p.o_stride[2]);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const int c = 2 * s + half;
+      if (valid && c * 8 < p.dim) {
+        const auto ov = *reinterpret_cast<const typename Elem<DT>::vec8*>(orow + c * 16);
+        const auto gv = __builtin_bit_cast(typename Elem<DT>::vec8, gf[s]);
+#pragma unroll
+        for (int v = 0; v < 8; ++v) delta = __builtin_fmaf((float)gv[v], (float)ov[v], delta);
+      }
+    }
+    delta = xor32_sum(delta);
+    if (valid) {
+      const float lse = p.lse_in[((int64_t)b * p.heads + h) * p.lq + i];
+      if (lse == -INFINITY) delta = 0.0f;
+      else lse2 = lse * kLog2e;
+    }
+    if (half == 0 && i < p.lq) p.stats[stats_row(p, b, hk, i) + x] = float2{lse2, delta};
+  }
+  const float c2 = p.scale * kLog2e;
+
+  f32x16 dq[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) dq[d][v] = 0.0f;
+
+  TileLoader<RB, kKeys, NW> lk, lv;
+  lk.init(p.k + 2 * (b * p.k_stride[0] + hk * p.k_stride[2]), 2 * p.k_stride[1], p.dim, wave, lane);
+  lv.init(p.v + 2 * (b * p.v_stride[0] + hk * p.v_stride[2]), 2 * p.v_stride[1], p.dim, wave, lane);
+  constexpr int LOADS = 2 * TileLoader<RB, kKeys, NW>::NB;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
+  auto tile_base = [&](int t) { return t < t_sink ? t * kKeys : lo + (t - t_sink) * kKeys; };
+  auto tile_end = [&](int t) { return t < t_sink ? s_end : end; };
+  auto issue = [&](int t) {
+    const int j0 = tile_base(t), n = t < t_all ? min(kKeys, tile_end(t) - j0) : 0;
+    const uint32_t st = lds0 + (uint32_t)t % L::STAGES * L::STAGE;
+    lk.issue(st, j0, n);
+    lv.issue(st + L::TILE, j0, n);
+  };
+#pragma unroll
+  for (int t = 0; t < L::STAGES - 1; ++t) issue(t);
+
+  for (int t = 0; t < t_all; ++t) {
+    wait_loads_barrier<LOADS*(L::STAGES - 2)>();
+    issue(t + L::STAGES - 1);
+    const int j0 = tile_base(t), j1 = tile_end(t);
+    const uint8_t* kt = smem + t % L::STAGES * L::STAGE;
+    const uint8_t* vt = kt + L::TILE;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int k0 = j0 + 32 * u;
+      const bool below = t >= t_sink && (int64_t)k0 + 31 + p.window <= w_lo && k0 >= p.sinks;
+      if (!w_any || k0 > w_hi || k0 >= j1 || below) continue;
+      f32x16 s, g;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
+#pragma unroll
+      for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(kt, 32 * u, st, lane), qf[st], s);
+#pragma unroll
+      for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(vt, 32 * u, st, lane), gf[st], g);
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c2, -lse2)) * (g[v] - delta);
+      if (k0 + 32 > j1 || k0 + 31 > w_lo || (t >= t_sink && (int64_t)k0 + p.window <= w_hi)) {
+        const int at = k0 + 4 * half;
+        const int top_c = min(pos, j1 - 1) - at;
+        const int low_c = (int)max((int64_t)pos - p.window - at, (int64_t)-1);
+        const int sink_c = p.sinks - at;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int c = 8 * (v >> 2) + (v & 3);
+          s[v] = c <= top_c && (c > low_c || c < sink_c) ? s[v] : 0.0f;
+        }
+      }
+      u32x4 df[2];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t w0, w1;
+        pack4<DT>(f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]}, &w0, &w1);
+        df[q >> 1][2 * (q & 1)] = w0;
+        df[q >> 1][2 * (q & 1) + 1] = w1;
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dq[d] = mfma32<DT>(col_frag<RB>(kt, 32 * u + 16 * st, 32 * d, lane), df[st], dq[d]);
+    }
+  }
+  wait_loads_barrier<0>();
+
+  bool nan = false;
+  uint8_t* stg = smem + wave * 32 * L::PITCH;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 y;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        y[v] = valid ? dq[d][4 * g + v] * p.scale : 0.0f;
+        nan |= y[v] != y[v];
+      }
+      uint32_t w0, w1;
+      pack4<DT>(y, &w0, &w1);
+      *reinterpret_cast<u32x2*>(stg + (lane & 31) * L::PITCH + (32 * d + 8 * g + 4 * half) * 2) = u32x2{w0, w1};
+    }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  constexpr int CPR = ND * 4;
+#pragma unroll 4
+  for (int y = lane; y < 32 * CPR; y += 64) {
+    const int row = y / CPR, c = y % CPR;
+    const int rr = r0 + wave * 32 + row, ii = rr / p.group, hh = hk * p.group + rr - ii * p.group;
+    if (ii < p.lq && c * 8 < p.dim)
+      *reinterpret_cast<u32x4*>(p.dq + 2 * ((((int64_t)b * p.lq + ii) * p.heads + hh) * p.dim) + c * 16) =
+          *reinterpret_cast<const u32x4*>(stg + row * L::PITCH + c * 16);
+  }
+  uint32_t redo = (uint32_t)(__ballot(nan && valid) | __ballot(nan && valid) >> 32);
+  while (redo) {
+    const int rr = r0 + wave * 32 + __builtin_ctz(redo);
+    dq_row<DT>(p, b, hk * p.group + rr % p.group, rr / p.group);
+    redo &= redo - 1;
+  }
+}
+
+// A workgroup takes kDkvKeys keys of one (sequence, key head), 32 a wave, their K
+// and V fragments in registers, and streams the queries that see them in tiles
+// of 64 packed rows: whole positions of up to 64 query heads of the group, so
+// that a lane's offset inside a tile is the same for every tile.
+//   S = Q . K^T, dP = dout . V^T (a lane holds 16 queries of one key)
+//   dV^T += dout^T . P, dK^T += Q^T . dS
+// The first tokens are seen by every later query.  A workgroup of their key
+// block streams, like the others, the queries whose window reaches the block; the
+// far queries go in p.far_chunks chunks to workgroups of their own (p.far_rows
+// positions each), and all of the block's sums as f32 to p.part_far, which
+// attention_far_kernel adds in order for the first tokens' keys.
+constexpr int kDkvWaves = 4;
+constexpr int kDkvKeys = 32 * kDkvWaves;
+constexpr int kQueries = 64;
+
+template <int ND> struct DkvLds {
+  static constexpr int RB = row_bytes(ND), STAGES = 2;
+  static constexpr int TILE = kQueries * RB, STATS = 2 * TILE, STAGE = 2 * TILE + 1024;
+  static constexpr int PITCH = ND * 64 + 16;
+  static constexpr int RING = STAGES * STAGE, OUT = kDkvWaves * 32 * PITCH;
+  static constexpr int TOTAL = RING > OUT ? RING : OUT;
+};
+
+// part_far: [batch][kv_heads][far_blocks][1 + far_chunks][kDkvKeys][dk, dv][dim]
+__device__ inline float* far_part(const AttnParams& p, int b, int hk, int kb, int slot) {
+  return p.part_far + ((((int64_t)b * p.kv_heads + hk) * p.far_blocks + kb) * (1 + p.far_chunks) + slot) * (kDkvKeys * 2) * p.dim;
+}
+
+template <int DT, int ND>
+__global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const AttnParams p) {
+  using L = DkvLds<ND>;
+  constexpr int RB = L::RB, NS = 2 * ND, NB = kQueries * RB / 1024 / kDkvWaves;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // workgroups of a (sequence, key head): the key blocks, then the far chunks
+  const int per = p.key_blocks + p.far_blocks * p.far_chunks;
+  const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
+  const int w = (int)(id % per), hk = (int)(id / per % p.kv_heads), b = (int)(id / per / p.kv_heads);
+  const bool far = w >= p.key_blocks;
+  const int kb = far ? (w - p.key_blocks) / p.far_chunks : w, chunk = far ? (w - p.key_blocks) % p.far_chunks : 0;
+  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
+  const int j_first = kb * kDkvKeys, j = j_first + wave * 32 + (lane & 31);
+  const bool valid = j < nk;
+  // queries: the near ones are those whose window may reach a key of the block
+  int i0 = min(max(0, j_first - shift), nq);
+  int i1 = (int)max((int64_t)i0, min((int64_t)nq, (int64_t)min(j_first + kDkvKeys, nk) - 1 + p.window - shift));
+  if (j_first >= nk) i1 = i0;
+  if (far) {
+    i0 = min(nq, (int)min((int64_t)nq, i1 + (int64_t)chunk * p.far_rows));
+    i1 = chunk + 1 == p.far_chunks ? nq : min(nq, (int)min((int64_t)nq, i0 + (int64_t)p.far_rows));
+    if (j_first >= nk) i1 = i0;
+  }
+  const int hg = min(p.group, kQueries), chunks = (p.group + hg - 1) / hg;  // query heads a tile, tiles a position
+  const int tp = kQueries / hg;                                             // positions a tile
+  const int steps = (i1 - i0 + tp - 1) / tp, t_all = steps * chunks;
+
+  u32x4 kf[NS], vf[NS];
+  load_row<NS>(p.k + 2 * (b * p.k_stride[0] + (int64_t)j * p.k_stride[1] + hk * p.k_stride[2]), valid, p.dim, half, kf);
+  load_row<NS>(p.v + 2 * (b * p.v_stride[0] + (int64_t)j * p.v_stride[1] + hk * p.v_stride[2]), valid, p.dim, half, vf);
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) dk[d][v] = dv[d][v] = 0.0f;
+
+  // loads of a tile: block q of this wave holds tile row `row[q]`, position row / hg, head row % hg
+  const uint8_t* q_base = p.q + 2 * (b * p.q_stride[0] + (int64_t)hk * p.group * p.q_stride[2]);
+  const uint8_t* g_base = p.dout + 2 * (b * p.do_stride[0] + (int64_t)hk * p.group * p.do_stride[2]);
+  uint32_t q_off[NB], g_off[NB];
+  int at_pos[NB], at_head[NB];
+#pragma unroll
+  for (int q = 0; q < NB; ++q) {
+    const int row = (int)block_row<RB>(wave * NB + q, lane);
+    const uint32_t c = block_chunk<RB>(wave * NB + q, lane) * 16u;
+    at_pos[q] = c < (uint32_t)p.dim * 2u ? row / hg : 1 << 30;
+    at_head[q] = row % hg;
+    q_off[q] = (uint32_t)(2 * (at_pos[q] * p.q_stride[1] + at_head[q] * p.q_stride[2])) + c;
+    g_off[q] = (uint32_t)(2 * (at_pos[q] * p.do_stride[1] + at_head[q] * p.do_stride[2])) + c;
+  }
+  const float2* st_base = p.stats + stats_row(p, b, hk, 0);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
+  constexpr int LOADS = 2 * NB;
+  auto issue = [&](int t) {
+    const int step = t / chunks, hc = t - step * chunks, i = i0 + step * tp;
+    const int npos = t < t_all ? min(tp, i1 - i) : 0, nhead = p.group - hc * hg;
+    const uint32_t st = lds0 + (uint32_t)t % L::STAGES * L::STAGE + (uint32_t)(wave * NB * 1024);
+    // what is in range is said by the offsets alone
+    const i32x4 rq = raw_rsrc(q_base + 2 * (i * p.q_stride[1] + hc * hg * p.q_stride[2]), 0x7FFFFFFFu);
+    const i32x4 rg = raw_rsrc(g_base + 2 * (i * p.do_stride[1] + hc * hg * p.do_stride[2]), 0x7FFFFFFFu);
+#pragma unroll
+    for (int q = 0; q < NB; ++q) {
+      const bool in = at_pos[q] < npos && at_head[q] < nhead;
+      dma16(rq, in ? q_off[q] : kOutOfRange, st + q * 1024);
+      dma16(rg, in ? g_off[q] : kOutOfRange, st + L::TILE + q * 1024);
+    }
+    if (wave == 0) {  // the rows' (lse, D): contiguous
+      const int rows = min(npos * hg, hg == p.group ? kQueries : nhead);
+      const i32x4 rs = raw_rsrc(st_base + (int64_t)i * p.group + hc * hg, rows > 0 ? (uint32_t)rows * 8u : 0u);
+      dma16(rs, lane * 16, lds0 + (uint32_t)t % L::STAGES * L::STAGE + L::STATS);
+    }
+  };
+  const float c2 = p.scale * kLog2e;
+  issue(0);
+  for (int t = 0; t < t_all; ++t) {
+    wait_loads_barrier<0>();  // tile t landed; every wave is done with tile t - 1
+    issue(t + 1);
+    const int step = t / chunks, hc = t - step * chunks, i = i0 + step * tp;
+    const uint8_t* qt = smem + t % L::STAGES * L::STAGE;
+    const uint8_t* gt = qt + L::TILE;
+    const uint8_t* stt = qt + L::STATS;
+    // tile row x is a query that sees this lane's key if t_lo <= x < t_hi
+    const int rows = min(min(tp, i1 - i) * hg, hg == p.group ? kQueries : p.group - hc * hg);
+    const int64_t back = (int64_t)j - shift - i;
+    const int t_lo = (int)min((int64_t)1 << 20, max((int64_t)0, back)) * hg;
+    const int64_t reach = j < p.sinks ? 1 << 20 : max((int64_t)0, min((int64_t)1 << 20, back + p.window)) * hg;
+    const int t_hi = valid ? (int)min((int64_t)rows, reach) : 0;
+    const bool all = __all(t_lo == 0 && t_hi == kQueries);
+    if (!all && !__any(t_lo < t_hi)) continue;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 s, g;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
+#pragma unroll
+      for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(qt, 32 * u, st, lane), kf[st], s);
+#pragma unroll
+      for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(gt, 32 * u, st, lane), vf[st], g);
+      u32x4 pf[2], df[2];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int row = 32 * u + 8 * q + 4 * half;
+        const f32x4 st0 = *reinterpret_cast<const f32x4*>(stt + row * 8), st1 = *reinterpret_cast<const f32x4*>(stt + row * 8 + 16);
+        const float lse[4] = {st0[0], st0[2], st1[0], st1[2]}, del[4] = {st0[1], st0[3], st1[1], st1[3]};
+        f32x4 pw, ds;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          pw[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + v], c2, -lse[v]));
+          ds[v] = pw[v] * (g[4 * q + v] - del[v]);
+          if (!all) {
+            const bool in = row + v >= t_lo && row + v < t_hi;
+            pw[v] = in ? pw[v] : 0.0f;
+            ds[v] = in ? ds[v] : 0.0f;
+          }
+        }
+        uint32_t w0, w1;
+        pack4<DT>(pw, &w0, &w1);
+        pf[q >> 1][2 * (q & 1)] = w0;
+        pf[q >> 1][2 * (q & 1) + 1] = w1;
+        pack4<DT>(ds, &w0, &w1);
+        df[q >> 1][2 * (q & 1)] = w0;
+        df[q >> 1][2 * (q & 1) + 1] = w1;
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          dv[d] = mfma32<DT>(col_frag<RB>(gt, 32 * u + 16 * st, 32 * d, lane), pf[st], dv[d]);
+          dk[d] = mfma32<DT>(col_frag<RB>(qt, 32 * u + 16 * st, 32 * d, lane), df[st], dk[d]);
+        }
+    }
+  }
+  wait_loads_barrier<0>();
+
+  const bool parts = kb < p.far_blocks && p.far_chunks > 0;
+  if (parts) {
+    float* dst = far_part(p, b, hk, kb, far ? 1 + chunk : 0) + (int64_t)(wave * 32 + (lane & 31)) * 2 * p.dim;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * d + 8 * g + 4 * half;
+        if (c < p.dim) {
+          *reinterpret_cast<f32x4*>(dst + c) = f32x4{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
+          *reinterpret_cast<f32x4*>(dst + p.dim + c) = f32x4{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
+        }
+      }
+    if (far) return;
+  }
+  bool nan = false;
+  uint8_t* stg = smem + wave * 32 * L::PITCH;
+  constexpr int CPR = ND * 4;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x4 y;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          y[v] = !valid ? 0.0f : which ? dv[d][4 * g + v] : dk[d][4 * g + v] * p.scale;
+          nan |= y[v] != y[v];
+        }
+        uint32_t w0, w1;
+        pack4<DT>(y, &w0, &w1);
+        *reinterpret_cast<u32x2*>(stg + (lane & 31) * L::PITCH + (32 * d + 8 * g + 4 * half) * 2) = u32x2{w0, w1};
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 4
+    for (int y = lane; y < 32 * CPR; y += 64) {
+      const int row = y / CPR, c = y % CPR, jj = j_first + wave * 32 + row;
+      if (jj < p.lk && c * 8 < p.dim && !(parts && jj < p.sinks))
+        *reinterpret_cast<u32x4*>((which ? p.dv : p.dk) + 2 * ((((int64_t)b * p.lk + jj) * p.kv_heads + hk) * p.dim) + c * 16) =
+            *reinterpret_cast<const u32x4*>(stg + row * L::PITCH + c * 16);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  nan = nan && !(parts && j < p.sinks);
+  uint32_t redo = (uint32_t)(__ballot(nan) | __ballot(nan) >> 32);
+  while (redo) {
+    dkv_row<DT>(p, b, hk, j_first + wave * 32 + __builtin_ctz(redo));
+    redo &= redo - 1;
+  }
+}
+
+// dk and dv of the first tokens: the sums of their blocks' chunks in order.  One wave a key.
+template <int DT>
+__global__ void __launch_bounds__(64) attention_far_kernel(const AttnParams p) {
+  using T = typename Elem<DT>::type;
+  const int lane = threadIdx.x;
+  const int j = (int)(blockIdx.x % p.sinks), hk = (int)(blockIdx.x / p.sinks % p.kv_heads), b = (int)(blockIdx.x / p.sinks / p.kv_heads);
+  bool nan = false;
+  for (int c = lane; c < 2 * p.dim; c += 64) {
+    const bool is_dv = c >= p.dim;
+    float sum = 0.0f;
+    for (int s = 0; s <= p.far_chunks; ++s)
+      sum += far_part(p, b, hk, j / kDkvKeys, s)[(int64_t)(j % kDkvKeys) * 2 * p.dim + c];
+    if (!is_dv) sum *= p.scale;
+    if (j >= seq_keys(p, b)) sum = 0.0f;
+    nan |= sum != sum;
+    T* dst = (T*)(is_dv ? p.dv : p.dk) + (((int64_t)b * p.lk + j) * p.kv_heads + hk) * p.dim;
+    dst[is_dv ? c - p.dim : c] = (T)sum;
+  }
+  if (__any(nan)) dkv_row<DT>(p, b, hk, j);
 }
 
 hipError_t launch(const void* fn, int64_t grid, int threads, const AttnParams& p, hipStream_t stream) {
@@ -443,13 +838,64 @@ hipError_t launch_attention(const AttnParams& params, const AttnPlan& plan, int 
   return launch(WTC_BY_TYPE(attention_join_kernel, dt), ((int64_t)p.batch * p.lq * p.heads + 3) / 4, 256, p, stream);
 }
 
-hipError_t launch_attention_backward(const AttnParams& p, int dt, hipStream_t stream) {
+namespace {
+template <int DT, int NW> const void* dq_kernel(int nd) {
+  switch (nd) {
+    case 1: return (const void*)&attention_dq_kernel<DT, 1, NW>;
+    case 2: return (const void*)&attention_dq_kernel<DT, 2, NW>;
+    case 3: return (const void*)&attention_dq_kernel<DT, 3, NW>;
+  }
+  return (const void*)&attention_dq_kernel<DT, 4, NW>;
+}
+template <int DT> const void* dkv_kernel(int nd) {
+  switch (nd) {
+    case 1: return (const void*)&attention_dkv_kernel<DT, 1>;
+    case 2: return (const void*)&attention_dkv_kernel<DT, 2>;
+    case 3: return (const void*)&attention_dkv_kernel<DT, 3>;
+  }
+  return (const void*)&attention_dkv_kernel<DT, 4>;
+}
+}  // namespace
+
+// Far chunks: about as many positions as a block's near queries, so that no
+// workgroup runs much longer than the others.
+AttnBackwardPlan plan_attention_backward(const AttnParams& p) {
+  AttnBackwardPlan plan{};
+  plan.key_blocks = (p.lk + kDkvKeys - 1) / kDkvKeys;
+  // queries past the near ones of the first block: at most the keys past them
+  const int64_t near = p.window + kDkvKeys, far = std::min<int64_t>(p.lq, (int64_t)p.lk - near + 1);
+  if (p.sinks > 0 && far > 0) {
+    plan.far_blocks = (p.sinks + kDkvKeys - 1) / kDkvKeys;
+    plan.far_chunks = (int)std::min<int64_t>((far + near - 1) / near, 64);
+    plan.far_rows = (int)((far + plan.far_chunks - 1) / plan.far_chunks);
+  }
+  const int64_t rows = (int64_t)p.batch * p.lq * p.heads;
+  plan.part_at = (rows * 8 + 255) / 256 * 256;
+  plan.workspace = plan.part_at + ((int64_t)p.batch * p.kv_heads * plan.far_blocks * (1 + plan.far_chunks) * kDkvKeys * 2 * p.dim * 4 + 255) / 256 * 256;
+  return plan;
+}
+
+hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwardPlan& plan, int dt, hipStream_t stream) {
+  AttnParams p = params;
+  p.part_far = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.stats) + plan.part_at);
+  p.key_blocks = plan.key_blocks;
+  p.far_blocks = plan.far_blocks;
+  p.far_chunks = plan.far_chunks;
+  p.far_rows = plan.far_rows;
+  const int nd = (p.dim + 31) / 32;
+  const int64_t seqs = (int64_t)p.batch * p.kv_heads;
   if (p.lq) {
-    const hipError_t e = launch(WTC_BY_TYPE(attention_dq_rows_kernel, dt), (int64_t)p.batch * p.lq * p.heads, 64, p, stream);
+    constexpr int waves = 4;
+    p.row_blocks = (int)(((int64_t)p.lq * p.group + waves * 32 - 1) / (waves * 32));
+    const hipError_t e = launch(dt == DT_F16 ? dq_kernel<DT_F16, waves>(nd) : dq_kernel<DT_BF16, waves>(nd), seqs * p.row_blocks,
+                                waves * 64, p, stream);
     if (e != hipSuccess) return e;
   }
   if (!p.lk) return hipSuccess;
-  return launch(WTC_BY_TYPE(attention_dkv_rows_kernel, dt), (int64_t)p.batch * p.lk * p.kv_heads, 64, p, stream);
+  const hipError_t e = launch(dt == DT_F16 ? dkv_kernel<DT_F16>(nd) : dkv_kernel<DT_BF16>(nd),
+                              seqs * (p.key_blocks + p.far_blocks * p.far_chunks), kDkvWaves * 64, p, stream);
+  if (e != hipSuccess || !p.far_chunks) return e;
+  return launch(WTC_BY_TYPE(attention_far_kernel, dt), seqs * p.sinks, 64, p, stream);
 }
 
 }  // namespace wtc
