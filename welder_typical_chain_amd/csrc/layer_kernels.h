@@ -42,6 +42,9 @@ struct AttnBackwardPlan {
 AttnBackwardPlan plan_attention_backward(const AttnParams& p);
 // p.stats: plan.workspace bytes
 hipError_t launch_attention_backward(const AttnParams& p, const AttnBackwardPlan& plan, int dt, hipStream_t stream);
-hipError_t launch_attention_decode(const AttnParams& p, int dt, hipStream_t stream);
+int plan_decode(const AttnParams& p, int cu_count);  // splits
+int64_t decode_workspace(const AttnParams& p, int splits);
+// p.part_out: decode_workspace() bytes; p.window: at most p.lk - p.sinks
+hipError_t launch_attention_decode(const AttnParams& p, int splits, int dt, hipStream_t stream);
 
 }  // namespace wtc

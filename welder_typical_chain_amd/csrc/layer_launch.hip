@@ -178,6 +178,13 @@ AttnParams attention_params(const wtc_attention_args& p) {
   return q;
 }
 
+// The cache keeps lk - sinks tokens behind the first ones: the window is at most that.
+AttnParams decode_params(const wtc_attention_args& p) {
+  AttnParams q = attention_params(p);
+  q.window = std::min<int64_t>(q.window, p.lk - p.sinks);
+  return q;
+}
+
 // The gradient addresses a tile's query rows (64 positions or one group of query
 // heads) with 32-bit offsets.
 int check_group_span(const wtc_attention_args& p, const int64_t* s, const char* what) {
@@ -379,7 +386,8 @@ int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout,
 int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p) {
   if (!p) return bad("NULL arguments"), -1;
   if (guarded([&] { return check_attention(*p, true); })) return -1;
-  return 0;
+  const AttnParams a = decode_params(*p);
+  return align256(decode_workspace(a, plan_decode(a, cu_count())));
 }
 
 int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void* k, void* v, const void* k_new,
@@ -398,15 +406,17 @@ int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void
     if (!q || !k || !v || !out) return bad("NULL operand");
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(k_new) || !aligned16(v_new))
       return bad("pointers must be 16-byte aligned");
-    AttnParams a = attention_params(*p);
-    a.window = std::min<int64_t>(a.window, p->lk - p->sinks);
+    AttnParams a = decode_params(*p);
+    const int splits = plan_decode(a, cu_count());
+    if (int rc = check_workspace(workspace, workspace_bytes, align256(decode_workspace(a, splits)))) return rc;
+    a.part_out = static_cast<float*>(workspace);
     a.q = static_cast<const uint8_t*>(q);
     a.k = static_cast<const uint8_t*>(k);
     a.v = static_cast<const uint8_t*>(v);
     a.k_new = static_cast<const uint8_t*>(k_new);
     a.v_new = static_cast<const uint8_t*>(v_new);
     a.out = static_cast<uint8_t*>(out);
-    return launched(launch_attention_decode(a, (int)p->dtype, static_cast<hipStream_t>(stream)),
+    return launched(launch_attention_decode(a, splits, (int)p->dtype, static_cast<hipStream_t>(stream)),
                     "window_attention_decode");
   });
 }

@@ -1,78 +1,298 @@
-// window_decode.hip -- kernels of wtc_window_attention_decode.
-#include "layer_common.h"
+// window_decode.hip -- kernels of wtc_window_attention_decode: one query row a
+// sequence and head against a cache that may have wrapped.
+//
+// What bounds it is reading the visible rows of K and V once.  The rows stand in
+// at most three runs of the cache (the first tokens, and the window's tokens,
+// which may wrap); a run is cut into tiles of 32 rows, so that a tile's rows
+// are consecutive and no tile needs a mask but for its length.  A workgroup
+// takes the tiles of one (sequence, key head, split); its 4 waves take them in
+// turn, each with a ring of its own of direct-to-LDS loads and no barrier until
+// the end, so that a wave's loads are in flight while it computes.  All query
+// heads of the group (up to 32) are columns of the same products:
+//   S^T = K . Q^T, O^T += V^T . P^T, online softmax as in window_attention.hip.
+// The waves' results are joined through LDS; splits by a second kernel.
+#include <algorithm>
+
+#include "attention_common.h"
 #include "layer_kernels.h"
 
 namespace wtc {
 namespace {
 
-// One wave a query head: 64 keys at a time.  The wave of a key head's first
-// query head writes the new row; the others read it from k_new / v_new, and
-// no wave reads the row it replaces.
-template <int DT>
-__global__ void __launch_bounds__(64) decode_rows_kernel(const AttnParams p) {
+using namespace attn;
+
+constexpr int kRows = 32;   // cache rows a tile
+constexpr int kWaves = 4;
+constexpr int kHeads = 32;  // query heads a workgroup
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int ND> struct DecodeLds {
+  static constexpr int RB = row_bytes(ND);
+  static constexpr int TILE = kRows * RB, STAGE = 2 * TILE;
+  static constexpr int STAGES = RB == 256 ? 2 : 4;  // 128 KiB over the waves
+  static constexpr int RING = kWaves * STAGES * STAGE;
+  static constexpr int PITCH = ND * 32 + 4;          // floats of a head's result
+  static constexpr int JOIN = kWaves * kHeads * PITCH * 4;
+  static constexpr int TOTAL = (RING > JOIN ? RING : JOIN) + kWaves * kHeads * 8;
+  static_assert(TOTAL <= 160 * 1024, "LDS");
+};
+
+template <int DT, int ND>
+__global__ void __launch_bounds__(kWaves * 64, 1) decode_kernel(const AttnParams p) {
+  using L = DecodeLds<ND>;
+  constexpr int RB = L::RB, NS = 2 * ND;
   using T = typename Elem<DT>::type;
-  const int lane = threadIdx.x;
-  const int h = blockIdx.x % p.heads, b = blockIdx.x / p.heads, hk = h / p.group;
-  const int rest = p.lk - p.sinks;
-  const int n = max(p.k_lens[b], 0), pos = n - 1;
-  const T* q = (const T*)p.q + b * p.q_stride[0] + h * p.q_stride[2];
-  T* k = (T*)p.k + b * p.k_stride[0] + hk * p.k_stride[2];
-  T* v = (T*)p.v + b * p.v_stride[0] + hk * p.v_stride[2];
-  const T* kn = p.k_new ? (const T*)p.k_new + b * p.kn_stride[0] + hk * p.kn_stride[1] : nullptr;
-  const T* vn = p.v_new ? (const T*)p.v_new + b * p.vn_stride[0] + hk * p.vn_stride[1] : nullptr;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int blocks = (p.group + kHeads - 1) / kHeads;
+  int id = blockIdx.x;
+  const int split = id % p.splits;
+  id /= p.splits;
+  const int hb = id % blocks;
+  id /= blocks;
+  const int hk = id % p.kv_heads, b = id / p.kv_heads;
+  const int h0 = hk * p.group + hb * kHeads, heads = min(kHeads, p.group - hb * kHeads);
+
+  // the runs of visible rows
+  const int n = max(p.k_lens[b], 0), pos = n - 1, rest = p.lk - p.sinks;
   const int lo = (int)max((int64_t)0, (int64_t)pos - p.window + 1);
-  const int first = min(p.sinks, lo), count = n == 0 ? 0 : first + pos - lo + 1;
-  auto key = [&](int t) { return t < first ? t : lo + t - first; };
-  auto row = [&](int j) { return (int64_t)(j < p.lk ? j : p.sinks + (j - p.sinks) % rest); };
-  float top = -INFINITY, total = 0.0f, acc[2] = {0.0f, 0.0f};
-  for (int t0 = 0; t0 < count; t0 += 64) {
-    const bool in = t0 + lane < count;
-    float s = -INFINITY;
-    if (in) {
-      const int j = key(t0 + lane);
-      const T* kr = j == pos && kn ? kn : k + row(j) * p.k_stride[1];
-      s = 0.0f;
-      for (int d = 0; d < p.dim; ++d) s = __builtin_fmaf((float)q[d], (float)kr[d], s);
-      s *= p.scale;
-    }
-    float next = s;
-    for (int o = 32; o; o >>= 1) next = fmaxf(next, __shfl_xor(next, o));
-    next = fmaxf(top, next);
-    const float keep = next == -INFINITY ? 1.0f : __expf(top - next);
-    const float e = in ? (next == -INFINITY ? (s != s ? s : 0.0f) : __expf(s - next)) : 0.0f;
-    float sum = e;
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    total = total * keep + sum;
-    acc[0] *= keep;
-    acc[1] *= keep;
-    top = next;
-    for (int t = 0; t < min(64, count - t0); ++t) {
-      const float w = __shfl(e, t);
-      const int j = key(t0 + t);
-      const T* vr = j == pos && vn ? vn : v + row(j) * p.v_stride[1];
-      for (int c = 0; c < 2; ++c)
-        if (lane + 64 * c < p.dim) acc[c] = __builtin_fmaf(w, (float)vr[lane + 64 * c], acc[c]);
-    }
+  const int first = n ? min(p.sinks, lo) : 0;
+  const int row_lo = lo < p.lk ? lo : p.sinks + (lo - p.sinks) % rest;
+  const int len1 = n ? min(pos - lo + 1, p.lk - row_lo) : 0, len2 = n ? pos - lo + 1 - len1 : 0;
+  const int tiles0 = (first + kRows - 1) / kRows, tiles1 = (len1 + kRows - 1) / kRows, tiles2 = (len2 + kRows - 1) / kRows;
+  const int t_all = tiles0 + tiles1 + tiles2;
+  const int t0 = (int)((int64_t)t_all * split / p.splits), t1 = (int)((int64_t)t_all * (split + 1) / p.splits);
+
+  u32x4 qf[NS];
+  const int hq = lane & 31;
+  load_row<NS>(p.q + 2 * (b * p.q_stride[0] + (int64_t)(h0 + hq) * p.q_stride[2]), hq < heads, p.dim, half, qf);
+  float c2 = p.scale * kLog2e;
+  if (c2 < 0.0f) {
+    c2 = -c2;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] ^= 0x80008000u;
   }
-  T* out = (T*)p.out + b * p.o_stride[0] + h * p.o_stride[2];
-  const float r = total == 0.0f ? 0.0f : 1.0f / total;
-  for (int c = 0; c < 2; ++c)
-    if (lane + 64 * c < p.dim) {
-      out[lane + 64 * c] = (T)(acc[c] * r);
-      if (kn && n && h % p.group == 0) {
-        k[row(pos) * p.k_stride[1] + lane + 64 * c] = kn[lane + 64 * c];
-        v[row(pos) * p.v_stride[1] + lane + 64 * c] = vn[lane + 64 * c];
+  f32x16 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
+  float top = -INFINITY, total = 0.0f;
+
+  TileLoader<RB, kRows, 1> lk, lv;
+  lk.init(p.k + 2 * (b * p.k_stride[0] + hk * p.k_stride[2]), 2 * p.k_stride[1], p.dim, 0, lane);
+  lv.init(p.v + 2 * (b * p.v_stride[0] + hk * p.v_stride[2]), 2 * p.v_stride[1], p.dim, 0, lane);
+  constexpr int LOADS = 2 * TileLoader<RB, kRows, 1>::NB;
+  uint8_t* ring = smem + wave * L::STAGES * L::STAGE;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)ring;
+  // first row and length of tile t; the tile's last row is the newest token's if `newest`
+  auto tile = [&](int t, int* row, int* rows, bool* newest) {
+    int at = t, base = 0, len = first;
+    if (at >= tiles0) {
+      at -= tiles0;
+      base = row_lo;
+      len = len1;
+      if (at >= tiles1) {
+        at -= tiles1;
+        base = p.sinks;
+        len = len2;
       }
     }
+    *row = base + at * kRows;
+    *rows = t < t1 ? min(kRows, len - at * kRows) : 0;
+    *newest = t == t_all - 1;
+  };
+  auto issue = [&](int x) {  // this wave's x-th tile
+    int row, rows;
+    bool newest;
+    tile(t0 + wave + x * kWaves, &row, &rows, &newest);
+    const uint32_t st = lds0 + (uint32_t)x % L::STAGES * L::STAGE;
+    lk.issue(st, row, rows);
+    lv.issue(st + L::TILE, row, rows);
+  };
+#pragma unroll
+  for (int x = 0; x < L::STAGES; ++x) issue(x);
+
+  for (int x = 0; t0 + wave + x * kWaves < t1; ++x) {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS * (L::STAGES - 1)) : "memory");
+    int row, rows;
+    bool newest;
+    tile(t0 + wave + x * kWaves, &row, &rows, &newest);
+    uint8_t* kt = ring + x % L::STAGES * L::STAGE;
+    uint8_t* vt = kt + L::TILE;
+    if (newest && p.k_new && lane * 8 < p.dim) {  // the new token: over what the cache held in its row
+      const u32x4 kn = *reinterpret_cast<const u32x4*>(p.k_new + 2 * (b * p.kn_stride[0] + hk * p.kn_stride[1]) + lane * 16);
+      const u32x4 vn = *reinterpret_cast<const u32x4*>(p.v_new + 2 * (b * p.vn_stride[0] + hk * p.vn_stride[1]) + lane * 16);
+      *reinterpret_cast<u32x4*>(kt + tile_offset<RB>(rows - 1, lane)) = kn;
+      *reinterpret_cast<u32x4*>(vt + tile_offset<RB>(rows - 1, lane)) = vn;
+      if (hb == 0) {
+        const int64_t to = row + rows - 1;
+        *reinterpret_cast<u32x4*>(const_cast<uint8_t*>(p.k) + 2 * (b * p.k_stride[0] + to * p.k_stride[1] + hk * p.k_stride[2]) + lane * 16) = kn;
+        *reinterpret_cast<u32x4*>(const_cast<uint8_t*>(p.v) + 2 * (b * p.v_stride[0] + to * p.v_stride[1] + hk * p.v_stride[2]) + lane * 16) = vn;
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    f32x16 s;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+#pragma unroll
+    for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(kt, 0, st, lane), qf[st], s);
+    float m = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      if (8 * (v >> 2) + (v & 3) + 4 * half >= rows) s[v] = -INFINITY;
+      m = fmaxf(m, s[v]);
+    }
+    m = xor32_max(m);
+    m = m == -INFINITY ? m : m * c2;
+    const float next = fmaxf(top, m);
+    const float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - next);
+    if (__any(next > top)) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] *= keep;
+    }
+    top = next;
+    const float ref = top == -INFINITY ? 0.0f : -top;
+    u32x4 pf[2];
+    float sum = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 e;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float y = s[4 * g + v];
+        e[v] = y == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(y, c2, ref));
+        sum += e[v];
+      }
+      uint32_t w0, w1;
+      pack4<DT>(e, &w0, &w1);
+      pf[g >> 1][2 * (g & 1)] = w0;
+      pf[g >> 1][2 * (g & 1) + 1] = w1;
+    }
+    total = __builtin_fmaf(total, keep, sum);
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] = mfma32<DT>(col_frag<RB>(vt, 16 * st, 32 * d, lane), pf[st], o[d]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its stage may be filled again
+    issue(x + L::STAGES);
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+
+  // ---- join the waves: head q's result at [wave][q][PITCH], its (maximum, sum) behind them
+  total = xor32_sum(total);
+  float* res = reinterpret_cast<float*>(smem);
+  float2* stat = reinterpret_cast<float2*>(smem + L::TOTAL - kWaves * kHeads * 8);
+  if (hq < heads) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(res + (wave * kHeads + hq) * L::PITCH + 32 * d + 8 * g + 4 * half) =
+            f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+    if (half == 0) stat[wave * kHeads + hq] = float2{top, total};
+  }
+  __syncthreads();
+  const int per = p.dim / 8;  // 8 elements a thread
+  for (int x = threadIdx.x; x < heads * per; x += kWaves * 64) {
+    const int q = x / per, c = x % per * 8;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, stat[w * kHeads + q].x);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f, y[8] = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float2 st = stat[w * kHeads + q];
+      const float f = st.x == -INFINITY && st.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(st.x - ref);
+      if (f == 0.0f) continue;  // (nothing there, or NaN times a weight of 0)
+      sum = __builtin_fmaf(st.y, f, sum);
+      const float* src = res + (w * kHeads + q) * L::PITCH + c;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) y[u] = __builtin_fmaf(src[u], f, y[u]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) y[u] *= inv;
+    if (p.splits > 1) {
+      const int64_t row = ((int64_t)b * p.heads + h0 + q) * p.splits + split;
+      f32x4* dst = reinterpret_cast<f32x4*>(p.part_out + row * p.dim + c);
+      dst[0] = f32x4{y[0], y[1], y[2], y[3]};
+      dst[1] = f32x4{y[4], y[5], y[6], y[7]};
+      if (c == 0) p.part_lse[row] = sum == 0.0f ? -INFINITY : m + __builtin_amdgcn_logf(sum);
+    } else {
+      uint32_t w[4];
+      pack4<DT>(f32x4{y[0], y[1], y[2], y[3]}, &w[0], &w[1]);
+      pack4<DT>(f32x4{y[4], y[5], y[6], y[7]}, &w[2], &w[3]);
+      *reinterpret_cast<u32x4*>(p.out + 2 * (b * p.o_stride[0] + (int64_t)(h0 + q) * p.o_stride[2] + c)) = u32x4{w[0], w[1], w[2], w[3]};
+    }
+  }
+}
+
+// The splits of a head's row, in their order (log2 domain).  One wave a row.
+template <int DT>
+__global__ void __launch_bounds__(256) decode_join_kernel(const AttnParams p) {
+  using T = typename Elem<DT>::type;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)p.batch * p.heads) return;
+  const int h = (int)(row % p.heads), b = (int)(row / p.heads);
+  const float* part = p.part_lse + row * p.splits;
+  float m = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, part[s]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f, acc[2] = {0.0f, 0.0f};
+  for (int s = 0; s < p.splits; ++s) {
+    const float w = __builtin_amdgcn_exp2f(part[s] - ref);
+    sum += w;
+    for (int c = 0; c < 2; ++c)
+      if (lane + 64 * c < p.dim) acc[c] = __builtin_fmaf(w, p.part_out[(row * p.splits + s) * p.dim + lane + 64 * c], acc[c]);
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  T* out = (T*)p.out + b * p.o_stride[0] + h * p.o_stride[2];
+  for (int c = 0; c < 2; ++c)
+    if (lane + 64 * c < p.dim) out[lane + 64 * c] = (T)(acc[c] * inv);
+}
+
+template <int DT> const void* kernel_for(int nd) {
+  switch (nd) {
+    case 1: return (const void*)&decode_kernel<DT, 1>;
+    case 2: return (const void*)&decode_kernel<DT, 2>;
+    case 3: return (const void*)&decode_kernel<DT, 3>;
+  }
+  return (const void*)&decode_kernel<DT, 4>;
 }
 
 }  // namespace
 
-hipError_t launch_attention_decode(const AttnParams& p, int dt, hipStream_t stream) {
-  AttnParams q = p;
-  void* args[] = {&q};
-  const void* fn = dt == DT_F16 ? (const void*)&decode_rows_kernel<DT_F16> : (const void*)&decode_rows_kernel<DT_BF16>;
-  return hipLaunchKernel(fn, dim3((unsigned)(p.batch * p.heads)), dim3(64), args, 0, stream);
+// Splits of a (sequence, key head): while CUs are idle and a wave keeps at least 4 tiles.
+int plan_decode(const AttnParams& p, int cu_count) {
+  const int64_t grid = (int64_t)p.batch * p.kv_heads * ((p.group + kHeads - 1) / kHeads);
+  const int64_t tiles = (std::min<int64_t>(p.lk, p.window + p.sinks) + kRows - 1) / kRows;
+  int splits = 1;
+  while (splits < 64 && grid * splits * 2 <= cu_count && tiles / (2 * splits) >= 4 * kWaves) splits *= 2;
+  return splits;
+}
+int64_t decode_workspace(const AttnParams& p, int splits) {
+  return splits > 1 ? (int64_t)p.batch * p.heads * splits * (p.dim + 1) * 4 : 0;
+}
+
+hipError_t launch_attention_decode(const AttnParams& params, int splits, int dt, hipStream_t stream) {
+  AttnParams p = params;
+  p.splits = splits;
+  p.part_lse = p.part_out + (int64_t)p.batch * p.heads * splits * p.dim;
+  void* args[] = {&p};
+  const int nd = (p.dim + 31) / 32;
+  const int64_t grid = (int64_t)p.batch * p.kv_heads * ((p.group + kHeads - 1) / kHeads) * splits;
+  const hipError_t e = hipLaunchKernel(dt == DT_F16 ? kernel_for<DT_F16>(nd) : kernel_for<DT_BF16>(nd), dim3((unsigned)grid),
+                                       dim3(kWaves * 64), args, 0, stream);
+  if (e != hipSuccess || splits == 1) return e;
+  return hipLaunchKernel(dt == DT_F16 ? (const void*)&decode_join_kernel<DT_F16> : (const void*)&decode_join_kernel<DT_BF16>,
+                         dim3((unsigned)(((int64_t)p.batch * p.heads + 3) / 4)), dim3(256), args, 0, stream);
 }
 
 }  // namespace wtc
