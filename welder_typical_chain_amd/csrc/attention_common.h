@@ -59,22 +59,34 @@ template <int RB, int ROWS, int NW> struct TileLoader {
   }
 };
 
-// Fragment of 32 token rows as MFMA rows, k-step s (16 elements of dim): lane l
-// reads row l % 32, chunk 2 s + l / 32.
-template <int RB> __device__ inline u32x4 row_frag(const uint8_t* tile, int row0, int s, int lane) {
-  const uint32_t row = (uint32_t)(row0 + (lane & 31));
-  return *reinterpret_cast<const u32x4*>(tile + tile_offset<RB>(row, (uint32_t)(2 * s + (lane >> 5))));
+// Where a lane reads its fragments in a tile.  The swizzle makes every other
+// address of the tile an exclusive or of these with a constant (the tile starts
+// 256-byte aligned, so that this holds for the address in LDS too), plus an
+// offset that the instruction takes: one register for a tile instead of one a
+// fragment.  fresh() keeps the compiler from holding the results over the loop,
+// where they cost registers (and, in the dk/dv kernel, spills).
+__device__ inline void fresh(uint32_t& x) { asm volatile("" : "+v"(x)); }
+template <int RB> __device__ inline uint32_t row_addr(int lane) {
+  const uint32_t row = (uint32_t)(lane & 31);
+  return row * RB + (((uint32_t)(lane >> 5) ^ row_swizzle<RB>(row)) << 4);
 }
-// Fragment of 32 columns (elements of dim) as MFMA rows, the 16 token rows from
-// row0 as its k.  A 32 x 32 accumulator holds, in registers 4 g .. 4 g + 3 of
-// lane half h, its rows 8 g + 4 h ..; packed to 16 bits, registers 8 s .. 8 s + 7
+template <int RB> __device__ inline uint32_t col_addr(int lane) {
+  const uint32_t row = (uint32_t)(4 * (lane >> 5) + ((lane & 15) >> 2)), chunk = (uint32_t)(2 * ((lane >> 4) & 1) + ((lane & 3) >> 1));
+  return row * RB + ((chunk ^ row_swizzle<RB>(row)) << 4) + (uint32_t)(lane & 1) * 8;
+}
+// 32 token rows as MFMA rows, k-step s (16 elements of dim): lane l reads row
+// l % 32, chunk 2 s + l / 32.  `at`: row_addr + the tile; row0 a multiple of 32.
+template <int RB> __device__ inline u32x4 row_frag(const uint8_t* lds, uint32_t at, int row0, int s) {
+  return *reinterpret_cast<const u32x4*>(lds + (at ^ (uint32_t)(s << 5)) + row0 * RB);
+}
+// 32 columns (elements 32 d .. of dim) as MFMA rows, the 16 token rows from row0 (a
+// multiple of 16) as its k.  A 32 x 32 accumulator holds, in registers 4 g .. 4 g + 3
+// of lane half h, its rows 8 g + 4 h ..; packed to 16 bits, registers 8 s .. 8 s + 7
 // are the other operand of k-step s with k in that order, so this reads token
-// rows row0 + 4 h .. + 3, then row0 + 8 + 4 h .. + 3.
-template <int RB> __device__ inline u32x4 col_frag(const uint8_t* tile, int row0, int col0, int lane) {
-  const uint32_t row = (uint32_t)(row0 + 4 * (lane >> 5) + ((lane & 15) >> 2));
-  const uint32_t col = (uint32_t)(col0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
-  const u32x2 lo = tr_read(tile + tile_offset<RB>(row, col >> 3) + (col & 7) * 2);
-  const u32x2 hi = tr_read(tile + tile_offset<RB>(row + 8, col >> 3) + (col & 7) * 2);
+// rows row0 + 4 h .. + 3, then row0 + 8 + 4 h .. + 3.  `at`: col_addr + the tile.
+template <int RB> __device__ inline u32x4 col_frag(const uint8_t* lds, uint32_t at, int row0, int d) {
+  const u32x2 lo = tr_read(lds + (at ^ (uint32_t)(d << 6)) + row0 * RB);
+  const u32x2 hi = tr_read(lds + (at ^ (uint32_t)((d << 6) | 32)) + (row0 + 8) * RB);
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 

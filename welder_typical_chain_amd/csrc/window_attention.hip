@@ -138,6 +138,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
 #pragma unroll
   for (int t = 0; t < L::STAGES - 1; ++t) issue(t0 + t);
 
+  const uint32_t k_at = row_addr<RB>(lane), v_at = L::TILE + col_addr<RB>(lane);
   for (int t = t0; t < t1; ++t) {
     wait_loads_barrier<LOADS*(L::STAGES - 2)>();  // tile t landed; every wave is done with tile t - 1
     issue(t + L::STAGES - 1);
@@ -145,8 +146,10 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
     // (in the window's part the first tokens may lie below the window too)
     const bool below = t >= t_sink && (int64_t)j0 + kKeys - 1 + p.window <= w_lo && j0 >= p.sinks;
     if (!w_any || j0 > w_hi || below) continue;
-    const uint8_t* kt = smem + (t - t0) % L::STAGES * L::STAGE;
-    const uint8_t* vt = kt + L::TILE;
+    const uint32_t stage = (uint32_t)(t - t0) % L::STAGES * L::STAGE;
+    uint32_t ka = k_at + stage, va = v_at + stage;
+    fresh(ka);
+    fresh(va);
 
     f32x16 s[2];
 #pragma unroll
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[u][v] = 0.0f;
 #pragma unroll
-      for (int st = 0; st < NS; ++st) s[u] = mfma32<DT>(row_frag<RB>(kt, 32 * u, st, lane), qf[st], s[u]);
+      for (int st = 0; st < NS; ++st) s[u] = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u, st), qf[st], s[u]);
     }
     if (j0 + kKeys > j1 || j0 + kKeys - 1 > w_lo || (t >= t_sink && (int64_t)j0 + p.window <= w_hi)) {
       // key j0 + 4 half + c is seen if c <= top_c and (c > low_c or c < sink_c)
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
 #pragma unroll
     for (int st = 0; st < 4; ++st)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] = mfma32<DT>(col_frag<RB>(vt, 16 * st, 32 * d, lane), pf[st], o[d]);
+      for (int d = 0; d < ND; ++d) o[d] = mfma32<DT>(col_frag<RB>(smem, va, 16 * st, d), pf[st], o[d]);
   }
   wait_loads_barrier<0>();
 
@@ -467,12 +470,15 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnPara
 #pragma unroll
   for (int t = 0; t < L::STAGES - 1; ++t) issue(t);
 
+  const uint32_t k_at = row_addr<RB>(lane), kc_at = col_addr<RB>(lane);
   for (int t = 0; t < t_all; ++t) {
     wait_loads_barrier<LOADS*(L::STAGES - 2)>();
     issue(t + L::STAGES - 1);
     const int j0 = tile_base(t), j1 = tile_end(t);
-    const uint8_t* kt = smem + t % L::STAGES * L::STAGE;
-    const uint8_t* vt = kt + L::TILE;
+    const uint32_t stage = (uint32_t)t % L::STAGES * L::STAGE;
+    uint32_t ka = k_at + stage, kc = kc_at + stage;
+    fresh(ka);
+    fresh(kc);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int k0 = j0 + 32 * u;
@@ -482,9 +488,9 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnPara
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
 #pragma unroll
-      for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(kt, 32 * u, st, lane), qf[st], s);
+      for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u, st), qf[st], s);
 #pragma unroll
-      for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(vt, 32 * u, st, lane), gf[st], g);
+      for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u + kKeys, st), gf[st], g);
 #pragma unroll
       for (int v = 0; v < 16; ++v)
         s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c2, -lse2)) * (g[v] - delta);
@@ -510,7 +516,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnPara
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dq[d] = mfma32<DT>(col_frag<RB>(kt, 32 * u + 16 * st, 32 * d, lane), df[st], dq[d]);
+        for (int d = 0; d < ND; ++d) dq[d] = mfma32<DT>(col_frag<RB>(smem, kc, 32 * u + 16 * st, d), df[st], dq[d]);
     }
   }
   wait_loads_barrier<0>();
@@ -549,27 +555,33 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnPara
   }
 }
 
-// A workgroup takes kDkvKeys keys of one (sequence, key head), 32 a wave, their K
-// and V fragments in registers, and streams the queries that see them in tiles
-// of 64 packed rows: whole positions of up to 64 query heads of the group, so
-// that a lane's offset inside a tile is the same for every tile.
+// A workgroup takes kDkvKeys keys of one (sequence, key head) and streams the
+// queries that see them in tiles of 64 packed rows: whole positions of up to 64
+// query heads of the group, so that a lane's offset inside a tile is the same
+// for every tile.  Wave w holds the K and V fragments of keys 32 (w % 4) .. + 31
+// in registers and takes the tile's rows 32 (w / 4) .. + 31, so that a SIMD has
+// two waves (one computes weights while the other's products run) and the key
+// block stays at 128:
 //   S = Q . K^T, dP = dout . V^T (a lane holds 16 queries of one key)
 //   dV^T += dout^T . P, dK^T += Q^T . dS
+// At the end the two waves of a key join their sums through LDS, one of them dk,
+// the other dv.
 // The first tokens are seen by every later query.  A workgroup of their key
 // block streams, like the others, the queries whose window reaches the block; the
 // far queries go in p.far_chunks chunks to workgroups of their own (p.far_rows
 // positions each), and all of the block's sums as f32 to p.part_far, which
 // attention_far_kernel adds in order for the first tokens' keys.
-constexpr int kDkvWaves = 4;
-constexpr int kDkvKeys = 32 * kDkvWaves;
+constexpr int kDkvWaves = 8;
+constexpr int kDkvKeys = 128;
 constexpr int kQueries = 64;
 
 template <int ND> struct DkvLds {
   static constexpr int RB = row_bytes(ND), STAGES = 2;
   static constexpr int TILE = kQueries * RB, STATS = 2 * TILE, STAGE = 2 * TILE + 1024;
-  static constexpr int PITCH = ND * 64 + 16;
+  static constexpr int PITCH = ND * 128 + 16;  // bytes of a key's sums
   static constexpr int RING = STAGES * STAGE, OUT = kDkvWaves * 32 * PITCH;
-  static constexpr int TOTAL = RING > OUT ? RING : OUT;
+  static constexpr int TOTAL = (RING > OUT ? RING : OUT) + kDkvWaves * 4;
+  static_assert(TOTAL <= 160 * 1024, "LDS");
 };
 
 // part_far: [batch][kv_heads][far_blocks][1 + far_chunks][kDkvKeys][dk, dv][dim]
@@ -591,7 +603,8 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
   const bool far = w >= p.key_blocks;
   const int kb = far ? (w - p.key_blocks) / p.far_chunks : w, chunk = far ? (w - p.key_blocks) % p.far_chunks : 0;
   const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
-  const int j_first = kb * kDkvKeys, j = j_first + wave * 32 + (lane & 31);
+  const int sub = wave >> 2;  // rows of a tile
+  const int j_wave = kb * kDkvKeys + (wave & 3) * 32, j_first = kb * kDkvKeys, j = j_wave + (lane & 31);
   const bool valid = j < nk;
   // queries: the near ones are those whose window may reach a key of the block
   int i0 = min(max(0, j_first - shift), nq);
@@ -653,114 +666,142 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
   };
   const float c2 = p.scale * kLog2e;
   issue(0);
+  const int row0 = 32 * sub;
+  const uint32_t r_at = row_addr<RB>(lane) + (uint32_t)row0 * RB, c_at = col_addr<RB>(lane) + (uint32_t)row0 * RB;
   for (int t = 0; t < t_all; ++t) {
     wait_loads_barrier<0>();  // tile t landed; every wave is done with tile t - 1
     issue(t + 1);
     const int step = t / chunks, hc = t - step * chunks, i = i0 + step * tp;
-    const uint8_t* qt = smem + t % L::STAGES * L::STAGE;
-    const uint8_t* gt = qt + L::TILE;
-    const uint8_t* stt = qt + L::STATS;
+    const uint32_t stage = (uint32_t)t % L::STAGES * L::STAGE;
+    const uint8_t* stt = smem + stage + L::STATS;
     // tile row x is a query that sees this lane's key if t_lo <= x < t_hi
     const int rows = min(min(tp, i1 - i) * hg, hg == p.group ? kQueries : p.group - hc * hg);
     const int64_t back = (int64_t)j - shift - i;
     const int t_lo = (int)min((int64_t)1 << 20, max((int64_t)0, back)) * hg;
     const int64_t reach = j < p.sinks ? 1 << 20 : max((int64_t)0, min((int64_t)1 << 20, back + p.window)) * hg;
     const int t_hi = valid ? (int)min((int64_t)rows, reach) : 0;
-    const bool all = __all(t_lo == 0 && t_hi == kQueries);
-    if (!all && !__any(t_lo < t_hi)) continue;
+    const bool all = __all(t_lo <= row0 && t_hi >= row0 + 32);
+    if (!all && !__any(max(t_lo, row0) < min(t_hi, row0 + 32))) continue;
+    uint32_t ra = r_at + stage, ca = c_at + stage;
+    fresh(ra);
+    fresh(ca);
+    f32x16 s, g;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      f32x16 s, g;
+    for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
 #pragma unroll
-      for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
+    for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ra, 0, st), kf[st], s);
 #pragma unroll
-      for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(qt, 32 * u, st, lane), kf[st], s);
+    for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(smem, ra, kQueries, st), vf[st], g);
+    u32x4 pf[2], df[2];
 #pragma unroll
-      for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(gt, 32 * u, st, lane), vf[st], g);
-      u32x4 pf[2], df[2];
+    for (int q = 0; q < 4; ++q) {
+      const int row = row0 + 8 * q + 4 * half;
+      const f32x4 st0 = *reinterpret_cast<const f32x4*>(stt + row * 8), st1 = *reinterpret_cast<const f32x4*>(stt + row * 8 + 16);
+      const float lse[4] = {st0[0], st0[2], st1[0], st1[2]}, del[4] = {st0[1], st0[3], st1[1], st1[3]};
+      f32x4 pw, ds;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int row = 32 * u + 8 * q + 4 * half;
-        const f32x4 st0 = *reinterpret_cast<const f32x4*>(stt + row * 8), st1 = *reinterpret_cast<const f32x4*>(stt + row * 8 + 16);
-        const float lse[4] = {st0[0], st0[2], st1[0], st1[2]}, del[4] = {st0[1], st0[3], st1[1], st1[3]};
-        f32x4 pw, ds;
+      for (int v = 0; v < 4; ++v) {
+        pw[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + v], c2, -lse[v]));
+        ds[v] = pw[v] * (g[4 * q + v] - del[v]);
+      }
+      if (!all) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          pw[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + v], c2, -lse[v]));
-          ds[v] = pw[v] * (g[4 * q + v] - del[v]);
-          if (!all) {
-            const bool in = row + v >= t_lo && row + v < t_hi;
-            pw[v] = in ? pw[v] : 0.0f;
-            ds[v] = in ? ds[v] : 0.0f;
-          }
+          const bool in = row + v >= t_lo && row + v < t_hi;
+          pw[v] = in ? pw[v] : 0.0f;
+          ds[v] = in ? ds[v] : 0.0f;
         }
-        uint32_t w0, w1;
-        pack4<DT>(pw, &w0, &w1);
-        pf[q >> 1][2 * (q & 1)] = w0;
-        pf[q >> 1][2 * (q & 1) + 1] = w1;
-        pack4<DT>(ds, &w0, &w1);
-        df[q >> 1][2 * (q & 1)] = w0;
-        df[q >> 1][2 * (q & 1) + 1] = w1;
       }
-#pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          dv[d] = mfma32<DT>(col_frag<RB>(gt, 32 * u + 16 * st, 32 * d, lane), pf[st], dv[d]);
-          dk[d] = mfma32<DT>(col_frag<RB>(qt, 32 * u + 16 * st, 32 * d, lane), df[st], dk[d]);
-        }
+      uint32_t w0, w1;
+      pack4<DT>(pw, &w0, &w1);
+      pf[q >> 1][2 * (q & 1)] = w0;
+      pf[q >> 1][2 * (q & 1) + 1] = w1;
+      pack4<DT>(ds, &w0, &w1);
+      df[q >> 1][2 * (q & 1)] = w0;
+      df[q >> 1][2 * (q & 1) + 1] = w1;
     }
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        dv[d] = mfma32<DT>(col_frag<RB>(smem, ca, kQueries + 16 * st, d), pf[st], dv[d]);
+        dk[d] = mfma32<DT>(col_frag<RB>(smem, ca, 16 * st, d), df[st], dk[d]);
+      }
   }
   wait_loads_barrier<0>();
 
+  // ---- join: waves 0-3 hand over dv and finish dk, waves 4-7 the other way round
+  uint8_t* mine = smem + wave * 32 * L::PITCH;          // what this wave finishes
+  uint8_t* other = smem + (wave ^ 4) * 32 * L::PITCH;   // what it hands over
+  const uint32_t at = (uint32_t)((lane & 31) * L::PITCH + half * 16);
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x16& y = sub ? dk[d] : dv[d];
+      *reinterpret_cast<f32x4*>(other + at + (32 * d + 8 * q) * 4) = f32x4{y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]};
+    }
+  __syncthreads();
+#pragma unroll
+  for (int d = 0; d < ND; ++d) {
+    f32x16& y = sub ? dv[d] : dk[d];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 z = *reinterpret_cast<const f32x4*>(mine + at + (32 * d + 8 * q) * 4);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) dk[d][4 * q + v] = y[4 * q + v] + z[v];  // (the result in dk from here on)
+    }
+  }
   const bool parts = kb < p.far_blocks && p.far_chunks > 0;
   if (parts) {
-    float* dst = far_part(p, b, hk, kb, far ? 1 + chunk : 0) + (int64_t)(wave * 32 + (lane & 31)) * 2 * p.dim;
+    float* dst = far_part(p, b, hk, kb, far ? 1 + chunk : 0) + (int64_t)((wave & 3) * 32 + (lane & 31)) * 2 * p.dim + sub * p.dim;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int c = 32 * d + 8 * g + 4 * half;
-        if (c < p.dim) {
-          *reinterpret_cast<f32x4*>(dst + c) = f32x4{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
-          *reinterpret_cast<f32x4*>(dst + p.dim + c) = f32x4{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
-        }
+        if (c < p.dim) *reinterpret_cast<f32x4*>(dst + c) = f32x4{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
       }
     if (far) return;
   }
   bool nan = false;
-  uint8_t* stg = smem + wave * 32 * L::PITCH;
-  constexpr int CPR = ND * 4;
+  const float scale = sub ? 1.0f : p.scale;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
+  for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+    for (int g = 0; g < 4; ++g) {
+      f32x4 y;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4 y;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          y[v] = !valid ? 0.0f : which ? dv[d][4 * g + v] : dk[d][4 * g + v] * p.scale;
-          nan |= y[v] != y[v];
-        }
-        uint32_t w0, w1;
-        pack4<DT>(y, &w0, &w1);
-        *reinterpret_cast<u32x2*>(stg + (lane & 31) * L::PITCH + (32 * d + 8 * g + 4 * half) * 2) = u32x2{w0, w1};
+      for (int v = 0; v < 4; ++v) {
+        y[v] = valid ? dk[d][4 * g + v] * scale : 0.0f;
+        nan |= y[v] != y[v];
       }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 4
-    for (int y = lane; y < 32 * CPR; y += 64) {
-      const int row = y / CPR, c = y % CPR, jj = j_first + wave * 32 + row;
-      if (jj < p.lk && c * 8 < p.dim && !(parts && jj < p.sinks))
-        *reinterpret_cast<u32x4*>((which ? p.dv : p.dk) + 2 * ((((int64_t)b * p.lk + jj) * p.kv_heads + hk) * p.dim) + c * 16) =
-            *reinterpret_cast<const u32x4*>(stg + row * L::PITCH + c * 16);
+      uint32_t w0, w1;
+      pack4<DT>(y, &w0, &w1);
+      *reinterpret_cast<u32x2*>(mine + (lane & 31) * L::PITCH + (32 * d + 8 * g + 4 * half) * 2) = u32x2{w0, w1};
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  constexpr int CPR = ND * 4;
+  uint8_t* dst = sub ? p.dv : p.dk;
+#pragma unroll 4
+  for (int y = lane; y < 32 * CPR; y += 64) {
+    const int row = y / CPR, c = y % CPR, jj = j_wave + row;
+    if (jj < p.lk && c * 8 < p.dim && !(parts && jj < p.sinks))
+      *reinterpret_cast<u32x4*>(dst + 2 * ((((int64_t)b * p.lk + jj) * p.kv_heads + hk) * p.dim) + c * 16) =
+          *reinterpret_cast<const u32x4*>(mine + row * L::PITCH + c * 16);
   }
+  // rows that came out as NaN, once both waves' results are written
   nan = nan && !(parts && j < p.sinks);
-  uint32_t redo = (uint32_t)(__ballot(nan) | __ballot(nan) >> 32);
+  uint32_t* marks = reinterpret_cast<uint32_t*>(smem + L::TOTAL - kDkvWaves * 4);
+  const uint64_t ballot = __ballot(nan);
+  if (lane == 0) marks[wave] = (uint32_t)(ballot | ballot >> 32);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (sub) return;
+  uint32_t redo = __builtin_amdgcn_readfirstlane(marks[wave] | marks[wave + 4]);
   while (redo) {
-    dkv_row<DT>(p, b, hk, j_first + wave * 32 + __builtin_ctz(redo));
+    dkv_row<DT>(p, b, hk, j_wave + __builtin_ctz(redo));
     redo &= redo - 1;
   }
 }

@@ -133,11 +133,14 @@ __global__ void __launch_bounds__(kWaves * 64, 1) decode_kernel(const AttnParams
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    uint32_t ka = row_addr<RB>(lane) + (uint32_t)(kt - smem), va = col_addr<RB>(lane) + (uint32_t)(vt - smem);
+    fresh(ka);
+    fresh(va);
     f32x16 s;
 #pragma unroll
     for (int v = 0; v < 16; ++v) s[v] = 0.0f;
 #pragma unroll
-    for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(kt, 0, st, lane), qf[st], s);
+    for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ka, 0, st), qf[st], s);
     float m = -INFINITY;
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) decode_kernel(const AttnParams
 #pragma unroll
     for (int st = 0; st < 2; ++st)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] = mfma32<DT>(col_frag<RB>(vt, 16 * st, 32 * d, lane), pf[st], o[d]);
+      for (int d = 0; d < ND; ++d) o[d] = mfma32<DT>(col_frag<RB>(smem, va, 16 * st, d), pf[st], o[d]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its stage may be filled again
     issue(x + L::STAGES);
   }
