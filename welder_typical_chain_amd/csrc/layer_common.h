@@ -116,7 +116,7 @@ struct AttnParams {
   float *part_out, *part_lse;  // of a row's splits: normalised results and log-sum-exp
   float* part_far;
   int32_t splits, row_blocks;
-  int32_t key_blocks, far_blocks, far_chunks, far_rows;
+  int32_t key_blocks, far_blocks, far_chunks, far_keys;
   int32_t batch, heads, kv_heads, group, lq, lk, dim, sinks;
   float scale;
 };

@@ -36,7 +36,7 @@ int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);
 // p.part_out: attention_workspace() bytes
 hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, hipStream_t stream);
 struct AttnBackwardPlan {
-  int key_blocks, far_blocks, far_chunks, far_rows;
+  int key_blocks, far_blocks, far_chunks, far_keys;
   int64_t part_at, workspace;  // bytes
 };
 AttnBackwardPlan plan_attention_backward(const AttnParams& p);

@@ -566,11 +566,13 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnPara
 //   dV^T += dout^T . P, dK^T += Q^T . dS
 // At the end the two waves of a key join their sums through LDS, one of them dk,
 // the other dv.
-// The first tokens are seen by every later query.  A workgroup of their key
-// block streams, like the others, the queries whose window reaches the block; the
-// far queries go in p.far_chunks chunks to workgroups of their own (p.far_rows
-// positions each), and all of the block's sums as f32 to p.part_far, which
-// attention_far_kernel adds in order for the first tokens' keys.
+// The first tokens are seen by every later query, more queries than see any other
+// key.  A workgroup of their key block takes, like the others, the queries whose
+// window reaches the block; the far queries go in p.far_chunks short chunks to
+// workgroups of their own behind the key blocks.  All sums of the first tokens go
+// to p.part_far in f32, and attention_far_kernel adds them in order.  (In chunks as
+// long as a block's near queries they made 280 equal workgroups on 256 CUs for
+// train_bf16, a second round: 240 us against FAR_US.)
 constexpr int kDkvWaves = 8;
 constexpr int kDkvKeys = 128;
 constexpr int kQueries = 64;
@@ -578,15 +580,20 @@ constexpr int kQueries = 64;
 template <int ND> struct DkvLds {
   static constexpr int RB = row_bytes(ND), STAGES = 2;
   static constexpr int TILE = kQueries * RB, STATS = 2 * TILE, STAGE = 2 * TILE + 1024;
+  // At dim 128 the registers do not hold all of K's and V's fragments beside the
+  // sums (a spilled one is loaded through vmcnt, behind the next tile's loads):
+  // the last KEPT of V's k-steps are read from LDS, 1 KiB a wave and step.
+  static constexpr int KEPT = ND == 4 ? 3 : 0, KEPT_AT = STAGES * STAGE;
   static constexpr int PITCH = ND * 128 + 16;  // bytes of a key's sums
-  static constexpr int RING = STAGES * STAGE, OUT = kDkvWaves * 32 * PITCH;
+  static constexpr int RING = KEPT_AT + 4 * KEPT * 1024, OUT = kDkvWaves * 32 * PITCH;
   static constexpr int TOTAL = (RING > OUT ? RING : OUT) + kDkvWaves * 4;
   static_assert(TOTAL <= 160 * 1024, "LDS");
 };
 
-// part_far: [batch][kv_heads][far_blocks][1 + far_chunks][kDkvKeys][dk, dv][dim]
-__device__ inline float* far_part(const AttnParams& p, int b, int hk, int kb, int slot) {
-  return p.part_far + ((((int64_t)b * p.kv_heads + hk) * p.far_blocks + kb) * (1 + p.far_chunks) + slot) * (kDkvKeys * 2) * p.dim;
+// part_far: [batch][kv_heads][far_blocks][1 + far_chunks][far_keys][dk, dv][dim];
+// slot 0 holds the near queries' sums
+__device__ inline float* far_part(const AttnParams& p, int b, int hk, int kb, int slot, int key) {
+  return p.part_far + (((((int64_t)b * p.kv_heads + hk) * p.far_blocks + kb) * (1 + p.far_chunks) + slot) * p.far_keys + key) * 2 * p.dim;
 }
 
 template <int DT, int ND>
@@ -604,47 +611,52 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
   const int kb = far ? (w - p.key_blocks) / p.far_chunks : w, chunk = far ? (w - p.key_blocks) % p.far_chunks : 0;
   const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
   const int sub = wave >> 2;  // rows of a tile
-  const int j_wave = kb * kDkvKeys + (wave & 3) * 32, j_first = kb * kDkvKeys, j = j_wave + (lane & 31);
+  const int j_first = kb * kDkvKeys, j_wave = j_first + (wave & 3) * 32, j = j_wave + (lane & 31);
   const bool valid = j < nk;
   // queries: the near ones are those whose window may reach a key of the block
   int i0 = min(max(0, j_first - shift), nq);
   int i1 = (int)max((int64_t)i0, min((int64_t)nq, (int64_t)min(j_first + kDkvKeys, nk) - 1 + p.window - shift));
-  if (j_first >= nk) i1 = i0;
   if (far) {
-    i0 = min(nq, (int)min((int64_t)nq, i1 + (int64_t)chunk * p.far_rows));
-    i1 = chunk + 1 == p.far_chunks ? nq : min(nq, (int)min((int64_t)nq, i0 + (int64_t)p.far_rows));
-    if (j_first >= nk) i1 = i0;
+    const int first = i1, share = (nq - first + p.far_chunks - 1) / p.far_chunks;
+    i0 = (int)min((int64_t)nq, first + (int64_t)chunk * share);
+    i1 = min(nq, i0 + share);
   }
+  if (j_first >= nk) i1 = i0;
   const int hg = min(p.group, kQueries), chunks = (p.group + hg - 1) / hg;  // query heads a tile, tiles a position
   const int tp = kQueries / hg;                                             // positions a tile
-  const int steps = (i1 - i0 + tp - 1) / tp, t_all = steps * chunks;
 
+  // loads of a tile: block q of this wave holds tile row `row[q]`, position row / hg, head row % hg
+  const uint8_t* q_base = p.q + 2 * (b * p.q_stride[0] + (int64_t)hk * p.group * p.q_stride[2]);
+  const uint8_t* g_base = p.dout + 2 * (b * p.do_stride[0] + (int64_t)hk * p.group * p.do_stride[2]);
+  uint32_t q_off[NB], g_off[NB];
+  uint32_t at_row[NB];  // position and head (high half)
+#pragma unroll
+  for (int q = 0; q < NB; ++q) {
+    const int row = (int)block_row<RB>(wave * NB + q, lane);
+    const uint32_t c = block_chunk<RB>(wave * NB + q, lane) * 16u;
+    at_row[q] = c < (uint32_t)p.dim * 2u ? (uint32_t)(row / hg | row % hg << 16) : 0xFFFFu;
+    q_off[q] = (uint32_t)(2 * (row / hg * p.q_stride[1] + row % hg * p.q_stride[2])) + c;
+    g_off[q] = (uint32_t)(2 * (row / hg * p.do_stride[1] + row % hg * p.do_stride[2])) + c;
+  }
+  const float2* st_base = p.stats + stats_row(p, b, hk, 0);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
+  const float c2 = p.scale * kLog2e;
+  const int row0 = 32 * sub;
+  const int steps = (i1 - i0 + tp - 1) / tp, t_all = steps * chunks;
   u32x4 kf[NS], vf[NS];
   load_row<NS>(p.k + 2 * (b * p.k_stride[0] + (int64_t)j * p.k_stride[1] + hk * p.k_stride[2]), valid, p.dim, half, kf);
   load_row<NS>(p.v + 2 * (b * p.v_stride[0] + (int64_t)j * p.v_stride[1] + hk * p.v_stride[2]), valid, p.dim, half, vf);
+  const uint32_t kept_at = (uint32_t)(L::KEPT_AT + (wave & 3) * L::KEPT * 1024 + lane * 16);
+  if (!sub) {
+#pragma unroll
+    for (int x = 0; x < L::KEPT; ++x) *reinterpret_cast<u32x4*>(smem + kept_at + x * 1024) = vf[NS - L::KEPT + x];
+  }
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int v = 0; v < 16; ++v) dk[d][v] = dv[d][v] = 0.0f;
 
-  // loads of a tile: block q of this wave holds tile row `row[q]`, position row / hg, head row % hg
-  const uint8_t* q_base = p.q + 2 * (b * p.q_stride[0] + (int64_t)hk * p.group * p.q_stride[2]);
-  const uint8_t* g_base = p.dout + 2 * (b * p.do_stride[0] + (int64_t)hk * p.group * p.do_stride[2]);
-  uint32_t q_off[NB], g_off[NB];
-  int at_pos[NB], at_head[NB];
-#pragma unroll
-  for (int q = 0; q < NB; ++q) {
-    const int row = (int)block_row<RB>(wave * NB + q, lane);
-    const uint32_t c = block_chunk<RB>(wave * NB + q, lane) * 16u;
-    at_pos[q] = c < (uint32_t)p.dim * 2u ? row / hg : 1 << 30;
-    at_head[q] = row % hg;
-    q_off[q] = (uint32_t)(2 * (at_pos[q] * p.q_stride[1] + at_head[q] * p.q_stride[2])) + c;
-    g_off[q] = (uint32_t)(2 * (at_pos[q] * p.do_stride[1] + at_head[q] * p.do_stride[2])) + c;
-  }
-  const float2* st_base = p.stats + stats_row(p, b, hk, 0);
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
-  constexpr int LOADS = 2 * NB;
   auto issue = [&](int t) {
     const int step = t / chunks, hc = t - step * chunks, i = i0 + step * tp;
     const int npos = t < t_all ? min(tp, i1 - i) : 0, nhead = p.group - hc * hg;
@@ -654,7 +666,7 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
     const i32x4 rg = raw_rsrc(g_base + 2 * (i * p.do_stride[1] + hc * hg * p.do_stride[2]), 0x7FFFFFFFu);
 #pragma unroll
     for (int q = 0; q < NB; ++q) {
-      const bool in = at_pos[q] < npos && at_head[q] < nhead;
+      const bool in = (int)(at_row[q] & 0xFFFFu) < npos && (int)(at_row[q] >> 16) < nhead;
       dma16(rq, in ? q_off[q] : kOutOfRange, st + q * 1024);
       dma16(rg, in ? g_off[q] : kOutOfRange, st + L::TILE + q * 1024);
     }
@@ -664,9 +676,7 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
       dma16(rs, lane * 16, lds0 + (uint32_t)t % L::STAGES * L::STAGE + L::STATS);
     }
   };
-  const float c2 = p.scale * kLog2e;
   issue(0);
-  const int row0 = 32 * sub;
   const uint32_t r_at = row_addr<RB>(lane) + (uint32_t)row0 * RB, c_at = col_addr<RB>(lane) + (uint32_t)row0 * RB;
   for (int t = 0; t < t_all; ++t) {
     wait_loads_barrier<0>();  // tile t landed; every wave is done with tile t - 1
@@ -691,7 +701,11 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
 #pragma unroll
     for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ra, 0, st), kf[st], s);
 #pragma unroll
-    for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(smem, ra, kQueries, st), vf[st], g);
+    for (int st = 0; st < NS; ++st) {
+      const int x = st - (NS - L::KEPT);
+      g = mfma32<DT>(row_frag<RB>(smem, ra, kQueries, st), x < 0 ? vf[st] : *reinterpret_cast<const u32x4*>(smem + kept_at + x * 1024), g);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     u32x4 pf[2], df[2];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -720,6 +734,7 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
       df[q >> 1][2 * (q & 1)] = w0;
       df[q >> 1][2 * (q & 1) + 1] = w1;
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int st = 0; st < 2; ++st)
 #pragma unroll
@@ -752,16 +767,18 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
       for (int v = 0; v < 4; ++v) dk[d][4 * q + v] = y[4 * q + v] + z[v];  // (the result in dk from here on)
     }
   }
-  const bool parts = kb < p.far_blocks && p.far_chunks > 0;
+  const bool parts = kb < p.far_blocks;
   if (parts) {
-    float* dst = far_part(p, b, hk, kb, far ? 1 + chunk : 0) + (int64_t)((wave & 3) * 32 + (lane & 31)) * 2 * p.dim + sub * p.dim;
+    if (j < p.sinks) {
+      float* dst = far_part(p, b, hk, kb, far ? 1 + chunk : 0, j - j_first) + sub * p.dim;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+      for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int c = 32 * d + 8 * g + 4 * half;
-        if (c < p.dim) *reinterpret_cast<f32x4*>(dst + c) = f32x4{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
-      }
+        for (int g = 0; g < 4; ++g) {
+          const int c = 32 * d + 8 * g + 4 * half;
+          if (c < p.dim) *reinterpret_cast<f32x4*>(dst + c) = f32x4{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
+        }
+    }
     if (far) return;
   }
   bool nan = false;
@@ -816,8 +833,15 @@ __global__ void __launch_bounds__(64) attention_far_kernel(const AttnParams p) {
   for (int c = lane; c < 2 * p.dim; c += 64) {
     const bool is_dv = c >= p.dim;
     float sum = 0.0f;
-    for (int s = 0; s <= p.far_chunks; ++s)
-      sum += far_part(p, b, hk, j / kDkvKeys, s)[(int64_t)(j % kDkvKeys) * 2 * p.dim + c];
+    const float* part = far_part(p, b, hk, j / kDkvKeys, 0, j % kDkvKeys) + c;
+    const int64_t step = (int64_t)p.far_keys * 2 * p.dim;
+    for (int s = 0; s <= p.far_chunks; s += 16) {  // 16 loads at a time, added in their order
+      float x[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) x[u] = s + u <= p.far_chunks ? part[(s + u) * step] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) sum += x[u];
+    }
     if (!is_dv) sum *= p.scale;
     if (j >= seq_keys(p, b)) sum = 0.0f;
     nan |= sum != sum;
@@ -898,21 +922,20 @@ template <int DT> const void* dkv_kernel(int nd) {
 }
 }  // namespace
 
-// Far chunks: about as many positions as a block's near queries, so that no
-// workgroup runs much longer than the others.
 AttnBackwardPlan plan_attention_backward(const AttnParams& p) {
   AttnBackwardPlan plan{};
   plan.key_blocks = (p.lk + kDkvKeys - 1) / kDkvKeys;
   // queries past the near ones of the first block: at most the keys past them
-  const int64_t near = p.window + kDkvKeys, far = std::min<int64_t>(p.lq, (int64_t)p.lk - near + 1);
+  const int64_t far = std::min<int64_t>(p.lq, (int64_t)p.lk - (p.window + kDkvKeys) + 1);
   if (p.sinks > 0 && far > 0) {
     plan.far_blocks = (p.sinks + kDkvKeys - 1) / kDkvKeys;
-    plan.far_chunks = (int)std::min<int64_t>((far + near - 1) / near, 64);
-    plan.far_rows = (int)((far + plan.far_chunks - 1) / plan.far_chunks);
+    plan.far_keys = std::min(p.sinks, kDkvKeys);
+    // short ones, in the end of the key blocks' round: 64 positions or a key block's share
+    plan.far_chunks = (int)std::max<int64_t>(1, std::min<int64_t>(plan.key_blocks, far / 64));
   }
   const int64_t rows = (int64_t)p.batch * p.lq * p.heads;
   plan.part_at = (rows * 8 + 255) / 256 * 256;
-  plan.workspace = plan.part_at + ((int64_t)p.batch * p.kv_heads * plan.far_blocks * (1 + plan.far_chunks) * kDkvKeys * 2 * p.dim * 4 + 255) / 256 * 256;
+  plan.workspace = plan.part_at + ((int64_t)p.batch * p.kv_heads * plan.far_blocks * (1 + plan.far_chunks) * plan.far_keys * 2 * p.dim * 4 + 255) / 256 * 256;
   return plan;
 }
 
@@ -921,8 +944,8 @@ hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwar
   p.part_far = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.stats) + plan.part_at);
   p.key_blocks = plan.key_blocks;
   p.far_blocks = plan.far_blocks;
+  p.far_keys = plan.far_keys;
   p.far_chunks = plan.far_chunks;
-  p.far_rows = plan.far_rows;
   const int nd = (p.dim + 31) / 32;
   const int64_t seqs = (int64_t)p.batch * p.kv_heads;
   if (p.lq) {
@@ -935,7 +958,7 @@ hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwar
   if (!p.lk) return hipSuccess;
   const hipError_t e = launch(dt == DT_F16 ? dkv_kernel<DT_F16>(nd) : dkv_kernel<DT_BF16>(nd),
                               seqs * (p.key_blocks + p.far_blocks * p.far_chunks), kDkvWaves * 64, p, stream);
-  if (e != hipSuccess || !p.far_chunks) return e;
+  if (e != hipSuccess || !p.far_blocks) return e;
   return launch(WTC_BY_TYPE(attention_far_kernel, dt), seqs * p.sinks, 64, p, stream);
 }
 
