@@ -109,10 +109,12 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
   u32x4 qf[NS];
   load_row<NS>(p.q + 2 * (b * p.q_stride[0] + (int64_t)i * p.q_stride[1] + h * p.q_stride[2]), valid, p.dim, half, qf);
   float c2 = p.scale * kLog2e;
-  if (c2 < 0.0f) {  // then the largest score is the smallest product: negate the queries instead
-    c2 = -c2;
+  if (!(c2 > 0.0f)) {
+    // a negative scale: the largest score is the smallest product, so negate the
+    // queries instead; a scale of 0: all scores are 0
 #pragma unroll
-    for (int s = 0; s < NS; ++s) qf[s] ^= 0x80008000u;
+    for (int s = 0; s < NS; ++s) qf[s] = c2 < 0.0f ? qf[s] ^ 0x80008000u : qf[s] & 0u;
+    c2 = c2 < 0.0f ? -c2 : 1.0f;
   }
 
   f32x16 o[ND];
@@ -173,13 +175,10 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
           s[u][v] = c <= top_c && (c > low_c || c < sink_c) ? s[u][v] : -INFINITY;
         }
     }
-    float m = s[0][0];
+    float m = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-    for (int v = 1; v < 16; ++v) m = fmaxf(m, s[0][v]);
-#pragma unroll
-    for (int v = 0; v < 16; ++v) m = fmaxf(m, s[1][v]);
-    m = xor32_max(m);
-    m = m == -INFINITY ? m : m * c2;  // (a scale of 0 times -inf)
+    for (int v = 1; v < 16; ++v) m = fmaxf(m, fmaxf(s[0][v], s[1][v]));
+    m = xor32_max(m) * c2;
     if (__any(m > top + kSlack || (top == -INFINITY && m > top))) {
       const float next = fmaxf(top, m);
       const float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - next);
@@ -193,16 +192,13 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
     const float ref = top == -INFINITY ? 0.0f : -top;
     u32x4 pf[4];
     float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
+    auto weights = [&](int u) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         f32x4 e;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const float x = s[u][4 * g + v];
-          e[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c2, ref));
-          if (c2 == 0.0f) e[v] = x == -INFINITY ? 0.0f : e[v];  // a scale of 0 keeps the mask
+          e[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][4 * g + v], c2, ref));
           sum[v & 1] += e[v];
         }
         uint32_t w0, w1;
@@ -210,11 +206,27 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
         pf[2 * u + (g >> 1)][2 * (g & 1)] = w0;
         pf[2 * u + (g >> 1)][2 * (g & 1) + 1] = w1;
       }
+    };
+    auto values = [&](int u) {
+#pragma unroll
+      for (int st = 2 * u; st < 2 * u + 2; ++st)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = mfma32<DT>(col_frag<RB>(smem, va, 16 * st, d), pf[st], o[d]);
+    };
+    weights(0);
+    __builtin_amdgcn_sched_barrier(0);
+    // the second half's exponentials among the first half's products
+    values(0);
+    weights(1);
+#pragma unroll
+    for (int x = 0; x < 2 * ND; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // fragment reads
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+      __builtin_amdgcn_sched_group_barrier(0x002, 9, 0);  // vector work
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    values(1);
     total += sum[0] + sum[1];
-#pragma unroll
-    for (int st = 0; st < 4; ++st)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] = mfma32<DT>(col_frag<RB>(smem, va, 16 * st, d), pf[st], o[d]);
   }
   wait_loads_barrier<0>();
 
