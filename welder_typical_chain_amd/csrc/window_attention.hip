@@ -161,6 +161,13 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
 #pragma unroll
       for (int st = 0; st < NS; ++st) s[u] = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u, st), qf[st], s[u]);
     }
+    __builtin_amdgcn_sched_group_barrier(0x100, 5, 0);
+#pragma unroll
+    for (int x = 0; x < 2 * NS - 5; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     if (j0 + kKeys > j1 || j0 + kKeys - 1 > w_lo || (t >= t_sink && (int64_t)j0 + p.window <= w_hi)) {
       // key j0 + 4 half + c is seen if c <= top_c and (c > low_c or c < sink_c)
       const int at = j0 + 4 * half;
@@ -218,14 +225,21 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
     // the second half's exponentials among the first half's products
     values(0);
     weights(1);
+    values(1);
+    // reads run four fragments ahead of the products that take them
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
 #pragma unroll
     for (int x = 0; x < 2 * ND; ++x) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // fragment reads
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // a fragment's reads
       __builtin_amdgcn_sched_group_barrier(0x002, 9, 0);  // vector work
     }
+#pragma unroll
+    for (int x = 0; x < 2 * ND - 4; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
     __builtin_amdgcn_sched_barrier(0);
-    values(1);
     total += sum[0] + sum[1];
   }
   wait_loads_barrier<0>();
