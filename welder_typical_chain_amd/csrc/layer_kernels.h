@@ -40,7 +40,7 @@ struct AttnBackwardPlan {
   int64_t part_at, workspace;  // bytes
 };
 AttnBackwardPlan plan_attention_backward(const AttnParams& p);
-// p.stats: plan.workspace bytes
+// p.row_lse: plan.workspace bytes
 hipError_t launch_attention_backward(const AttnParams& p, const AttnBackwardPlan& plan, int dt, hipStream_t stream);
 int plan_decode(const AttnParams& p, int cu_count);  // splits
 int64_t decode_workspace(const AttnParams& p, int splits);

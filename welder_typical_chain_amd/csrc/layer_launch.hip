@@ -374,7 +374,7 @@ int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout,
     a.o = static_cast<const uint8_t*>(out);
     a.dout = static_cast<const uint8_t*>(dout);
     a.lse_in = lse;
-    a.stats = static_cast<float2*>(workspace);
+    a.row_lse = static_cast<float*>(workspace);
     a.dq = static_cast<uint8_t*>(dq);
     a.dk = static_cast<uint8_t*>(dk);
     a.dv = static_cast<uint8_t*>(dv);

@@ -64,6 +64,16 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // of once a tile.
 constexpr float kSlack = 8.0f;
 
+// Scores in the log2 domain are c2 times the products, c2 > 0: with a negative scale
+// one operand's fragments are negated, with a scale of 0 they are zero.
+template <int NS> __device__ inline float positive_scale(float scale, u32x4 (&f)[NS]) {
+  const float c2 = scale * kLog2e;
+  if (c2 > 0.0f) return c2;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) f[s] = c2 < 0.0f ? f[s] ^ 0x80008000u : f[s] & 0u;
+  return c2 < 0.0f ? -c2 : 1.0f;
+}
+
 template <int ND, int NW> struct FwdLds {
   static constexpr int RB = row_bytes(ND), STAGES = NW == 8 ? 3 : 2;
   static constexpr int TILE = kKeys * RB, STAGE = 2 * TILE;
@@ -108,14 +118,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
 
   u32x4 qf[NS];
   load_row<NS>(p.q + 2 * (b * p.q_stride[0] + (int64_t)i * p.q_stride[1] + h * p.q_stride[2]), valid, p.dim, half, qf);
-  float c2 = p.scale * kLog2e;
-  if (!(c2 > 0.0f)) {
-    // a negative scale: the largest score is the smallest product, so negate the
-    // queries instead; a scale of 0: all scores are 0
-#pragma unroll
-    for (int s = 0; s < NS; ++s) qf[s] = c2 < 0.0f ? qf[s] ^ 0x80008000u : qf[s] & 0u;
-    c2 = c2 < 0.0f ? -c2 : 1.0f;
-  }
+  const float c2 = positive_scale<NS>(p.scale, qf);
 
   f32x16 o[ND];
 #pragma unroll
@@ -340,8 +343,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 //                          per key block, queries streamed (attention_dkv_kernel)
 // Two kernels, each recomputing S and dP (7 products instead of 5): no dq sums
 // through atomics, whose order would change the result, and no f32 dq in memory.
-// The first writes each row's (lse in the log2 domain, D) as p.stats, rows packed
-// as the tiles are: [batch][kv_heads][lq][G].
+// The first writes each row's lse (in the log2 domain) and D as p.row_lse and
+// p.row_delta, rows packed as the tiles are: [batch][kv_heads][lq][G].
 __device__ inline int64_t stats_row(const AttnParams& p, int b, int hk, int i) {
   return (((int64_t)b * p.kv_heads + hk) * p.lq + i) * p.group;
 }
@@ -399,9 +402,9 @@ template <int DT> __device__ inline void dkv_row(const AttnParams& p, int b, int
       float w = 0.0f, ds = 0.0f;
       const int i = t0 + lane;
       if (i < i1) {
-        const float2 st = p.stats[stats_row(p, b, hk, i) + x];
-        w = __builtin_amdgcn_exp2f(c2 * dot_rows<DT>(q + i * p.q_stride[1], k, p.dim) - st.x);
-        ds = p.scale * w * (dot_rows<DT>(g + i * p.do_stride[1], v, p.dim) - st.y);
+        const int64_t row = stats_row(p, b, hk, i) + x;
+        w = __builtin_amdgcn_exp2f(c2 * dot_rows<DT>(q + i * p.q_stride[1], k, p.dim) - p.row_lse[row]);
+        ds = p.scale * w * (dot_rows<DT>(g + i * p.do_stride[1], v, p.dim) - p.row_delta[row]);
       }
       for (int t = 0; t < min(64, i1 - t0); ++t) {
         const float wt = __shfl(w, t), dt = __shfl(ds, t);
@@ -470,9 +473,12 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnPara
       if (lse == -INFINITY) delta = 0.0f;
       else lse2 = lse * kLog2e;
     }
-    if (half == 0 && i < p.lq) p.stats[stats_row(p, b, hk, i) + x] = float2{lse2, delta};
+    if (half == 0 && i < p.lq) {
+      p.row_lse[stats_row(p, b, hk, i) + x] = lse2;
+      p.row_delta[stats_row(p, b, hk, i) + x] = delta;
+    }
   }
-  const float c2 = p.scale * kLog2e;
+  const float c2 = positive_scale<NS>(p.scale, qf);
 
   f32x16 dq[ND];
 #pragma unroll
@@ -515,11 +521,6 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnPara
       for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
 #pragma unroll
       for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u, st), qf[st], s);
-#pragma unroll
-      for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u + kKeys, st), gf[st], g);
-#pragma unroll
-      for (int v = 0; v < 16; ++v)
-        s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c2, -lse2)) * (g[v] - delta);
       if (k0 + 32 > j1 || k0 + 31 > w_lo || (t >= t_sink && (int64_t)k0 + p.window <= w_hi)) {
         const int at = k0 + 4 * half;
         const int top_c = min(pos, j1 - 1) - at;
@@ -528,14 +529,31 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnPara
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           const int c = 8 * (v >> 2) + (v & 3);
-          s[v] = c <= top_c && (c > low_c || c < sink_c) ? s[v] : 0.0f;
+          s[v] = c <= top_c && (c > low_c || c < sink_c) ? s[v] : -INFINITY;
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      // the exponentials among the products of dP
+#pragma unroll
+      for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u + kKeys, st), gf[st], g);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c2, -lse2));
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 32 / NS, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
       u32x4 df[2];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
+        f32x4 ds;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) ds[v] = s[4 * q + v] * (g[4 * q + v] - delta);
         uint32_t w0, w1;
-        pack4<DT>(f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]}, &w0, &w1);
+        pack4<DT>(ds, &w0, &w1);
         df[q >> 1][2 * (q & 1)] = w0;
         df[q >> 1][2 * (q & 1) + 1] = w1;
       }
@@ -605,11 +623,11 @@ constexpr int kQueries = 64;
 
 template <int ND> struct DkvLds {
   static constexpr int RB = row_bytes(ND), STAGES = 2;
-  static constexpr int TILE = kQueries * RB, STATS = 2 * TILE, STAGE = 2 * TILE + 1024;
+  static constexpr int TILE = kQueries * RB, STATS = 2 * TILE, STAGE = 2 * TILE + 2048;
   // At dim 128 the registers do not hold all of K's and V's fragments beside the
   // sums (a spilled one is loaded through vmcnt, behind the next tile's loads):
-  // the last KEPT of V's k-steps are read from LDS, 1 KiB a wave and step.
-  static constexpr int KEPT = ND == 4 ? 3 : 0, KEPT_AT = STAGES * STAGE;
+  // the last KEPT of the k-steps of V are read from LDS, 1 KiB a wave and step.
+  static constexpr int KEPT = ND == 4 ? 6 : 0, KEPT_AT = STAGES * STAGE;
   static constexpr int PITCH = ND * 128 + 16;  // bytes of a key's sums
   static constexpr int RING = KEPT_AT + 4 * KEPT * 1024, OUT = kDkvWaves * 32 * PITCH;
   static constexpr int TOTAL = (RING > OUT ? RING : OUT) + kDkvWaves * 4;
@@ -664,14 +682,14 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
     q_off[q] = (uint32_t)(2 * (row / hg * p.q_stride[1] + row % hg * p.q_stride[2])) + c;
     g_off[q] = (uint32_t)(2 * (row / hg * p.do_stride[1] + row % hg * p.do_stride[2])) + c;
   }
-  const float2* st_base = p.stats + stats_row(p, b, hk, 0);
+  const int64_t st_row = stats_row(p, b, hk, 0);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
-  const float c2 = p.scale * kLog2e;
   const int row0 = 32 * sub;
   const int steps = (i1 - i0 + tp - 1) / tp, t_all = steps * chunks;
   u32x4 kf[NS], vf[NS];
   load_row<NS>(p.k + 2 * (b * p.k_stride[0] + (int64_t)j * p.k_stride[1] + hk * p.k_stride[2]), valid, p.dim, half, kf);
   load_row<NS>(p.v + 2 * (b * p.v_stride[0] + (int64_t)j * p.v_stride[1] + hk * p.v_stride[2]), valid, p.dim, half, vf);
+  const float c2 = positive_scale<NS>(p.scale, kf);
   const uint32_t kept_at = (uint32_t)(L::KEPT_AT + (wave & 3) * L::KEPT * 1024 + lane * 16);
   if (!sub) {
 #pragma unroll
@@ -696,10 +714,12 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
       dma16(rq, in ? q_off[q] : kOutOfRange, st + q * 1024);
       dma16(rg, in ? g_off[q] : kOutOfRange, st + L::TILE + q * 1024);
     }
-    if (wave == 0) {  // the rows' (lse, D): contiguous
+    if (wave == 0) {  // the rows' lse and D: contiguous
       const int rows = min(npos * hg, hg == p.group ? kQueries : nhead);
-      const i32x4 rs = raw_rsrc(st_base + (int64_t)i * p.group + hc * hg, rows > 0 ? (uint32_t)rows * 8u : 0u);
-      dma16(rs, lane * 16, lds0 + (uint32_t)t % L::STAGES * L::STAGE + L::STATS);
+      const int64_t row = st_row + (int64_t)i * p.group + hc * hg;
+      const uint32_t bytes = rows > 0 ? (uint32_t)rows * 4u : 0u, at = lds0 + (uint32_t)t % L::STAGES * L::STAGE + L::STATS;
+      dma16(raw_rsrc(p.row_lse + row, bytes), lane * 16, at);
+      dma16(raw_rsrc(p.row_delta + row, bytes), lane * 16, at + 1024);
     }
   };
   issue(0);
@@ -726,48 +746,65 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
     for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
 #pragma unroll
     for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ra, 0, st), kf[st], s);
+    if (!all) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int row = row0 + 8 * (v >> 2) + 4 * half + (v & 3);
+        s[v] = row >= t_lo && row < t_hi ? s[v] : -INFINITY;
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // the exponentials among the products of dP
 #pragma unroll
     for (int st = 0; st < NS; ++st) {
       const int x = st - (NS - L::KEPT);
       g = mfma32<DT>(row_frag<RB>(smem, ra, kQueries, st), x < 0 ? vf[st] : *reinterpret_cast<const u32x4*>(smem + kept_at + x * 1024), g);
     }
-    __builtin_amdgcn_sched_barrier(0);
     u32x4 pf[2], df[2];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int row = row0 + 8 * q + 4 * half;
-      const f32x4 st0 = *reinterpret_cast<const f32x4*>(stt + row * 8), st1 = *reinterpret_cast<const f32x4*>(stt + row * 8 + 16);
-      const float lse[4] = {st0[0], st0[2], st1[0], st1[2]}, del[4] = {st0[1], st0[3], st1[1], st1[3]};
-      f32x4 pw, ds;
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(stt + (row0 + 8 * q + 4 * half) * 4);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        pw[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + v], c2, -lse[v]));
-        ds[v] = pw[v] * (g[4 * q + v] - del[v]);
-      }
-      if (!all) {
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const bool in = row + v >= t_lo && row + v < t_hi;
-          pw[v] = in ? pw[v] : 0.0f;
-          ds[v] = in ? ds[v] : 0.0f;
-        }
-      }
+      for (int v = 0; v < 4; ++v) s[4 * q + v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + v], c2, -lse[v]));
       uint32_t w0, w1;
-      pack4<DT>(pw, &w0, &w1);
+      pack4<DT>(f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]}, &w0, &w1);
       pf[q >> 1][2 * (q & 1)] = w0;
       pf[q >> 1][2 * (q & 1) + 1] = w1;
+    }
+#pragma unroll
+    for (int x = 0; x < NS; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 40 / NS, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // dS among the products of dv
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) dv[d] = mfma32<DT>(col_frag<RB>(smem, ca, kQueries + 16 * st, d), pf[st], dv[d]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 del = *reinterpret_cast<const f32x4*>(stt + 1024 + (row0 + 8 * q + 4 * half) * 4);
+      f32x4 ds;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) ds[v] = s[4 * q + v] * (g[4 * q + v] - del[v]);
+      uint32_t w0, w1;
       pack4<DT>(ds, &w0, &w1);
       df[q >> 1][2 * (q & 1)] = w0;
       df[q >> 1][2 * (q & 1) + 1] = w1;
+    }
+#pragma unroll
+    for (int x = 0; x < 2 * ND; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 40 / (2 * ND), 0);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int st = 0; st < 2; ++st)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        dv[d] = mfma32<DT>(col_frag<RB>(smem, ca, kQueries + 16 * st, d), pf[st], dv[d]);
-        dk[d] = mfma32<DT>(col_frag<RB>(smem, ca, 16 * st, d), df[st], dk[d]);
-      }
+      for (int d = 0; d < ND; ++d) dk[d] = mfma32<DT>(col_frag<RB>(smem, ca, 16 * st, d), df[st], dk[d]);
   }
   wait_loads_barrier<0>();
 
@@ -967,7 +1004,8 @@ AttnBackwardPlan plan_attention_backward(const AttnParams& p) {
 
 hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwardPlan& plan, int dt, hipStream_t stream) {
   AttnParams p = params;
-  p.part_far = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.stats) + plan.part_at);
+  p.part_far = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.row_lse) + plan.part_at);
+  p.row_delta = p.row_lse + (int64_t)p.batch * p.lq * p.heads;
   p.key_blocks = plan.key_blocks;
   p.far_blocks = plan.far_blocks;
   p.far_keys = plan.far_keys;
