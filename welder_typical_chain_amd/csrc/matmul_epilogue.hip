@@ -11,8 +11,8 @@
 //       transposing ds_read_b64_tr_b16 (btr_offset)
 // 4 waves in a 2 x 2 grid, each a quarter of the tile in 32 x 32 MFMA subtiles
 // (v_mfma_f32_32x32x16, D = B^T . A^T: a lane's accumulators belong to one
-// output row).  Slabs go through a ring of 4 stages filled by direct-to-LDS
-// loads, three ahead of the one whose MFMAs run; the fragments of a slab's
+// output row).  Slabs go through a ring of stages filled by direct-to-LDS
+// loads, all but one ahead of the one whose MFMAs run; the fragments of a slab's
 // second half are read while the MFMAs of the first issue, and the next
 // slab's first half under those of the second.
 #include "layer_common.h"
@@ -23,7 +23,6 @@ namespace {
 
 constexpr int kSlab = 64;    // bytes of k per ring stage and operand row
 constexpr int kSlabK = 32;   // elements
-constexpr int kStages = 4;
 constexpr int kThreads = 256;
 
 __device__ inline float load_elem(const void* p, int64_t i, int dt) {
@@ -147,9 +146,9 @@ template <bool KS, int W> struct Frags {
   }
 };
 
-template <int TM, int TN> struct TileLds {
+template <int TM, int TN, int STAGES> struct TileLds {
   static constexpr int A_STAGE = TM * kSlab, STAGE = (TM + TN) * kSlab;
-  static constexpr int RING = kStages * STAGE;
+  static constexpr int RING = STAGES * STAGE;
   // epilogue: a wave stages 32 rows of its quarter in f32
   static constexpr int PITCH = TN / 2 * 4 + 16;
   static constexpr int TOTAL = RING > 4 * 32 * PITCH ? RING : 4 * 32 * PITCH;
@@ -158,9 +157,9 @@ template <int TM, int TN> struct TileLds {
 
 // Grid: tiles * splits; split s takes k-slabs [s * slabs, (s + 1) * slabs) and, where
 // there are several, writes f32 partial products [split][m][n] to p.partial.
-template <int DT, int OUT_DT, bool AKS, bool BKS, int TM, int TN>
-__global__ void __launch_bounds__(kThreads, TM == 256 ? 1 : 2) matmul_tile_kernel(const MatmulParams p) {
-  using L = TileLds<TM, TN>;
+template <int DT, int OUT_DT, bool AKS, bool BKS, int TM, int TN, int STAGES>
+__global__ void __launch_bounds__(kThreads, (TM + TN) * kSlab * STAGES > 80 * 1024 ? 1 : 2) matmul_tile_kernel(const MatmulParams p) {
+  using L = TileLds<TM, TN, STAGES>;
   constexpr int WM = TM / 64, WN = TN / 64;
   __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
   const int lane = threadIdx.x & 63;
@@ -192,57 +191,66 @@ __global__ void __launch_bounds__(kThreads, TM == 256 ? 1 : 2) matmul_tile_kerne
   Frags<BKS, WN> fb;
   fa.init(0, wm * (TM / 2), lane);
   fb.init(L::A_STAGE, wn * (TN / 2), lane);
-  constexpr int NA = Loader<AKS, TM>::NB, LOADS = NA + Loader<BKS, TN>::NB;
+  constexpr int NA = Loader<AKS, TM>::NB, NB = Loader<BKS, TN>::NB, LOADS = NA + NB, ALT = 2 * (NA < NB ? NA : NB);
   constexpr int RA = Frags<AKS, WM>::READS, R = RA + Frags<BKS, WN>::READS;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
   auto load = [&](uint32_t stage, int kt, int j) {
-    // A and B blocks alternate
-    if (j & 1) lb.issue(stage + L::A_STAGE, kt0 + kt, k_end, j >> 1);
-    else la.issue(stage, kt0 + kt, k_end, j >> 1);
+    // A and B blocks alternate, then what is left of the larger one
+    const bool of_a = j < ALT ? !(j & 1) : NA > NB;
+    const int q = j < ALT ? j >> 1 : j - ALT / 2;
+    if (of_a) la.issue(stage, kt0 + kt, k_end, q);
+    else lb.issue(stage + L::A_STAGE, kt0 + kt, k_end, q);
   };
-  static_assert(NA * 2 == LOADS, "square tiles");
   auto read = [&](const uint8_t* st, int s, int u, u32x4 (&a)[WM], u32x4 (&b)[WN]) {
     if (u < RA) fa.read(st, s, u, a);
-    else if (u < R) fb.read(st, s, u - RA, b);
+    else fb.read(st, s, u - RA, b);
   };
-  constexpr int RG = (R + WM - 1) / WM, LG = LOADS / WM;  // reads and loads per group of MFMAs
+  // Of `total` things, those that go with MFMA x of a part.
+  constexpr int M = WM * WN;
+  auto first = [](int total, int x) { return total * x / M; };
   if (nk > 0) {
 #pragma unroll
-    for (int q = 0; q < kStages; ++q)
+    for (int q = 0; q < STAGES; ++q)
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) load(lds0 + q * L::STAGE, q, j);
-    wait_loads_barrier<LOADS*(kStages - 1)>();
+    wait_loads_barrier<LOADS*(STAGES - 1)>();
     u32x4 a0[WM], b0[WN], a1[WM], b1[WN];
 #pragma unroll
     for (int u = 0; u < R; ++u) read(smem, 0, u, a0, b0);
+    int stage = 0;
     for (int kt = 0; kt < nk; ++kt) {
-      const uint8_t* cur = smem + (kt % kStages) * L::STAGE;
-      const uint8_t* nxt = smem + ((kt + 1) % kStages) * L::STAGE;
-      const uint32_t fill = lds0 + (kt % kStages) * L::STAGE;
+      const int next = stage + 1 == STAGES ? 0 : stage + 1;
+      const uint8_t* cur = smem + stage * L::STAGE;
+      const uint8_t* nxt = smem + next * L::STAGE;
+      const uint32_t fill = lds0 + stage * L::STAGE;
+      stage = next;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < WM; ++g) {
 #pragma unroll
-        for (int u = 0; u < RG; ++u) read(cur, 1, RG * g + u, a1, b1);
+        for (int u = first(R, g * WN); u < first(R, (g + 1) * WN); ++u) read(cur, 1, u, a1, b1);
 #pragma unroll
         for (int j = 0; j < WN; ++j) acc[g][j] = mfma32<DT>(b0[j], a0[g], acc[g][j]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      wait_loads_barrier<LOADS*(kStages - 2)>();  // slab kt+1 landed; slab kt read
+      wait_loads_barrier<LOADS*(STAGES - 2)>();  // slab kt+1 landed; slab kt read
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < WM; ++g) {
 #pragma unroll
         for (int j = 0; j < WN; ++j) {
+          // each load right behind an MFMA, in the first half of a group
           acc[g][j] = mfma32<DT>(b1[j], a1[g], acc[g][j]);
-          if (j < LG) {  // each load right behind an MFMA
+          constexpr int H = WN / 2;
+          if (j < H) {
             __builtin_amdgcn_sched_barrier(0);
-            load(fill, kt + kStages, LG * g + j);
+#pragma unroll
+            for (int x = LOADS * (g * H + j) / (WM * H); x < LOADS * (g * H + j + 1) / (WM * H); ++x) load(fill, kt + STAGES, x);
             __builtin_amdgcn_sched_barrier(0);
           }
-          if (j == LG - 1) {
+          if (j == H - 1) {
 #pragma unroll
-            for (int u = 0; u < RG; ++u) read(nxt, 0, RG * g + u, a0, b0);
+            for (int u = first(R, g * WN); u < first(R, (g + 1) * WN); ++u) read(nxt, 0, u, a0, b0);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -300,6 +308,7 @@ __global__ void __launch_bounds__(256) matmul_join_kernel(const MatmulParams p) 
   if (at >= total) return;
   float z[8], y[8];
   load8<DT_F32>(p.partial, at, z);
+#pragma unroll 4
   for (int s = 1; s < p.splits; ++s) {
     load8<DT_F32>(p.partial, s * total + at, y);
 #pragma unroll
@@ -360,7 +369,13 @@ __global__ void __launch_bounds__(256) sum_chunks_kernel(const ActBackwardParams
   const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (j >= p.n) return;
   float s = 0.0f;
-  for (int c = 0; c < p.chunks; ++c) s += p.partial[c * p.n + j];
+  for (int c = 0; c < p.chunks; c += 16) {  // 16 loads at a time, added in their order
+    float x[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) x[u] = c + u < p.chunks ? p.partial[(c + u) * p.n + j] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) s += x[u];
+  }
   p.dbias[j] = s;
 }
 
@@ -370,36 +385,60 @@ template <typename P> hipError_t run(const void* fn, int64_t grid, int threads, 
   return hipLaunchKernel(fn, dim3((unsigned)grid), dim3(threads), args, 0, stream);
 }
 
-template <int DT, int OUT_DT, int T> const void* tile_by_kind(bool aks, bool bks) {
-  if (aks) return (const void*)&matmul_tile_kernel<DT, DT, true, true, T, T>;  // db: out is of the input type
-  return bks ? (const void*)&matmul_tile_kernel<DT, OUT_DT, false, true, T, T>
-             : (const void*)&matmul_tile_kernel<DT, OUT_DT, false, false, T, T>;
+template <int DT, int OUT_DT, int TM, int TN, int S> const void* tile_by_kind(bool aks, bool bks) {
+  if constexpr (TM > 64)
+    if (aks) return (const void*)&matmul_tile_kernel<DT, DT, true, true, TM, TN, S>;  // db: out is of the input type
+  return bks ? (const void*)&matmul_tile_kernel<DT, OUT_DT, false, true, TM, TN, S>
+             : (const void*)&matmul_tile_kernel<DT, OUT_DT, false, false, TM, TN, S>;
 }
-template <int DT, int OUT_DT> const void* tile_by_size(int tile, bool aks, bool bks) {
-  return tile == 256 ? tile_by_kind<DT, OUT_DT, 256>(aks, bks) : tile_by_kind<DT, OUT_DT, 128>(aks, bks);
+template <int DT, int OUT_DT> const void* tile_by_size(int v, bool aks, bool bks) {
+  switch (v) {
+    case 0: return tile_by_kind<DT, OUT_DT, 256, 256, 4>(aks, bks);
+    case 1: return tile_by_kind<DT, OUT_DT, 256, 128, 6>(aks, bks);
+    case 2: return tile_by_kind<DT, OUT_DT, 128, 128, 4>(aks, bks);
+  }
+  return tile_by_kind<DT, OUT_DT, 64, 128, 6>(aks, bks);
 }
+
+// The tile kernels and what they take, in us (read off graph replays of 14 shapes
+// from 8 x 4096 x 4096 to 8192 x 8192 x 4096, the three operand kinds, every
+// tile with 1 to 16 splits): a slab of 32 k on a CU, more with every CU busy
+// (the clock falls), and what a round of tiles costs besides.
+//   256 x 256 is the fastest per product where its tiles fill the chip (8192 x
+//   8192 x 4096: 465 us, 256 x 128 550, 128 x 128 580); 256 x 128 where those
+//   are half of the chip (4096 x 2048 x 4096: 72, against 92 and 78); 128 x 128
+//   for smaller products, one or two workgroups a CU (2048 x 2048 x 1024: 15,
+//   against 30 and 21); 64 x 128 for few rows (8 x 4096 x 4096 in 8 splits:
+//   11.2, 128 x 128 12.2).
+struct Variant {
+  int tm, tn;
+  double slab_us, busy_us, fixed_us;
+};
+constexpr Variant kVariants[] = {{256, 256, 0.58, 0.34, 10.0}, {256, 128, 0.34, 0.19, 7.0}, {128, 128, 0.28, 0.0, 5.0}, {64, 128, 0.22, 0.0, 3.5}};
+constexpr int kFewRows = 64;  // at most so many rows for the 64-row tile
 
 }  // namespace
 
-// The tile and the number of k-splits: as many workgroups as the chip holds at
-// once (256 of the large tile, 512 of the small one), each with at least 8 slabs.
-MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, int cu_count) {
+// The tile and the number of k-splits with the least estimate.  Splits cost a second
+// kernel (3.5 us) and their partial products' way to memory and back (6 TB/s).
+MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, bool aks, int cu_count) {
   MatmulPlan best{};
   double best_us = 0;
   const int64_t slabs = (k + kSlabK - 1) / kSlabK;
-  for (int tile : {256, 128}) {
-    const int64_t tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
-    const int64_t slots = tile == 256 ? cu_count : 2 * cu_count;
+  for (int v = 0; v < 4; ++v) {
+    const Variant& t = kVariants[v];
+    if (t.tm == 64 && (m > kFewRows || aks)) continue;
+    const int64_t tiles = ((m + t.tm - 1) / t.tm) * ((n + t.tn - 1) / t.tn);
     for (int64_t s = 1; s <= 16 && (s == 1 || slabs / s >= 4); s *= 2) {
       const int64_t per = (slabs + s - 1) / s;
       const int64_t splits = per ? (slabs + per - 1) / per : 1;
-      const int64_t waves = (tiles * splits + slots - 1) / slots;
-      const double slab_us = tile == 256 ? 0.62 : 0.40;
-      double us = waves * (per * slab_us + (tile == 256 ? 6.0 : 3.0));
-      if (splits > 1) us += 4.0 + (double)m * n * 4 * (splits + 1) * 2 / 4.0e6;
+      const int64_t groups = tiles * splits, full = groups / cu_count, rest = groups % cu_count;
+      double us = t.fixed_us + (double)(full * per) * (t.slab_us + t.busy_us);
+      if (rest) us += (double)per * (t.slab_us + t.busy_us * (double)rest / cu_count);
+      if (splits > 1) us += 3.5 + 2.0 * (double)(splits * m * n) * 4 / 6.0e6;
       if (best_us == 0 || us < best_us) {
         best_us = us;
-        best = MatmulPlan{tile, (int)splits, (int)per};
+        best = MatmulPlan{v, (int)splits, (int)per};
       }
     }
   }
@@ -414,10 +453,11 @@ hipError_t launch_matmul(const MatmulParams& params, const MatmulPlan& plan, int
   MatmulParams p = params;
   p.splits = plan.splits;
   p.slabs = plan.slabs;
-  const int64_t grid = ((int64_t)(p.m + plan.tile - 1) / plan.tile) * ((p.n + plan.tile - 1) / plan.tile) * p.splits;
+  const Variant& v = kVariants[plan.variant];
+  const int64_t grid = ((int64_t)(p.m + v.tm - 1) / v.tm) * ((p.n + v.tn - 1) / v.tn) * p.splits;
   const bool f32 = out_dt == DT_F32;
-  const void* fn = dt == DT_F16 ? (f32 ? tile_by_size<DT_F16, DT_F32>(plan.tile, aks, bks) : tile_by_size<DT_F16, DT_F16>(plan.tile, aks, bks))
-                                : (f32 ? tile_by_size<DT_BF16, DT_F32>(plan.tile, aks, bks) : tile_by_size<DT_BF16, DT_BF16>(plan.tile, aks, bks));
+  const void* fn = dt == DT_F16 ? (f32 ? tile_by_size<DT_F16, DT_F32>(plan.variant, aks, bks) : tile_by_size<DT_F16, DT_F16>(plan.variant, aks, bks))
+                                : (f32 ? tile_by_size<DT_BF16, DT_F32>(plan.variant, aks, bks) : tile_by_size<DT_BF16, DT_BF16>(plan.variant, aks, bks));
   const hipError_t e = run(fn, grid, kThreads, p, stream);
   if (e != hipSuccess || p.splits == 1) return e;
   fn = dt == DT_F16 ? (f32 ? (const void*)&matmul_join_kernel<DT_F16, DT_F32> : (const void*)&matmul_join_kernel<DT_F16, DT_F16>)

@@ -993,8 +993,8 @@ AttnBackwardPlan plan_attention_backward(const AttnParams& p) {
   if (p.sinks > 0 && far > 0) {
     plan.far_blocks = (p.sinks + kDkvKeys - 1) / kDkvKeys;
     plan.far_keys = std::min(p.sinks, kDkvKeys);
-    // short ones, in the end of the key blocks' round: 64 positions or a key block's share
-    plan.far_chunks = (int)std::max<int64_t>(1, std::min<int64_t>(plan.key_blocks, far / 64));
+    // short ones, in the end of the key blocks' round: 256 positions or a key block's share
+    plan.far_chunks = (int)std::max<int64_t>(1, std::min<int64_t>(plan.key_blocks, far / 256));
   }
   const int64_t rows = (int64_t)p.batch * p.lq * p.heads;
   plan.part_at = (rows * 8 + 255) / 256 * 256;
