@@ -26,20 +26,26 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 # The C structs are eight-byte fields throughout, packed here into bytes.
 _pack_matmul = struct.Struct("13q").pack
 _pack_attention = struct.Struct("28q2qd").pack
+_SIZES_END = 28 * 8  # where sizes and strides end: addresses and the scale follow
 
 
+# A decode step's kernels take 5 to 10 us, less than a careless host call, so
+# the helpers read each property of a tensor once and build no intermediate
+# objects: 17 -> HOST_US us on the host for a window_attention_decode.
 def _check_inputs(dtype, *named):
+    """Device index of the tensors (None among them are skipped), all of `dtype` if it is given."""
     grad = torch.is_grad_enabled()
-    device = None
+    device = -2
     for name, t in named:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be on the GPU")
-        if device is None:
-            device = t.get_device()
-        elif t.get_device() != device:
-            raise ValueError(f"{name} is on another device")
+        at = t.get_device()  # -1 on the CPU
+        if at != device:
+            if at < 0:
+                raise ValueError(f"{name} must be on the GPU")
+            if device >= 0:
+                raise ValueError(f"{name} is on another device")
+            device = at
         if dtype is not None and t.dtype != dtype:
             raise TypeError(f"{name} must be {dtype}, is {t.dtype}")
         if grad and t.requires_grad:
@@ -60,10 +66,21 @@ def _launch(device, fn, *args):
         _lib.check(rc)
 
 
-def _scratch(size, device):
-    """(tensor, pointer, bytes) of a workspace; none for size 0."""
-    if size < 0:
-        _lib.check(_lib.WTC_ERR_ARG)
+_sizes: dict = {}  # (function, arguments without addresses) -> bytes
+
+
+def _scratch(name, args, device, keyed=None):
+    """(tensor, pointer, bytes) of a call's workspace; none for size 0."""
+    key = (name, device, args if keyed is None else args[:keyed])
+    size = _sizes.get(key)
+    if size is None:
+        with torch.cuda.device(device):  # the plan goes by its compute units
+            size = getattr(_lib.lib(), name)(args)
+        if size < 0:
+            _lib.check(_lib.WTC_ERR_ARG)
+        if len(_sizes) >= 4096:
+            _sizes.clear()
+        _sizes[key] = size
     if size == 0:
         return None, None, 0
     t = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", device))
@@ -129,46 +146,48 @@ def matmul_epilogue(a: torch.Tensor, b: torch.Tensor, *, bias: torch.Tensor | No
     needs for an activation (rounded to 16 bits it would move dbias by 5e-4).
     """
     code = _code_of(a, "a")
-    k = a.shape[-1] if a.dim() else 0
-    if a.dim() < 1:
+    a_shape = a.shape
+    if not a_shape:
         raise ValueError("a must have at least one dimension")
-    lead = a.shape[:-1]
-    a2 = a if a.dim() == 2 else a.reshape(-1, k) if a.numel() else a.new_empty((lead.numel(), k))
+    k = a_shape[-1]
+    flat = len(a_shape) == 2
+    a2 = a if flat else a.reshape(-1, k) if a.numel() else a.new_empty((a_shape[:-1].numel(), k))
     m = a2.shape[0]
     n, ldb, trans = _weights(b, k)
     device = _check_inputs(None, ("a", a), ("b", b), ("bias", bias), ("residual", residual), ("out", out))
-    if b.dtype != a.dtype:
+    dtype = a.dtype
+    if b.dtype != dtype:
         raise TypeError("a and b must have the same element type")
     act = _activation(activation)
     if out_dtype is None:
-        out_dtype = a.dtype if out is None else out.dtype
-    if out_dtype not in (a.dtype, torch.float32):
-        raise TypeError(f"out_dtype must be {a.dtype} or float32")
-    shape = lead + (n,)
+        out_dtype = dtype if out is None else out.dtype
+    if out_dtype != dtype and out_dtype != torch.float32:
+        raise TypeError(f"out_dtype must be {dtype} or float32")
+    shape = (m, n) if flat else (*a_shape[:-1], n)
     if out is None:
         out = torch.empty(shape, dtype=out_dtype, device=a.device)
     elif out.shape != shape or out.dtype != out_dtype:
         raise ValueError("out has the wrong shape or dtype")
-    out2 = out if out.dim() == 2 else out.view(-1, n) if out.numel() else out.new_empty((m, n))
+    out2 = out if flat else out.view(-1, n) if out.numel() else out.new_empty((m, n))
     bias_code = code
     if bias is not None:
         if bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
             raise ValueError(f"bias must be a contiguous [{n}]")
-        if bias.dtype not in (a.dtype, torch.float32):
-            raise TypeError(f"bias must be {a.dtype} or float32")
+        if bias.dtype != dtype and bias.dtype != torch.float32:
+            raise TypeError(f"bias must be {dtype} or float32")
         bias_code = _FLOATS[bias.dtype]
     ldo = ldr = _row_stride(out2, "out")
     if residual is not None:
         if residual.shape != shape or residual.dtype != out_dtype:
             raise ValueError(f"residual must be {tuple(shape)} of {out_dtype}")
-        r2 = residual if residual.dim() == 2 else residual.reshape(-1, n) if residual.numel() else out2
+        r2 = residual if flat else residual.reshape(-1, n) if residual.numel() else out2
         ldr = _row_stride(r2, "residual")
         residual = r2
     pre = torch.empty(shape, dtype=torch.float32, device=a.device) if return_pre else None
     lib = _lib.lib()
     args = _pack_matmul(m, n, k, _row_stride(a2, "a"), ldb, ldr, ldo, trans, code, _FLOATS[out_dtype], bias_code,
                         act, n)
-    ws, ws_ptr, ws_bytes = _scratch(lib.wtc_matmul_epilogue_workspace_size(args), device)
+    ws, ws_ptr, ws_bytes = _scratch("wtc_matmul_epilogue_workspace_size", args, device)
     _launch(device, lib.wtc_matmul_epilogue, args, a2.data_ptr(), b.data_ptr(), _ptr(bias), _ptr(residual),
             out2.data_ptr(), _ptr(pre), ws_ptr, ws_bytes)
     return (out, pre) if return_pre else out
@@ -210,7 +229,7 @@ def matmul_epilogue_backward(dout: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     lib = _lib.lib()
     args = _pack_matmul(m, n, k, _row_stride(a2, "a"), ldb, n, n, trans, code, code, code, act,
                         _row_stride(d2, "dout"))
-    ws, ws_ptr, ws_bytes = _scratch(lib.wtc_matmul_epilogue_backward_workspace_size(args), device)
+    ws, ws_ptr, ws_bytes = _scratch("wtc_matmul_epilogue_backward_workspace_size", args, device)
     _launch(device, lib.wtc_matmul_epilogue_backward, args, d2.data_ptr(), a2.data_ptr(), b.data_ptr(),
             _ptr(pre) if act else None, _ptr(da), _ptr(db), _ptr(dbias), ws_ptr, ws_bytes)
     return da, db.t() if trans and db is not None else db, dbias
@@ -218,16 +237,26 @@ def matmul_epilogue_backward(dout: torch.Tensor, a: torch.Tensor, b: torch.Tenso
 
 def _strides(t, name):
     """Strides of [batch, tokens, heads, dim], dim contiguous; dimensions of one element get a harmless one."""
-    s = t.stride()
-    if t.shape[3] > 1 and s[3] != 1:
+    n0, n1, n2, n3 = t.shape
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 and n3 > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    return tuple(s[i] if t.shape[i] > 1 else 0 for i in range(3))
+    return s0 if n0 > 1 else 0, s1 if n1 > 1 else 0, s2 if n2 > 1 else 0
+
+
+def _row_strides(t, name):
+    """_strides of [batch, heads, dim]: sequence, token (one), head."""
+    n0, n1, n2 = t.shape
+    s0, s1, s2 = t.stride()
+    if s2 != 1 and n2 > 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    return s0 if n0 > 1 else 0, 0, s1 if n1 > 1 else 0
 
 
 def _lens(t, batch, name, device):
     if t is None:
         return 0
-    if t.dtype != torch.int32 or t.shape != (batch,) or not t.is_cuda or t.get_device() != device or \
+    if t.dtype != torch.int32 or t.shape != (batch,) or t.get_device() != device or \
             (batch > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be a contiguous int32 [{batch}] on the tensors' device")
     return t.data_ptr()
@@ -242,12 +271,13 @@ def _mask(window, sinks):
 
 
 def _attention_args(q, k, v, window, sinks, scale, q_lens, k_lens, device):
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+    k_shape = k.shape
+    if q.dim() != 4 or len(k_shape) != 4 or v.shape != k_shape:
         raise ValueError("q must be [B, Lq, H, D], k and v [B, Lk, Hkv, D]")
     b, lq, h, d = q.shape
-    lk, kv = k.shape[1], k.shape[2]
-    if k.shape[0] != b or k.shape[3] != d or kv == 0 or h % kv:
-        raise ValueError(f"shape mismatch: q {tuple(q.shape)} k {tuple(k.shape)}")
+    bk, lk, kv, dk = k_shape
+    if bk != b or dk != d or kv == 0 or h % kv:
+        raise ValueError(f"shape mismatch: q {tuple(q.shape)} k {tuple(k_shape)}")
     w, s = _mask(window, sinks)
     return (b, h, kv, lq, lk, d, w, s, _code_of(q, "q"), *_strides(q, "q"), *_strides(k, "k"),
             *_strides(v, "v")), (_lens(q_lens, b, "q_lens", device), _lens(k_lens, b, "k_lens", device),
@@ -283,7 +313,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if return_lse else None
     args = _pack_attention(*head, *_strides(out, "out"), 0, 0, 0, 0, 0, 0, 0, *tail)
     lib = _lib.lib()
-    ws, ws_ptr, ws_bytes = _scratch(lib.wtc_window_attention_workspace_size(args), device)
+    ws, ws_ptr, ws_bytes = _scratch("wtc_window_attention_workspace_size", args, device, _SIZES_END)
     _launch(device, lib.wtc_window_attention, args, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
             _ptr(lse), ws_ptr, ws_bytes)
     return (out, lse) if return_lse else out
@@ -310,7 +340,7 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     lib = _lib.lib()
     args = _pack_attention(*head, *_strides(out, "out"), *_strides(dout, "dout"), 0, 0, 0, 0, *tail)
-    ws, ws_ptr, ws_bytes = _scratch(lib.wtc_window_attention_backward_workspace_size(args), device)
+    ws, ws_ptr, ws_bytes = _scratch("wtc_window_attention_backward_workspace_size", args, device, _SIZES_END)
     _launch(device, lib.wtc_window_attention_backward, args, dout.data_ptr(), q.data_ptr(), k.data_ptr(),
             v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws_ptr,
             ws_bytes)
@@ -332,30 +362,34 @@ def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     k_new, v_new: [B, Hkv, D], the new token's key and value, written to the
     caches in the same pass; without them the caches hold it already.
     """
-    if q.dim() != 3 or k_cache.dim() != 4:
+    shape, cache = q.shape, k_cache.shape
+    if len(shape) != 3 or len(cache) != 4 or v_cache.shape != cache:
         raise ValueError("q must be [B, H, D], the caches [B, C, Hkv, D]")
     device = _check_inputs(q.dtype, ("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("k_new", k_new),
                            ("v_new", v_new), ("out", out))
     if lengths is None:
         raise ValueError("lengths must be given")
-    q4 = q.unsqueeze(1)
-    head, tail = _attention_args(q4, k_cache, v_cache, window, sinks, scale, None, lengths, device)
-    b, _, kv, d = k_cache.shape
+    b, h, d = shape
+    bk, cap, kv, dk = cache
+    if bk != b or dk != d or kv == 0 or h % kv:
+        raise ValueError(f"shape mismatch: q {tuple(shape)} caches {tuple(cache)}")
+    w, s = _mask(window, sinks)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != shape:
         raise ValueError("out must have q's shape")
-    new = (0, 0, 0, 0)
-    if (k_new is None) != (v_new is None):
-        raise ValueError("k_new and v_new go together")
-    if k_new is not None:
+    kn = vn = (0, 0, 0)
+    if k_new is not None and v_new is not None:
         if k_new.shape != (b, kv, d) or v_new.shape != (b, kv, d):
             raise ValueError(f"k_new and v_new must be {(b, kv, d)}")
-        kn, vn = _strides(k_new.unsqueeze(1), "k_new"), _strides(v_new.unsqueeze(1), "v_new")
-        new = (kn[0], kn[2], vn[0], vn[2])
-    lib = _lib.lib()
-    args = _pack_attention(*head, *_strides(out.unsqueeze(1), "out"), 0, 0, 0, *new, *tail)
-    ws, ws_ptr, ws_bytes = _scratch(lib.wtc_window_attention_decode_workspace_size(args), device)
-    _launch(device, lib.wtc_window_attention_decode, args, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            _ptr(k_new), _ptr(v_new), out.data_ptr(), ws_ptr, ws_bytes)
+        kn, vn = _row_strides(k_new, "k_new"), _row_strides(v_new, "v_new")
+    elif k_new is not v_new:
+        raise ValueError("k_new and v_new go together")
+    args = _pack_attention(b, h, kv, 1, cap, d, w, s, _code_of(q, "q"), *_row_strides(q, "q"),
+                           *_strides(k_cache, "k_cache"), *_strides(v_cache, "v_cache"), *_row_strides(out, "out"),
+                           0, 0, 0, kn[0], kn[2], vn[0], vn[2], 0, _lens(lengths, b, "lengths", device),
+                           d ** -0.5 if scale is None else float(scale))
+    ws, ws_ptr, ws_bytes = _scratch("wtc_window_attention_decode_workspace_size", args, device, _SIZES_END)
+    _launch(device, _lib.lib().wtc_window_attention_decode, args, q.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), _ptr(k_new), _ptr(v_new), out.data_ptr(), ws_ptr, ws_bytes)
     return out
