@@ -15,6 +15,8 @@
 // loads, all but one ahead of the one whose MFMAs run; the fragments of a slab's
 // second half are read while the MFMAs of the first issue, and the next
 // slab's first half under those of the second.
+#include <type_traits>
+
 #include "layer_common.h"
 #include "layer_kernels.h"
 
@@ -260,44 +262,96 @@ __global__ void __launch_bounds__(kThreads, (TM + TN) * kSlab * STAGES > 80 * 10
   }
 
   // ---- epilogue: each wave by itself, 32 rows at a time through its part of LDS,
-  // from a row a lane to eight columns a lane
-  constexpr int CW = TN / 2, LPR = CW / 8, RPI = 64 / LPR;
+  // from a row a lane to eight columns a lane.  A lane's columns are the same in
+  // every step, so the bias is read once; the residual of the next 32 rows is
+  // requested before the current ones are worked on (loaded where it is added,
+  // its latency made up a third of a product with k = 1000: 33.8 -> RES_US us).
+  constexpr int CW = TN / 2, LPR = CW / 8, RPI = 64 / LPR, ITS = 32 / RPI;
   uint8_t* stg = smem + wave * 32 * L::PITCH;
-  auto epilogue = [&](auto finish) {
+  const int c = lane % LPR * 8;
+  const int64_t m0 = (int64_t)row0 + wm * (TM / 2) + lane / LPR, n = (int64_t)n0 + wn * CW + c;
+  auto stage = [&](int mt) {
+#pragma unroll
+    for (int j = 0; j < WN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(stg + acc_j(lane) * L::PITCH + (j * 32 + acc_i(lane, 4 * g)) * 4) =
+            f32x4{acc[mt][j][4 * g], acc[mt][j][4 * g + 1], acc[mt][j][4 * g + 2], acc[mt][j][4 * g + 3]};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  auto staged = [&](int it, float (&z)[8]) {
+    const f32x4* src = reinterpret_cast<const f32x4*>(stg + (it * RPI + lane / LPR) * L::PITCH + c * 4);
+    const f32x4 lo = src[0], hi = src[1];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) z[u] = lo[u], z[4 + u] = hi[u];
+  };
+  if (p.splits > 1) {
+    float* part = p.partial + (int64_t)split * p.m * p.n;
 #pragma unroll
     for (int mt = 0; mt < WM; ++mt) {
+      stage(mt);
 #pragma unroll
-      for (int j = 0; j < WN; ++j)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(stg + acc_j(lane) * L::PITCH + (j * 32 + acc_i(lane, 4 * g)) * 4) =
-              f32x4{acc[mt][j][4 * g], acc[mt][j][4 * g + 1], acc[mt][j][4 * g + 2], acc[mt][j][4 * g + 3]};
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 2
-      for (int it = 0; it < 32 / RPI; ++it) {
-        const int r = it * RPI + lane / LPR, c = lane % LPR * 8;
-        const int64_t m = (int64_t)row0 + wm * (TM / 2) + mt * 32 + r, n = (int64_t)n0 + wn * CW + c;
+      for (int it = 0; it < ITS; ++it) {
+        const int64_t m = m0 + mt * 32 + it * RPI;
         float z[8];
-        const f32x4* src = reinterpret_cast<const f32x4*>(stg + r * L::PITCH + c * 4);
-        const f32x4 lo = src[0], hi = src[1];
+        staged(it, z);
+        if (m < p.m && n < p.n) store8<DT_F32>(part, m * p.n + n, z);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    return;
+  }
+  constexpr int RV = OUT_DT == DT_F32 ? 2 : 1;  // 16-byte words of eight values
+  const int64_t n_in = n < p.n ? n : 0;
+  float bias[8] = {};
+  if (p.bias) {
+    if (p.bias_f32) load8<DT_F32>(p.bias, n_in, bias);
+    else load8<DT>(p.bias, n_in, bias);
+  }
+  u32x4 res[2][ITS][RV];
+  auto request = [&](int mt) {
+    if (!p.residual) return;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) z[u] = lo[u], z[4 + u] = hi[u];
-        if (m < p.m && n < p.n) finish(m, n, z);
+    for (int it = 0; it < ITS; ++it) {
+      const int64_t m = min(m0 + mt * 32 + it * RPI, (int64_t)p.m - 1);
+      const u32x4* src = reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(p.residual) + (m * p.ldr + n_in) * dtype_bytes(OUT_DT));
+#pragma unroll
+      for (int w = 0; w < RV; ++w) res[mt & 1][it][w] = src[w];
+    }
+  };
+  auto epilogue = [&](auto act) {
+    request(0);
+#pragma unroll
+    for (int mt = 0; mt < WM; ++mt) {
+      if (mt + 1 < WM) request(mt + 1);
+      stage(mt);
+#pragma unroll
+      for (int it = 0; it < ITS; ++it) {
+        const int64_t m = m0 + mt * 32 + it * RPI;
+        float z[8], y[8];
+        staged(it, z);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) z[u] += bias[u];
+        const bool in = m < p.m && n < p.n;
+        if (p.pre && in) store8<DT_F32>(p.pre, m * p.ldp + n, z);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) z[u] = act_value<decltype(act)::value>(z[u]);
+        if (p.residual) {
+          load8<OUT_DT>(res[mt & 1][it], 0, y);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) z[u] += y[u];
+        }
+        if (in) store8<OUT_DT>(p.out, m * p.ldo + n, z);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
   };
-  if (p.splits > 1) {
-    float* part = p.partial + (int64_t)split * p.m * p.n;
-    epilogue([&](int64_t m, int64_t n, float (&z)[8]) { store8<DT_F32>(part, m * p.n + n, z); });
-    return;
-  }
   switch (p.act) {
-    case WTC_ACT_NONE: return epilogue([&](int64_t m, int64_t n, float (&z)[8]) { finish8<DT, OUT_DT, WTC_ACT_NONE>(p, m, n, z); });
-    case WTC_ACT_RELU: return epilogue([&](int64_t m, int64_t n, float (&z)[8]) { finish8<DT, OUT_DT, WTC_ACT_RELU>(p, m, n, z); });
-    case WTC_ACT_GELU: return epilogue([&](int64_t m, int64_t n, float (&z)[8]) { finish8<DT, OUT_DT, WTC_ACT_GELU>(p, m, n, z); });
-    case WTC_ACT_GELU_TANH: return epilogue([&](int64_t m, int64_t n, float (&z)[8]) { finish8<DT, OUT_DT, WTC_ACT_GELU_TANH>(p, m, n, z); });
-    case WTC_ACT_SILU: return epilogue([&](int64_t m, int64_t n, float (&z)[8]) { finish8<DT, OUT_DT, WTC_ACT_SILU>(p, m, n, z); });
+    case WTC_ACT_NONE: return epilogue(std::integral_constant<int, WTC_ACT_NONE>{});
+    case WTC_ACT_RELU: return epilogue(std::integral_constant<int, WTC_ACT_RELU>{});
+    case WTC_ACT_GELU: return epilogue(std::integral_constant<int, WTC_ACT_GELU>{});
+    case WTC_ACT_GELU_TANH: return epilogue(std::integral_constant<int, WTC_ACT_GELU_TANH>{});
+    case WTC_ACT_SILU: return epilogue(std::integral_constant<int, WTC_ACT_SILU>{});
   }
 }
 
