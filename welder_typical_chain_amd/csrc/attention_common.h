@@ -99,6 +99,22 @@ template <int NS> __device__ inline void load_row(const uint8_t* row, bool valid
   }
 }
 
+// Masks as bits, a lane's own: bit c of bits_below(n) is set for c < n.  One bit
+// then costs an element two vector instructions; compares would go through scalar
+// masks, three to an element and each waiting for the last.
+__device__ inline uint64_t bits_below(int64_t n) {
+  return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+}
+__device__ inline float keep_bit(float x, uint64_t bits, int c) {  // x, or -inf where bit c is clear
+  const uint32_t w = c < 32 ? (uint32_t)bits : (uint32_t)(bits >> 32);
+  const uint32_t in = (uint32_t)__builtin_amdgcn_sbfe((int)w, c & 31, 1);
+  return __builtin_bit_cast(float, (in & __builtin_bit_cast(uint32_t, x)) | (~in & 0xFF800000u));
+}
+// Of the 64 keys from j on, those below `end` that a query at `pos` sees.
+__device__ inline uint64_t seen_bits(int64_t j, int64_t end, int64_t pos, int64_t window, int64_t sinks) {
+  return bits_below(min(pos + 1, end) - j) & (~bits_below(pos - window + 1 - j) | bits_below(sinks - j));
+}
+
 // Keys that the query at position `pos` sees: the first `first` ones and then lo .. pos.
 struct Seen {
   int lo, first, count;
@@ -123,6 +139,39 @@ __device__ inline float wave_max(float x) {
 __device__ inline float wave_sum(float x) {
   for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
   return x;
+}
+
+// Joins the normalised results of a row's splits, [splits][dim] at `part` with their
+// log2-sum-exps at `lse`, in their order: a lane takes elements c .. c + 3.  Returns
+// the row's log2-sum-exp (-inf: no split has keys).  Four splits are read at a
+// time, so that a row costs a few trips to memory and not one a split.
+__device__ inline float join_splits(const float* part, const float* lse, int splits, int dim, int c, f32x4* out) {
+  float m = -INFINITY;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, lse[s]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float total = 0.0f;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = 0; s0 < splits; s0 += 4) {
+    f32x4 x[4];
+    float w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = min(s0 + u, splits - 1);
+      x[u] = *reinterpret_cast<const f32x4*>(part + (int64_t)s * dim + c);
+      w[u] = s0 + u < splits ? __builtin_amdgcn_exp2f(lse[s] - ref) : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (w[u] == 0.0f) continue;  // nothing there: whatever it holds does not count
+      total += w[u];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) acc[v] = __builtin_fmaf(w[u], x[u][v], acc[v]);
+    }
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) (*out)[v] = acc[v] * inv;
+  return total == 0.0f ? -INFINITY : m + __builtin_amdgcn_logf(total);
 }
 
 }  // namespace attn

@@ -29,7 +29,7 @@ int64_t act_backward_chunk_rows(int64_t m, int64_t n, int cu_count);
 hipError_t launch_act_backward(const ActBackwardParams& p, int dt, hipStream_t stream);
 
 struct AttnPlan {
-  int waves, splits;
+  int key_groups, splits;
 };
 AttnPlan plan_attention(const AttnParams& p, int cu_count);
 int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);

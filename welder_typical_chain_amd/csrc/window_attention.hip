@@ -47,7 +47,7 @@ template <int DT> __device__ inline void attention_row(const AttnParams& p, int 
 }
 
 // ---- forward -----------------------------------------------------------------
-// A workgroup takes NW * 32 query rows of one sequence and key head.  The rows
+// A workgroup takes 256 / KG query rows of one sequence and key head.  The rows
 // of the query heads that share the key head are packed (row r = query r / G,
 // head r % G), so that a tile of keys serves all of them and the window's
 // edges cost G times fewer tiles.  A wave owns 32 rows, one a lane pair:
@@ -55,8 +55,13 @@ template <int DT> __device__ inline void attention_row(const AttnParams& p, int 
 //   online softmax  (in registers; the two lanes of a query share its maximum)
 //   O^T += V^T . P^T (P^T straight from the registers, see col_frag)
 // Keys come in tiles of 64 through a ring of (K, V) stages filled by
-// direct-to-LDS loads; one barrier a tile.  Workgroups of 8 waves have 3 stages
-// (one workgroup a CU at dim 128), those of 4 waves 2 (two a CU).
+// direct-to-LDS loads; one barrier a tile.
+// With one wave a SIMD a tile takes about 1.9 us whatever its loads do (deeper
+// rings changed nothing): the chain from scores through maximum and exponentials
+// to the values' product is serial.  So a SIMD always gets two waves: where 256
+// rows a workgroup would leave CUs idle, KG = 2 gives each row to two waves that
+// take every other tile and join their results through LDS at the end
+// (chunk_bf16 39 -> KG_US us, prompt_ragged_f16 17 -> KG2_US).
 constexpr int kKeys = 64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // The running maximum is only moved when a score exceeds it by 2^8: the weights
@@ -74,29 +79,32 @@ template <int NS> __device__ inline float positive_scale(float scale, u32x4 (&f)
   return c2 < 0.0f ? -c2 : 1.0f;
 }
 
-template <int ND, int NW> struct FwdLds {
-  static constexpr int RB = row_bytes(ND), STAGES = NW == 8 ? 3 : 2;
-  static constexpr int TILE = kKeys * RB, STAGE = 2 * TILE;
-  static constexpr int PITCH = ND * 64 + 16;  // bytes of a row staged for the output
-  static constexpr int RING = STAGES * STAGE, OUT = NW * 32 * PITCH;
-  static constexpr int TOTAL = RING > OUT ? RING : OUT;
+template <int ND, int KG> struct FwdLds {
+  static constexpr int RB = row_bytes(ND), STAGES = KG == 2 ? 2 : 3;
+  static constexpr int TILE = kKeys * RB, STAGE = KG * 2 * TILE;
+  static constexpr int PITCH = ND * 64 + 16;    // bytes of a row staged for the output
+  static constexpr int JPITCH = ND * 128 + 16;  // bytes of a row handed over (KG = 2), its maximum and sum in the last 16
+  static constexpr int RING = STAGES * STAGE, OUT = 256 / KG * PITCH, JOIN = KG == 2 ? 128 * JPITCH : 0;
+  static constexpr int MOST = RING > OUT ? RING : OUT;
+  static constexpr int TOTAL = MOST > JOIN ? MOST : JOIN;
   static_assert(TOTAL <= 160 * 1024, "LDS");
 };
 
-template <int DT, int ND, int NW>
-__global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnParams p) {
-  using L = FwdLds<ND, NW>;
-  constexpr int RB = L::RB, NS = 2 * ND;
+template <int DT, int ND, int KG>
+__global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams p) {
+  using L = FwdLds<ND, KG>;
+  constexpr int RB = L::RB, NS = 2 * ND, ROWS = 256 / KG;
   __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = wave_id % (8 / KG), group = wave_id / (8 / KG);  // rows, tiles
   const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
   const int split = (int)(id % p.splits);
   const uint32_t rest = id / p.splits;
   const int blk = p.row_blocks - 1 - (int)(rest % p.row_blocks);  // the longest rows first
   const int hk = (int)(rest / p.row_blocks % p.kv_heads), b = (int)(rest / p.row_blocks / p.kv_heads);
   const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
-  const int r0 = blk * NW * 32;
+  const int r0 = blk * ROWS;
 
   // this lane's row
   const int r = r0 + wave * 32 + (lane & 31), i = r / p.group, h = hk * p.group + r - i * p.group;
@@ -104,7 +112,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
   const int pos = valid ? i + shift : -1;
 
   // keys of the block: [0, s_end) and [lo, end)
-  const int i_last = min((r0 + NW * 32 - 1) / p.group, nq - 1);
+  const int i_last = min((r0 + ROWS - 1) / p.group, nq - 1);
   const int p_lo = r0 / p.group + shift, p_hi = i_last + shift;
   const int lo = (int)max((int64_t)0, (int64_t)p_lo - p.window + 1);
   const int end = r0 / p.group < nq ? max(p_hi + 1, 0) : 0;
@@ -127,31 +135,35 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
     for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
   float top = -INFINITY, total = 0.0f;  // log2 domain; total: this lane's half of the keys
 
-  TileLoader<RB, kKeys, NW> lk, lv;
+  TileLoader<RB, kKeys, 8 / KG> lk, lv;
   lk.init(p.k + 2 * (b * p.k_stride[0] + hk * p.k_stride[2]), 2 * p.k_stride[1], p.dim, wave, lane);
   lv.init(p.v + 2 * (b * p.v_stride[0] + hk * p.v_stride[2]), 2 * p.v_stride[1], p.dim, wave, lane);
-  constexpr int LOADS = 2 * TileLoader<RB, kKeys, NW>::NB;
+  constexpr int LOADS = 2 * TileLoader<RB, kKeys, 8 / KG>::NB;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
   auto tile_base = [&](int t) { return t < t_sink ? t * kKeys : lo + (t - t_sink) * kKeys; };
   auto tile_end = [&](int t) { return t < t_sink ? s_end : end; };
-  auto issue = [&](int t) {
+  // step x: tile t0 + x KG + group
+  const int steps = (t1 - t0 + KG - 1) / KG;
+  auto issue = [&](int x) {
+    const int t = t0 + x * KG + group;
     const int j0 = tile_base(t), n = t < t1 ? min(kKeys, tile_end(t) - j0) : 0;
-    const uint32_t st = lds0 + (uint32_t)(t - t0) % L::STAGES * L::STAGE;
+    const uint32_t st = lds0 + (uint32_t)x % L::STAGES * L::STAGE + group * 2 * L::TILE;
     lk.issue(st, j0, n);
     lv.issue(st + L::TILE, j0, n);
   };
 #pragma unroll
-  for (int t = 0; t < L::STAGES - 1; ++t) issue(t0 + t);
+  for (int x = 0; x < L::STAGES - 1; ++x) issue(x);
 
-  const uint32_t k_at = row_addr<RB>(lane), v_at = L::TILE + col_addr<RB>(lane);
-  for (int t = t0; t < t1; ++t) {
-    wait_loads_barrier<LOADS*(L::STAGES - 2)>();  // tile t landed; every wave is done with tile t - 1
-    issue(t + L::STAGES - 1);
+  const uint32_t k_at = row_addr<RB>(lane) + group * 2 * L::TILE, v_at = L::TILE + col_addr<RB>(lane) + group * 2 * L::TILE;
+  for (int x = 0; x < steps; ++x) {
+    wait_loads_barrier<LOADS*(L::STAGES - 2)>();  // the step's tiles landed; every wave is done with the last one's
+    issue(x + L::STAGES - 1);
+    const int t = t0 + x * KG + group;
     const int j0 = tile_base(t), j1 = tile_end(t);
     // (in the window's part the first tokens may lie below the window too)
     const bool below = t >= t_sink && (int64_t)j0 + kKeys - 1 + p.window <= w_lo && j0 >= p.sinks;
-    if (!w_any || j0 > w_hi || below) continue;
-    const uint32_t stage = (uint32_t)(t - t0) % L::STAGES * L::STAGE;
+    if (t >= t1 || !w_any || j0 > w_hi || below) continue;
+    const uint32_t stage = (uint32_t)x % L::STAGES * L::STAGE;
     uint32_t ka = k_at + stage, va = v_at + stage;
     fresh(ka);
     fresh(va);
@@ -172,18 +184,11 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
     }
     __builtin_amdgcn_sched_barrier(0);
     if (j0 + kKeys > j1 || j0 + kKeys - 1 > w_lo || (t >= t_sink && (int64_t)j0 + p.window <= w_hi)) {
-      // key j0 + 4 half + c is seen if c <= top_c and (c > low_c or c < sink_c)
-      const int at = j0 + 4 * half;
-      const int top_c = min(pos, j1 - 1) - at;
-      const int low_c = (int)max((int64_t)pos - p.window - at, (int64_t)-1);
-      const int sink_c = p.sinks - at;
+      const uint64_t seen = seen_bits(j0 + 4 * half, j1, pos, p.window, p.sinks);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int c = 32 * u + 8 * (v >> 2) + (v & 3);
-          s[u][v] = c <= top_c && (c > low_c || c < sink_c) ? s[u][v] : -INFINITY;
-        }
+        for (int v = 0; v < 16; ++v) s[u][v] = keep_bit(s[u][v], seen, 32 * u + 8 * (v >> 2) + (v & 3));
     }
     float m = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
@@ -250,12 +255,40 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
   // ---- the rows' results
   // (a row behind the end took part in tiles that needed no mask)
   total = valid ? xor32_sum(total) : 0.0f;
+  if constexpr (KG == 2) {
+    uint8_t* at = smem + (wave * 32 + (lane & 31)) * L::JPITCH + half * 16;
+    float2* stat = reinterpret_cast<float2*>(smem + (wave * 32 + (lane & 31)) * L::JPITCH + ND * 128);
+    if (group) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(at + (32 * d + 8 * g) * 4) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+      if (half == 0) *stat = float2{top, total};
+    }
+    __syncthreads();
+    if (group) return;
+    const float2 other = *stat;
+    const float next = fmaxf(top, other.x), base = next == -INFINITY ? 0.0f : next;
+    const float f = __builtin_amdgcn_exp2f(top - base), g2 = __builtin_amdgcn_exp2f(other.x - base);
+    total = total * f + other.y * g2;
+    top = next;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(at + (32 * d + 8 * g) * 4);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o[d][4 * g + v] = o[d][4 * g + v] * f + y[v] * g2;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   const float lse = (top + __builtin_amdgcn_logf(total)) * kLn2;  // (v_log_f32: log2)
   if (p.splits > 1) {
     const int64_t row = (((int64_t)b * p.lq + i) * p.heads + h) * p.splits + split;
     if (valid) {
-      if (half == 0) p.part_lse[row] = total == 0.0f ? -INFINITY : lse;
+      if (half == 0) p.part_lse[row] = total == 0.0f ? -INFINITY : top + __builtin_amdgcn_logf(total);
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -269,7 +302,8 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
     return;
   }
   bool nan = lse != lse && total != 0.0f;
-  uint8_t* stg = smem + wave * 32 * L::PITCH;
+  // (with KG = 2 inside the rows that this wave alone has read)
+  uint8_t* stg = smem + wave * 32 * (KG == 2 ? L::JPITCH : L::PITCH);
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -303,37 +337,34 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_tile_kernel(const AttnPa
   }
 }
 
-// Joins the splits of a row: one wave a row.
+// Joins the splits of a row: half a wave a row.
 template <int DT>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p) {
-  using T = typename Elem<DT>::type;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)p.batch * p.lq * p.heads) return;
+  const int lane = threadIdx.x & 63, c = (lane & 31) * 4;
+  const int64_t rows = (int64_t)p.batch * p.lq * p.heads, at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t row = min(at, rows - 1);
   const int h = (int)(row % p.heads), i = (int)(row / p.heads % p.lq), b = (int)(row / p.heads / p.lq);
-  const float* part = p.part_lse + row * p.splits;
-  const int splits = i < seq_queries(p, b) ? p.splits : 0;  // rows behind the end were not written
-  float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, part[s]);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  float total = 0.0f, acc[2] = {0.0f, 0.0f};
-  for (int s = 0; s < splits; ++s) {
-    const float w = __expf(part[s] - ref);
-    total += w;
-    for (int c = 0; c < 2; ++c)
-      if (lane + 64 * c < p.dim) acc[c] = __builtin_fmaf(w, p.part_out[(row * p.splits + s) * p.dim + lane + 64 * c], acc[c]);
-  }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  T* out = (T*)p.out + b * p.o_stride[0] + i * p.o_stride[1] + h * p.o_stride[2];
-  bool nan = total != total;
-  for (int c = 0; c < 2; ++c)
-    if (lane + 64 * c < p.dim) {
-      const float x = acc[c] * inv;
-      nan |= x != x;
-      out[lane + 64 * c] = (T)x;
+  const bool valid = i < seq_queries(p, b);  // rows behind the end were not written
+  bool nan = false;
+  if (c < p.dim) {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    float lse = -INFINITY;
+    if (valid) lse = join_splits(p.part_out + row * p.splits * p.dim, p.part_lse + row * p.splits, p.splits, p.dim, c, &x);
+    nan = lse != lse;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) nan |= x[v] != x[v];
+    if (at < rows) {
+      uint32_t w0, w1;
+      pack4<DT>(x, &w0, &w1);
+      *reinterpret_cast<u32x2*>(p.out + 2 * (b * p.o_stride[0] + (int64_t)i * p.o_stride[1] + h * p.o_stride[2] + c)) = u32x2{w0, w1};
+      if (p.lse && c == 0) p.lse[((int64_t)b * p.heads + h) * p.lq + i] = lse * kLn2;
     }
-  if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + h) * p.lq + i] = top + __logf(total);
-  if (__any(nan) && i < seq_queries(p, b)) attention_row<DT>(p, b, h, i);
+  }
+  const uint64_t redo = __ballot(nan && at < rows);
+  for (int half = 0; half < 2; ++half) {
+    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 6) * 2 + half;
+    if (redo >> (32 * half) & 0xFFFFFFFFu) attention_row<DT>(p, (int)(r / p.heads / p.lq), (int)(r % p.heads), (int)(r / p.heads % p.lq));
+  }
 }
 
 // ---- gradients ------------------------------------------------------------------
@@ -426,9 +457,18 @@ template <int DT> __device__ inline void dkv_row(const AttnParams& p, int b, int
 
 // Row blocks and key tiles as in attention_tile_kernel; keys in subtiles of 32:
 //   S^T = K . Q^T, dP^T = V . dout^T, dq^T += K^T . dS^T
-template <int DT, int ND, int NW>
-__global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnParams p) {
-  using L = FwdLds<ND, NW>;
+constexpr int kDqWaves = 4;  // two workgroups a CU at dim 128
+template <int ND> struct DqLds {
+  static constexpr int RB = row_bytes(ND), STAGES = 2;
+  static constexpr int TILE = kKeys * RB, STAGE = 2 * TILE;
+  static constexpr int PITCH = ND * 64 + 16;
+  static constexpr int RING = STAGES * STAGE, OUT = kDqWaves * 32 * PITCH;
+  static constexpr int TOTAL = RING > OUT ? RING : OUT;
+};
+template <int DT, int ND>
+__global__ void __launch_bounds__(kDqWaves * 64, 2) attention_dq_kernel(const AttnParams p) {
+  using L = DqLds<ND>;
+  constexpr int NW = kDqWaves;
   constexpr int RB = L::RB, NS = 2 * ND;
   __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -522,15 +562,9 @@ __global__ void __launch_bounds__(NW * 64, 2) attention_dq_kernel(const AttnPara
 #pragma unroll
       for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u, st), qf[st], s);
       if (k0 + 32 > j1 || k0 + 31 > w_lo || (t >= t_sink && (int64_t)k0 + p.window <= w_hi)) {
-        const int at = k0 + 4 * half;
-        const int top_c = min(pos, j1 - 1) - at;
-        const int low_c = (int)max((int64_t)pos - p.window - at, (int64_t)-1);
-        const int sink_c = p.sinks - at;
+        const uint64_t seen = seen_bits(k0 + 4 * half, j1, pos, p.window, p.sinks);
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int c = 8 * (v >> 2) + (v & 3);
-          s[v] = c <= top_c && (c > low_c || c < sink_c) ? s[v] : -INFINITY;
-        }
+        for (int v = 0; v < 16; ++v) s[v] = keep_bit(s[v], seen, 8 * (v >> 2) + (v & 3));
       }
       __builtin_amdgcn_sched_barrier(0);
       // the exponentials among the products of dP
@@ -722,11 +756,14 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
       dma16(raw_rsrc(p.row_delta + row, bytes), lane * 16, at + 1024);
     }
   };
-  issue(0);
+#pragma unroll
+  for (int t = 0; t < L::STAGES - 1; ++t) issue(t);
   const uint32_t r_at = row_addr<RB>(lane) + (uint32_t)row0 * RB, c_at = col_addr<RB>(lane) + (uint32_t)row0 * RB;
   for (int t = 0; t < t_all; ++t) {
-    wait_loads_barrier<0>();  // tile t landed; every wave is done with tile t - 1
-    issue(t + 1);
+    // tile t landed; every wave is done with tile t - 1 (wave 0 has two more loads a tile)
+    if (wave == 0) wait_loads_barrier<(2 * NB + 2) * (L::STAGES - 2)>();
+    else wait_loads_barrier<2 * NB * (L::STAGES - 2)>();
+    issue(t + L::STAGES - 1);
     const int step = t / chunks, hc = t - step * chunks, i = i0 + step * tp;
     const uint32_t stage = (uint32_t)t % L::STAGES * L::STAGE;
     const uint8_t* stt = smem + stage + L::STATS;
@@ -747,11 +784,10 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
 #pragma unroll
     for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ra, 0, st), kf[st], s);
     if (!all) {
+      const int at = row0 + 4 * half;
+      const uint64_t in = bits_below(t_hi - at) & ~bits_below(t_lo - at);
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int row = row0 + 8 * (v >> 2) + 4 * half + (v & 3);
-        s[v] = row >= t_lo && row < t_hi ? s[v] : -INFINITY;
-      }
+      for (int v = 0; v < 16; ++v) s[v] = keep_bit(s[v], in, 8 * (v >> 2) + (v & 3));
     }
     __builtin_amdgcn_sched_barrier(0);
     // the exponentials among the products of dP
@@ -925,26 +961,27 @@ hipError_t launch(const void* fn, int64_t grid, int threads, const AttnParams& p
 #define WTC_BY_TYPE(kernel, dt) ((dt) == DT_F16 ? (const void*)&kernel<DT_F16> : (const void*)&kernel<DT_BF16>)
 
 namespace {
-template <int DT, int NW> const void* tile_kernel(int nd) {
+template <int DT, int KG> const void* tile_kernel(int nd) {
   switch (nd) {
-    case 1: return (const void*)&attention_tile_kernel<DT, 1, NW>;
-    case 2: return (const void*)&attention_tile_kernel<DT, 2, NW>;
-    case 3: return (const void*)&attention_tile_kernel<DT, 3, NW>;
+    case 1: return (const void*)&attention_tile_kernel<DT, 1, KG>;
+    case 2: return (const void*)&attention_tile_kernel<DT, 2, KG>;
+    case 3: return (const void*)&attention_tile_kernel<DT, 3, KG>;
   }
-  return (const void*)&attention_tile_kernel<DT, 4, NW>;
+  return (const void*)&attention_tile_kernel<DT, 4, KG>;
 }
 }  // namespace
 
-// Waves a workgroup (32 rows each) and splits of the keys, from the sizes alone.
+// Rows a workgroup (256 / key_groups) and splits of the keys, from the sizes alone:
+// splits while CUs are idle and a workgroup keeps 8 tiles.
 AttnPlan plan_attention(const AttnParams& p, int cu_count) {
-  AttnPlan plan{8, 1};
+  AttnPlan plan{1, 1};
   const int64_t rows = (int64_t)p.lq * p.group, seqs = (int64_t)p.batch * p.kv_heads;
-  if (seqs * ((rows + 255) / 256) < cu_count) plan.waves = 4;
-  const int64_t grid = seqs * ((rows + plan.waves * 32 - 1) / (plan.waves * 32));
+  if (seqs * ((rows + 255) / 256) < cu_count) plan.key_groups = 2;
+  const int64_t block = 256 / plan.key_groups, grid = seqs * ((rows + block - 1) / block);
   // keys that a row block sees at most
-  const int64_t reach = std::min<int64_t>(p.lk, p.window + (plan.waves * 32 + p.group - 1) / p.group + p.sinks);
+  const int64_t reach = std::min<int64_t>(p.lk, p.window + (block + p.group - 1) / p.group + p.sinks);
   const int64_t tiles = (reach + kKeys - 1) / kKeys;
-  while (plan.splits < 16 && grid * plan.splits < cu_count && tiles / (2 * plan.splits) >= 4) plan.splits *= 2;
+  while (plan.splits < 16 && grid * plan.splits < cu_count && tiles / (2 * plan.splits) >= 4 * plan.key_groups) plan.splits *= 2;
   return plan;
 }
 int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan) {
@@ -956,24 +993,24 @@ hipError_t launch_attention(const AttnParams& params, const AttnPlan& plan, int 
   AttnParams p = params;
   const int64_t rows = (int64_t)p.lq * p.group;
   p.splits = plan.splits;
-  p.row_blocks = (int)((rows + plan.waves * 32 - 1) / (plan.waves * 32));
+  p.row_blocks = (int)((rows * plan.key_groups + 255) / 256);
   p.part_lse = p.part_out + (int64_t)p.batch * p.lq * p.heads * p.splits * p.dim;
   const int nd = (p.dim + 31) / 32;
-  const void* fn = plan.waves == 8 ? (dt == DT_F16 ? tile_kernel<DT_F16, 8>(nd) : tile_kernel<DT_BF16, 8>(nd))
-                                   : (dt == DT_F16 ? tile_kernel<DT_F16, 4>(nd) : tile_kernel<DT_BF16, 4>(nd));
-  const hipError_t e = launch(fn, (int64_t)p.batch * p.kv_heads * p.row_blocks * p.splits, plan.waves * 64, p, stream);
+  const void* fn = plan.key_groups == 2 ? (dt == DT_F16 ? tile_kernel<DT_F16, 2>(nd) : tile_kernel<DT_BF16, 2>(nd))
+                                        : (dt == DT_F16 ? tile_kernel<DT_F16, 1>(nd) : tile_kernel<DT_BF16, 1>(nd));
+  const hipError_t e = launch(fn, (int64_t)p.batch * p.kv_heads * p.row_blocks * p.splits, 512, p, stream);
   if (e != hipSuccess || p.splits == 1) return e;
-  return launch(WTC_BY_TYPE(attention_join_kernel, dt), ((int64_t)p.batch * p.lq * p.heads + 3) / 4, 256, p, stream);
+  return launch(WTC_BY_TYPE(attention_join_kernel, dt), ((int64_t)p.batch * p.lq * p.heads + 7) / 8, 256, p, stream);
 }
 
 namespace {
-template <int DT, int NW> const void* dq_kernel(int nd) {
+template <int DT> const void* dq_kernel(int nd) {
   switch (nd) {
-    case 1: return (const void*)&attention_dq_kernel<DT, 1, NW>;
-    case 2: return (const void*)&attention_dq_kernel<DT, 2, NW>;
-    case 3: return (const void*)&attention_dq_kernel<DT, 3, NW>;
+    case 1: return (const void*)&attention_dq_kernel<DT, 1>;
+    case 2: return (const void*)&attention_dq_kernel<DT, 2>;
+    case 3: return (const void*)&attention_dq_kernel<DT, 3>;
   }
-  return (const void*)&attention_dq_kernel<DT, 4, NW>;
+  return (const void*)&attention_dq_kernel<DT, 4>;
 }
 template <int DT> const void* dkv_kernel(int nd) {
   switch (nd) {
@@ -1013,10 +1050,8 @@ hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwar
   const int nd = (p.dim + 31) / 32;
   const int64_t seqs = (int64_t)p.batch * p.kv_heads;
   if (p.lq) {
-    constexpr int waves = 4;
-    p.row_blocks = (int)(((int64_t)p.lq * p.group + waves * 32 - 1) / (waves * 32));
-    const hipError_t e = launch(dt == DT_F16 ? dq_kernel<DT_F16, waves>(nd) : dq_kernel<DT_BF16, waves>(nd), seqs * p.row_blocks,
-                                waves * 64, p, stream);
+    p.row_blocks = (int)(((int64_t)p.lq * p.group + kDqWaves * 32 - 1) / (kDqWaves * 32));
+    const hipError_t e = launch(dt == DT_F16 ? dq_kernel<DT_F16>(nd) : dq_kernel<DT_BF16>(nd), seqs * p.row_blocks, kDqWaves * 64, p, stream);
     if (e != hipSuccess) return e;
   }
   if (!p.lk) return hipSuccess;

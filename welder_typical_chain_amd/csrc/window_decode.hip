@@ -236,29 +236,18 @@ __global__ void __launch_bounds__(kWaves * 64, 1) decode_kernel(const AttnParams
   }
 }
 
-// The splits of a head's row, in their order (log2 domain).  One wave a row.
+// The splits of a head's row: half a wave a row.
 template <int DT>
 __global__ void __launch_bounds__(256) decode_join_kernel(const AttnParams p) {
-  using T = typename Elem<DT>::type;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)p.batch * p.heads) return;
+  const int c = (threadIdx.x & 31) * 4;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= (int64_t)p.batch * p.heads || c >= p.dim) return;
   const int h = (int)(row % p.heads), b = (int)(row / p.heads);
-  const float* part = p.part_lse + row * p.splits;
-  float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, part[s]);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f, acc[2] = {0.0f, 0.0f};
-  for (int s = 0; s < p.splits; ++s) {
-    const float w = __builtin_amdgcn_exp2f(part[s] - ref);
-    sum += w;
-    for (int c = 0; c < 2; ++c)
-      if (lane + 64 * c < p.dim) acc[c] = __builtin_fmaf(w, p.part_out[(row * p.splits + s) * p.dim + lane + 64 * c], acc[c]);
-  }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  T* out = (T*)p.out + b * p.o_stride[0] + h * p.o_stride[2];
-  for (int c = 0; c < 2; ++c)
-    if (lane + 64 * c < p.dim) out[lane + 64 * c] = (T)(acc[c] * inv);
+  f32x4 x;
+  join_splits(p.part_out + row * p.splits * p.dim, p.part_lse + row * p.splits, p.splits, p.dim, c, &x);
+  uint32_t w0, w1;
+  pack4<DT>(x, &w0, &w1);
+  *reinterpret_cast<u32x2*>(p.out + 2 * (b * p.o_stride[0] + h * p.o_stride[2] + c)) = u32x2{w0, w1};
 }
 
 template <int DT> const void* kernel_for(int nd) {
@@ -295,7 +284,7 @@ hipError_t launch_attention_decode(const AttnParams& params, int splits, int dt,
                                        dim3(kWaves * 64), args, 0, stream);
   if (e != hipSuccess || splits == 1) return e;
   return hipLaunchKernel(dt == DT_F16 ? (const void*)&decode_join_kernel<DT_F16> : (const void*)&decode_join_kernel<DT_BF16>,
-                         dim3((unsigned)(((int64_t)p.batch * p.heads + 3) / 4)), dim3(256), args, 0, stream);
+                         dim3((unsigned)(((int64_t)p.batch * p.heads + 7) / 8)), dim3(256), args, 0, stream);
 }
 
 }  // namespace wtc
