@@ -147,7 +147,7 @@ def test_matmul_backward_strided(W):
     want = W.matmul_epilogue_backward(dout.contiguous(), a.contiguous(), b)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
     # a gradient that autograd broadcast from one value
-    got = W.matmul_epilogue_backward(torch.ones((), dtype=BF16, device="cuda").expand(90, 136).contiguous(), a, b)
+    got = W.matmul_epilogue_backward(torch.ones((), dtype=BF16, device="cuda").expand(90, 136), a, b)
     want = W.matmul_epilogue_backward(torch.ones(90, 136, dtype=BF16, device="cuda"), a, b)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
@@ -275,6 +275,70 @@ def test_attention_bad_values_stay_where_they_are_seen(W, bad, name, lq):
         U.assert_within(x[:, ~touched], want[:, ~touched], bound[:, ~touched], (name, what))
         if one_head and x.shape[2] == 2:
             U.assert_within(x[:, :, 1], want[:, :, 1], bound[:, :, 1], (name, what, "other head"))
+
+
+def test_attention_full_of_nan(W):
+    """Everything NaN stays NaN (and ends soon)."""
+    q, k, v, g = qkv(75, 1, 700, 700, 4, 2, 64, BF16)
+    out, lse = W.window_attention(q, k, torch.full_like(v, NAN), return_lse=True)
+    assert bool(out.isnan().all()) and bool(lse.isfinite().all())
+    nan = torch.full_like(q, NAN)
+    out, lse = W.window_attention(nan, k, v, return_lse=True)
+    assert bool(out.isnan().all()) and bool(lse.isnan().all())
+    out, lse = W.window_attention(q, k, v, return_lse=True)
+    dq, dk, dv = W.window_attention_backward(nan, q, k, v, out, lse)
+    assert bool(dq.isnan().all()) and bool(dk.isnan().all()) and bool(dv.isnan().all())
+
+
+def test_attention_bad_value_in_a_first_token(W):
+    """A NaN in one column of a first token's value reaches that column of every row and no other."""
+    q, k, v, g = qkv(76, 1, 600, 600, 2, 2, 64, F16)
+    kw = dict(window=40, sinks=2)
+    ref = U.attention_reference(q, k, v, **kw)["out"]
+    v[0, 1, 0, 7] = NAN
+    out = W.window_attention(q, k, v, **kw)
+    assert bool(out[0, 1:, 0, 7].isnan().all())
+    clean = out.clone()
+    clean[0, 1:, 0, 7] = ref[0][0, 1:, 0, 7].to(F16)
+    U.assert_within(clean, *ref, "out")
+
+
+@pytest.mark.parametrize("b,lq,lk,window,sinks", [(1, 900, 900, 5, 850), (2, 40, 900, 17, 300), (1, 1500, 1500, 1, 1)])
+def test_attention_many_or_far_first_tokens(W, b, lq, lk, window, sinks):
+    q, k, v, g = qkv(77, b, lq, lk, 2, 1, 32, BF16)
+    check_attention(W, q, k, v, g, window=window, sinks=sinks)
+
+
+def test_attention_backward_of_a_broadcast_gradient(W):
+    q, k, v, _ = qkv(78, 1, 70, 70, 2, 2, 64, BF16)
+    out, lse = W.window_attention(q, k, v, return_lse=True)
+    one = torch.ones((), dtype=BF16, device="cuda").expand(q.shape)
+    got = W.window_attention_backward(one, q, k, v, out, lse)
+    want = W.window_attention_backward(one.contiguous(), q, k, v, out, lse)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_offsets_past_32_bits(W):
+    """A cache of over 4 GiB: its last rows, its wrapped rows and its first ones."""
+    kv, d, cap, sinks = 32, 128, 600_000, 3
+    cache = torch.zeros(1, cap, kv, d, dtype=BF16, device="cuda")  # 4.9 GB, keys and values alike
+    assert cache.numel() * 2 > 1 << 32
+    cache[:, :400] = rand(1, 1, 400, kv, d, dtype=BF16)
+    cache[:, -400:] = rand(2, 1, 400, kv, d, dtype=BF16)
+    q = rand(3, 1, 64, d, dtype=BF16)
+    for n in (cap, cap + 150):  # the second wraps: 150 rows behind the first ones, the rest at the end
+        n_t = torch.tensor([n], dtype=torch.int32, device="cuda")
+        ref, bound, _, _ = U.decode_reference(q, cache, cache, [n], window=300, sinks=sinks)
+        U.assert_within(W.window_attention_decode(q, cache, cache, n_t, window=300, sinks=sinks), ref, bound, f"n {n}")
+    # the last tokens of a prompt of that length, and the same with heads before tokens
+    q = rand(4, 1, 5, 32, d, dtype=BF16)
+    rows = torch.cat([torch.arange(sinks), torch.arange(cap - 104, cap)]).cuda()
+    ref = U.attention_reference(q, cache[:, rows], cache[:, rows], window=100, sinks=sinks)["out"]
+    U.assert_within(W.window_attention(q, cache, cache, window=100, sinks=sinks), *ref, "prompt")
+    turned = cache.view(1, kv, cap, d)  # another tensor of the same values: [B, H, L, D]
+    turned = turned.transpose(1, 2)
+    ref = U.attention_reference(q, turned[:, rows], turned[:, rows], window=100, sinks=sinks)["out"]
+    U.assert_within(W.window_attention(q, turned, turned, window=100, sinks=sinks), *ref, "turned")
 
 
 def test_attention_all_scores_minus_infinity(W):
@@ -551,6 +615,9 @@ def test_refusals_on_the_gpu(W):
         W.matmul_epilogue(rand(1, 4, 60, dtype=F16), rand(1, 60, 32, dtype=F16))
     with pytest.raises(W._lib.WtcError):
         W.matmul_epilogue(rand(1, 4, 65, dtype=F16)[:, 1:], b)  # rows not 16-byte aligned
+    square = rand(2, 64, 64, dtype=F16)
+    with pytest.raises(ValueError):
+        W.matmul_epilogue(a, square, out=a)
     with pytest.raises(ValueError):
         W.matmul_epilogue(a.requires_grad_(), b)
     a = a.detach()
@@ -559,6 +626,8 @@ def test_refusals_on_the_gpu(W):
     q, k, v, _ = qkv(1, 1, 8, 8, 2, 2, 64, F16)
     with pytest.raises(ValueError):
         W.window_attention(q, k[:, :, :, :32], v)
+    with pytest.raises(ValueError):
+        W.window_attention(q, k, v, out=q)
     with pytest.raises(ValueError):
         W.window_attention(q, k, v, window=0)
     with pytest.raises(ValueError):

@@ -99,6 +99,18 @@ template <int NS> __device__ inline void load_row(const uint8_t* row, bool valid
   }
 }
 
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Scores in the log2 domain are c2 times the products, c2 > 0: with a negative scale
+// one operand's fragments are negated, with a scale of 0 they are zero.
+template <int NS> __device__ inline float positive_scale(float scale, u32x4 (&f)[NS]) {
+  const float c2 = scale * kLog2e;
+  if (c2 > 0.0f) return c2;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) f[s] = c2 < 0.0f ? f[s] ^ 0x80008000u : f[s] & 0u;
+  return c2 < 0.0f ? -c2 : 1.0f;
+}
+
 // Masks as bits, a lane's own: bit c of bits_below(n) is set for c < n.  One bit
 // then costs an element two vector instructions; compares would go through scalar
 // masks, three to an element and each waiting for the last.

@@ -9,10 +9,40 @@ namespace {
 
 using namespace attn;
 
-// One query row by a whole wave, 64 keys at a time, with nothing but the keys it
-// sees: what the tile kernel's rows fall back on that come out as NaN (a NaN or an
-// infinity in a key or value that the mask hides would reach them through the
-// tile's products, as 0 * NaN).
+// Where the mask hides a NaN or an infinity.  The tiles' products meet it as 0 * NaN,
+// so an output element that comes out as NaN is computed again by a whole wave
+// from the keys (queries) that it sees, 64 at a time.  Only those elements are,
+// and only until each of them is NaN again, which an element that sees the bad
+// value is as soon as it is met: an input full of NaN costs one step a row.
+constexpr int kCols = 2;  // columns a lane: lane, lane + 64
+template <int DT> struct Redo {
+  using T = typename Elem<DT>::type;
+  T* row;
+  bool bad[kCols];
+  float acc[kCols];
+  __device__ inline Redo(void* base, int64_t at, int dim, int lane) : row(static_cast<T*>(base) + at) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const float x = lane + 64 * c < dim ? (float)row[lane + 64 * c] : 0.0f;
+      bad[c] = x != x;
+      acc[c] = 0.0f;
+    }
+  }
+  __device__ inline void add(float w, const T* x, int lane) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+      if (bad[c]) acc[c] = __builtin_fmaf(w, (float)x[lane + 64 * c], acc[c]);
+  }
+  __device__ inline bool settled() const {  // every one of them is NaN for good
+    return __all((!bad[0] || acc[0] != acc[0]) && (!bad[1] || acc[1] != acc[1]));
+  }
+  __device__ inline void store(float by, int lane) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+      if (bad[c]) row[lane + 64 * c] = (T)(acc[c] * by);
+  }
+};
+
 template <int DT> __device__ inline void attention_row(const AttnParams& p, int b, int h, int i) {
   using T = typename Elem<DT>::type;
   const int lane = threadIdx.x & 63;
@@ -21,29 +51,20 @@ template <int DT> __device__ inline void attention_row(const AttnParams& p, int 
   const T* k = (const T*)p.k + b * p.k_stride[0] + h / p.group * p.k_stride[2];
   const T* v = (const T*)p.v + b * p.v_stride[0] + h / p.group * p.v_stride[2];
   const Seen seen(p.window, p.sinks, pos);
-  float top = -INFINITY, total = 0.0f, acc[2] = {0.0f, 0.0f};
-  for (int t0 = 0; t0 < seen.count; t0 += 64) {
+  Redo<DT> out(p.out, b * p.o_stride[0] + i * p.o_stride[1] + h * p.o_stride[2], p.dim, lane);
+  float top = -INFINITY, total = 0.0f;
+  for (int t0 = 0; t0 < seen.count && !out.settled(); t0 += 64) {
     const bool in = t0 + lane < seen.count;
     const float s = in ? p.scale * dot_rows<DT>(q, k + seen.key(t0 + lane) * p.k_stride[1], p.dim) : -INFINITY;
     const float next = fmaxf(top, wave_max(s));
     const float keep = next == -INFINITY ? 1.0f : __expf(top - next);
     const float e = in ? (next == -INFINITY ? (s != s ? s : 0.0f) : __expf(s - next)) : 0.0f;
     total = total * keep + wave_sum(e);
-    acc[0] *= keep;
-    acc[1] *= keep;
+    for (int c = 0; c < kCols; ++c) out.acc[c] *= keep;
     top = next;
-    for (int t = 0; t < min(64, seen.count - t0); ++t) {
-      const float w = __shfl(e, t);
-      const T* row = v + seen.key(t0 + t) * p.v_stride[1];
-      for (int c = 0; c < 2; ++c)
-        if (lane + 64 * c < p.dim) acc[c] = __builtin_fmaf(w, (float)row[lane + 64 * c], acc[c]);
-    }
+    for (int t = 0; t < min(64, seen.count - t0); ++t) out.add(__shfl(e, t), v + seen.key(t0 + t) * p.v_stride[1], lane);
   }
-  T* out = (T*)p.out + b * p.o_stride[0] + i * p.o_stride[1] + h * p.o_stride[2];
-  const float r = total == 0.0f ? 0.0f : 1.0f / total;
-  for (int c = 0; c < 2; ++c)
-    if (lane + 64 * c < p.dim) out[lane + 64 * c] = (T)(acc[c] * r);
-  if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + h) * p.lq + i] = top + __logf(total);
+  out.store(total == 0.0f ? 0.0f : 1.0f / total, lane);
 }
 
 // ---- forward -----------------------------------------------------------------
@@ -63,21 +84,10 @@ template <int DT> __device__ inline void attention_row(const AttnParams& p, int 
 // take every other tile and join their results through LDS at the end
 // (chunk_bf16 39 -> KG_US us, prompt_ragged_f16 17 -> KG2_US).
 constexpr int kKeys = 64;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // The running maximum is only moved when a score exceeds it by 2^8: the weights
 // stay below 2^8, and the accumulators are rescaled a few times a row instead
 // of once a tile.
 constexpr float kSlack = 8.0f;
-
-// Scores in the log2 domain are c2 times the products, c2 > 0: with a negative scale
-// one operand's fragments are negated, with a scale of 0 they are zero.
-template <int NS> __device__ inline float positive_scale(float scale, u32x4 (&f)[NS]) {
-  const float c2 = scale * kLog2e;
-  if (c2 > 0.0f) return c2;
-#pragma unroll
-  for (int s = 0; s < NS; ++s) f[s] = c2 < 0.0f ? f[s] ^ 0x80008000u : f[s] & 0u;
-  return c2 < 0.0f ? -c2 : 1.0f;
-}
 
 template <int ND, int KG> struct FwdLds {
   static constexpr int RB = row_bytes(ND), STAGES = KG == 2 ? 2 : 3;
@@ -301,7 +311,7 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
     }
     return;
   }
-  bool nan = lse != lse && total != 0.0f;
+  bool nan = false;
   // (with KG = 2 inside the rows that this wave alone has read)
   uint8_t* stg = smem + wave * 32 * (KG == 2 ? L::JPITCH : L::PITCH);
 #pragma unroll
@@ -330,6 +340,7 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
           *reinterpret_cast<const u32x4*>(stg + row * L::PITCH + c * 16);
   }
   uint32_t redo = (uint32_t)(__ballot(nan && valid) | __ballot(nan && valid) >> 32);
+  if (redo) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the rows are read back
   while (redo) {
     const int rr = r0 + wave * 32 + __builtin_ctz(redo);
     attention_row<DT>(p, b, hk * p.group + rr % p.group, rr / p.group);
@@ -350,7 +361,6 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     float lse = -INFINITY;
     if (valid) lse = join_splits(p.part_out + row * p.splits * p.dim, p.part_lse + row * p.splits, p.splits, p.dim, c, &x);
-    nan = lse != lse;
 #pragma unroll
     for (int v = 0; v < 4; ++v) nan |= x[v] != x[v];
     if (at < rows) {
@@ -361,6 +371,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
     }
   }
   const uint64_t redo = __ballot(nan && at < rows);
+  if (redo) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   for (int half = 0; half < 2; ++half) {
     const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 6) * 2 + half;
     if (redo >> (32 * half) & 0xFFFFFFFFu) attention_row<DT>(p, (int)(r / p.heads / p.lq), (int)(r % p.heads), (int)(r / p.heads % p.lq));
@@ -380,7 +391,6 @@ __device__ inline int64_t stats_row(const AttnParams& p, int b, int hk, int i) {
   return (((int64_t)b * p.kv_heads + hk) * p.lq + i) * p.group;
 }
 
-// dq of one row by a whole wave, for the rows that come out as NaN (see attention_row).
 template <int DT> __device__ inline void dq_row(const AttnParams& p, int b, int h, int i) {
   using T = typename Elem<DT>::type;
   const int lane = threadIdx.x & 63;
@@ -393,27 +403,20 @@ template <int DT> __device__ inline void dq_row(const AttnParams& p, int b, int 
   const float delta = dot_rows<DT>(g, o, p.dim);
   const float lse = p.lse_in[((int64_t)b * p.heads + h) * p.lq + i];
   const Seen seen(p.window, p.sinks, pos);
-  float acc[2] = {0.0f, 0.0f};
-  for (int t0 = 0; t0 < seen.count; t0 += 64) {
+  Redo<DT> dq(p.dq, (((int64_t)b * p.lq + i) * p.heads + h) * p.dim, p.dim, lane);
+  for (int t0 = 0; t0 < seen.count && !dq.settled(); t0 += 64) {
     float ds = 0.0f;
     if (t0 + lane < seen.count) {
       const int j = seen.key(t0 + lane);
       const float w = __expf(p.scale * dot_rows<DT>(q, k + j * p.k_stride[1], p.dim) - lse);
       ds = p.scale * w * (dot_rows<DT>(g, v + j * p.v_stride[1], p.dim) - delta);
     }
-    for (int t = 0; t < min(64, seen.count - t0); ++t) {
-      const float w = __shfl(ds, t);
-      const T* row = k + seen.key(t0 + t) * p.k_stride[1];
-      for (int c = 0; c < 2; ++c)
-        if (lane + 64 * c < p.dim) acc[c] = __builtin_fmaf(w, (float)row[lane + 64 * c], acc[c]);
-    }
+    for (int t = 0; t < min(64, seen.count - t0); ++t) dq.add(__shfl(ds, t), k + seen.key(t0 + t) * p.k_stride[1], lane);
   }
-  T* dq = (T*)p.dq + (((int64_t)b * p.lq + i) * p.heads + h) * p.dim;
-  for (int c = 0; c < 2; ++c)
-    if (lane + 64 * c < p.dim) dq[lane + 64 * c] = (T)acc[c];
+  dq.store(1.0f, lane);
 }
 
-// dk and dv of one key by a whole wave, 64 queries at a time, likewise.
+// dk and dv of one key.
 template <int DT> __device__ inline void dkv_row(const AttnParams& p, int b, int hk, int j) {
   using T = typename Elem<DT>::type;
   const int lane = threadIdx.x & 63;
@@ -424,12 +427,13 @@ template <int DT> __device__ inline void dkv_row(const AttnParams& p, int b, int
   const int i0 = max(0, j - shift);
   const int i1 = j < p.sinks ? nq : (int)min((int64_t)nq, j + p.window - shift);
   const float c2 = p.scale * kLog2e;
-  float ak[2] = {0.0f, 0.0f}, av[2] = {0.0f, 0.0f};
+  const int64_t at = (((int64_t)b * p.lk + j) * p.kv_heads + hk) * p.dim;
+  Redo<DT> dk(p.dk, at, p.dim, lane), dv(p.dv, at, p.dim, lane);
   for (int x = 0; x < p.group; ++x) {
     const int h = hk * p.group + x;
     const T* q = (const T*)p.q + b * p.q_stride[0] + h * p.q_stride[2];
     const T* g = (const T*)p.dout + b * p.do_stride[0] + h * p.do_stride[2];
-    for (int t0 = i0; t0 < i1; t0 += 64) {
+    for (int t0 = i0; t0 < i1 && !(dk.settled() && dv.settled()); t0 += 64) {
       float w = 0.0f, ds = 0.0f;
       const int i = t0 + lane;
       if (i < i1) {
@@ -438,21 +442,13 @@ template <int DT> __device__ inline void dkv_row(const AttnParams& p, int b, int
         ds = p.scale * w * (dot_rows<DT>(g + i * p.do_stride[1], v, p.dim) - p.row_delta[row]);
       }
       for (int t = 0; t < min(64, i1 - t0); ++t) {
-        const float wt = __shfl(w, t), dt = __shfl(ds, t);
-        for (int c = 0; c < 2; ++c)
-          if (lane + 64 * c < p.dim) {
-            av[c] = __builtin_fmaf(wt, (float)g[(t0 + t) * p.do_stride[1] + lane + 64 * c], av[c]);
-            ak[c] = __builtin_fmaf(dt, (float)q[(t0 + t) * p.q_stride[1] + lane + 64 * c], ak[c]);
-          }
+        dv.add(__shfl(w, t), g + (t0 + t) * p.do_stride[1], lane);
+        dk.add(__shfl(ds, t), q + (t0 + t) * p.q_stride[1], lane);
       }
     }
   }
-  const int64_t at = (((int64_t)b * p.lk + j) * p.kv_heads + hk) * p.dim;
-  for (int c = 0; c < 2; ++c)
-    if (lane + 64 * c < p.dim) {
-      ((T*)p.dk)[at + lane + 64 * c] = (T)ak[c];
-      ((T*)p.dv)[at + lane + 64 * c] = (T)av[c];
-    }
+  dk.store(1.0f, lane);
+  dv.store(1.0f, lane);
 }
 
 // Row blocks and key tiles as in attention_tile_kernel; keys in subtiles of 32:
@@ -626,6 +622,7 @@ __global__ void __launch_bounds__(kDqWaves * 64, 2) attention_dq_kernel(const At
           *reinterpret_cast<const u32x4*>(stg + row * L::PITCH + c * 16);
   }
   uint32_t redo = (uint32_t)(__ballot(nan && valid) | __ballot(nan && valid) >> 32);
+  if (redo) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   while (redo) {
     const int rr = r0 + wave * 32 + __builtin_ctz(redo);
     dq_row<DT>(p, b, hk * p.group + rr % p.group, rr / p.group);
@@ -947,7 +944,9 @@ __global__ void __launch_bounds__(64) attention_far_kernel(const AttnParams p) {
     T* dst = (T*)(is_dv ? p.dv : p.dk) + (((int64_t)b * p.lk + j) * p.kv_heads + hk) * p.dim;
     dst[is_dv ? c - p.dim : c] = (T)sum;
   }
-  if (__any(nan)) dkv_row<DT>(p, b, hk, j);
+  if (!__any(nan)) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  dkv_row<DT>(p, b, hk, j);
 }
 
 hipError_t launch(const void* fn, int64_t grid, int threads, const AttnParams& p, hipStream_t stream) {
@@ -1030,8 +1029,9 @@ AttnBackwardPlan plan_attention_backward(const AttnParams& p) {
   if (p.sinks > 0 && far > 0) {
     plan.far_blocks = (p.sinks + kDkvKeys - 1) / kDkvKeys;
     plan.far_keys = std::min(p.sinks, kDkvKeys);
-    // short ones, in the end of the key blocks' round: 256 positions or a key block's share
-    plan.far_chunks = (int)std::max<int64_t>(1, std::min<int64_t>(plan.key_blocks, far / 256));
+    // short ones, in the end of the key blocks' round: 256 positions or a key block's
+    // share, and no more in all than there are key blocks (their sums take memory)
+    plan.far_chunks = (int)std::max<int64_t>(1, std::min<int64_t>(plan.key_blocks / plan.far_blocks, far / 256));
   }
   const int64_t rows = (int64_t)p.batch * p.lq * p.heads;
   plan.part_at = (rows * 8 + 255) / 256 * 256;

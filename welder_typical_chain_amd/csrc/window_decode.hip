@@ -24,7 +24,6 @@ using namespace attn;
 constexpr int kRows = 32;   // cache rows a tile
 constexpr int kWaves = 4;
 constexpr int kHeads = 32;  // query heads a workgroup
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int ND> struct DecodeLds {
   static constexpr int RB = row_bytes(ND);
@@ -67,12 +66,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) decode_kernel(const AttnParams
   u32x4 qf[NS];
   const int hq = lane & 31;
   load_row<NS>(p.q + 2 * (b * p.q_stride[0] + (int64_t)(h0 + hq) * p.q_stride[2]), hq < heads, p.dim, half, qf);
-  float c2 = p.scale * kLog2e;
-  if (c2 < 0.0f) {
-    c2 = -c2;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) qf[s] ^= 0x80008000u;
-  }
+  const float c2 = positive_scale<NS>(p.scale, qf);
   f32x16 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -147,8 +141,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) decode_kernel(const AttnParams
       if (8 * (v >> 2) + (v & 3) + 4 * half >= rows) s[v] = -INFINITY;
       m = fmaxf(m, s[v]);
     }
-    m = xor32_max(m);
-    m = m == -INFINITY ? m : m * c2;
+    m = xor32_max(m) * c2;
     const float next = fmaxf(top, m);
     const float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - next);
     if (__any(next > top)) {
@@ -166,8 +159,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) decode_kernel(const AttnParams
       f32x4 e;
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const float y = s[4 * g + v];
-        e[v] = y == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(y, c2, ref));
+        e[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + v], c2, ref));
         sum += e[v];
       }
       uint32_t w0, w1;

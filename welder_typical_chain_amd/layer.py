@@ -168,6 +168,8 @@ def matmul_epilogue(a: torch.Tensor, b: torch.Tensor, *, bias: torch.Tensor | No
         out = torch.empty(shape, dtype=out_dtype, device=a.device)
     elif out.shape != shape or out.dtype != out_dtype:
         raise ValueError("out has the wrong shape or dtype")
+    elif m and n and out.data_ptr() in (a.data_ptr(), b.data_ptr()):
+        raise ValueError("out may not be a or b")
     out2 = out if flat else out.view(-1, n) if out.numel() else out.new_empty((m, n))
     bias_code = code
     if bias is not None:
@@ -220,7 +222,10 @@ def matmul_epilogue_backward(dout: torch.Tensor, a: torch.Tensor, b: torch.Tenso
         raise ValueError("the gradient of an activation needs pre")
     if pre is not None and (pre.shape != dout.shape or not pre.is_contiguous() or pre.get_device() != device):
         raise ValueError("pre must be contiguous, of dout's shape and on its device")
-    d2 = dout if dout.dim() == 2 else dout.reshape(-1, n) if dout.numel() else dout.new_empty((m, n))
+    if dout.dim() == 2:  # (a gradient that autograd broadcast is copied)
+        d2 = dout if dout.stride(1) == 1 and dout.stride(0) >= n or not dout.numel() else dout.contiguous()
+    else:
+        d2 = dout.reshape(-1, n).contiguous() if dout.numel() else dout.new_empty((m, n))
     da = torch.empty(a.shape, dtype=a.dtype, device=a.device) if need_a else None
     db = None
     if need_b:
@@ -309,6 +314,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape:
         raise ValueError("out must have q's shape")
+    elif out.numel() and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+        raise ValueError("out may not be an input")
     b, lq, h, _ = q.shape
     lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if return_lse else None
     args = _pack_attention(*head, *_strides(out, "out"), 0, 0, 0, 0, 0, 0, 0, *tail)
@@ -337,6 +344,8 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     if lse.shape != (b, h, lq) or lse.dtype != torch.float32 or not lse.is_contiguous() or \
             not lse.is_cuda or lse.get_device() != device:
         raise ValueError("lse must be window_attention's: float32, contiguous, [B, H, Lq]")
+    if dout.stride(3) != 1 or 0 in dout.stride():  # a gradient that autograd broadcast
+        dout = dout.contiguous()
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     lib = _lib.lib()
     args = _pack_attention(*head, *_strides(out, "out"), *_strides(dout, "dout"), 0, 0, 0, 0, *tail)
@@ -378,6 +387,8 @@ def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape:
         raise ValueError("out must have q's shape")
+    elif out.numel() and out.data_ptr() == q.data_ptr():
+        raise ValueError("out may not be q")
     kn = vn = (0, 0, 0)
     if k_new is not None and v_new is not None:
         if k_new.shape != (b, kv, d) or v_new.shape != (b, kv, d):
