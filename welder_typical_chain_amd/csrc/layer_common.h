@@ -114,9 +114,9 @@ struct AttnParams {
   int64_t kn_stride[2], vn_stride[2];
   int64_t window;  // INT32_MAX at most (no limit)
   float *part_out, *part_lse;  // of a row's splits: normalised results and log-sum-exp
-  float* part_far;
+  float *part_near, *part_far;
   int32_t splits, row_blocks;
-  int32_t key_blocks, far_blocks, far_chunks, far_keys;
+  int32_t key_blocks, near_blocks, near_chunks, far_blocks, far_chunks, far_keys;
   int32_t batch, heads, kv_heads, group, lq, lk, dim, sinks;
   float scale;
 };

@@ -36,10 +36,10 @@ int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);
 // p.part_out: attention_workspace() bytes
 hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, hipStream_t stream);
 struct AttnBackwardPlan {
-  int key_blocks, far_blocks, far_chunks, far_keys;
-  int64_t part_at, workspace;  // bytes
+  int key_blocks, near_blocks, near_chunks, far_blocks, far_chunks, far_keys, cu_count;
+  int64_t part_at, far_at, workspace;  // bytes
 };
-AttnBackwardPlan plan_attention_backward(const AttnParams& p);
+AttnBackwardPlan plan_attention_backward(const AttnParams& p, int cu_count);
 // p.row_lse: plan.workspace bytes
 hipError_t launch_attention_backward(const AttnParams& p, const AttnBackwardPlan& plan, int dt, hipStream_t stream);
 int plan_decode(const AttnParams& p, int cu_count);  // splits

@@ -350,7 +350,7 @@ int wtc_window_attention(const wtc_attention_args* p, const void* q, const void*
 int64_t wtc_window_attention_backward_workspace_size(const wtc_attention_args* p) {
   if (!p) return bad("NULL arguments"), -1;
   if (guarded([&] { return check_attention_backward(*p); })) return -1;
-  return plan_attention_backward(attention_params(*p)).workspace;
+  return plan_attention_backward(attention_params(*p), cu_count()).workspace;
 }
 
 int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout, const void* q, const void* k,
@@ -366,7 +366,7 @@ int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout,
         !aligned16(dk) || !aligned16(dv))
       return bad("pointers must be 16-byte aligned");
     AttnParams a = attention_params(*p);
-    const AttnBackwardPlan plan = plan_attention_backward(a);
+    const AttnBackwardPlan plan = plan_attention_backward(a, cu_count());
     if (int rc = check_workspace(workspace, workspace_bytes, plan.workspace)) return rc;
     a.q = static_cast<const uint8_t*>(q);
     a.k = static_cast<const uint8_t*>(k);

@@ -453,22 +453,27 @@ template <int DT> __device__ inline void dkv_row(const AttnParams& p, int b, int
 
 // Row blocks and key tiles as in attention_tile_kernel; keys in subtiles of 32:
 //   S^T = K . Q^T, dP^T = V . dout^T, dq^T += K^T . dS^T
-constexpr int kDqWaves = 4;  // two workgroups a CU at dim 128
-template <int ND> struct DqLds {
+// 128 rows a workgroup: 4 waves, two workgroups a CU at dim 128, or with KG = 2 eight
+// waves that take every other tile for a row (where the grid leaves each workgroup
+// a CU of its own: train_ragged_f16 36 -> DQ_US us).
+constexpr int kDqRows = 128;
+template <int ND, int KG> struct DqLds {
   static constexpr int RB = row_bytes(ND), STAGES = 2;
-  static constexpr int TILE = kKeys * RB, STAGE = 2 * TILE;
-  static constexpr int PITCH = ND * 64 + 16;
-  static constexpr int RING = STAGES * STAGE, OUT = kDqWaves * 32 * PITCH;
+  static constexpr int TILE = kKeys * RB, STAGE = KG * 2 * TILE;
+  static constexpr int PITCH = ND * 64 + 16, JPITCH = ND * 128 + 16;
+  static constexpr int RING = STAGES * STAGE, OUT = kDqRows * (KG == 2 ? JPITCH : PITCH);
   static constexpr int TOTAL = RING > OUT ? RING : OUT;
+  static_assert(TOTAL <= 160 * 1024, "LDS");
 };
-template <int DT, int ND>
-__global__ void __launch_bounds__(kDqWaves * 64, 2) attention_dq_kernel(const AttnParams p) {
-  using L = DqLds<ND>;
-  constexpr int NW = kDqWaves;
+template <int DT, int ND, int KG>
+__global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnParams p) {
+  using L = DqLds<ND, KG>;
+  constexpr int NW = 4;
   constexpr int RB = L::RB, NS = 2 * ND;
   __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = wave_id % 4, group = wave_id / 4;  // rows, tiles
   const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
   const int blk = p.row_blocks - 1 - (int)(id % p.row_blocks);
   const int hk = (int)(id / p.row_blocks % p.kv_heads), b = (int)(id / p.row_blocks / p.kv_heads);
@@ -509,7 +514,7 @@ __global__ void __launch_bounds__(kDqWaves * 64, 2) attention_dq_kernel(const At
       if (lse == -INFINITY) delta = 0.0f;
       else lse2 = lse * kLog2e;
     }
-    if (half == 0 && i < p.lq) {
+    if (half == 0 && group == 0 && i < p.lq) {
       p.row_lse[stats_row(p, b, hk, i) + x] = lse2;
       p.row_delta[stats_row(p, b, hk, i) + x] = delta;
     }
@@ -529,21 +534,26 @@ __global__ void __launch_bounds__(kDqWaves * 64, 2) attention_dq_kernel(const At
   const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
   auto tile_base = [&](int t) { return t < t_sink ? t * kKeys : lo + (t - t_sink) * kKeys; };
   auto tile_end = [&](int t) { return t < t_sink ? s_end : end; };
-  auto issue = [&](int t) {
+  // step x: tile x KG + group
+  const int steps = (t_all + KG - 1) / KG;
+  auto issue = [&](int x) {
+    const int t = x * KG + group;
     const int j0 = tile_base(t), n = t < t_all ? min(kKeys, tile_end(t) - j0) : 0;
-    const uint32_t st = lds0 + (uint32_t)t % L::STAGES * L::STAGE;
+    const uint32_t st = lds0 + (uint32_t)x % L::STAGES * L::STAGE + group * 2 * L::TILE;
     lk.issue(st, j0, n);
     lv.issue(st + L::TILE, j0, n);
   };
 #pragma unroll
-  for (int t = 0; t < L::STAGES - 1; ++t) issue(t);
+  for (int x = 0; x < L::STAGES - 1; ++x) issue(x);
 
-  const uint32_t k_at = row_addr<RB>(lane), kc_at = col_addr<RB>(lane);
-  for (int t = 0; t < t_all; ++t) {
+  const uint32_t k_at = row_addr<RB>(lane) + group * 2 * L::TILE, kc_at = col_addr<RB>(lane) + group * 2 * L::TILE;
+  for (int x = 0; x < steps; ++x) {
     wait_loads_barrier<LOADS*(L::STAGES - 2)>();
-    issue(t + L::STAGES - 1);
+    issue(x + L::STAGES - 1);
+    const int t = x * KG + group;
+    if (t >= t_all) continue;
     const int j0 = tile_base(t), j1 = tile_end(t);
-    const uint32_t stage = (uint32_t)t % L::STAGES * L::STAGE;
+    const uint32_t stage = (uint32_t)x % L::STAGES * L::STAGE;
     uint32_t ka = k_at + stage, kc = kc_at + stage;
     fresh(ka);
     fresh(kc);
@@ -594,9 +604,30 @@ __global__ void __launch_bounds__(kDqWaves * 64, 2) attention_dq_kernel(const At
     }
   }
   wait_loads_barrier<0>();
+  if constexpr (KG == 2) {
+    uint8_t* at = smem + (wave * 32 + (lane & 31)) * L::JPITCH + half * 16;
+    if (group) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(at + (32 * d + 8 * g) * 4) = f32x4{dq[d][4 * g], dq[d][4 * g + 1], dq[d][4 * g + 2], dq[d][4 * g + 3]};
+    }
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(at + (32 * d + 8 * g) * 4);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) dq[d][4 * g + v] += y[v];
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
 
   bool nan = false;
-  uint8_t* stg = smem + wave * 32 * L::PITCH;
+  uint8_t* stg = smem + wave * 32 * (KG == 2 ? L::JPITCH : L::PITCH);
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -645,9 +676,11 @@ __global__ void __launch_bounds__(kDqWaves * 64, 2) attention_dq_kernel(const At
 // key.  A workgroup of their key block takes, like the others, the queries whose
 // window reaches the block; the far queries go in p.far_chunks short chunks to
 // workgroups of their own behind the key blocks.  All sums of the first tokens go
-// to p.part_far in f32, and attention_far_kernel adds them in order.  (In chunks as
+// to p.part_far in f32, and attention_sum_kernel adds them in order.  (In chunks as
 // long as a block's near queries they made 280 equal workgroups on 256 CUs for
 // train_bf16, a second round: 240 us against FAR_US.)
+// Where the key blocks alone leave CUs idle, the near queries go in p.near_chunks
+// parts as well, and every key's sums that way (train_ragged_f16 65 -> NEAR_US us).
 constexpr int kDkvWaves = 8;
 constexpr int kDkvKeys = 128;
 constexpr int kQueries = 64;
@@ -665,10 +698,13 @@ template <int ND> struct DkvLds {
   static_assert(TOTAL <= 160 * 1024, "LDS");
 };
 
-// part_far: [batch][kv_heads][far_blocks][1 + far_chunks][far_keys][dk, dv][dim];
-// slot 0 holds the near queries' sums
+// Sums of a part, [dk, dv][dim] of a key: part_near [batch][kv_heads][near_blocks]
+// [near_chunks][kDkvKeys], part_far [batch][kv_heads][far_blocks][far_chunks][far_keys].
+__device__ inline float* near_part(const AttnParams& p, int b, int hk, int kb, int slot, int key) {
+  return p.part_near + (((((int64_t)b * p.kv_heads + hk) * p.near_blocks + kb) * p.near_chunks + slot) * kDkvKeys + key) * 2 * p.dim;
+}
 __device__ inline float* far_part(const AttnParams& p, int b, int hk, int kb, int slot, int key) {
-  return p.part_far + (((((int64_t)b * p.kv_heads + hk) * p.far_blocks + kb) * (1 + p.far_chunks) + slot) * p.far_keys + key) * 2 * p.dim;
+  return p.part_far + (((((int64_t)b * p.kv_heads + hk) * p.far_blocks + kb) * p.far_chunks + slot) * p.far_keys + key) * 2 * p.dim;
 }
 
 template <int DT, int ND>
@@ -678,12 +714,13 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
   __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // workgroups of a (sequence, key head): the key blocks, then the far chunks
-  const int per = p.key_blocks + p.far_blocks * p.far_chunks;
+  // workgroups of a (sequence, key head): the key blocks' near chunks, then the far ones
+  const int near = p.key_blocks * p.near_chunks, per = near + p.far_blocks * p.far_chunks;
   const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
   const int w = (int)(id % per), hk = (int)(id / per % p.kv_heads), b = (int)(id / per / p.kv_heads);
-  const bool far = w >= p.key_blocks;
-  const int kb = far ? (w - p.key_blocks) / p.far_chunks : w, chunk = far ? (w - p.key_blocks) % p.far_chunks : 0;
+  const bool far = w >= near;
+  const int parts_of = far ? p.far_chunks : p.near_chunks;
+  const int kb = (far ? w - near : w) / parts_of, chunk = (far ? w - near : w) % parts_of;
   const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
   const int sub = wave >> 2;  // rows of a tile
   const int j_first = kb * kDkvKeys, j_wave = j_first + (wave & 3) * 32, j = j_wave + (lane & 31);
@@ -692,11 +729,15 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
   int i0 = min(max(0, j_first - shift), nq);
   int i1 = (int)max((int64_t)i0, min((int64_t)nq, (int64_t)min(j_first + kDkvKeys, nk) - 1 + p.window - shift));
   if (far) {
-    const int first = i1, share = (nq - first + p.far_chunks - 1) / p.far_chunks;
-    i0 = (int)min((int64_t)nq, first + (int64_t)chunk * share);
-    i1 = min(nq, i0 + share);
+    i0 = i1;
+    i1 = nq;
   }
   if (j_first >= nk) i1 = i0;
+  {
+    const int first = i0, last = i1, share = (last - first + parts_of - 1) / parts_of;
+    i0 = (int)min((int64_t)last, first + (int64_t)chunk * share);
+    i1 = min(last, i0 + share);
+  }
   const int hg = min(p.group, kQueries), chunks = (p.group + hg - 1) / hg;  // query heads a tile, tiles a position
   const int tp = kQueries / hg;                                             // positions a tile
 
@@ -863,10 +904,11 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
       for (int v = 0; v < 4; ++v) dk[d][4 * q + v] = y[4 * q + v] + z[v];  // (the result in dk from here on)
     }
   }
-  const bool parts = kb < p.far_blocks;
-  if (parts) {
-    if (j < p.sinks) {
-      float* dst = far_part(p, b, hk, kb, far ? 1 + chunk : 0, j - j_first) + sub * p.dim;
+  // keys whose sums the last kernel adds up: all, or the first tokens'
+  const int summed = p.near_chunks > 1 ? p.lk : kb < p.far_blocks ? p.sinks : 0;
+  if (summed > j_first) {
+    if (j < (far ? p.sinks : summed)) {
+      float* dst = (far ? far_part(p, b, hk, kb, chunk, j - j_first) : near_part(p, b, hk, kb, chunk, j - j_first)) + sub * p.dim;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -875,7 +917,7 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
           if (c < p.dim) *reinterpret_cast<f32x4*>(dst + c) = f32x4{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
         }
     }
-    if (far) return;
+    if (far || p.near_chunks > 1) return;
   }
   bool nan = false;
   const float scale = sub ? 1.0f : p.scale;
@@ -900,12 +942,12 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
 #pragma unroll 4
   for (int y = lane; y < 32 * CPR; y += 64) {
     const int row = y / CPR, c = y % CPR, jj = j_wave + row;
-    if (jj < p.lk && c * 8 < p.dim && !(parts && jj < p.sinks))
+    if (jj < p.lk && c * 8 < p.dim && jj >= summed)
       *reinterpret_cast<u32x4*>(dst + 2 * ((((int64_t)b * p.lk + jj) * p.kv_heads + hk) * p.dim) + c * 16) =
           *reinterpret_cast<const u32x4*>(mine + row * L::PITCH + c * 16);
   }
   // rows that came out as NaN, once both waves' results are written
-  nan = nan && !(parts && j < p.sinks);
+  nan = nan && j >= summed;
   uint32_t* marks = reinterpret_cast<uint32_t*>(smem + L::TOTAL - kDkvWaves * 4);
   const uint64_t ballot = __ballot(nan);
   if (lane == 0) marks[wave] = (uint32_t)(ballot | ballot >> 32);
@@ -919,30 +961,45 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
   }
 }
 
-// dk and dv of the first tokens: the sums of their blocks' chunks in order.  One wave a key.
+// dk and dv of the keys whose sums came in parts, the parts in order.  One wave a
+// key, four elements a lane.
 template <int DT>
-__global__ void __launch_bounds__(64) attention_far_kernel(const AttnParams p) {
-  using T = typename Elem<DT>::type;
-  const int lane = threadIdx.x;
-  const int j = (int)(blockIdx.x % p.sinks), hk = (int)(blockIdx.x / p.sinks % p.kv_heads), b = (int)(blockIdx.x / p.sinks / p.kv_heads);
+__global__ void __launch_bounds__(256) attention_sum_kernel(const AttnParams p) {
+  const int lane = threadIdx.x & 63;
+  const int keys = p.near_chunks > 1 ? p.lk : p.sinks;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= (int64_t)p.batch * p.kv_heads * keys) return;
+  const int j = (int)(at % keys), hk = (int)(at / keys % p.kv_heads), b = (int)(at / keys / p.kv_heads);
+  const int kb = j / kDkvKeys, key = j % kDkvKeys, c = lane * 4;
   bool nan = false;
-  for (int c = lane; c < 2 * p.dim; c += 64) {
-    const bool is_dv = c >= p.dim;
-    float sum = 0.0f;
-    const float* part = far_part(p, b, hk, j / kDkvKeys, 0, j % kDkvKeys) + c;
-    const int64_t step = (int64_t)p.far_keys * 2 * p.dim;
-    for (int s = 0; s <= p.far_chunks; s += 16) {  // 16 loads at a time, added in their order
-      float x[16];
+  if (c < 2 * p.dim) {
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto add = [&](const float* part, int64_t step, int count) {
+      for (int s = 0; s < count; s += 8) {  // 8 loads at a time, added in their order
+        f32x4 x[8];
 #pragma unroll
-      for (int u = 0; u < 16; ++u) x[u] = s + u <= p.far_chunks ? part[(s + u) * step] : 0.0f;
+        for (int u = 0; u < 8; ++u)
+          if (s + u < count) x[u] = *reinterpret_cast<const f32x4*>(part + (s + u) * step);
 #pragma unroll
-      for (int u = 0; u < 16; ++u) sum += x[u];
+        for (int u = 0; u < 8; ++u)
+          if (s + u < count) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) sum[v] += x[u][v];
+          }
+      }
+    };
+    add(near_part(p, b, hk, kb, 0, key) + c, (int64_t)kDkvKeys * 2 * p.dim, p.near_chunks);
+    if (p.far_chunks && j < p.sinks) add(far_part(p, b, hk, kb, 0, key) + c, (int64_t)p.far_keys * 2 * p.dim, p.far_chunks);
+    const bool is_dv = c >= p.dim, valid = j < seq_keys(p, b);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      sum[v] = valid ? sum[v] * (is_dv ? 1.0f : p.scale) : 0.0f;
+      nan |= sum[v] != sum[v];
     }
-    if (!is_dv) sum *= p.scale;
-    if (j >= seq_keys(p, b)) sum = 0.0f;
-    nan |= sum != sum;
-    T* dst = (T*)(is_dv ? p.dv : p.dk) + (((int64_t)b * p.lk + j) * p.kv_heads + hk) * p.dim;
-    dst[is_dv ? c - p.dim : c] = (T)sum;
+    uint32_t w0, w1;
+    pack4<DT>(sum, &w0, &w1);
+    uint8_t* dst = (is_dv ? p.dv : p.dk) + 2 * ((((int64_t)b * p.lk + j) * p.kv_heads + hk) * p.dim + (is_dv ? c - p.dim : c));
+    *reinterpret_cast<u32x2*>(dst) = u32x2{w0, w1};
   }
   if (!__any(nan)) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1003,13 +1060,13 @@ hipError_t launch_attention(const AttnParams& params, const AttnPlan& plan, int 
 }
 
 namespace {
-template <int DT> const void* dq_kernel(int nd) {
+template <int DT, int KG> const void* dq_kernel(int nd) {
   switch (nd) {
-    case 1: return (const void*)&attention_dq_kernel<DT, 1>;
-    case 2: return (const void*)&attention_dq_kernel<DT, 2>;
-    case 3: return (const void*)&attention_dq_kernel<DT, 3>;
+    case 1: return (const void*)&attention_dq_kernel<DT, 1, KG>;
+    case 2: return (const void*)&attention_dq_kernel<DT, 2, KG>;
+    case 3: return (const void*)&attention_dq_kernel<DT, 3, KG>;
   }
-  return (const void*)&attention_dq_kernel<DT, 4>;
+  return (const void*)&attention_dq_kernel<DT, 4, KG>;
 }
 template <int DT> const void* dkv_kernel(int nd) {
   switch (nd) {
@@ -1021,8 +1078,9 @@ template <int DT> const void* dkv_kernel(int nd) {
 }
 }  // namespace
 
-AttnBackwardPlan plan_attention_backward(const AttnParams& p) {
+AttnBackwardPlan plan_attention_backward(const AttnParams& p, int cu_count) {
   AttnBackwardPlan plan{};
+  plan.cu_count = cu_count;
   plan.key_blocks = (p.lk + kDkvKeys - 1) / kDkvKeys;
   // queries past the near ones of the first block: at most the keys past them
   const int64_t far = std::min<int64_t>(p.lq, (int64_t)p.lk - (p.window + kDkvKeys) + 1);
@@ -1033,15 +1091,25 @@ AttnBackwardPlan plan_attention_backward(const AttnParams& p) {
     // share, and no more in all than there are key blocks (their sums take memory)
     plan.far_chunks = (int)std::max<int64_t>(1, std::min<int64_t>(plan.key_blocks / plan.far_blocks, far / 256));
   }
+  // near chunks while CUs are idle and a chunk keeps 8 tiles of 64 rows
+  const int64_t seqs = (int64_t)p.batch * p.kv_heads;
+  const int64_t tiles = std::min<int64_t>(p.lq, p.window + kDkvKeys) * p.group / kQueries;
+  plan.near_chunks = 1;
+  while (plan.near_chunks < 16 && seqs * plan.key_blocks * plan.near_chunks * 2 <= cu_count && tiles / (2 * plan.near_chunks) >= 4) plan.near_chunks *= 2;
+  plan.near_blocks = plan.near_chunks > 1 ? plan.key_blocks : plan.far_blocks;
   const int64_t rows = (int64_t)p.batch * p.lq * p.heads;
   plan.part_at = (rows * 8 + 255) / 256 * 256;
-  plan.workspace = plan.part_at + ((int64_t)p.batch * p.kv_heads * plan.far_blocks * (1 + plan.far_chunks) * plan.far_keys * 2 * p.dim * 4 + 255) / 256 * 256;
+  plan.far_at = plan.part_at + (seqs * plan.near_blocks * plan.near_chunks * kDkvKeys * 2 * p.dim * 4 + 255) / 256 * 256;
+  plan.workspace = plan.far_at + (seqs * plan.far_blocks * plan.far_chunks * plan.far_keys * 2 * p.dim * 4 + 255) / 256 * 256;
   return plan;
 }
 
 hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwardPlan& plan, int dt, hipStream_t stream) {
   AttnParams p = params;
-  p.part_far = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.row_lse) + plan.part_at);
+  p.part_near = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.row_lse) + plan.part_at);
+  p.part_far = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.row_lse) + plan.far_at);
+  p.near_blocks = plan.near_blocks;
+  p.near_chunks = plan.near_chunks;
   p.row_delta = p.row_lse + (int64_t)p.batch * p.lq * p.heads;
   p.key_blocks = plan.key_blocks;
   p.far_blocks = plan.far_blocks;
@@ -1050,15 +1118,18 @@ hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwar
   const int nd = (p.dim + 31) / 32;
   const int64_t seqs = (int64_t)p.batch * p.kv_heads;
   if (p.lq) {
-    p.row_blocks = (int)(((int64_t)p.lq * p.group + kDqWaves * 32 - 1) / (kDqWaves * 32));
-    const hipError_t e = launch(dt == DT_F16 ? dq_kernel<DT_F16>(nd) : dq_kernel<DT_BF16>(nd), seqs * p.row_blocks, kDqWaves * 64, p, stream);
+    p.row_blocks = (int)(((int64_t)p.lq * p.group + kDqRows - 1) / kDqRows);
+    const bool pairs = seqs * p.row_blocks <= plan.cu_count;
+    const void* fn = pairs ? (dt == DT_F16 ? dq_kernel<DT_F16, 2>(nd) : dq_kernel<DT_BF16, 2>(nd))
+                           : (dt == DT_F16 ? dq_kernel<DT_F16, 1>(nd) : dq_kernel<DT_BF16, 1>(nd));
+    const hipError_t e = launch(fn, seqs * p.row_blocks, pairs ? 512 : 256, p, stream);
     if (e != hipSuccess) return e;
   }
   if (!p.lk) return hipSuccess;
   const hipError_t e = launch(dt == DT_F16 ? dkv_kernel<DT_F16>(nd) : dkv_kernel<DT_BF16>(nd),
-                              seqs * (p.key_blocks + p.far_blocks * p.far_chunks), kDkvWaves * 64, p, stream);
-  if (e != hipSuccess || !p.far_blocks) return e;
-  return launch(WTC_BY_TYPE(attention_far_kernel, dt), seqs * p.sinks, 64, p, stream);
+                              seqs * (p.key_blocks * p.near_chunks + p.far_blocks * p.far_chunks), kDkvWaves * 64, p, stream);
+  if (e != hipSuccess || (p.near_chunks == 1 && !p.far_blocks)) return e;
+  return launch(WTC_BY_TYPE(attention_sum_kernel, dt), (seqs * (p.near_chunks > 1 ? p.lk : p.sinks) + 3) / 4, 256, p, stream);
 }
 
 }  // namespace wtc
