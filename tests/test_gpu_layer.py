@@ -42,7 +42,7 @@ def check_matmul(W, m, n, k, dtype, out_dtype, kind, bias, residual, trans, a=No
     assert torch.equal(out, again), "two calls differ"
 
 
-SIZES = [(1, 8, 8), (1, 64, 4096), (3, 136, 72), (8, 1024, 512), (16, 4096, 256), (33, 264, 1000), (64, 128, 64),
+SIZES = [(1, 8, 8), (1, 64, 4096), (16, 24, 2056), (17, 40, 4160), (7, 4104, 1032), (3, 136, 72), (8, 1024, 512), (16, 4096, 256), (33, 264, 1000), (64, 128, 64),
          (65, 72, 40), (127, 520, 128), (128, 128, 128), (129, 136, 136), (256, 256, 32), (257, 264, 2056),
          (300, 1000, 96), (513, 776, 520), (1024, 2048, 256)]
 

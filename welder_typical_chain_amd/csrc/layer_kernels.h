@@ -9,7 +9,7 @@ namespace wtc {
 struct MatmulPlan {
   int variant, splits, slabs;
 };
-MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, bool aks, int cu_count);
+MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, bool aks, bool bks, int cu_count);
 int64_t matmul_workspace(const MatmulPlan& plan, int64_t m, int64_t n);
 // aks / bks: the operand is strided along k (element (row, k) at k * ld + row) instead
 // of contiguous (row * ld + k); aks only with bks and out_dt == dt.

@@ -94,8 +94,8 @@ MatmulBackwardPlan plan_backward(const wtc_matmul_args& p) {
   const int cus = cu_count();
   q.chunk_rows = act_backward_chunk_rows(p.m, p.n, cus);
   q.chunks = std::max<int64_t>(1, (p.m + q.chunk_rows - 1) / q.chunk_rows);
-  q.da = plan_matmul(p.m, p.k, p.n, false, cus);
-  q.db = p.b_trans ? plan_matmul(p.n, p.k, p.m, true, cus) : plan_matmul(p.k, p.n, p.m, true, cus);
+  q.da = plan_matmul(p.m, p.k, p.n, false, p.b_trans, cus);
+  q.db = p.b_trans ? plan_matmul(p.n, p.k, p.m, true, true, cus) : plan_matmul(p.k, p.n, p.m, true, true, cus);
   q.sums_at = p.activation == WTC_ACT_NONE ? 0 : align256(p.m * p.n * 2);
   q.partial_at = q.sums_at + (q.chunks > 1 ? align256(q.chunks * p.n * 4) : 0);
   q.total = q.partial_at + align256(std::max(matmul_workspace(q.da, p.m, p.k), matmul_workspace(q.db, p.k, p.n)));
@@ -208,7 +208,7 @@ extern "C" {
 int64_t wtc_matmul_epilogue_workspace_size(const wtc_matmul_args* p) {
   if (!p) return bad("NULL arguments"), -1;
   if (guarded([&] { return check_matmul(*p, false); })) return -1;
-  return align256(matmul_workspace(plan_matmul(p->m, p->n, p->k, false, cu_count()), p->m, p->n));
+  return align256(matmul_workspace(plan_matmul(p->m, p->n, p->k, false, !p->b_trans, cu_count()), p->m, p->n));
 }
 
 int wtc_matmul_epilogue(const wtc_matmul_args* p, const void* a, const void* b, const void* bias,
@@ -221,7 +221,7 @@ int wtc_matmul_epilogue(const wtc_matmul_args* p, const void* a, const void* b, 
     if (!out || (p->k && (!a || !b))) return bad("NULL operand");
     if (!aligned16(a) || !aligned16(b) || !aligned16(out) || !aligned16(pre) || !aligned16(residual) || !aligned16(bias))
       return bad("pointers must be 16-byte aligned");
-    const MatmulPlan plan = plan_matmul(p->m, p->n, p->k, false, cu_count());
+    const MatmulPlan plan = plan_matmul(p->m, p->n, p->k, false, !p->b_trans, cu_count());
     if (int rc = check_workspace(workspace, workspace_bytes, align256(matmul_workspace(plan, p->m, p->n)))) return rc;
     MatmulParams q{};
     q.a = static_cast<const uint8_t*>(a);

@@ -79,6 +79,16 @@ __device__ inline void finish8(const MatmulParams& p, int64_t m, int64_t n, floa
   store8<OUT_DT>(p.out, m * p.ldo + n, z);
 }
 
+template <int DT, int OUT_DT> __device__ inline void finish(const MatmulParams& p, int64_t m, int64_t n, float (&z)[8]) {
+  switch (p.act) {
+    case WTC_ACT_NONE: return finish8<DT, OUT_DT, WTC_ACT_NONE>(p, m, n, z);
+    case WTC_ACT_RELU: return finish8<DT, OUT_DT, WTC_ACT_RELU>(p, m, n, z);
+    case WTC_ACT_GELU: return finish8<DT, OUT_DT, WTC_ACT_GELU>(p, m, n, z);
+    case WTC_ACT_GELU_TANH: return finish8<DT, OUT_DT, WTC_ACT_GELU_TANH>(p, m, n, z);
+    case WTC_ACT_SILU: return finish8<DT, OUT_DT, WTC_ACT_SILU>(p, m, n, z);
+  }
+}
+
 // Direct-to-LDS loads of one operand: wave w fills blocks nb*w .. of 1 KiB.
 // Rows (KC) and columns (KS) past the operand's end are parked at kOutOfRange,
 // whose loads give zeros; so are slabs from k_end on.
@@ -355,6 +365,65 @@ __global__ void __launch_bounds__(kThreads, (TM + TN) * kSlab * STAGES > 80 * 10
   }
 }
 
+// At most 16 rows against weights stored as [n][k] (decode): what counts is reading B
+// once.  A workgroup takes 16 rows of B (columns of the output) and all of k: its 8
+// waves take 64-element chunks of k in turn, straight from memory to registers as
+// MFMA fragments (v_mfma_f32_16x16x32, D = B . A^T: a chunk is one 128-byte line
+// of each row), and join their sums through LDS: one launch, and no partial
+// products in memory.  Against 64-row tiles with k-splits, us: 8 x 4096 x 4096 8.8
+// (10.7), 8 x 4096 x 1024 4.3 (7.7), 8 x 2048 x 2048 5.5 (8.5); what it reads of A
+// grows with the workgroups and a wave's chunks come 8 at a time, so large n and
+// long k go to the tiles (8 x 8192 x 8192 31.7 against 24.9).
+constexpr int kRowsWaves = 8;
+template <int DT> __device__ inline f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (DT == DT_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <int DT, int OUT_DT>
+__global__ void __launch_bounds__(kRowsWaves * 64, 2) matmul_rows_kernel(const MatmulParams p) {
+  __shared__ __attribute__((aligned(16))) float red[kRowsWaves][16][16];  // [.][m][n]
+  const int lane = threadIdx.x & 63, r = lane & 15, kq = (lane >> 4) * 8;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16;
+  // rows past the end take the last one's values; their results are not written
+  const uint8_t* b = p.b + 2 * ((int64_t)min(n0 + r, p.n - 1) * p.ldb + kq);
+  const uint8_t* a = p.a + 2 * ((int64_t)min(r, p.m - 1) * p.lda + kq);
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int U = 8;  // chunks requested at a time
+  for (int c0 = wave; c0 * 64 < p.k; c0 += kRowsWaves * U) {
+    u32x4 bf[U][2], af[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int k = (c0 + u * kRowsWaves) * 64 + s * 32;
+        const bool in = k + kq < p.k;
+        bf[u][s] = in ? *reinterpret_cast<const u32x4*>(b + 2 * (int64_t)k) : u32x4{0, 0, 0, 0};
+        af[u][s] = in ? *reinterpret_cast<const u32x4*>(a + 2 * (int64_t)k) : u32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) acc = mfma16<DT>(bf[u][s], af[u][s], acc);
+  }
+  *reinterpret_cast<f32x4*>(&red[wave][r][(lane >> 4) * 4]) = acc;
+  __syncthreads();
+  const int m = threadIdx.x >> 1, half = (threadIdx.x & 1) * 8;
+  const int64_t n = n0 + half;
+  if (m >= p.m || n >= p.n) return;
+  float z[8] = {};
+#pragma unroll
+  for (int w = 0; w < kRowsWaves; ++w) {
+    const f32x4* src = reinterpret_cast<const f32x4*>(&red[w][m][half]);
+    const f32x4 lo = src[0], hi = src[1];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) z[u] += lo[u], z[4 + u] += hi[u];
+  }
+  finish<DT, OUT_DT>(p, m, n, z);
+}
+
 // The partial products of all splits, summed in their order, and the epilogue.
 template <int DT, int OUT_DT>
 __global__ void __launch_bounds__(256) matmul_join_kernel(const MatmulParams p) {
@@ -368,14 +437,8 @@ __global__ void __launch_bounds__(256) matmul_join_kernel(const MatmulParams p) 
 #pragma unroll
     for (int u = 0; u < 8; ++u) z[u] += y[u];
   }
-  const int64_t m = at / p.n, n = at - m * p.n;
-  switch (p.act) {
-    case WTC_ACT_NONE: return finish8<DT, OUT_DT, WTC_ACT_NONE>(p, m, n, z);
-    case WTC_ACT_RELU: return finish8<DT, OUT_DT, WTC_ACT_RELU>(p, m, n, z);
-    case WTC_ACT_GELU: return finish8<DT, OUT_DT, WTC_ACT_GELU>(p, m, n, z);
-    case WTC_ACT_GELU_TANH: return finish8<DT, OUT_DT, WTC_ACT_GELU_TANH>(p, m, n, z);
-    case WTC_ACT_SILU: return finish8<DT, OUT_DT, WTC_ACT_SILU>(p, m, n, z);
-  }
+  const int64_t m = at / p.n;
+  finish<DT, OUT_DT>(p, m, at - m * p.n, z);
 }
 
 // dz = dout * act'(pre), rounded for the products; the columns' sums in f32 of
@@ -470,12 +533,13 @@ struct Variant {
 };
 constexpr Variant kVariants[] = {{256, 256, 0.58, 0.34, 10.0}, {256, 128, 0.34, 0.19, 7.0}, {128, 128, 0.28, 0.0, 5.0}, {64, 128, 0.22, 0.0, 3.5}};
 constexpr int kFewRows = 64;  // at most so many rows for the 64-row tile
+constexpr int kRowsVariant = 4, kRowsMost = 16;  // matmul_rows_kernel
 
 }  // namespace
 
 // The tile and the number of k-splits with the least estimate.  Splits cost a second
 // kernel (3.5 us) and their partial products' way to memory and back (6 TB/s).
-MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, bool aks, int cu_count) {
+MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, bool aks, bool bks, int cu_count) {
   MatmulPlan best{};
   double best_us = 0;
   const int64_t slabs = (k + kSlabK - 1) / kSlabK;
@@ -496,6 +560,9 @@ MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, bool aks, int cu_count) 
       }
     }
   }
+  // matmul_rows_kernel: a round of 16 columns a CU takes as long as k
+  const double rows_us = 2.5 + (double)((n + 16 * cu_count - 1) / (16 * cu_count)) * (0.5 + 1.45e-3 * (double)k);
+  if (!aks && !bks && m <= kRowsMost && rows_us < best_us) best = MatmulPlan{kRowsVariant, 1, 0};
   return best;
 }
 int64_t matmul_workspace(const MatmulPlan& plan, int64_t m, int64_t n) {
@@ -507,6 +574,11 @@ hipError_t launch_matmul(const MatmulParams& params, const MatmulPlan& plan, int
   MatmulParams p = params;
   p.splits = plan.splits;
   p.slabs = plan.slabs;
+  if (plan.variant == kRowsVariant) {
+    const void* fn = dt == DT_F16 ? (out_dt == DT_F32 ? (const void*)&matmul_rows_kernel<DT_F16, DT_F32> : (const void*)&matmul_rows_kernel<DT_F16, DT_F16>)
+                                  : (out_dt == DT_F32 ? (const void*)&matmul_rows_kernel<DT_BF16, DT_F32> : (const void*)&matmul_rows_kernel<DT_BF16, DT_BF16>);
+    return run(fn, ((int64_t)p.n + 15) / 16, kRowsWaves * 64, p, stream);
+  }
   const Variant& v = kVariants[plan.variant];
   const int64_t grid = ((int64_t)(p.m + v.tm - 1) / v.tm) * ((p.n + v.tn - 1) / v.tn) * p.splits;
   const bool f32 = out_dt == DT_F32;
