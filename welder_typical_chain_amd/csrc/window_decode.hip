@@ -11,6 +11,10 @@
 // heads of the group (up to 32) are columns of the same products:
 //   S^T = K . Q^T, O^T += V^T . P^T, online softmax as in window_attention.hip.
 // The waves' results are joined through LDS; splits by a second kernel.
+// 64 sequences of up to 16384 tokens, 32 / 8 heads of 128, 4100 visible keys: 172 us,
+// 5.5 TB/s in all and 6.2 on the CUs that still have work (sequences shorter than
+// the window end early).  Refilling a stage's K as soon as it is read, before its
+// V, changed nothing.
 #include <algorithm>
 
 #include "attention_common.h"

