@@ -8,6 +8,7 @@ namespace wtc {
 
 struct MatmulPlan {
   int variant, splits, slabs;
+  double us;  // estimate
 };
 MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, bool aks, bool bks, int cu_count);
 int64_t matmul_workspace(const MatmulPlan& plan, int64_t m, int64_t n);
@@ -15,6 +16,12 @@ int64_t matmul_workspace(const MatmulPlan& plan, int64_t m, int64_t n);
 // of contiguous (row * ld + k); aks only with bks and out_dt == dt.
 hipError_t launch_matmul(const MatmulParams& p, const MatmulPlan& plan, int dt, int out_dt, bool aks, bool bks,
                          hipStream_t stream);
+
+// da = x . y and db of an [m][k] . [k][n] product, whether one launch for both is
+// faster; bks: of da's second operand.
+bool pair_pays(const MatmulPlan& da, const MatmulPlan& db, int64_t m, int64_t n, int64_t k, int cu_count);
+MatmulPlan pair_plan(int64_t k);  // of one of them alone, k elements summed
+hipError_t launch_matmul_pair(const MatmulParams& da, const MatmulParams& db, int dt, bool bks, hipStream_t stream);
 
 struct ActBackwardParams {
   const void* dout;

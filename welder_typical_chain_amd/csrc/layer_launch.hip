@@ -87,6 +87,7 @@ int cu_count() {
 struct MatmulBackwardPlan {
   int64_t chunk_rows, chunks;
   MatmulPlan da, db;
+  bool pair;
   int64_t sums_at, partial_at, total;
 };
 MatmulBackwardPlan plan_backward(const wtc_matmul_args& p) {
@@ -96,6 +97,11 @@ MatmulBackwardPlan plan_backward(const wtc_matmul_args& p) {
   q.chunks = std::max<int64_t>(1, (p.m + q.chunk_rows - 1) / q.chunk_rows);
   q.da = plan_matmul(p.m, p.k, p.n, false, p.b_trans, cus);
   q.db = p.b_trans ? plan_matmul(p.n, p.k, p.m, true, true, cus) : plan_matmul(p.k, p.n, p.m, true, true, cus);
+  q.pair = pair_pays(q.da, q.db, p.m, p.n, p.k, cus);
+  if (q.pair) {  // da or db alone: the same tiles, so the same bits
+    q.da = pair_plan(p.n);
+    q.db = pair_plan(p.m);
+  }
   q.sums_at = p.activation == WTC_ACT_NONE ? 0 : align256(p.m * p.n * 2);
   q.partial_at = q.sums_at + (q.chunks > 1 ? align256(q.chunks * p.n * 4) : 0);
   q.total = q.partial_at + align256(std::max(matmul_workspace(q.da, p.m, p.k), matmul_workspace(q.db, p.k, p.n)));
@@ -287,33 +293,35 @@ int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, con
       q.act = (int)p->activation;
       if (int rc = launched(launch_act_backward(q, dt, stream), "activation gradient")) return rc;
     }
-    MatmulParams q{};
-    q.partial = reinterpret_cast<float*>(ws + plan.partial_at);
-    if (da && p->m && p->k) {  // dz [m][n] . B^T: B stored by rows is contiguous along n
-      q.a = dz;
-      q.b = static_cast<const uint8_t*>(b);
-      q.lda = ldz;
-      q.ldb = p->ldb;
-      q.out = da;
-      q.ldo = p->k;
-      q.m = (int)p->m;
-      q.n = (int)p->k;
-      q.k = (int)p->n;
-      if (int rc = launched(launch_matmul(q, plan.da, dt, dt, false, p->b_trans, stream), "da")) return rc;
-    }
-    if (db && p->n && p->k) {  // A^T . dz, or its transpose dz^T . A: both strided along m
-      const uint8_t* x = static_cast<const uint8_t*>(a);
-      q.a = p->b_trans ? dz : x;
-      q.b = p->b_trans ? x : dz;
-      q.lda = p->b_trans ? ldz : p->lda;
-      q.ldb = p->b_trans ? p->lda : ldz;
-      q.out = db;
-      q.m = (int)(p->b_trans ? p->n : p->k);
-      q.n = (int)(p->b_trans ? p->k : p->n);
-      q.ldo = q.n;
-      q.k = (int)p->m;
-      if (int rc = launched(launch_matmul(q, plan.db, dt, dt, true, true, stream), "db")) return rc;
-    }
+    const bool want_da = da && p->m && p->k, want_db = db && p->n && p->k;
+    MatmulParams x{}, y{};
+    x.partial = y.partial = reinterpret_cast<float*>(ws + plan.partial_at);
+    // dz [m][n] . B^T: B stored by rows is contiguous along n
+    x.a = dz;
+    x.b = static_cast<const uint8_t*>(b);
+    x.lda = ldz;
+    x.ldb = p->ldb;
+    x.out = da;
+    x.ldo = p->k;
+    x.m = (int)p->m;
+    x.n = (int)p->k;
+    x.k = (int)p->n;
+    // A^T . dz, or its transpose dz^T . A: both strided along m
+    const uint8_t* rows = static_cast<const uint8_t*>(a);
+    y.a = p->b_trans ? dz : rows;
+    y.b = p->b_trans ? rows : dz;
+    y.lda = p->b_trans ? ldz : p->lda;
+    y.ldb = p->b_trans ? p->lda : ldz;
+    y.out = db;
+    y.m = (int)(p->b_trans ? p->n : p->k);
+    y.n = (int)(p->b_trans ? p->k : p->n);
+    y.ldo = y.n;
+    y.k = (int)p->m;
+    if (want_da && want_db && plan.pair) return launched(launch_matmul_pair(x, y, dt, p->b_trans, stream), "da and db");
+    if (want_da)
+      if (int rc = launched(launch_matmul(x, plan.da, dt, dt, false, p->b_trans, stream), "da")) return rc;
+    if (want_db)
+      if (int rc = launched(launch_matmul(y, plan.db, dt, dt, true, true, stream), "db")) return rc;
     return WTC_OK;
   });
 }

@@ -18,6 +18,7 @@
 // bf16 8192 x 8192 x 4096: 465 us, 1180 TFLOP/s (a library product of that size
 // 1270); with bias and gelu 508.  Full tiles are bound by the matrix cores at the
 // clock that the power limit leaves; small ones by the tiles' count and latency.
+#include <algorithm>
 #include <type_traits>
 
 #include "layer_common.h"
@@ -173,16 +174,15 @@ template <int TM, int TN, int STAGES> struct TileLds {
 // Grid: tiles * splits; split s takes k-slabs [s * slabs, (s + 1) * slabs) and, where
 // there are several, writes f32 partial products [split][m][n] to p.partial.
 template <int DT, int OUT_DT, bool AKS, bool BKS, int TM, int TN, int STAGES>
-__global__ void __launch_bounds__(kThreads, (TM + TN) * kSlab * STAGES > 80 * 1024 ? 1 : 2) matmul_tile_kernel(const MatmulParams p) {
+__device__ inline void matmul_tile(const MatmulParams& p, uint32_t block, uint32_t grid, uint8_t* smem) {
   using L = TileLds<TM, TN, STAGES>;
   constexpr int WM = TM / 64, WN = TN / 64;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
   const uint32_t rows = (uint32_t)(p.m + TM - 1) / TM, cols = (uint32_t)(p.n + TN - 1) / TN;
   uint32_t rt, ct;  // all splits of a tile row are rows of the map
-  tile_of_block(blockIdx.x, gridDim.x, rows * p.splits, cols, &rt, &ct);
+  tile_of_block(block, grid, rows * p.splits, cols, &rt, &ct);
   const uint32_t split = rt / rows;
   rt -= split * rows;
   const uint32_t row0 = rt * TM, n0 = ct * TN;
@@ -366,6 +366,25 @@ __global__ void __launch_bounds__(kThreads, (TM + TN) * kSlab * STAGES > 80 * 10
     case WTC_ACT_GELU_TANH: return epilogue(std::integral_constant<int, WTC_ACT_GELU_TANH>{});
     case WTC_ACT_SILU: return epilogue(std::integral_constant<int, WTC_ACT_SILU>{});
   }
+}
+
+constexpr int waves_per_simd(int tm, int tn, int stages) { return (tm + tn) * kSlab * stages > 80 * 1024 ? 1 : 2; }
+template <int DT, int OUT_DT, bool AKS, bool BKS, int TM, int TN, int STAGES>
+__global__ void __launch_bounds__(kThreads, waves_per_simd(TM, TN, STAGES)) matmul_tile_kernel(const MatmulParams p) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[TileLds<TM, TN, STAGES>::TOTAL];
+  matmul_tile<DT, OUT_DT, AKS, BKS, TM, TN, STAGES>(p, blockIdx.x, gridDim.x, smem);
+}
+
+// da (x) and db (y) of a small layer in one launch: neither fills the chip alone.
+// The one with more slabs a tile comes first.  The whole backward call, us: 1000 x
+// 1000 x 1000 37.1 -> 24.9, 2048 x 2048 x 1024 53.7 -> 36.8, 128 x 512 x 512 17.6 ->
+// 13.0; 4096 x 1024 x 1024 49.8 -> 49.0, where it ends to pay.
+template <int DT, bool BKS>
+__global__ void __launch_bounds__(kThreads, 2) matmul_pair_kernel(const MatmulParams x, const MatmulParams y, const uint32_t x_from, const uint32_t x_tiles, const uint32_t y_from) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[TileLds<128, 128, 4>::TOTAL];
+  const uint32_t b = blockIdx.x;
+  if (b >= x_from && b - x_from < x_tiles) matmul_tile<DT, DT, false, BKS, 128, 128, 4>(x, b - x_from, x_tiles, smem);
+  else matmul_tile<DT, DT, true, true, 128, 128, 4>(y, b - y_from, gridDim.x - x_tiles, smem);
 }
 
 // At most 16 rows against weights stored as [n][k] (decode): what counts is reading B
@@ -559,15 +578,42 @@ MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, bool aks, bool bks, int 
       if (splits > 1) us += 3.5 + 2.0 * (double)(splits * m * n) * 4 / 6.0e6;
       if (best_us == 0 || us < best_us) {
         best_us = us;
-        best = MatmulPlan{v, (int)splits, (int)per};
+        best = MatmulPlan{v, (int)splits, (int)per, us};
       }
     }
   }
   // matmul_rows_kernel: a round of 16 columns a CU takes as long as k
   const double rows_us = 2.5 + (double)((n + 16 * cu_count - 1) / (16 * cu_count)) * (0.5 + 1.45e-3 * (double)k);
-  if (!aks && !bks && m <= kRowsMost && rows_us < best_us) best = MatmulPlan{kRowsVariant, 1, 0};
+  if (!aks && !bks && m <= kRowsMost && rows_us < best_us) best = MatmulPlan{kRowsVariant, 1, 0, rows_us};
   return best;
 }
+// Both products of a backward pass as 128 x 128 tiles of one launch: the sum of their
+// work over the chip, at least the longer one's tile; against one after the other
+// with a launch (4 us) between.
+bool pair_pays(const MatmulPlan& da, const MatmulPlan& db, int64_t m, int64_t n, int64_t k, int cu_count) {
+  const Variant& t = kVariants[2];
+  auto tiles = [](int64_t a, int64_t b) { return ((a + 127) / 128) * ((b + 127) / 128); };
+  auto slabs = [](int64_t x) { return (x + kSlabK - 1) / kSlabK; };
+  const double work = (double)(tiles(m, k) * slabs(n) + tiles(k, n) * slabs(m)) / cu_count;
+  const double longest = (double)std::max(slabs(n), slabs(m));
+  // (a CU takes whole tiles: on average half of one more than its share)
+  return t.fixed_us + t.slab_us * (std::max(work, longest) + 0.5 * longest) < da.us + db.us + 4.0;
+}
+MatmulPlan pair_plan(int64_t k) { return MatmulPlan{2, 1, (int)((k + kSlabK - 1) / kSlabK), 0.0}; }
+hipError_t launch_matmul_pair(const MatmulParams& da, const MatmulParams& db, int dt, bool bks, hipStream_t stream) {
+  MatmulParams x = da, y = db;
+  x.splits = y.splits = 1;
+  x.slabs = (x.k + kSlabK - 1) / kSlabK;
+  y.slabs = (y.k + kSlabK - 1) / kSlabK;
+  auto tiles = [](const MatmulParams& p) { return (uint32_t)(((p.m + 127) / 128) * ((p.n + 127) / 128)); };
+  uint32_t x_tiles = tiles(x), y_tiles = tiles(y);
+  uint32_t x_from = x.slabs >= y.slabs ? 0 : y_tiles, y_from = x.slabs >= y.slabs ? x_tiles : 0;
+  void* args[] = {&x, &y, &x_from, &x_tiles, &y_from};
+  const void* fn = dt == DT_F16 ? (bks ? (const void*)&matmul_pair_kernel<DT_F16, true> : (const void*)&matmul_pair_kernel<DT_F16, false>)
+                                : (bks ? (const void*)&matmul_pair_kernel<DT_BF16, true> : (const void*)&matmul_pair_kernel<DT_BF16, false>);
+  return hipLaunchKernel(fn, dim3(x_tiles + y_tiles), dim3(kThreads), args, 0, stream);
+}
+
 int64_t matmul_workspace(const MatmulPlan& plan, int64_t m, int64_t n) {
   return plan.splits > 1 ? plan.splits * m * n * 4 : 0;
 }
