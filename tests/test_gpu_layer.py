@@ -86,6 +86,12 @@ def test_matmul_empty(W):
     bias = rand(3, 32, dtype=F16)
     out = W.matmul_epilogue(rand(1, 5, 0, dtype=F16), rand(2, 0, 32, dtype=F16), bias=bias, activation="relu")
     assert torch.equal(out, torch.relu(bias).expand(5, 32))
+    out = W.matmul_epilogue(rand(1, 5, 64, dtype=F16), rand(2, 64, 0, dtype=F16), activation="silu")
+    assert out.shape == (5, 0)
+    for m in (5, 40):
+        x, w = rand(1, m, 64, dtype=F16), rand(2, 64, 0, dtype=F16)
+        da, db, dbias = W.matmul_epilogue_backward(rand(1, m, 0, dtype=F16), x, w)
+        assert bool((da == 0).all()) and db.shape == (64, 0) and dbias.shape == (0,)
     da, db, dbias = W.matmul_epilogue_backward(rand(1, 0, 32, dtype=F16), a, b)
     assert da.shape == (0, 64) and bool((db == 0).all()) and bool((dbias == 0).all())
 
@@ -202,7 +208,7 @@ def test_attention_scales(W, scale):
     check_decode(W, [3, 100, 300], 120, 2, 2, 64, BF16, window=50, sinks=2, scale=scale)
 
 
-@pytest.mark.parametrize("h,kv", [(1, 1), (8, 1), (6, 2), (7, 7), (12, 4), (32, 2)])
+@pytest.mark.parametrize("h,kv", [(1, 1), (8, 1), (6, 2), (7, 7), (12, 4), (32, 2), (64, 1), (80, 1), (140, 1)])
 def test_attention_heads(W, h, kv):
     q, k, v, g = qkv(31, 2, 90, 90, h, kv, 64, F16)
     check_attention(W, q, k, v, g, window=33, sinks=3)
@@ -596,6 +602,40 @@ def test_two_graphs_and_streams_at_once(W):
     for rounds, want in zip(eager, (want1, want2)):
         for r in rounds:
             assert all(torch.equal(x, y) for x, y in zip(r, want))
+
+
+def test_calls_from_several_host_threads(W):
+    import threading
+    args = []
+    for i in range(4):
+        q, k, v, g = qkv(20 + 10 * i, 1, 300 + 50 * i, 300 + 50 * i, 4, 2, 64, BF16)
+        args.append((q, k, v, g, rand(5 + i, 8 + 30 * i, 512, dtype=BF16), rand(50 + i, 256, 512, dtype=BF16).t()))
+
+    def work(q, k, v, g, a, b):
+        out, lse = W.window_attention(q, k, v, window=70, sinks=4, return_lse=True)
+        n = torch.full((1,), k.shape[1], dtype=torch.int32, device="cuda")
+        return [out, *W.window_attention_backward(g, q, k, v, out, lse, window=70, sinks=4),
+                W.window_attention_decode(q[:, 0], k, v, n), W.matmul_epilogue(a, b, activation="gelu")]
+
+    want = [work(*x) for x in args]
+    torch.cuda.synchronize()
+    got, streams = [[] for _ in args], [torch.cuda.Stream() for _ in args]
+
+    def run(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(10):
+                got[i].append(work(*args[i]))
+        streams[i].synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(args))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for rounds, ref in zip(got, want):
+        assert len(rounds) == 10
+        for r in rounds:
+            assert all(torch.equal(x, y) for x, y in zip(r, ref))
 
 
 def test_refusals_on_the_gpu(W):

@@ -116,7 +116,9 @@ def _weights(b, k):
     if b.dim() != 2 or b.shape[0] != k:
         raise ValueError(f"b must be [{k}, N], is {tuple(b.shape)}")
     n = b.shape[1]
-    if b.stride(1) == 1 and (b.stride(0) >= n or k <= 1) or n == 0 or k == 0:
+    if n == 0 or k == 0:
+        return n, n, 0
+    if b.stride(1) == 1 and (b.stride(0) >= n or k <= 1):
         return n, max(b.stride(0) if k > 1 else n, n), 0
     if b.stride(0) == 1 and (b.stride(1) >= k or n <= 1):
         return n, max(b.stride(1) if n > 1 else k, k), 1
