@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
   const int hk = (int)(id / p.row_blocks % p.kv_heads), b = (int)(id / p.row_blocks / p.kv_heads);
   const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
   const int r0 = blk * NW * 32;
-  const int r = r0 + wave * 32 + (lane & 31), i = r / p.group, x = r - i * p.group, h = hk * p.group + x;
+  const int r = r0 + wave * 32 + (lane & 31), i = r / p.group, x_head = r - i * p.group, h = hk * p.group + x_head;
   const bool valid = i < nq;
   const int pos = valid ? i + shift : -1;
   const int i_last = min((r0 + NW * 32 - 1) / p.group, nq - 1);
@@ -517,18 +517,8 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
       if (lse == -INFINITY) delta = 0.0f;
       else lse2 = lse * kLog2e;
     }
-    if (half == 0 && group == 0 && i < p.lq) {
-      p.row_lse[stats_row(p, b, hk, i) + x] = lse2;
-      p.row_delta[stats_row(p, b, hk, i) + x] = delta;
-    }
   }
   const float c2 = positive_scale<NS>(p.scale, qf);
-
-  f32x16 dq[ND];
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) dq[d][v] = 0.0f;
 
   TileLoader<RB, kKeys, NW> lk, lv;
   lk.init(p.k + 2 * (b * p.k_stride[0] + hk * p.k_stride[2]), 2 * p.k_stride[1], p.dim, wave, lane);
@@ -546,49 +536,98 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
     lk.issue(st, j0, n);
     lv.issue(st + L::TILE, j0, n);
   };
+  const uint32_t k_at = row_addr<RB>(lane) + group * 2 * L::TILE, kc_at = col_addr<RB>(lane) + group * 2 * L::TILE;
+  // Weights s and dP g of subtile u of step x; false: none of the wave's rows sees it.
+  auto weights = [&](int x, int u, uint32_t ka, f32x16& s, f32x16& g) {
+    const int t = x * KG + group;
+    const int j0 = tile_base(t), j1 = tile_end(t);
+    const int k0 = j0 + 32 * u;
+    const bool below = t >= t_sink && (int64_t)k0 + 31 + p.window <= w_lo && k0 >= p.sinks;
+    if (t >= t_all || !w_any || k0 > w_hi || k0 >= j1 || below) return false;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
+#pragma unroll
+    for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u, st), qf[st], s);
+    if (k0 + 32 > j1 || k0 + 31 > w_lo || (t >= t_sink && (int64_t)k0 + p.window <= w_hi)) {
+      const uint64_t seen = seen_bits(k0 + 4 * half, j1, pos, p.window, p.sinks);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[v] = keep_bit(s[v], seen, 8 * (v >> 2) + (v & 3));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // the exponentials among the products of dP
+#pragma unroll
+    for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u + kKeys, st), gf[st], g);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c2, -lse2));
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+    for (int x = 0; x < NS; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 32 / NS, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    return true;
+  };
+  auto weights_at = [&](int x) {
+    uint32_t ka = k_at + (uint32_t)x % L::STAGES * L::STAGE;
+    fresh(ka);
+    return ka;
+  };
+
+  // D from the rounded `out` is off by that rounding times |dout|, which shows where
+  // weights are large: in rows of few keys.  Blocks of at most two tiles sum it
+  // themselves first, D = sum_j P dP (dq of causal rows in f16 1.48 -> 1.42
+  // roundings off 64 bits; the D of later rows changes nothing there).
+  if (t_all <= 2) {
+#pragma unroll
+    for (int x = 0; x < L::STAGES - 1; ++x) issue(x);
+    float sum = 0.0f;
+    for (int x = 0; x < steps; ++x) {
+      wait_loads_barrier<LOADS*(L::STAGES - 2)>();
+      issue(x + L::STAGES - 1);
+#pragma unroll 1
+      for (int u = 0; u < 2; ++u) {
+        f32x16 s, g;
+        if (!weights(x, u, weights_at(x), s, g)) continue;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sum += s[v] == 0.0f ? 0.0f : s[v] * g[v];  // (a hidden key's dP may be anything)
+      }
+    }
+    wait_loads_barrier<0>();
+    sum = xor32_sum(sum);
+    if constexpr (KG == 2) {  // the other group's tiles
+      float* part = reinterpret_cast<float*>(smem);
+      if (half == 0) part[wave_id * 32 + (lane & 31)] = sum;
+      __syncthreads();
+      sum = part[wave * 32 + (lane & 31)] + part[(4 + wave) * 32 + (lane & 31)];
+      __syncthreads();
+    }
+    delta = sum;
+  }
+  if (half == 0 && group == 0 && i < p.lq) {
+    p.row_lse[stats_row(p, b, hk, i) + x_head] = lse2;
+    p.row_delta[stats_row(p, b, hk, i) + x_head] = delta;
+  }
+
+  f32x16 dq[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) dq[d][v] = 0.0f;
+
 #pragma unroll
   for (int x = 0; x < L::STAGES - 1; ++x) issue(x);
-
-  const uint32_t k_at = row_addr<RB>(lane) + group * 2 * L::TILE, kc_at = col_addr<RB>(lane) + group * 2 * L::TILE;
   for (int x = 0; x < steps; ++x) {
     wait_loads_barrier<LOADS*(L::STAGES - 2)>();
     issue(x + L::STAGES - 1);
-    const int t = x * KG + group;
-    if (t >= t_all) continue;
-    const int j0 = tile_base(t), j1 = tile_end(t);
-    const uint32_t stage = (uint32_t)x % L::STAGES * L::STAGE;
-    uint32_t ka = k_at + stage, kc = kc_at + stage;
-    fresh(ka);
+    uint32_t kc = kc_at + (uint32_t)x % L::STAGES * L::STAGE;
     fresh(kc);
+    const uint32_t ka = weights_at(x);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int k0 = j0 + 32 * u;
-      const bool below = t >= t_sink && (int64_t)k0 + 31 + p.window <= w_lo && k0 >= p.sinks;
-      if (!w_any || k0 > w_hi || k0 >= j1 || below) continue;
       f32x16 s, g;
-#pragma unroll
-      for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
-#pragma unroll
-      for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u, st), qf[st], s);
-      if (k0 + 32 > j1 || k0 + 31 > w_lo || (t >= t_sink && (int64_t)k0 + p.window <= w_hi)) {
-        const uint64_t seen = seen_bits(k0 + 4 * half, j1, pos, p.window, p.sinks);
-#pragma unroll
-        for (int v = 0; v < 16; ++v) s[v] = keep_bit(s[v], seen, 8 * (v >> 2) + (v & 3));
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      // the exponentials among the products of dP
-#pragma unroll
-      for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u + kKeys, st), gf[st], g);
-#pragma unroll
-      for (int v = 0; v < 16; ++v) s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c2, -lse2));
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-#pragma unroll
-      for (int x = 0; x < NS; ++x) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 32 / NS, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      if (!weights(x, u, ka, s, g)) continue;
       u32x4 df[2];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
