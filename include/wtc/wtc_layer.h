@@ -16,7 +16,9 @@
  * buffers are the caller's.  Where a *_workspace_size function says that a
  * call needs scratch memory, the caller passes it (256-byte aligned,
  * uninitialised; calls that may overlap must not share one); too little of it
- * is WTC_ERR_WORKSPACE.  Calls may come from any host thread.  Results do not
+ * is WTC_ERR_WORKSPACE.  Outputs may not overlap inputs, but for the residual,
+ * which may be the output itself, and the caches that decode appends to.  Calls
+ * may come from any host thread.  Results do not
  * depend on timing: nothing is summed by atomics.
  */
 #ifndef WTC_LAYER_H
