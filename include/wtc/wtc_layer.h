@@ -18,8 +18,8 @@
  * uninitialised; calls that may overlap must not share one); too little of it
  * is WTC_ERR_WORKSPACE.  Outputs may not overlap inputs, but for the residual,
  * which may be the output itself, and the caches that decode appends to.  Calls
- * may come from any host thread.  Results do not
- * depend on timing: nothing is summed by atomics.
+ * may come from any host thread.  Results do not depend on timing: nothing is
+ * summed by atomics.
  */
 #ifndef WTC_LAYER_H
 #define WTC_LAYER_H

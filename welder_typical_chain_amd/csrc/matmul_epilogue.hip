@@ -31,12 +31,6 @@ constexpr int kSlab = 64;    // bytes of k per ring stage and operand row
 constexpr int kSlabK = 32;   // elements
 constexpr int kThreads = 256;
 
-__device__ inline float load_elem(const void* p, int64_t i, int dt) {
-  if (dt == DT_F32) return static_cast<const float*>(p)[i];
-  if (dt == DT_F16) return (float)static_cast<const _Float16*>(p)[i];
-  return (float)static_cast<const __bf16*>(p)[i];
-}
-
 // Eight consecutive values, 16-byte aligned.
 template <int DT> __device__ inline void load8(const void* p, int64_t i, float (&x)[8]) {
   if constexpr (DT == DT_F32) {

@@ -723,8 +723,8 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
 // 4096 tokens, 8 key heads, window 1024, 4 first tokens, a second round: 240 us
 // against 210.)
 // Where the key blocks alone leave CUs idle, the near queries go in p.near_chunks
-// parts as well, and every key's sums that way (3 x 1000
-// causal tokens, 6 / 3 heads of 80: 65 -> 40 us, and 6 for the sums).
+// parts as well, and every key's sums that way (3 x 1000 causal tokens, 6 / 3 heads
+// of 80: 65 -> 40 us, and 6 for the sums).
 // Both kernels on 4 x 4096 causal tokens, 32 / 8 heads of 128: 2017 us, 682 TFLOP/s by
 // the usual count of 5 products and 955 by the 7 that they run.
 constexpr int kDkvWaves = 8;
@@ -1074,7 +1074,7 @@ template <int DT, int KG> const void* tile_kernel(int nd) {
 }  // namespace
 
 // Rows a workgroup (256 / key_groups) and splits of the keys, from the sizes alone:
-// splits while CUs are idle and a workgroup keeps 8 tiles.
+// splits while CUs are idle and a wave keeps 4 tiles.
 AttnPlan plan_attention(const AttnParams& p, int cu_count) {
   AttnPlan plan{1, 1};
   const int64_t rows = (int64_t)p.lq * p.group, seqs = (int64_t)p.batch * p.kv_heads;
@@ -1137,7 +1137,7 @@ AttnBackwardPlan plan_attention_backward(const AttnParams& p, int cu_count) {
     // share, and no more in all than there are key blocks (their sums take memory)
     plan.far_chunks = (int)std::max<int64_t>(1, std::min<int64_t>(plan.key_blocks / plan.far_blocks, far / 256));
   }
-  // near chunks while CUs are idle and a chunk keeps 8 tiles of 64 rows
+  // near chunks while CUs are idle and a chunk keeps 4 tiles of 64 rows
   const int64_t seqs = (int64_t)p.batch * p.kv_heads;
   const int64_t tiles = std::min<int64_t>(p.lq, p.window + kDkvKeys) * p.group / kQueries;
   plan.near_chunks = 1;
