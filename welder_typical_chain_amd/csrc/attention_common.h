@@ -165,19 +165,22 @@ __device__ inline float join_splits(const float* part, const float* lse, int spl
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int s0 = 0; s0 < splits; s0 += 4) {
     f32x4 x[4];
-    float w[4];
+    float l[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int s = min(s0 + u, splits - 1);
       x[u] = *reinterpret_cast<const f32x4*>(part + (int64_t)s * dim + c);
-      w[u] = s0 + u < splits ? __builtin_amdgcn_exp2f(lse[s] - ref) : 0.0f;
+      l[u] = s0 + u < splits ? lse[s] : -INFINITY;
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (w[u] == 0.0f) continue;  // nothing there: whatever it holds does not count
-      total += w[u];
+      // No keys there: whatever it holds does not count.  Where there are keys a NaN
+      // counts, also if their weight beside the others' is 0, as it does inside a tile.
+      if (l[u] == -INFINITY) continue;
+      const float w = __builtin_amdgcn_exp2f(l[u] - ref);
+      total += w;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) acc[v] = __builtin_fmaf(w[u], x[u][v], acc[v]);
+      for (int v = 0; v < 4; ++v) acc[v] = __builtin_fmaf(w, x[u][v], acc[v]);
     }
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;

@@ -206,9 +206,10 @@ __global__ void __launch_bounds__(kWaves * 64, 1) decode_kernel(const AttnParams
     float sum = 0.0f, y[8] = {};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
+      // (a wave without keys has a maximum of -inf and zeros; one whose scores are all NaN
+      // has that maximum too, which leaves NaN out, and its sum says so)
       const float2 st = stat[w * kHeads + q];
-      const float f = st.x == -INFINITY && st.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(st.x - ref);
-      if (f == 0.0f) continue;  // (nothing there, or NaN times a weight of 0)
+      const float f = __builtin_amdgcn_exp2f(st.x - ref);
       sum = __builtin_fmaf(st.y, f, sum);
       const float* src = res + (w * kHeads + q) * L::PITCH + c;
 #pragma unroll
