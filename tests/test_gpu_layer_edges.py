@@ -95,3 +95,108 @@ def test_decode_all_scores_minus_infinity(W):
     assert bool((W.window_attention_decode(q, kc, vc, lens(40)) == 0).all())
     assert bool((W.window_attention_decode(q, kc, vc, lens(100)) == 1).all())
     assert bool((W.window_attention_decode(q, kc, vc, lens(0)) == 0).all())
+
+
+# ---------------------------------------------------------------------------
+# activations: relative to their own size, also in the tails
+# ---------------------------------------------------------------------------
+E = U.E32
+#: error of an activation relative to |act(z)| besides the argument's own, in half
+#: steps of float32.  gelu: the tail's variable t = 1 / (1 + p u) is off by 3 (an fma, a
+#: reciprocal of one step), which the tail takes 3.4 times at most (near u = 0); its ten
+#: Horner steps 6; exp 2 and two roundings of its correction; three products.
+#: sigmoid: exp 4, sum 1, reciprocal 2, products 3.
+ACT_STEPS = {"gelu": 28, "silu": 14, "gelu_tanh": 14}
+
+
+#: exponentials and sigmoids below float32's normal numbers may become 0
+FLUSH = 2.0 ** -126
+
+
+def tanh_argument(z):
+    return 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+
+
+def act64(z, kind):
+    if kind == "gelu_tanh":  # (1 + tanh loses the negative tail even in 64 bits)
+        return z * torch.sigmoid(tanh_argument(z))
+    return U.act(z, kind)
+
+
+def slope64(z, kind):
+    if kind == "gelu":
+        return 0.5 * torch.erfc(-z / math.sqrt(2)) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    c = 2 * math.sqrt(2 / math.pi)
+    x = tanh_argument(z) if kind == "gelu_tanh" else z
+    dx = c * (1 + 3 * 0.044715 * z * z) if kind == "gelu_tanh" else 1.0
+    return torch.sigmoid(x) * (1 + z * dx * torch.sigmoid(-x))
+
+
+def argument_error(z, kind):
+    """Relative change of the tail by what the argument of the exponential is off: gelu_tanh
+    takes a polynomial that five roundings touch; the others keep theirs whole."""
+    if kind != "gelu_tanh":
+        return 0.0
+    return 5 * E * tanh_argument(z).abs()
+
+
+@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("out_dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows", [16, 4096])
+def test_activation_values_relative(W, kind, out_dtype, rows):
+    """z over [-12, 12], exact in 16 bits: what a (one column) times ones gives."""
+    dtype = BF16 if out_dtype == BF16 else F16
+    a = torch.zeros(rows, 8, dtype=dtype, device="cuda")
+    a[:, 0] = torch.linspace(-12, 12, rows, device="cuda").to(dtype)
+    trans = rows <= 16  # (few rows against [n, k] weights: the kernel without tiles)
+    b = torch.zeros(264, 8, dtype=dtype, device="cuda") if trans else torch.zeros(8, 264, dtype=dtype, device="cuda")
+    if trans:
+        b[:, 0] = 1
+        b = b.t()
+    else:
+        b[0] = 1
+    out = W.matmul_epilogue(a, b, activation=kind, out_dtype=out_dtype)
+    z = a[:, :1].double()
+    y = act64(z, kind)
+    err = (ACT_STEPS[kind] * E + argument_error(z, kind)) * y.abs() + FLUSH * z.abs()
+    if out_dtype != F32:
+        # for a 16-bit result the exponential's argument has three roundings more, and
+        # gelu's polynomial is off by 1.1e-6
+        size = {"gelu": z * z / 2, "silu": z.abs(), "gelu_tanh": tanh_argument(z).abs()}[kind]
+        err = err + (1.2e-6 + 3 * E * size) * y.abs()
+    bound = U.rounded(y, err, out_dtype)
+    U.assert_within(out, y.expand(out.shape), bound.expand(out.shape), kind)
+
+
+@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh", "silu"])
+def test_activation_slopes_relative(W, kind):
+    """dbias of one row with dout 1 is the slope, in float32.  Each of its two terms is off by
+    its own share, so near its zero the bound is that of the terms."""
+    n = 8192
+    pre = torch.linspace(-12, 12, n, device="cuda")[None].contiguous()
+    dout = torch.ones(1, n, dtype=F16, device="cuda")
+    a, b = torch.zeros(1, 8, dtype=F16, device="cuda"), torch.zeros(8, n, dtype=F16, device="cuda")
+    _, _, slope = W.matmul_epilogue_backward(dout, a, b, pre=pre, activation=kind, need_a=False, need_b=False)
+    z = pre[0].double()
+    want = slope64(z, kind)
+    first = act64(z, kind) / z  # Phi or the sigmoid
+    steps = ACT_STEPS[kind] + 6
+    # (what is flushed goes into the result times 1 + z times the argument's slope: 400 at most)
+    U.assert_within(slope, want, (steps * E + argument_error(z, kind)) * (first.abs() + (want - first).abs()) + 400 * FLUSH, kind)
+
+
+@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("z,value,slope", [(math.inf, math.inf, 1.0), (-math.inf, 0.0, 0.0), (3e38, 3e38, 1.0), (-3e38, 0.0, 0.0),
+                                           (1e19, 1e19, 1.0), (-1e19, 0.0, 0.0), (-200.0, 0.0, 0.0), (200.0, 200.0, 1.0), (0.0, 0.0, 0.5),
+                                           (NAN, NAN, NAN)])
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+def test_activation_limits(W, kind, z, value, slope, out_dtype):
+    a, b = torch.zeros(5, 0, dtype=BF16, device="cuda"), torch.zeros(0, 8, dtype=BF16, device="cuda")
+    bias = torch.full((8,), z, device="cuda")
+    out = W.matmul_epilogue(a, b, bias=bias, activation=kind, out_dtype=out_dtype)
+    want = torch.full_like(out, value)
+    assert bool(out.isnan().all()) if z != z else torch.equal(out, want), out[0, 0]
+    pre = bias[None].contiguous()
+    got = W.matmul_epilogue_backward(torch.ones(1, 8, dtype=BF16, device="cuda"), torch.zeros(1, 8, dtype=BF16, device="cuda"),
+                                     torch.zeros(8, 8, dtype=BF16, device="cuda"), pre=pre, activation=kind)[2]
+    assert bool(got.isnan().all()) if z != z else bool((got == slope).all()), got[0]

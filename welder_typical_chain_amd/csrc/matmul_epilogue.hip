@@ -68,7 +68,7 @@ __device__ inline void finish8(const MatmulParams& p, int64_t m, int64_t n, floa
   }
   if (p.pre) store8<DT_F32>(p.pre, m * p.ldp + n, z);
 #pragma unroll
-  for (int u = 0; u < 8; ++u) z[u] = act_value<ACT>(z[u]);
+  for (int u = 0; u < 8; ++u) z[u] = act_value<ACT, OUT_DT == DT_F32>(z[u]);
   if (p.residual) {
     load8<OUT_DT>(p.residual, m * p.ldr + n, y);
 #pragma unroll
@@ -342,7 +342,7 @@ __device__ inline void matmul_tile(const MatmulParams& p, uint32_t block, uint32
         const bool in = m < p.m && n < p.n;
         if (p.pre && in) store8<DT_F32>(p.pre, m * p.ldp + n, z);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) z[u] = act_value<decltype(act)::value>(z[u]);
+        for (int u = 0; u < 8; ++u) z[u] = act_value<decltype(act)::value, OUT_DT == DT_F32>(z[u]);
         if (p.residual) {
           load8<OUT_DT>(res[mt & 1][it], 0, y);
 #pragma unroll
