@@ -1,6 +1,7 @@
 """The layer operators on the GPU at values, sizes and calls at the edges of what
 their documentation allows, against plain 64-bit forms (tests/layer_util.py)."""
 import math
+from unittest import mock
 
 import pytest
 import torch
@@ -23,6 +24,11 @@ def rand(seed, *shape, dtype=F32, by=1.0):
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
     return (torch.randn(shape, generator=g, device="cuda") * by).to(dtype)
+
+
+def qkv(seed, b, lq, lk, h, kv, d, dtype):
+    return (rand(seed, b, lq, h, d, dtype=dtype), rand(seed + 1, b, lk, kv, d, dtype=dtype),
+            rand(seed + 2, b, lk, kv, d, dtype=dtype), rand(seed + 3, b, lq, h, d, dtype=dtype))
 
 
 # ---------------------------------------------------------------------------
@@ -200,3 +206,61 @@ def test_activation_limits(W, kind, z, value, slope, out_dtype):
     got = W.matmul_epilogue_backward(torch.ones(1, 8, dtype=BF16, device="cuda"), torch.zeros(1, 8, dtype=BF16, device="cuda"),
                                      torch.zeros(8, 8, dtype=BF16, device="cuda"), pre=pre, activation=kind)[2]
     assert bool(got.isnan().all()) if z != z else bool((got == slope).all()), got[0]
+
+
+# ---------------------------------------------------------------------------
+# float16 gradients of any size that their results have
+# ---------------------------------------------------------------------------
+def check_gradients(W, q, k, v, g, **kw):
+    """Bounds without the absolute error that weights and their gradients would have as plain
+    float16 numbers (2^-25): only the results' own rounding has one."""
+    with mock.patch.object(U, "least", lambda dtype: 0.0):
+        ref = U.attention_reference(q, k, v, dout=g, **kw)
+    out, lse = W.window_attention(q, k, v, return_lse=True, **kw)
+    for name, x in zip(("dq", "dk", "dv"), W.window_attention_backward(g, q, k, v, out, lse, **kw)):
+        want, bound = ref[name]
+        # a packed gradient below 2^-37 of its row's largest, a weight below 2^-28, keeps 2^-39 at least
+        bound = bound + U.least(q.dtype) + 2.0 ** -37 * want.abs().max()
+        assert float(want.abs().max()) < 6e4, "the test's own results leave float16's range"
+        U.assert_within(x, want, bound, name)
+
+
+SHAPES = [(1, 40, 40, 2, 1, 64, dict()), (1, 300, 300, 4, 2, 80, dict(window=100, sinks=4)),
+          (1, 1000, 1000, 2, 1, 128, dict(window=90, sinks=140)), (1, 20, 700, 6, 2, 32, dict())]
+
+
+@pytest.mark.parametrize("b,lq,lk,h,kv,d,kw", SHAPES)
+def test_large_gradients(W, b, lq, lk, h, kv, d, kw):
+    """Loss-scaled: dP - D of 10^5 and more, whose product with the weights passes 65504, while
+    dq, dk and dv fit float16."""
+    q, k, v, g = qkv(5, b, lq, lk, h, kv, d, F16)
+    q, k = q * 0.02, k * 0.02
+    v, g = v * 30, g * (4000 if lq < lk else 1500)
+    check_gradients(W, q, k, v, g, **kw)
+
+
+@pytest.mark.parametrize("b,lq,lk,h,kv,d,kw", SHAPES)
+@pytest.mark.parametrize("big", ["q", "k"])
+def test_small_gradients(W, b, lq, lk, h, kv, d, kw, big):
+    """dS of 10^-8 and below, whose sums with large keys or queries are ordinary numbers."""
+    q, k, v, g = qkv(6, b, lq, lk, h, kv, d, F16)
+    q, k = (q * 60, k * 0.01) if big == "q" else (q * 0.01, k * 60)
+    check_gradients(W, q, k, v * 0.02, g * 2e-4, **kw)
+
+
+def test_gradients_of_rows_of_very_different_size(W):
+    """Rows of 10^4 and rows of 10^-5 in one call: where only the small ones meet, they keep
+    their size; a key that both see has the large ones' error."""
+    q, k, v, g = qkv(7, 1, 600, 600, 2, 2, 64, F16)
+    g = g * torch.logspace(-5, 3, 600, device="cuda")[None, :, None, None].to(F16)
+    check_gradients(W, q * 0.3, k * 0.3, v, g, window=30)
+    check_gradients(W, q * 0.3, k * 0.3, v, g.flip(1).contiguous(), window=30)
+
+
+def test_gradients_of_small_weights(W):
+    """Beside a key of weight 1 all others have about e^-14 = 8e-7, less than float16's normal
+    numbers: the values' gradient adds them as they are."""
+    q, k, v, g = qkv(8, 1, 700, 700, 1, 1, 64, F16)
+    q, k = q * 0.1 + 1, k * 0.1
+    k[0, 0] = 1.75
+    check_gradients(W, q, k, v, g * 200)

@@ -163,7 +163,7 @@ struct AttnParams {
   uint8_t *out, *dq, *dk, *dv;
   const float* lse_in;
   float* lse;
-  float *row_lse, *row_delta;  // backward: a row's lse in the log2 domain, sum of dout * out
+  float *row_lse, *row_delta;  // backward: a row's lse in the log2 domain, less its weights' bits; -sum of dout * out
   const int32_t *q_lens, *k_lens;
   const uint8_t *k_new, *v_new;
   int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3], do_stride[3];  // elements

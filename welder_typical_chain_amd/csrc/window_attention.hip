@@ -388,11 +388,70 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 //                          per key block, queries streamed (attention_dkv_kernel)
 // Two kernels, each recomputing S and dP (7 products instead of 5): no dq sums
 // through atomics, whose order would change the result, and no f32 dq in memory.
-// The first writes each row's lse (in the log2 domain) and D as p.row_lse and
+// The first writes each row's lse (in the log2 domain) and -D as p.row_lse and
 // p.row_delta, rows packed as the tiles are: [batch][kv_heads][lq][G].
 __device__ inline int64_t stats_row(const AttnParams& p, int b, int hk, int i) {
   return (((int64_t)b * p.kv_heads + hk) * p.lq + i) * p.group;
 }
+
+// float16 holds 2^-24 to 2^16, 2^-14 with all its bits.  Weights of 1 / keys, and a dS that
+// goes with the gradient's size (loss-scaled ones pass 2^16 where dq and dk do not, small
+// ones vanish), do not fit that range as they are.
+// P: dk / dv works with P times 2^kWeightBits (row_lse is stored less by that).
+template <int DT> constexpr int kWeightBits = DT == DT_F16 ? 14 : 0;
+__device__ inline float power_of_2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
+// dS: taken times 2^ex, ex of each row (dq) or key (dk) its own.  It starts higher than any
+// use, short of where f32 would overflow, and is lowered, together with the sums so
+// far, when a value reaches 2^15, to put that value at 2^12 or more.  What a lane packs is
+// then off by 2^-11 of itself or 2^-37 of the largest so far.  The factor and the test
+// cost f16 2 to 5 % (forward and gradients, 4096 causal tokens, 32 / 8 heads of 128: 922 ->
+// 937 us; 4 x 2048, 16 heads of 64: 329 -> 345).  bf16 has f32's range.
+template <int DT> struct DsRange {
+  int ex;
+  // Two fragments of `ds`, which is times 2^ex already; the largest magnitude.
+  __device__ inline float pack(const f32x16& ds, u32x4 (&df)[2]) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t w0, w1;
+      pack4<DT>(f32x4{ds[4 * q], ds[4 * q + 1], ds[4 * q + 2], ds[4 * q + 3]}, &w0, &w1);
+      df[q >> 1][2 * (q & 1)] = w0;
+      df[q >> 1][2 * (q & 1) + 1] = w1;
+    }
+    float m = 0.0f;
+    if constexpr (DT == DT_F16) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) m = fmaxf(m, fabsf(ds[v]));
+    }
+    return m;
+  }
+  // Where that is too large: ex moves, `sums` follow, the fragments are packed again.
+  template <int ND> __device__ inline void fit(float m, f32x16& ds, f32x16 (&sums)[ND], u32x4 (&df)[2]) {
+    if constexpr (DT == DT_F16) {
+      if (!__any(m >= 32768.0f)) return;
+      m = xor32_max(m);
+      const int by = m >= 32768.0f ? min(0, 13 - __builtin_amdgcn_frexp_expf(m)) : 0;  // (0 for an infinity)
+      const float keep = power_of_2(by);
+      ex += by;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sums[d][v] *= keep;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) ds[v] *= keep;
+      pack(ds, df);
+    }
+  }
+  // sums without 2^(ex + bits)
+  template <int ND> __device__ inline void undo(f32x16 (&sums)[ND], int bits) const {
+    if constexpr (DT == DT_F16) {
+      const float by = power_of_2(-ex - bits);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sums[d][v] *= by;
+    }
+  }
+};
 
 template <int DT> __device__ inline void dq_row(const AttnParams& p, int b, int h, int i) {
   using T = typename Elem<DT>::type;
@@ -441,8 +500,8 @@ template <int DT> __device__ inline void dkv_row(const AttnParams& p, int b, int
       const int i = t0 + lane;
       if (i < i1) {
         const int64_t row = stats_row(p, b, hk, i) + x;
-        w = __builtin_amdgcn_exp2f(c2 * dot_rows<DT>(q + i * p.q_stride[1], k, p.dim) - p.row_lse[row]);
-        ds = p.scale * w * (dot_rows<DT>(g + i * p.do_stride[1], v, p.dim) - p.row_delta[row]);
+        w = __builtin_amdgcn_exp2f(c2 * dot_rows<DT>(q + i * p.q_stride[1], k, p.dim) - (p.row_lse[row] + kWeightBits<DT>));
+        ds = p.scale * w * (dot_rows<DT>(g + i * p.do_stride[1], v, p.dim) + p.row_delta[row]);
       }
       for (int t = 0; t < min(64, i1 - t0); ++t) {
         dv.add(__shfl(w, t), g + (t0 + t) * p.do_stride[1], lane);
@@ -519,6 +578,19 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
     }
   }
   const float c2 = positive_scale<NS>(p.scale, qf);
+  // |P (dP - D)| is at most 2 dim max|dout| max|v|, 2^24 max|dout| for any f16 v
+  DsRange<DT> range{0};
+  if constexpr (DT == DT_F16) {
+    float m = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const auto gv = __builtin_bit_cast(typename Elem<DT>::vec8, gf[s]);
+#pragma unroll
+      for (int v = 0; v < 8; ++v) m = fmaxf(m, fabsf((float)gv[v]));
+    }
+    range.ex = 30 - __builtin_amdgcn_frexp_expf(xor32_max(m));
+  }
+  float weight_off = -lse2;  // of the exponents
 
   TileLoader<RB, kKeys, NW> lk, lv;
   lk.init(p.k + 2 * (b * p.k_stride[0] + hk * p.k_stride[2]), 2 * p.k_stride[1], p.dim, wave, lane);
@@ -537,7 +609,7 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
     lv.issue(st + L::TILE, j0, n);
   };
   const uint32_t k_at = row_addr<RB>(lane) + group * 2 * L::TILE, kc_at = col_addr<RB>(lane) + group * 2 * L::TILE;
-  // Weights s and dP g of subtile u of step x; false: none of the wave's rows sees it.
+  // Weights s (times 2^(weight_off + lse2)) and dP g of subtile u of step x; false: none of the wave's rows sees it.
   auto weights = [&](int x, int u, uint32_t ka, f32x16& s, f32x16& g) {
     const int t = x * KG + group;
     const int j0 = tile_base(t), j1 = tile_end(t);
@@ -558,7 +630,7 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
 #pragma unroll
     for (int st = 0; st < NS; ++st) g = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u + kKeys, st), gf[st], g);
 #pragma unroll
-    for (int v = 0; v < 16; ++v) s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c2, -lse2));
+    for (int v = 0; v < 16; ++v) s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c2, weight_off));
     __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
     for (int x = 0; x < NS; ++x) {
@@ -606,8 +678,8 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
     delta = sum;
   }
   if (half == 0 && group == 0 && i < p.lq) {
-    p.row_lse[stats_row(p, b, hk, i) + x_head] = lse2;
-    p.row_delta[stats_row(p, b, hk, i) + x_head] = delta;
+    p.row_lse[stats_row(p, b, hk, i) + x_head] = lse2 - kWeightBits<DT>;
+    p.row_delta[stats_row(p, b, hk, i) + x_head] = -delta;
   }
 
   f32x16 dq[ND];
@@ -627,18 +699,12 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f32x16 s, g;
+      weight_off = (float)range.ex - lse2;
       if (!weights(x, u, ka, s, g)) continue;
       u32x4 df[2];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        f32x4 ds;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) ds[v] = s[4 * q + v] * (g[4 * q + v] - delta);
-        uint32_t w0, w1;
-        pack4<DT>(ds, &w0, &w1);
-        df[q >> 1][2 * (q & 1)] = w0;
-        df[q >> 1][2 * (q & 1) + 1] = w1;
-      }
+      for (int v = 0; v < 16; ++v) s[v] *= g[v] - delta;
+      range.fit(range.pack(s, df), s, dq, df);
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
@@ -646,6 +712,7 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
     }
   }
   wait_loads_barrier<0>();
+  range.undo(dq, 0);
   if constexpr (KG == 2) {
     uint8_t* at = smem + (wave * 32 + (lane & 31)) * L::JPITCH + half * 16;
     if (group) {
@@ -818,6 +885,7 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int v = 0; v < 16; ++v) dk[d][v] = dv[d][v] = 0.0f;
+  DsRange<DT> range{DT == DT_F16 ? 60 : 0};  // (2^14 P (dP - D) is below 2^56 for f16 inputs)
 
   auto issue = [&](int t) {
     const int step = t / chunks, hc = t - step * chunks, i = i0 + step * tp;
@@ -864,7 +932,7 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
     fresh(ca);
     f32x16 s, g;
 #pragma unroll
-    for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
+    for (int v = 0; v < 16; ++v) s[v] = 0.0f;
 #pragma unroll
     for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ra, 0, st), kf[st], s);
     if (!all) {
@@ -874,7 +942,13 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
       for (int v = 0; v < 16; ++v) s[v] = keep_bit(s[v], in, 8 * (v >> 2) + (v & 3));
     }
     __builtin_amdgcn_sched_barrier(0);
-    // the exponentials among the products of dP
+    // the exponentials among the products of dP - D, which start from -D
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 del = *reinterpret_cast<const f32x4*>(stt + 1024 + (row0 + 8 * q + 4 * half) * 4);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) g[4 * q + v] = del[v];
+    }
 #pragma unroll
     for (int st = 0; st < NS; ++st) {
       const int x = st - (NS - L::KEPT);
@@ -903,30 +977,31 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
     for (int st = 0; st < 2; ++st)
 #pragma unroll
       for (int d = 0; d < ND; ++d) dv[d] = mfma32<DT>(col_frag<RB>(smem, ca, kQueries + 16 * st, d), pf[st], dv[d]);
+    const float by = power_of_2(range.ex);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 del = *reinterpret_cast<const f32x4*>(stt + 1024 + (row0 + 8 * q + 4 * half) * 4);
-      f32x4 ds;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) ds[v] = s[4 * q + v] * (g[4 * q + v] - del[v]);
-      uint32_t w0, w1;
-      pack4<DT>(ds, &w0, &w1);
-      df[q >> 1][2 * (q & 1)] = w0;
-      df[q >> 1][2 * (q & 1) + 1] = w1;
-    }
+    for (int v = 0; v < 16; ++v) s[v] = DT == DT_F16 ? s[v] * by * g[v] : s[v] * g[v];
+    const float most = range.pack(s, df);
 #pragma unroll
     for (int x = 0; x < 2 * ND; ++x) {
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 40 / (2 * ND), 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, (DT == DT_F16 ? 48 : 24) / (2 * ND), 0);
     }
     __builtin_amdgcn_sched_barrier(0);
+    range.fit(most, s, dk, df);
 #pragma unroll
     for (int st = 0; st < 2; ++st)
 #pragma unroll
       for (int d = 0; d < ND; ++d) dk[d] = mfma32<DT>(col_frag<RB>(smem, ca, 16 * st, d), df[st], dk[d]);
   }
   wait_loads_barrier<0>();
+  range.undo(dk, kWeightBits<DT>);
+  if constexpr (kWeightBits<DT> != 0) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) dv[d][v] *= power_of_2(-kWeightBits<DT>);
+  }
 
   // ---- join: waves 0-3 hand over dv and finish dk, waves 4-7 the other way round
   uint8_t* mine = smem + wave * 32 * L::PITCH;          // what this wave finishes

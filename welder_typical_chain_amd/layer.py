@@ -205,8 +205,9 @@ def matmul_epilogue_backward(dout: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     da = dz @ b.T, db = a.T @ dz (stored as b is) and dbias = the column sums of
     dz in float32; None for what is not needed.  dout: [..., N] of a's type; pre:
     what return_pre=True gave (not needed with activation "none").  The
-    products take dz rounded to a's type and sum in float32.  The residual's
-    gradient is dout itself.
+    products take dz rounded to a's type and sum in float32: a float16 dz has
+    float16's range, so dout is best scaled to well above 6e-5 and below 5e4.
+    The residual's gradient is dout itself.
     """
     code = _code_of(a, "a")
     if a.dim() < 1:
@@ -337,7 +338,9 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     `out` and `lse`.  Contiguous, in the shapes and type of q, k, v; a key
     head's gradient is the sum over the query heads that share it.  Sums are
     float32; the products take the weights and their gradients rounded to q's
-    type.  Two calls give the same bits.
+    type (float16: times a power of two that keeps them in its range, so a
+    gradient may have any size that its results have).  Two calls give the same
+    bits.
     """
     device = _check_inputs(q.dtype, ("dout", dout), ("q", q), ("k", k), ("v", v), ("out", out))
     head, tail = _attention_args(q, k, v, window, sinks, scale, q_lens, k_lens, device)
