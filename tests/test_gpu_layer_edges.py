@@ -264,3 +264,56 @@ def test_gradients_of_small_weights(W):
     q, k = q * 0.1 + 1, k * 0.1
     k[0, 0] = 1.75
     check_gradients(W, q, k, v, g * 200)
+
+
+# ---------------------------------------------------------------------------
+# calls that autograd would track
+# ---------------------------------------------------------------------------
+def test_tangents_are_refused(W):
+    """A dual tensor does not require a gradient, and its tangent would be lost."""
+    import torch.autograd.forward_ad as fwad
+    a, b = rand(1, 16, 64, dtype=F16), rand(2, 64, 32, dtype=F16)
+    q, k, v, g = qkv(1, 1, 8, 8, 2, 2, 64, F16)
+    out, lse = W.window_attention(q, k, v, return_lse=True)
+    n = torch.tensor([8], dtype=torch.int32, device="cuda")
+    want = W.matmul_epilogue(a, b)
+
+    class Product(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return W.matmul_epilogue(x, b)
+
+        @staticmethod
+        def jvp(ctx, dx):
+            return W.matmul_epilogue(dx.contiguous(), b)
+
+    with fwad.dual_level():
+        def dual(t):
+            return fwad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: W.matmul_epilogue(dual(a), b), lambda: W.matmul_epilogue(a, dual(b)),
+                     lambda: W.matmul_epilogue(a, b, bias=dual(rand(3, 32, dtype=F16))),
+                     lambda: W.matmul_epilogue_backward(want, dual(a), b),
+                     lambda: W.window_attention(dual(q), k, v), lambda: W.window_attention(q, k, dual(v)),
+                     lambda: W.window_attention_backward(dual(g), q, k, v, out, lse),
+                     lambda: W.window_attention_backward(g, q, k, v, out, dual(lse)),
+                     lambda: W.window_attention_decode(dual(q)[:, 0], k, v, n)):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+            with pytest.raises(ValueError, match="gradient"), torch.no_grad():  # (which keeps tangents)
+                call()
+        assert torch.equal(W.matmul_epilogue(a, b), want)  # others are not held up
+        y, dy = fwad.unpack_dual(Product.apply(dual(a)))  # inside a Function's forward they are its own affair
+        assert torch.equal(y, want) and torch.equal(dy, W.matmul_epilogue(torch.ones_like(a), b))
+    assert torch.equal(W.matmul_epilogue(a, b), want)
+
+
+def test_lse_that_requires_a_gradient_is_refused(W):
+    q, k, v, g = qkv(1, 1, 8, 8, 2, 2, 64, F16)
+    out, lse = W.window_attention(q, k, v, return_lse=True)
+    want = W.window_attention_backward(g, q, k, v, out, lse)
+    lse.requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        W.window_attention_backward(g, q, k, v, out, lse)
+    with torch.no_grad():
+        got = W.window_attention_backward(g, q, k, v, out, lse)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))

@@ -7,15 +7,17 @@ and every byte is computed by the HIP kernels behind ``include/wtc/wtc_layer.h``
 Every call runs on the current stream of its tensors' device, may be captured
 into a graph, and takes its scratch memory from PyTorch's allocator (so that
 calls and graphs never share any).  The gradients are functions of their own:
-a call on tensors that autograd would track raises, instead of dropping the
-gradient in silence (``torch.no_grad()``, or the ``forward`` of a
-``torch.autograd.Function``, is where these are called).
+a call on tensors that autograd would track, in reverse or in forward mode,
+raises, instead of dropping the gradient in silence (``torch.no_grad()``, or
+the ``forward`` of a ``torch.autograd.Function``, is where these are called; a
+dual tensor's tangent needs the latter).
 """
 from __future__ import annotations
 
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -52,6 +54,10 @@ def _check_inputs(dtype, *named):
         if grad and t.requires_grad:
             raise ValueError(f"{name} requires a gradient, which this call does not record: call it under "
                              "torch.no_grad() and use the backward function")
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for name, t in named:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has a tangent (a forward-mode gradient), which this call does not carry on")
     return device
 
 
@@ -350,6 +356,7 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     if lse.shape != (b, h, lq) or lse.dtype != torch.float32 or not lse.is_contiguous() or \
             not lse.is_cuda or lse.get_device() != device:
         raise ValueError("lse must be window_attention's: float32, contiguous, [B, H, Lq]")
+    _check_inputs(None, ("lse", lse))
     if dout.stride(3) != 1 or 0 in dout.stride():  # a gradient that autograd broadcast
         dout = dout.contiguous()
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
