@@ -317,3 +317,53 @@ def test_lse_that_requires_a_gradient_is_refused(W):
     with torch.no_grad():
         got = W.window_attention_backward(g, q, k, v, out, lse)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+# ---------------------------------------------------------------------------
+# outputs that lie over inputs
+# ---------------------------------------------------------------------------
+def test_outputs_over_inputs_are_refused(W):
+    flat = rand(1, 4096 + 64, dtype=F16)
+    a, b = flat[:4096].view(64, 64), rand(2, 64, 64, dtype=F16)
+    over = flat[64:].view(64, 64)  # one row further on
+    bias = over[3]
+    with pytest.raises(ValueError, match="out may not"):
+        W.matmul_epilogue(a, b, out=over)
+    with pytest.raises(ValueError, match="out may not"):
+        W.matmul_epilogue(b, a, out=over)
+    with pytest.raises(ValueError, match="out may not"):
+        W.matmul_epilogue(b, a.t(), out=over)
+    with pytest.raises(ValueError, match="out may not"):
+        W.matmul_epilogue(b, b, bias=bias, out=over)
+    with pytest.raises(ValueError, match="out may not"):
+        W.matmul_epilogue(b, b, residual=a, out=over)
+    wide = rand(3, 64, 128, dtype=F16)
+    with pytest.raises(ValueError, match="out may not"):  # the same start, other rows
+        W.matmul_epilogue(b, b, residual=wide.view(128, 64)[:64], out=wide[:, :64])
+    want = W.matmul_epilogue(b, b, residual=wide[:, :64].contiguous())
+    assert torch.equal(W.matmul_epilogue(b, b, residual=wide[:, :64], out=wide[:, :64]), want)
+    # columns side by side of one buffer do not overlap
+    joint = rand(4, 64, 192, dtype=F16)
+    want = W.matmul_epilogue(joint[:, :64], b)
+    assert torch.equal(W.matmul_epilogue(joint[:, :64], b, out=joint[:, 64:128]), want)
+
+    buf = rand(5, 2 * 8 * 2 * 64 + 128, dtype=F16)
+    q, o = buf[:2048].view(2, 8, 2, 64), buf[128:].view(2, 8, 2, 64)
+    k, v = rand(6, 2, 8, 2, 64, dtype=F16), rand(7, 2, 8, 2, 64, dtype=F16)
+    for x in ((q, k, v), (k, q, v), (k, v, q)):
+        with pytest.raises(ValueError, match="out may not"):
+            W.window_attention(*x, out=o)
+    n = torch.tensor([8, 8], dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="out may not"):
+        W.window_attention_decode(k[:, 0], q, v, n, out=buf[128:384].view(2, 2, 64))
+    with pytest.raises(ValueError, match="out may not"):
+        W.window_attention_decode(k[:, 0], k, v, n, k_new=buf[:256].view(2, 2, 64), v_new=v[:, 1], out=buf[128:384].view(2, 2, 64))
+
+
+def test_one_cache_for_keys_and_values_cannot_take_a_token(W):
+    q, kc, kn = rand(1, 1, 2, 64, dtype=F16), rand(2, 1, 8, 2, 64, dtype=F16), rand(3, 1, 2, 64, dtype=F16)
+    n = torch.tensor([5], dtype=torch.int32, device="cuda")
+    with pytest.raises(W._lib.WtcError, match="same"):
+        W.window_attention_decode(q, kc, kc, n, k_new=kn, v_new=kn + 1)
+    want = W.window_attention_decode(q, kc, kc.clone(), n)
+    assert torch.equal(W.window_attention_decode(q, kc, kc, n), want)

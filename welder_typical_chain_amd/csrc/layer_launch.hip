@@ -407,6 +407,7 @@ int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void
     if (int rc = check_distinct(p->o_stride, p->batch, 1, p->heads, p->dim, "out")) return rc;
     if (!k_new != !v_new) return bad("k_new and v_new go together");
     if (k_new) {
+      if (k && k == v) return bad("k and v are the same cache: it cannot take both k_new and v_new");
       if (int rc = check_distinct(p->k_stride, p->batch, p->lk, p->kv_heads, p->dim, "k")) return rc;
       if (int rc = check_distinct(p->v_stride, p->batch, p->lk, p->kv_heads, p->dim, "v")) return rc;
     }

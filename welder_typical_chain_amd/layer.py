@@ -94,6 +94,24 @@ def _scratch(name, args, device, keyed=None):
     return t, t.data_ptr(), size
 
 
+def _check_out(out, *named):
+    """Refuses an `out` that starts where an input does, or lies over one: of tensors
+    without gaps that is known, of others only the start (columns side by side in one
+    buffer share no element, but their ranges meet)."""
+    size = out.numel() * out.element_size()
+    if not size:
+        return
+    at = out.data_ptr()
+    end = at + size if out.is_contiguous() else at
+    for name, t in named:
+        if t is None or not t.numel():
+            continue
+        first = t.data_ptr()
+        if first == at or (end > at and t.is_contiguous() and first < end and
+                           at < first + t.numel() * t.element_size()):
+            raise ValueError(f"out may not be or lie over {name}")
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -150,7 +168,7 @@ def matmul_epilogue(a: torch.Tensor, b: torch.Tensor, *, bias: torch.Tensor | No
     the output type.  K and N are multiples of 8.  activation: "none", "relu",
     "gelu" (z Phi(z)), "gelu_tanh" or "silu".  Products and epilogue are
     float32, rounded once to `out_dtype` (a's type, or float32).  `out` may be
-    `residual` itself, and no other input.  With return_pre=True the result is
+    `residual` itself, and lie over no other input.  With return_pre=True the result is
     (out, pre), pre = a @ b + bias in float32, which matmul_epilogue_backward
     needs for an activation (rounded to 16 bits it would move dbias by 5e-4).
     """
@@ -177,8 +195,10 @@ def matmul_epilogue(a: torch.Tensor, b: torch.Tensor, *, bias: torch.Tensor | No
         out = torch.empty(shape, dtype=out_dtype, device=a.device)
     elif out.shape != shape or out.dtype != out_dtype:
         raise ValueError("out has the wrong shape or dtype")
-    elif m and n and out.data_ptr() in (a.data_ptr(), b.data_ptr()):
-        raise ValueError("out may not be a or b")
+    else:
+        itself = residual is not None and residual.shape == shape and out.data_ptr() == residual.data_ptr() and \
+            (out.stride() == residual.stride() or (out.is_contiguous() and residual.is_contiguous()))
+        _check_out(out, ("a", a), ("b", b.t() if trans else b), ("bias", bias), ("residual", None if itself else residual))
     out2 = out if flat else out.view(-1, n) if out.numel() else out.new_empty((m, n))
     bias_code = code
     if bias is not None:
@@ -324,8 +344,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape:
         raise ValueError("out must have q's shape")
-    elif out.numel() and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
-        raise ValueError("out may not be an input")
+    else:
+        _check_out(out, ("q", q), ("k", k), ("v", v))
     b, lq, h, _ = q.shape
     lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if return_lse else None
     args = _pack_attention(*head, *_strides(out, "out"), 0, 0, 0, 0, 0, 0, 0, *tail)
@@ -400,8 +420,8 @@ def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape:
         raise ValueError("out must have q's shape")
-    elif out.numel() and out.data_ptr() == q.data_ptr():
-        raise ValueError("out may not be q")
+    else:
+        _check_out(out, ("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("k_new", k_new), ("v_new", v_new))
     kn = vn = (0, 0, 0)
     if k_new is not None and v_new is not None:
         if k_new.shape != (b, kv, d) or v_new.shape != (b, kv, d):
