@@ -16,6 +16,7 @@ constexpr int64_t kMost = 1ll << 30;          // rows, tokens, heads, ...
 constexpr int64_t kSpan = 0x7FFFFFFFll;       // bytes of an operand of a product
 constexpr int64_t kTokenStride = 1ll << 23;   // elements: a tile's rows stay within 32-bit offsets
 constexpr int64_t kMaxDim = 128;
+constexpr int64_t kThreads = 1ll << 32;       // a launch takes fewer
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -49,9 +50,9 @@ int check_matmul(const wtc_matmul_args& p, bool backward) {
   if (p.m < 0 || p.n < 0 || p.k < 0) return bad("negative extent");
   if (p.m > kMost || p.n > kMost || p.k > kMost) return report(WTC_ERR_UNSUPPORTED, "extent above 2^30");
   if (p.n % 8 || p.k % 8) return bad("n and k must be multiples of 8");
-  // workgroups of the smallest tile with the most splits, of the forward product and of the gradients
+  // workgroups of the forward product and of the gradients (splits are for few of them)
   const int64_t mt = (p.m + 127) / 128, nt = (p.n + 127) / 128, kt = (p.k + 127) / 128;
-  if (std::max({mt * nt, mt * kt, kt * nt}) > kMost / 16) return report(WTC_ERR_UNSUPPORTED, "too many tiles");
+  if (std::max({mt * nt, mt * kt, kt * nt}) >= kThreads / 256) return report(WTC_ERR_UNSUPPORTED, "too many tiles");
   const int64_t b_cols = p.b_trans ? p.k : p.n, b_rows = p.b_trans ? p.n : p.k;
   if (p.lda < p.k || p.ldb < b_cols || p.lda % 8 || p.ldb % 8)
     return bad("lda and ldb must be multiples of 8 that hold a row");
@@ -129,6 +130,8 @@ int check_distinct(const int64_t* s, int64_t n0, int64_t n1, int64_t n2, int64_t
   return WTC_OK;
 }
 
+int too_many() { return report(WTC_ERR_UNSUPPORTED, "more sequences, heads and tokens than one launch takes"); }
+
 int check_attention(const wtc_attention_args& p, bool decode) {
   if (p.dtype != WTC_DTYPE_F16 && p.dtype != WTC_DTYPE_BF16) return bad("dtype must be f16 or bf16");
   if (p.batch < 0 || p.lq < 0 || p.lk < 0 || p.window < 0 || p.sinks < 0) return bad("negative extent");
@@ -137,6 +140,10 @@ int check_attention(const wtc_attention_args& p, bool decode) {
   if (p.batch > kMost || p.lq > kMost || p.lk > kMost || p.heads > (1 << 16) ||
       p.batch * p.heads > kMost || p.batch * p.heads * p.lq > kMost || p.batch * p.kv_heads > kMost / std::max<int64_t>(p.lk, 1))
     return report(WTC_ERR_UNSUPPORTED, "extent above 2^30");
+  // row blocks of 128 (splits are for few of them), query heads by 32 in decode
+  const int64_t group = p.heads / p.kv_heads, seqs = p.batch * p.kv_heads;
+  const int64_t groups = seqs * (decode ? (group + 31) / 32 : (p.lq * group + 127) / 128);
+  if (groups >= kThreads / (decode ? 256 : 512)) return too_many();
   if (!std::isfinite(p.scale)) return bad("scale must be finite");
   int rc;
   if ((rc = check_strides(p.q_stride, 3, p.lq, "q"))) return rc;
@@ -204,7 +211,13 @@ int check_attention_backward(const wtc_attention_args& p) {
   if (int rc = check_attention(p, false)) return rc;
   if (int rc = check_strides(p.do_stride, 3, p.lq, "dout")) return rc;
   if (int rc = check_group_span(p, p.q_stride, "q")) return rc;
-  return check_group_span(p, p.do_stride, "dout");
+  if (int rc = check_group_span(p, p.do_stride, "dout")) return rc;
+  const AttnParams a = attention_params(p);
+  const AttnBackwardPlan plan = plan_attention_backward(a, cu_count());
+  const int64_t seqs = p.batch * p.kv_heads;
+  const int64_t groups = seqs * ((int64_t)plan.key_blocks * plan.near_chunks + (int64_t)plan.far_blocks * plan.far_chunks);
+  if (groups >= kThreads / 512 || (plan.far_blocks && seqs * a.sinks >= kThreads / 64)) return too_many();
+  return WTC_OK;
 }
 
 }  // namespace
