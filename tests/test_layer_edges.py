@@ -48,3 +48,10 @@ def test_decode_of_too_many_workgroups(L):
     assert L.wtc_window_attention_decode_workspace_size(args) == -1
     assert L.wtc_window_attention_decode(args, A, A, 2 * A, A, A, A, A, 1 << 50, None) == ERR_UNSUPPORTED
     assert L.wtc_window_attention_decode_workspace_size(attention_args(**{**ONE, "batch": (1 << 24) - 1, "lq": 1, "lk": 1, "k_lens": A})) >= 0
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, 3.5e38])
+def test_scale_beyond_float32(L, scale):
+    assert L.wtc_window_attention(attention_args(scale=scale), A, A, A, A, None, A, 1 << 40, None) == ERR_ARG
+    assert L.wtc_window_attention_backward(attention_args(scale=scale), *[A] * 9, A, 1 << 40, None) == ERR_ARG
+    assert L.wtc_window_attention_decode(attention_args(lq=1, k_lens=A, scale=scale), A, A, 2 * A, A, A, A, A, 1 << 40, None) == ERR_ARG

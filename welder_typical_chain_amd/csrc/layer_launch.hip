@@ -144,7 +144,7 @@ int check_attention(const wtc_attention_args& p, bool decode) {
   const int64_t group = p.heads / p.kv_heads, seqs = p.batch * p.kv_heads;
   const int64_t groups = seqs * (decode ? (group + 31) / 32 : (p.lq * group + 127) / 128);
   if (groups >= kThreads / (decode ? 256 : 512)) return too_many();
-  if (!std::isfinite(p.scale)) return bad("scale must be finite");
+  if (!std::isfinite((float)p.scale)) return bad("scale must be finite in float32");
   int rc;
   if ((rc = check_strides(p.q_stride, 3, p.lq, "q"))) return rc;
   if ((rc = check_strides(p.k_stride, 3, p.lk, "k"))) return rc;
