@@ -367,3 +367,18 @@ def test_one_cache_for_keys_and_values_cannot_take_a_token(W):
         W.window_attention_decode(q, kc, kc, n, k_new=kn, v_new=kn + 1)
     want = W.window_attention_decode(q, kc, kc.clone(), n)
     assert torch.equal(W.window_attention_decode(q, kc, kc, n), want)
+
+
+@pytest.mark.parametrize("n", [40, 400])
+def test_a_nan_value_of_weight_0_in_the_gradients(W, n):
+    """0 * NaN in a row's result makes its D NaN, and with it the gradient of every key that the
+    row sees: also in rows of few keys, which sum D themselves."""
+    q, k = torch.ones(1, n, 1, 64, dtype=BF16, device="cuda"), rand(1, 1, n, 1, 64, dtype=BF16, by=0.1)
+    v, g = rand(2, 1, n, 1, 64, dtype=BF16), rand(3, 1, n, 1, 64, dtype=BF16)
+    k[0, 3] = -40  # its scores are 320 below the others'
+    v[0, 3, 0] = NAN
+    out, lse = W.window_attention(q, k, v, return_lse=True)
+    dq, dk, dv = W.window_attention_backward(g, q, k, v, out, lse)
+    assert bool(out[0, 3:].isnan().all()) and bool(out[0, :3].isfinite().all())
+    assert bool(dq[0, 3:].isnan().all()) and bool(dk.isnan().all())
+    assert bool(dq[0, :3].isfinite().all()) and bool(dv.isfinite().all())

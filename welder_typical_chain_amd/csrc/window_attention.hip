@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
       sum = part[wave * 32 + (lane & 31)] + part[(4 + wave) * 32 + (lane & 31)];
       __syncthreads();
     }
-    delta = sum;
+    delta = delta != delta ? delta : sum;  // (a NaN value that is seen, be its weight 0, is in out)
   }
   if (half == 0 && group == 0 && i < p.lq) {
     p.row_lse[stats_row(p, b, hk, i) + x_head] = lse2 - kWeightBits<DT>;
