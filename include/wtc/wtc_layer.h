@@ -71,6 +71,13 @@ int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, con
                                  const float* pre, void* da, void* db, float* dbias, void* workspace,
                                  size_t workspace_bytes, void* stream);
 
+/* The kernel that a product of these sizes runs on a device of `cu_count` compute
+ * units (0: the current one's): its output tile and the parts that k is split
+ * into.  part: 0 the forward product, 1 da, 2 db.  16 x 16: the kernel for few
+ * rows, which has no tiles. */
+int wtc_matmul_epilogue_plan(const wtc_matmul_args* p, int part, int cu_count, int64_t* tile_m, int64_t* tile_n,
+                             int64_t* splits);
+
 /*
  * Attention.  q, out and dout [batch][lq][heads][dim]; k and v
  * [batch][lk][kv_heads][dim]; heads a multiple of kv_heads, query head h
@@ -107,6 +114,12 @@ int64_t wtc_window_attention_backward_workspace_size(const wtc_attention_args* p
 int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout, const void* q, const void* k,
                                   const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* What the two calls above run on a device of `cu_count` compute units (0: the
+ * current one's), five numbers: waves that share a query row and key splits of
+ * the forward pass; waves that share a row in dq; parts of a key block's queries
+ * in dk / dv, and workgroups for the first tokens' far queries. */
+int wtc_window_attention_plan(const wtc_attention_args* p, int cu_count, int64_t* plan);
 
 int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p);
 /* One token a sequence (lq = 1).  k and v are caches of lk rows a sequence, lk

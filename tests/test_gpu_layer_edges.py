@@ -7,6 +7,8 @@ import pytest
 import torch
 
 from tests import layer_util as U
+from tests.layer_sizes import FULL_CHIP, LARGE_GRADIENTS, LARGE_PRODUCTS
+from welder_typical_chain_amd.layer import matmul_epilogue_plan, window_attention_plan
 
 pytestmark = pytest.mark.gpu
 
@@ -382,3 +384,108 @@ def test_a_nan_value_of_weight_0_in_the_gradients(W, n):
     assert bool(out[0, 3:].isnan().all()) and bool(out[0, :3].isfinite().all())
     assert bool(dq[0, 3:].isnan().all()) and bool(dk.isnan().all())
     assert bool(dq[0, :3].isfinite().all()) and bool(dv.isfinite().all())
+
+
+# ---------------------------------------------------------------------------
+# the kernels that large calls run
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("size,tile", LARGE_PRODUCTS)
+@pytest.mark.parametrize("dtype,out_dtype,kind,bias,residual,trans", [
+    (BF16, BF16, "gelu", BF16, True, False), (F16, F32, "silu", F32, True, True), (BF16, F32, "none", None, False, False),
+    (F16, F16, "gelu_tanh", F16, True, True), (BF16, BF16, "relu", None, False, True), (F16, F32, "gelu", F16, True, False)])
+def test_large_products(W, size, tile, dtype, out_dtype, kind, bias, residual, trans):
+    m, n, k = size
+    assert matmul_epilogue_plan(m, n, k, b_trans=trans)[:2] == tile
+    a = rand(1, m, k, dtype=dtype)
+    b = rand(2, n, k, dtype=dtype, by=0.1).t() if trans else rand(2, k, n, dtype=dtype, by=0.1)
+    bv = None if bias is None else rand(3, n, dtype=bias)
+    r = rand(4, m, n, dtype=out_dtype) if residual else None
+    out, pre = W.matmul_epilogue(a, b, bias=bv, residual=r, activation=kind, out_dtype=out_dtype, return_pre=True)
+    y, z, dz, dy = U.matmul_reference(a, b, bv, r, kind)
+    U.assert_within(out, y, U.rounded(y, dy, out_dtype), "out")
+    U.assert_within(pre, z, U.rounded(z, dz, F32), "pre")
+    wide = torch.full((m, n + 16), 7.0, dtype=out_dtype, device="cuda")  # what is between an out's rows stays
+    again = W.matmul_epilogue(a, b, bias=bv, residual=r, activation=kind, out=wide[:, 8:n + 8])
+    assert torch.equal(out, again) and bool((wide[:, :8] == 7).all()) and bool((wide[:, n + 8:] == 7).all())
+
+
+@pytest.mark.parametrize("size,part,tile,split", LARGE_GRADIENTS)
+@pytest.mark.parametrize("dtype,trans,kind", [(BF16, False, "none"), (F16, True, "silu"), (BF16, True, "relu"), (F16, False, "gelu")])
+def test_large_gradients_of_products(W, size, part, tile, split, dtype, trans, kind):
+    m, n, k = size
+    *got, splits = matmul_epilogue_plan(m, n, k, b_trans=trans, part=part)
+    assert tuple(got) == tile and (splits > 1) == split
+    a, dout, pre = rand(1, m, k, dtype=dtype), rand(3, m, n, dtype=dtype), rand(4, m, n)
+    b = rand(2, n, k, dtype=dtype, by=0.1).t() if trans else rand(2, k, n, dtype=dtype, by=0.1)
+    da, db, dbias = W.matmul_epilogue_backward(dout, a, b, pre=None if kind == "none" else pre, activation=kind)
+    dz = dout.double() * U.act_slope(pre.double(), kind)
+    # the slope's own error (64 half steps of its terms, which are at most 1 and |z| in size), then dz's rounding
+    ez = dout.double().abs() * (0 if kind in ("none", "relu") else 64 * U.E32 * (1 + pre.double().abs()))
+    err = 0 * dz if kind == "none" else ez + U.half_step(dtype) * (dz.abs() + ez) + U.least(dtype)
+    size_of = dz.abs() + err
+    bd, ad = b.double(), a.double()
+    ref = dz @ bd.t()
+    U.assert_within(da, ref, U.rounded(ref, (err + 2 * (n + 2) * U.E32 * size_of) @ bd.t().abs(), dtype), "da")
+    ref = ad.t() @ dz
+    U.assert_within(db, ref, U.rounded(ref, ad.t().abs() @ (err + 2 * (m + 2) * U.E32 * size_of), dtype), "db")
+    U.assert_within(dbias, dz.sum(0), (ez + 2 * (m + 2) * U.E32 * size_of).sum(0), "dbias")
+    again = W.matmul_epilogue_backward(dout, a, b, pre=None if kind == "none" else pre, activation=kind)
+    assert all(torch.equal(x, y) for x, y in zip((da, db, dbias), again))
+
+
+@pytest.mark.parametrize("b,h,kv,lq,lk,d,kw", FULL_CHIP)
+@pytest.mark.parametrize("dtype,ragged", [(BF16, False), (F16, True)])
+def test_attention_on_a_full_chip(W, b, h, kv, lq, lk, d, kw, dtype, ragged):
+    """A wave to each row: rings of three stages forward, four waves a block in dq."""
+    plan = window_attention_plan(b, h, kv, lq, lk, d, **kw)
+    assert plan["row_waves"] == 1 and plan["dq_row_waves"] == 1
+    q, k, v, g = qkv(91, b, lq, lk, h, kv, d, dtype)
+    if ragged:
+        q_lens = torch.tensor([(lq + 1) * i // b for i in range(b)], dtype=torch.int32, device="cuda")
+        k_lens = torch.tensor([(lk + 1) * ((7 * i + 3) % b + 1) // b for i in range(b)], dtype=torch.int32, device="cuda")
+        for i in range(b):  # nothing behind the ends is read
+            for t, n in ((q, q_lens), (g, q_lens), (k, k_lens), (v, k_lens)):
+                t[i, int(n[i]):] = NAN
+        kw = dict(kw, q_lens=q_lens, k_lens=k_lens)
+    ref = U.attention_reference(q, k, v, dout=g, **kw)
+    out, lse = W.window_attention(q, k, v, return_lse=True, **kw)
+    U.assert_within(out, *ref["out"], "out")
+    empty = ref["lse"][0] == -math.inf
+    assert torch.equal(lse == -math.inf, empty)
+    U.assert_within(torch.where(empty, 0.0, lse), torch.where(empty, 0.0, ref["lse"][0]), ref["lse"][1], "lse")
+    got = W.window_attention_backward(g, q, k, v, out, lse, **kw)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        U.assert_within(x, *ref[name], name)
+    assert torch.equal(out, W.window_attention(q, k, v, **kw))
+    again = W.window_attention_backward(g, q, k, v, out, lse, **kw)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+@pytest.mark.parametrize("bad", [NAN, -math.inf])
+@pytest.mark.parametrize("name", ["k", "v", "q", "g"])
+def test_bad_values_on_a_full_chip(W, bad, name):
+    """As with two waves a row: a bad value in one sequence reaches the rows of that sequence
+    that see it and no other."""
+    b, n, window, sinks, at = 280, 200, 30, 2, 150
+    kw = dict(window=window, sinks=sinks)
+    plan = window_attention_plan(b, 2, 1, n, n, 64, **kw)
+    assert plan["row_waves"] == 1 and plan["dq_row_waves"] == 1
+    q, k, v, g = qkv(95, b, n, n, 2, 1, 64, F16)
+    clean, lse = W.window_attention(q, k, v, return_lse=True, **kw)
+    want = (clean, *W.window_attention_backward(g, q, k, v, clean, lse, **kw))
+    dict(q=q, k=k, v=v, g=g)[name][5, at, 0, 9] = bad
+    out, lse = W.window_attention(q, k, v, return_lse=True, **kw)
+    got = (out, *W.window_attention_backward(g, q, k, v, out, lse, **kw))
+    pos = torch.arange(n, device="cuda")
+    one_head = name in ("q", "g")
+    rows = pos == at if one_head else (pos >= at) & (pos < at + window)
+    keys = U.seen_mask(n, n, n, n, window, sinks, "cuda")[rows].any(0)
+    none = torch.zeros_like(rows)
+    touched = (none if name == "g" else rows, rows, keys, none if name == "v" else keys)
+    others = [i for i in range(b) if i != 5]
+    clean5 = [t[5:6].clone() for t in qkv(95, b, n, n, 2, 1, 64, F16)]
+    ref = U.attention_reference(*clean5[:3], dout=clean5[3], **kw)
+    for what, x, y, t in zip(("out", "dq", "dk", "dv"), got, want, touched):
+        assert torch.equal(x[others], y[others]), (name, what)
+        r, bound = ref[what]
+        U.assert_within(x[5:6, ~t], r[:, ~t], bound[:, ~t], (name, what))

@@ -2,8 +2,9 @@
 points take (no GPU)."""
 import pytest
 
+from tests.layer_sizes import FULL_CHIP, LARGE_GRADIENTS, LARGE_PRODUCTS
 from tests.test_layer import A, ERR_ARG, ERR_UNSUPPORTED, attention_args
-from welder_typical_chain_amd import _lib
+from welder_typical_chain_amd import _lib, layer
 
 
 @pytest.fixture(scope="module")
@@ -55,3 +56,41 @@ def test_scale_beyond_float32(L, scale):
     assert L.wtc_window_attention(attention_args(scale=scale), A, A, A, A, None, A, 1 << 40, None) == ERR_ARG
     assert L.wtc_window_attention_backward(attention_args(scale=scale), *[A] * 9, A, 1 << 40, None) == ERR_ARG
     assert L.wtc_window_attention_decode(attention_args(lq=1, k_lens=A, scale=scale), A, A, 2 * A, A, A, A, A, 1 << 40, None) == ERR_ARG
+
+
+@pytest.mark.parametrize("size,tile", LARGE_PRODUCTS)
+@pytest.mark.parametrize("b_trans", [False, True])
+def test_plan_of_large_products(L, size, tile, b_trans):
+    assert layer.matmul_epilogue_plan(*size, b_trans=b_trans, cu_count=256) == (*tile, 1)
+
+
+@pytest.mark.parametrize("size,part,tile,split", LARGE_GRADIENTS)
+@pytest.mark.parametrize("b_trans", [False, True])
+def test_plan_of_large_gradients(L, size, part, tile, split, b_trans):
+    *got, splits = layer.matmul_epilogue_plan(*size, b_trans=b_trans, part=part, cu_count=256)
+    assert tuple(got) == tile and (splits > 1) == split
+
+
+def test_plan_of_few_rows(L):
+    assert layer.matmul_epilogue_plan(8, 4096, 4096, b_trans=True, cu_count=256) == (16, 16, 1)
+    assert layer.matmul_epilogue_plan(8, 4096, 4096, cu_count=256)[0] == 64
+
+
+@pytest.mark.parametrize("b,h,kv,lq,lk,d,kw", FULL_CHIP)
+def test_plan_of_a_full_chip(L, b, h, kv, lq, lk, d, kw):
+    plan = layer.window_attention_plan(b, h, kv, lq, lk, d, cu_count=256, **kw)
+    assert plan["row_waves"] == 1 and plan["dq_row_waves"] == 1 and plan["key_splits"] == 1
+    few = layer.window_attention_plan(1, h, kv, 90, 90, d, cu_count=256, **kw)
+    assert few["row_waves"] == 2 and few["dq_row_waves"] == 2
+
+
+def test_plan_refusals(L):
+    with pytest.raises(_lib.WtcError):
+        layer.matmul_epilogue_plan(8, 12, 8)
+    with pytest.raises(ValueError):
+        layer.matmul_epilogue_plan(8, 16, 8, part="dc")
+    with pytest.raises(_lib.WtcError):
+        layer.window_attention_plan(1, 3, 2, 8, 8, 64)
+    args = attention_args()
+    assert L.wtc_window_attention_plan(None, 0, None) == ERR_ARG and L.wtc_window_attention_plan(args, 0, None) == ERR_ARG
+    assert L.wtc_matmul_epilogue_plan(None, 0, 0, None, None, None) == ERR_ARG

@@ -85,6 +85,8 @@ SIGNATURES = {
     "wtc_matmul_epilogue": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 7 + [ctypes.c_size_t, _c_p]),
     "wtc_matmul_epilogue_backward_workspace_size": (_c_i64, [ctypes.c_char_p]),
     "wtc_matmul_epilogue_backward": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 8 + [ctypes.c_size_t, _c_p]),
+    "wtc_matmul_epilogue_plan": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_int, ctypes.c_int] + [ctypes.POINTER(_c_i64)] * 3),
+    "wtc_window_attention_plan": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(_c_i64)]),
     "wtc_window_attention_workspace_size": (_c_i64, [ctypes.c_char_p]),
     "wtc_window_attention": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 6 + [ctypes.c_size_t, _c_p]),
     "wtc_window_attention_backward_workspace_size": (_c_i64, [ctypes.c_char_p]),

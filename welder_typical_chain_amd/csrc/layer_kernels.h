@@ -12,6 +12,7 @@ struct MatmulPlan {
 };
 MatmulPlan plan_matmul(int64_t m, int64_t n, int64_t k, bool aks, bool bks, int cu_count);
 int64_t matmul_workspace(const MatmulPlan& plan, int64_t m, int64_t n);
+void matmul_tile_size(const MatmulPlan& plan, int64_t* tile_m, int64_t* tile_n);
 // aks / bks: the operand is strided along k (element (row, k) at k * ld + row) instead
 // of contiguous (row * ld + k); aks only with bks and out_dt == dt.
 hipError_t launch_matmul(const MatmulParams& p, const MatmulPlan& plan, int dt, int out_dt, bool aks, bool bks,
@@ -43,7 +44,8 @@ int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);
 // p.part_out: attention_workspace() bytes
 hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, hipStream_t stream);
 struct AttnBackwardPlan {
-  int key_blocks, near_blocks, near_chunks, far_blocks, far_chunks, far_keys, cu_count;
+  int dq_groups;  // waves that share a query row
+  int key_blocks, near_blocks, near_chunks, far_blocks, far_chunks, far_keys;
   int64_t part_at, far_at, workspace;  // bytes
 };
 AttnBackwardPlan plan_attention_backward(const AttnParams& p, int cu_count);

@@ -91,9 +91,8 @@ struct MatmulBackwardPlan {
   bool pair;
   int64_t sums_at, partial_at, total;
 };
-MatmulBackwardPlan plan_backward(const wtc_matmul_args& p) {
+MatmulBackwardPlan plan_backward(const wtc_matmul_args& p, int cus) {
   MatmulBackwardPlan q{};
-  const int cus = cu_count();
   q.chunk_rows = act_backward_chunk_rows(p.m, p.n, cus);
   q.chunks = std::max<int64_t>(1, (p.m + q.chunk_rows - 1) / q.chunk_rows);
   q.da = plan_matmul(p.m, p.k, p.n, false, p.b_trans, cus);
@@ -269,7 +268,7 @@ int wtc_matmul_epilogue(const wtc_matmul_args* p, const void* a, const void* b, 
 int64_t wtc_matmul_epilogue_backward_workspace_size(const wtc_matmul_args* p) {
   if (!p) return bad("NULL arguments"), -1;
   if (guarded([&] { return check_matmul(*p, true); })) return -1;
-  return plan_backward(*p).total;
+  return plan_backward(*p, cu_count()).total;
 }
 
 int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, const void* a, const void* b,
@@ -285,7 +284,7 @@ int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, con
     if (!aligned16(dout) || !aligned16(a) || !aligned16(b) || !aligned16(pre) || !aligned16(da) || !aligned16(db) ||
         !aligned16(dbias))
       return bad("pointers must be 16-byte aligned");
-    const MatmulBackwardPlan plan = plan_backward(*p);
+    const MatmulBackwardPlan plan = plan_backward(*p, cu_count());
     if (int rc = check_workspace(workspace, workspace_bytes, plan.total)) return rc;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint8_t* dz = act ? ws : static_cast<uint8_t*>(const_cast<void*>(dout));
@@ -335,6 +334,26 @@ int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, con
       if (int rc = launched(launch_matmul(x, plan.da, dt, dt, false, p->b_trans, stream), "da")) return rc;
     if (want_db)
       if (int rc = launched(launch_matmul(y, plan.db, dt, dt, true, true, stream), "db")) return rc;
+    return WTC_OK;
+  });
+}
+
+int wtc_matmul_epilogue_plan(const wtc_matmul_args* p, int part, int cus, int64_t* tile_m, int64_t* tile_n,
+                             int64_t* splits) {
+  return guarded([&]() -> int {
+    if (!p || !tile_m || !tile_n || !splits) return bad("NULL argument");
+    if (part < 0 || part > 2) return bad("part must be 0 (forward), 1 (da) or 2 (db)");
+    if (int rc = check_matmul(*p, part > 0)) return rc;
+    if (cus <= 0) cus = cu_count();
+    MatmulPlan plan;
+    if (part == 0) {
+      plan = plan_matmul(p->m, p->n, p->k, false, !p->b_trans, cus);
+    } else {
+      const MatmulBackwardPlan both = plan_backward(*p, cus);
+      plan = part == 1 ? both.da : both.db;
+    }
+    matmul_tile_size(plan, tile_m, tile_n);
+    *splits = plan.splits;
     return WTC_OK;
   });
 }
@@ -401,6 +420,23 @@ int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout,
     a.dv = static_cast<uint8_t*>(dv);
     return launched(launch_attention_backward(a, plan, (int)p->dtype, static_cast<hipStream_t>(stream)),
                     "window_attention_backward");
+  });
+}
+
+int wtc_window_attention_plan(const wtc_attention_args* p, int cus, int64_t* plan) {
+  return guarded([&]() -> int {
+    if (!p || !plan) return bad("NULL argument");
+    if (int rc = check_attention_backward(*p)) return rc;
+    if (cus <= 0) cus = cu_count();
+    const AttnParams a = attention_params(*p);
+    const AttnPlan forward = plan_attention(a, cus);
+    const AttnBackwardPlan backward = plan_attention_backward(a, cus);
+    plan[0] = forward.key_groups;
+    plan[1] = forward.splits;
+    plan[2] = backward.dq_groups;
+    plan[3] = backward.near_chunks;
+    plan[4] = (int64_t)backward.far_blocks * backward.far_chunks;
+    return WTC_OK;
   });
 }
 

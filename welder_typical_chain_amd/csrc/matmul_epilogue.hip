@@ -608,6 +608,11 @@ hipError_t launch_matmul_pair(const MatmulParams& da, const MatmulParams& db, in
   return hipLaunchKernel(fn, dim3(x_tiles + y_tiles), dim3(kThreads), args, 0, stream);
 }
 
+void matmul_tile_size(const MatmulPlan& plan, int64_t* tile_m, int64_t* tile_n) {
+  *tile_m = plan.variant == kRowsVariant ? kRowsMost : kVariants[plan.variant].tm;
+  *tile_n = plan.variant == kRowsVariant ? 16 : kVariants[plan.variant].tn;
+}
+
 int64_t matmul_workspace(const MatmulPlan& plan, int64_t m, int64_t n) {
   return plan.splits > 1 ? plan.splits * m * n * 4 : 0;
 }

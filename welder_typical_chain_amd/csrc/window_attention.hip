@@ -1201,7 +1201,8 @@ template <int DT> const void* dkv_kernel(int nd) {
 
 AttnBackwardPlan plan_attention_backward(const AttnParams& p, int cu_count) {
   AttnBackwardPlan plan{};
-  plan.cu_count = cu_count;
+  const int64_t row_blocks = ((int64_t)p.lq * p.group + kDqRows - 1) / kDqRows;
+  plan.dq_groups = (int64_t)p.batch * p.kv_heads * row_blocks <= cu_count ? 2 : 1;
   plan.key_blocks = (p.lk + kDkvKeys - 1) / kDkvKeys;
   // queries past the near ones of the first block: at most the keys past them
   const int64_t far = std::min<int64_t>(p.lq, (int64_t)p.lk - (p.window + kDkvKeys) + 1);
@@ -1240,7 +1241,7 @@ hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwar
   const int64_t seqs = (int64_t)p.batch * p.kv_heads;
   if (p.lq) {
     p.row_blocks = (int)(((int64_t)p.lq * p.group + kDqRows - 1) / kDqRows);
-    const bool pairs = seqs * p.row_blocks <= plan.cu_count;
+    const bool pairs = plan.dq_groups == 2;
     const void* fn = pairs ? (dt == DT_F16 ? dq_kernel<DT_F16, 2>(nd) : dq_kernel<DT_BF16, 2>(nd))
                            : (dt == DT_F16 ? dq_kernel<DT_F16, 1>(nd) : dq_kernel<DT_BF16, 1>(nd));
     const hipError_t e = launch(fn, seqs * p.row_blocks, pairs ? 512 : 256, p, stream);

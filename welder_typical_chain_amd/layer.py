@@ -14,6 +14,7 @@ dual tensor's tangent needs the latter).
 """
 from __future__ import annotations
 
+import ctypes
 import struct
 
 import torch
@@ -268,6 +269,32 @@ def matmul_epilogue_backward(dout: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     _launch(device, lib.wtc_matmul_epilogue_backward, args, d2.data_ptr(), a2.data_ptr(), b.data_ptr(),
             _ptr(pre) if act else None, _ptr(da), _ptr(db), _ptr(dbias), ws_ptr, ws_bytes)
     return da, db.t() if trans and db is not None else db, dbias
+
+
+def matmul_epilogue_plan(m: int, n: int, k: int, *, b_trans: bool = False, part: str = "forward",
+                         cu_count: int = 0) -> tuple:
+    """(tile rows, tile columns, splits of k) of the kernel that matmul_epilogue runs for
+    dense operands of these sizes on a device of `cu_count` compute units (0: the current
+    one), or of part "da" or "db" of its gradients.  (16, 16, 1): few rows, no tiles."""
+    args = _pack_matmul(m, n, k, k, k if b_trans else n, n, n, bool(b_trans), _lib.DTYPE_BF16, _lib.DTYPE_BF16,
+                        _lib.DTYPE_BF16, 0, n)
+    got = (ctypes.c_int64 * 3)()
+    at = [ctypes.cast(ctypes.byref(got, 8 * i), ctypes.POINTER(ctypes.c_int64)) for i in range(3)]
+    _lib.check(_lib.lib().wtc_matmul_epilogue_plan(args, ("forward", "da", "db").index(part), cu_count, *at))
+    return tuple(got)
+
+
+def window_attention_plan(batch: int, heads: int, kv_heads: int, lq: int, lk: int, dim: int, *,
+                          window: int | None = None, sinks: int = 0, cu_count: int = 0) -> dict:
+    """What window_attention and its gradients run for dense tensors of these sizes on a
+    device of `cu_count` compute units (0: the current one): "row_waves" and "key_splits" of
+    the forward pass, "dq_row_waves", "query_parts" and "far_parts" of the gradients."""
+    q, kv = (lq * heads * dim, heads * dim, dim), (lk * kv_heads * dim, kv_heads * dim, dim)
+    args = _pack_attention(batch, heads, kv_heads, lq, lk, dim, *_mask(window, sinks), _lib.DTYPE_BF16, *q, *kv, *kv,
+                           *q, *q, 0, 0, 0, 0, 0, 0, dim ** -0.5)
+    got = (ctypes.c_int64 * 5)()
+    _lib.check(_lib.lib().wtc_window_attention_plan(args, cu_count, got))
+    return dict(zip(("row_waves", "key_splits", "dq_row_waves", "query_parts", "far_parts"), got))
 
 
 def _strides(t, name):
