@@ -9,6 +9,7 @@
  *   wtc_window_attention_backward  dQ, dK, dV of it
  *   wtc_window_attention_decode    the same for one token a sequence against
  *                                  a cache, which it also appends to
+ *   wtc_*_plan                     what such a call runs
  *
  * Status codes, wtc_last_error() and element type codes are wtc_hip.h's.
  * Every call is asynchronous on `stream` (a hipStream_t, or NULL) and may be
@@ -42,9 +43,11 @@ extern "C" {
  * or with b_trans its transpose stored as [n][k]; out, residual and pre [m][n].
  * The ld* are row strides in elements.  dtype (WTC_DTYPE_F16 / BF16): A and B;
  * out_dtype (dtype or WTC_DTYPE_F32): out and residual; bias_dtype
- * (dtype or WTC_DTYPE_F32): bias.  A, B, dout, pre and out start 16-byte
- * aligned and their rows are 16-byte aligned; n and k are multiples of 8 (k
- * may be 0: then A . B is 0).  m and n may be 0.  No operand spans 2 GiB.
+ * (dtype or WTC_DTYPE_F32): bias.  Every pointer, bias, residual and the
+ * gradients too, is 16-byte aligned and every ld* a multiple of 8, and so are n and k
+ * (k may be 0: then A . B is 0).  m and n may be 0.  No operand spans 2 GiB.
+ * Activations and their slopes keep their relative accuracy out to both tails: to
+ * a few roundings with f32 outputs, below the output's rounding with 16-bit ones.
  */
 typedef struct wtc_matmul_args {
   int64_t m, n, k;
@@ -66,7 +69,9 @@ int64_t wtc_matmul_epilogue_backward_workspace_size(const wtc_matmul_args* p);
 /* dz = dout * act'(pre); da = dz . B^T (dense [m][k]), db = A^T . dz (dense, in
  * B's layout), both of `dtype`, and dbias = the column sums of dz in f32.  Each
  * of the three may be NULL (not computed).  dout is of `dtype`.  pre may be
- * NULL with WTC_ACT_NONE.  The residual's gradient is dout itself. */
+ * NULL with WTC_ACT_NONE.  The residual's gradient is dout itself.  The products
+ * take dz rounded to `dtype`: in f16, dout is best scaled to well above 6e-5 and
+ * below 5e4. */
 int wtc_matmul_epilogue_backward(const wtc_matmul_args* p, const void* dout, const void* a, const void* b,
                                  const float* pre, void* da, void* db, float* dbias, void* workspace,
                                  size_t workspace_bytes, void* stream);
@@ -90,7 +95,13 @@ int wtc_matmul_epilogue_plan(const wtc_matmul_args* p, int part, int cu_count, i
  * i of a sequence stands at position p = i + k_len - q_len and sees the keys
  * j <= p with p - j < window or j < sinks (window 0: no limit).  A query that
  * sees no key, or stands behind its sequence's end, gives zeros (log-sum-exp
- * -inf, gradient 0); keys behind the end are not read (gradient 0).
+ * -inf, gradient 0); keys behind the end are not read (gradient 0).  A NaN or an
+ * infinity that the mask hides from a row does not reach it; a NaN that the row
+ * sees does, whatever its weight.
+ *
+ * Sums and statistics are f32; the products take the softmax weights, and in the
+ * backward pass their gradients, rounded to dtype (f16: times powers of two that
+ * keep them in its range).
  */
 typedef struct wtc_attention_args {
   int64_t batch, heads, kv_heads, lq, lk, dim;
@@ -129,7 +140,8 @@ int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p);
  * tokens of each sequence with the new one, any number (0: an idle sequence;
  * its out is 0 and its cache is left alone).  k_new, v_new
  * [batch][kv_heads][dim]: the new token's key and value, written to the
- * caches and attended to; both NULL: the caches hold them already. */
+ * caches and attended to (the caches are two then); both NULL: the caches hold
+ * them already. */
 int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void* k, void* v, const void* k_new,
                                 const void* v_new, void* out, void* workspace, size_t workspace_bytes,
                                 void* stream);

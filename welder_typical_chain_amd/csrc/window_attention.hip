@@ -403,7 +403,8 @@ __device__ inline float power_of_2(int e) { return __builtin_amdgcn_ldexpf(1.0f,
 // dS: taken times 2^ex, ex of each row (dq) or key (dk) its own.  It starts higher than any
 // use, short of where f32 would overflow, and is lowered, together with the sums so
 // far, when a value reaches 2^15, to put that value at 2^12 or more.  What a lane packs is
-// then off by 2^-11 of itself or 2^-37 of the largest so far.  The factor and the test
+// then off by 2^-11 of itself or 2^-37 of the largest so far (where none has reached 2^12,
+// in dq, 2^-55 of the row's largest dout).  The factor and the test
 // cost f16 2 to 5 % (forward and gradients, 4096 causal tokens, 32 / 8 heads of 128: 922 ->
 // 937 us; 4 x 2048, 16 heads of 64: 329 -> 345).  bf16 has f32's range.
 template <int DT> struct DsRange {
@@ -792,8 +793,8 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
 // Where the key blocks alone leave CUs idle, the near queries go in p.near_chunks
 // parts as well, and every key's sums that way (3 x 1000 causal tokens, 6 / 3 heads
 // of 80: 65 -> 40 us, and 6 for the sums).
-// Both kernels on 4 x 4096 causal tokens, 32 / 8 heads of 128: 2017 us, 682 TFLOP/s by
-// the usual count of 5 products and 955 by the 7 that they run.
+// Both kernels on 4 x 4096 causal tokens, 32 / 8 heads of 128: 1993 us, 690 TFLOP/s by
+// the usual count of 5 products and 966 by the 7 that they run (f16, see DsRange: 2153).
 constexpr int kDkvWaves = 8;
 constexpr int kDkvKeys = 128;
 constexpr int kQueries = 64;
