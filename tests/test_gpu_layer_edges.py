@@ -95,6 +95,20 @@ def test_decode_nan_beside_far_larger_scores(W, cap, n, where):
         assert bool(out.isnan().all())
 
 
+@pytest.mark.parametrize("dtype,h,kv,d", [(BF16, 2, 2, 64), (F16, 40, 1, 80), (BF16, 4, 2, 128)])
+@pytest.mark.parametrize("cap,n", [(1, 1), (1, 7), (2, 2), (33, 33), (33, 70)])
+def test_decode_over_stale_nan(W, dtype, h, kv, d, cap, n):
+    """What the new token's row held before does not matter, in a cache of one row either."""
+    q, kn, vn = rand(1, 2, h, d, dtype=dtype), rand(2, 2, kv, d, dtype=dtype), rand(3, 2, kv, d, dtype=dtype)
+    kc, vc = rand(4, 2, cap, kv, d, dtype=dtype), rand(5, 2, cap, kv, d, dtype=dtype)
+    want, bound, rk, rv = U.decode_reference(q, kc, vc, [n, n], k_new=kn, v_new=vn)
+    kc[:, U.cache_row(n - 1, cap, 0)] = NAN
+    vc[:, U.cache_row(n - 1, cap, 0)] = NAN
+    out = W.window_attention_decode(q, kc, vc, lens(n, n), k_new=kn, v_new=vn)
+    U.assert_within(out, want, bound, "out")
+    assert torch.equal(kc, rk) and torch.equal(vc, rv)
+
+
 def test_decode_all_scores_minus_infinity(W):
     """Keys of -inf alone: a row without keys, as in the prompt form; beside others they count nothing."""
     q = torch.ones(1, 1, 64, dtype=F16, device="cuda")

@@ -168,9 +168,10 @@ AttnParams attention_params(const wtc_attention_args& p) {
     q.o_stride[i] = p.o_stride[i];
     q.do_stride[i] = p.do_stride[i];
   }
-  // the stride of a single token counts for nothing
+  // The stride of a single token counts for nothing.  A tile's rows behind a single key lie
+  // outside what its loads may read, and give zeros, only if they are apart from it.
   if (p.lq <= 1) q.q_stride[1] = q.o_stride[1] = q.do_stride[1] = 0;
-  if (p.lk <= 1) q.k_stride[1] = q.v_stride[1] = 0;
+  if (p.lk <= 1) q.k_stride[1] = q.v_stride[1] = p.dim;
   for (int i = 0; i < 2; ++i) {
     q.kn_stride[i] = p.kn_stride[i];
     q.vn_stride[i] = p.vn_stride[i];
