@@ -18,6 +18,15 @@ def test_one_cache_cannot_take_a_key_and_a_value(L):
     assert b"same cache" in L.wtc_last_error()
 
 
+@pytest.mark.parametrize("kw", [dict(k=(2048, 8, 64)), dict(v=(2048, 56, 64))])
+def test_decode_refuses_caches_of_overlapping_rows(L, kw):
+    args = attention_args(**{**dict(lq=1, k_lens=A), **kw})
+    assert L.wtc_window_attention_decode_workspace_size(args) == -1
+    assert L.wtc_window_attention_decode(args, A, A, 2 * A, None, None, A, A, 1 << 40, None) == ERR_ARG
+    same = attention_args(lq=1, k_lens=A, k=(2048, 0, 64), v=(2048, 0, 64))  # one row for all tokens
+    assert L.wtc_window_attention_decode_workspace_size(same) >= 0
+
+
 # A launch takes fewer than 2^32 threads: 2^23 workgroups of 512, 2^24 of 256.
 ONE = dict(heads=1, kv_heads=1, dim=8, q=(8, 8, 8), k=(8, 8, 8), v=(8, 8, 8), o=(8, 8, 8), do=(8, 8, 8), kn=(8, 8), vn=(8, 8))
 

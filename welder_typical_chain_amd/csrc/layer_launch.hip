@@ -153,6 +153,9 @@ int check_attention(const wtc_attention_args& p, bool decode) {
     if (p.lq != 1) return bad("decode takes one token a sequence");
     if (p.lk <= p.sinks) return bad("the cache must have more rows than sinks");
     if (!p.k_lens && p.batch) return bad("decode needs k_lens");
+    // (a tile's rows behind the last one would be parts of it, not zeros)
+    for (const int64_t s : {p.k_stride[1], p.v_stride[1]})
+      if (p.lk > 1 && s > 0 && s < p.dim) return bad("a cache's rows overlap");
     if ((rc = check_strides(p.kn_stride, 2, 0, "k_new"))) return rc;
     if ((rc = check_strides(p.vn_stride, 2, 0, "v_new"))) return rc;
   }
