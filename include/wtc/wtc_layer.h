@@ -141,7 +141,8 @@ int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p);
  * its out is 0 and its cache is left alone).  k_new, v_new
  * [batch][kv_heads][dim]: the new token's key and value, written to the
  * caches and attended to (the caches are two then); both NULL: the caches hold
- * them already. */
+ * them already.  A cache's rows do not overlap; stride 0, one row for all tokens,
+ * is for caches that are only read. */
 int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void* k, void* v, const void* k_new,
                                 const void* v_new, void* out, void* workspace, size_t workspace_bytes,
                                 void* stream);

@@ -109,6 +109,18 @@ def test_decode_over_stale_nan(W, dtype, h, kv, d, cap, n):
     assert torch.equal(kc, rk) and torch.equal(vc, rv)
 
 
+@pytest.mark.parametrize("cap,window,sinks", [(300, None, 3), (64, 16, 0), (5000, 4000, 100)])
+def test_decode_of_the_longest_sequences(W, cap, window, sinks):
+    """Lengths up to what int32 holds, and negative ones (idle)."""
+    n = [2 ** 31 - 1, 2 ** 31 - 17, 2 ** 30, -5]
+    q, kn, vn = rand(1, 4, 4, 64, dtype=BF16), rand(2, 4, 2, 64, dtype=BF16), rand(3, 4, 2, 64, dtype=BF16)
+    kc, vc = rand(4, 4, cap, 2, 64, dtype=BF16), rand(5, 4, cap, 2, 64, dtype=BF16)
+    want, bound, rk, rv = U.decode_reference(q, kc, vc, n, window=window, sinks=sinks, k_new=kn, v_new=vn)
+    out = W.window_attention_decode(q, kc, vc, lens(*n), window=window, sinks=sinks, k_new=kn, v_new=vn)
+    U.assert_within(out, want, bound, "out")
+    assert torch.equal(kc, rk) and torch.equal(vc, rv)
+
+
 def test_decode_all_scores_minus_infinity(W):
     """Keys of -inf alone: a row without keys, as in the prompt form; beside others they count nothing."""
     q = torch.ones(1, 1, 64, dtype=F16, device="cuda")
