@@ -9,6 +9,15 @@
  *   wtc_window_attention_backward  dQ, dK, dV of it
  *   wtc_window_attention_decode    the same for one token a sequence against
  *                                  a cache, which it also appends to
+ *   wtc_cross_attention            attention to another sequence: no order, every
+ *                                  query sees every key
+ *   wtc_cross_attention_backward   dQ, dK, dV of it
+ *   wtc_prefix_attention           causal attention of a batch behind a prefix that
+ *                                  its sequences share
+ *   wtc_prefix_attention_decode    the same for one token a sequence
+ *   wtc_window_attention_weights   what each key has received from the queries
+ *   wtc_window_attention_decode_weights  decode that adds up what its rows receive
+ *   wtc_cache_evict                a smaller cache of the rows of most weight
  *   wtc_*_plan                     what such a call runs
  *
  * Status codes, wtc_last_error() and element type codes are wtc_hip.h's.
@@ -18,7 +27,8 @@
  * call needs scratch memory, the caller passes it (256-byte aligned,
  * uninitialised; calls that may overlap must not share one); too little of it
  * is WTC_ERR_WORKSPACE.  Outputs may not overlap inputs, but for the residual,
- * which may be the output itself, and the caches that decode appends to.  Calls
+ * which may be the output itself, and the caches and weights that decode and
+ * wtc_window_attention_weights add to.  Calls
  * may come from any host thread.  Results do not depend on timing: nothing is
  * summed by atomics.
  */
@@ -146,6 +156,85 @@ int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p);
 int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void* k, void* v, const void* k_new,
                                 const void* v_new, void* out, void* workspace, size_t workspace_bytes,
                                 void* stream);
+
+/*
+ * Attention to another sequence: as wtc_window_attention, but query i < q_len sees
+ * every key j < k_len.  window and sinks are 0; lq + lk is at most 2^30.
+ */
+int64_t wtc_cross_attention_workspace_size(const wtc_attention_args* p);
+int wtc_cross_attention(const wtc_attention_args* p, const void* q, const void* k, const void* v, void* out,
+                        float* lse, void* workspace, size_t workspace_bytes, void* stream);
+int64_t wtc_cross_attention_backward_workspace_size(const wtc_attention_args* p);
+int wtc_cross_attention_backward(const wtc_attention_args* p, const void* dout, const void* q, const void* k,
+                                 const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A prefix that all sequences of a batch share, [prefix][kv_heads][dim], strides of
+ * token and head.  A query i < q_len sees every prefix key and, of its sequence's
+ * own keys, those that it sees in wtc_window_attention without a window (window and
+ * sinks are 0).  prefix and lk may be 0.
+ */
+typedef struct wtc_prefix_args {
+  int64_t prefix;
+  int64_t kp_stride[2], vp_stride[2];
+} wtc_prefix_args;
+
+int64_t wtc_prefix_attention_workspace_size(const wtc_attention_args* p, const wtc_prefix_args* x);
+/* lse: as in wtc_window_attention, over prefix and own keys (NULL: not written) */
+int wtc_prefix_attention(const wtc_attention_args* p, const wtc_prefix_args* x, const void* q, const void* k_prefix,
+                         const void* v_prefix, const void* k, const void* v, void* out, float* lse, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+int64_t wtc_prefix_attention_decode_workspace_size(const wtc_attention_args* p, const wtc_prefix_args* x);
+/* One token a sequence.  The own caches, their lengths (without the prefix) and the
+ * new token as in wtc_window_attention_decode without sinks: token j stands in row
+ * j % lk.  A sequence of length 0 is idle: its out is 0. */
+int wtc_prefix_attention_decode(const wtc_attention_args* p, const wtc_prefix_args* x, const void* q,
+                                const void* k_prefix, const void* v_prefix, void* k, void* v, const void* k_new,
+                                const void* v_new, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * What each key receives, f32 [batch][kv_heads][lk]: the sum over the query heads of
+ * its key head and the queries that see it of exp(scale q . k - lse), lse f32
+ * [batch][heads][lq] as wtc_window_attention gave it for the same arguments.  With
+ * add, it is added to what `weights` holds; otherwise it replaces it (keys behind
+ * their sequence's end: 0).
+ */
+int64_t wtc_window_attention_weights_workspace_size(const wtc_attention_args* p);
+int wtc_window_attention_weights(const wtc_attention_args* p, const void* q, const void* k, const float* lse,
+                                 float* weights, int add, void* workspace, size_t workspace_bytes, void* stream);
+
+/* wtc_window_attention_decode that also adds what each visible row of the cache
+ * receives from the token to `weights`, f32 [batch][kv_heads][lk].  The newest
+ * token's row is set to it: what it held was another token's. */
+int64_t wtc_window_attention_decode_weights_workspace_size(const wtc_attention_args* p);
+int wtc_window_attention_decode_weights(const wtc_attention_args* p, const void* q, void* k, void* v,
+                                        const void* k_new, const void* v_new, void* out, float* weights,
+                                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The rows of a cache that stay, in a smaller one.  k, v [batch][rows][kv_heads][dim],
+ * weights [batch][kv_heads][rows] f32 (dense), lengths int32 [batch] (clamped to 0 ..
+ * rows).  A sequence of up to `keep` rows keeps them all; of a longer one each key head
+ * keeps the first `sinks`, the last `recent` and, of those between, the ones of
+ * greatest weight (of equal ones the lowest rows; a NaN is the greatest).  They go,
+ * in their order, to k_out, v_out [batch][out_rows][kv_heads][dim] and weights_out
+ * [batch][kv_heads][out_rows], out_rows >= keep; rows [batch][kv_heads][keep] says
+ * which they were (-1 behind the last one), lengths_out how many.  Behind a sequence's
+ * last row, k_out and v_out are 0 up to row keep and left alone from there on;
+ * weights_out is 0 to its end.  recent + sinks <= keep.  Strides (elements,
+ * multiples of 8) of sequence, row and head; dtype f16 or bf16.
+ */
+typedef struct wtc_evict_args {
+  int64_t batch, kv_heads, rows, out_rows, dim, dtype;
+  int64_t keep, recent, sinks;
+  int64_t k_stride[3], v_stride[3], ko_stride[3], vo_stride[3];
+} wtc_evict_args;
+
+int wtc_cache_evict(const wtc_evict_args* p, const void* k, const void* v, const float* weights,
+                    const int32_t* lengths, void* k_out, void* v_out, float* weights_out, int32_t* rows,
+                    int32_t* lengths_out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -10,7 +10,8 @@ from . import _lib  # noqa: F401
 
 _CHAIN = ["matmul_softmax", "workspace_size", "new_workspace", "read_error_flags"]
 _LAYER = ["matmul_epilogue", "matmul_epilogue_backward", "window_attention", "window_attention_backward",
-          "window_attention_decode"]
+          "window_attention_decode", "cross_attention", "cross_attention_backward", "prefix_attention",
+          "prefix_attention_decode", "window_attention_weights", "cache_evict"]
 __all__ = _CHAIN + _LAYER
 
 

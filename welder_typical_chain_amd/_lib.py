@@ -93,6 +93,19 @@ SIGNATURES = {
     "wtc_window_attention_backward": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 10 + [ctypes.c_size_t, _c_p]),
     "wtc_window_attention_decode_workspace_size": (_c_i64, [ctypes.c_char_p]),
     "wtc_window_attention_decode": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 7 + [ctypes.c_size_t, _c_p]),
+    "wtc_cross_attention_workspace_size": (_c_i64, [ctypes.c_char_p]),
+    "wtc_cross_attention": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 6 + [ctypes.c_size_t, _c_p]),
+    "wtc_cross_attention_backward_workspace_size": (_c_i64, [ctypes.c_char_p]),
+    "wtc_cross_attention_backward": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 10 + [ctypes.c_size_t, _c_p]),
+    "wtc_prefix_attention_workspace_size": (_c_i64, [ctypes.c_char_p] * 2),
+    "wtc_prefix_attention": (ctypes.c_int, [ctypes.c_char_p] * 2 + [_c_p] * 8 + [ctypes.c_size_t, _c_p]),
+    "wtc_prefix_attention_decode_workspace_size": (_c_i64, [ctypes.c_char_p] * 2),
+    "wtc_prefix_attention_decode": (ctypes.c_int, [ctypes.c_char_p] * 2 + [_c_p] * 9 + [ctypes.c_size_t, _c_p]),
+    "wtc_window_attention_weights_workspace_size": (_c_i64, [ctypes.c_char_p]),
+    "wtc_window_attention_weights": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 4 + [ctypes.c_int, _c_p, ctypes.c_size_t, _c_p]),
+    "wtc_window_attention_decode_weights_workspace_size": (_c_i64, [ctypes.c_char_p]),
+    "wtc_window_attention_decode_weights": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 8 + [ctypes.c_size_t, _c_p]),
+    "wtc_cache_evict": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 10),
     "wtc_last_error": (ctypes.c_char_p, []),
     "wtc_version": (ctypes.c_char_p, []),
     "welder_compile_typical_chain_to_nvvm": (ctypes.c_int, [

@@ -53,6 +53,7 @@ ARCH = "gfx950"
 HIP_SOURCES = ["fused_matmul_softmax.hip", "wide_tile.hip", "rowblock_softmax.hip", "fewrows_softmax.hip",
                "unfused_chain.hip",
                "matmul_epilogue.hip", "window_attention.hip", "window_decode.hip",
+               "key_weights.hip", "cache_evict.hip",
                "launch.hip", "layer_launch.hip"]
 HOST_SOURCES = ["launch.hip", "layer_launch.hip"]  # no kernels to report on
 CXX_SOURCES = ["chain_recognizer.cpp", "variants.cpp", "tile_solver.cpp", "compile_capi.cpp"]

@@ -69,6 +69,18 @@ __device__ inline void dma16(i32x4 rsrc, uint32_t voff, uint32_t lds_base) {
                : "memory", "m0");
 }
 
+// 4 bytes per lane into LDS at lds_base + 4*lane.
+__device__ inline void dma4(i32x4 rsrc, uint32_t voff, uint32_t lds_base) {
+  i32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_base);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(m), "v"(voff), "s"(r)
+               : "memory", "m0");
+}
+
 // Wait until at most N of this wave's direct-to-LDS loads are in flight and
 // its LDS reads are done, then meet the other waves.
 template <int N>

@@ -175,6 +175,14 @@ struct AttnParams {
   int32_t key_blocks, near_blocks, near_chunks, far_blocks, far_chunks, far_keys;
   int32_t batch, heads, kv_heads, group, lq, lk, dim, sinks;
   float scale;
+  int32_t full;       // every query sees every key: it stands behind the last one
+  int32_t seq_rows;   // a batch's queries as one sequence: tokens of each in q (0: they are not)
+  int32_t slots, slot0;  // partial results of a row, and this launch's first (slots 0: it writes results)
+  const uint8_t *kp, *vp;  // keys that a batch shares, [prefix][kv_heads][dim]
+  int64_t kp_stride[2], vp_stride[2];
+  int32_t prefix;
+  float *weights, *scores;  // [batch][kv_heads][lk]; of a decode step, see window_decode.hip
+  int32_t add;              // weights: added to what is there
 };
 
 // Tokens of sequence b: queries and keys (clamped to what the tensors hold).
@@ -184,5 +192,7 @@ __device__ inline int seq_queries(const AttnParams& p, int b) {
 __device__ inline int seq_keys(const AttnParams& p, int b) {
   return p.k_lens ? min(max(p.k_lens[b], 0), p.lk) : p.lk;
 }
+// Position of a sequence's query 0 among its nk keys, of which a query sees those up to its own.
+__device__ inline int first_position(const AttnParams& p, int nq, int nk) { return p.full ? nk - 1 : nk - nq; }
 
 }  // namespace wtc

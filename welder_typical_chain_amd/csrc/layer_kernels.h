@@ -43,6 +43,8 @@ AttnPlan plan_attention(const AttnParams& p, int cu_count);
 int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);
 // p.part_out: attention_workspace() bytes
 hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, hipStream_t stream);
+// Results of the rows from p.slots partial ones, p.part_out [batch][lq][heads][slots][dim] and p.part_lse without dim.
+hipError_t launch_attention_join(const AttnParams& p, int dt, hipStream_t stream);
 struct AttnBackwardPlan {
   int dq_groups;  // waves that share a query row
   int key_blocks, near_blocks, near_chunks, far_blocks, far_chunks, far_keys;
@@ -55,5 +57,28 @@ int plan_decode(const AttnParams& p, int cu_count);  // splits
 int64_t decode_workspace(const AttnParams& p, int splits);
 // p.part_out: decode_workspace() bytes; p.window: at most p.lk - p.sinks
 hipError_t launch_attention_decode(const AttnParams& p, int splits, int dt, hipStream_t stream);
+// The same with p.weights; p.part_out: decode_weights_workspace() bytes
+int64_t decode_weights_workspace(const AttnParams& p, int splits);
+hipError_t launch_attention_decode_weights(const AttnParams& p, int splits, int dt, hipStream_t stream);
+
+struct KeyWeightsPlan {
+  int key_blocks, chunks, chunk_rows;  // chunks of the queries, positions of each
+  int64_t workspace;
+};
+KeyWeightsPlan plan_key_weights(const AttnParams& p, int cu_count);
+// p.lse_in, p.weights, p.add; p.part_out: plan.workspace bytes
+hipError_t launch_key_weights(const AttnParams& p, const KeyWeightsPlan& plan, int dt, hipStream_t stream);
+
+struct EvictParams {
+  const uint8_t *k, *v;
+  uint8_t *k_out, *v_out;
+  const float* weights;  // [batch][kv_heads][rows]
+  float* weights_out;    // [batch][kv_heads][out_rows]
+  const int32_t* lengths;
+  int32_t *kept, *lengths_out;  // [batch][kv_heads][keep]: source rows
+  int64_t k_stride[3], v_stride[3], ko_stride[3], vo_stride[3];  // bytes
+  int32_t batch, kv_heads, rows, out_rows, keep, recent, sinks, row_bytes;
+};
+hipError_t launch_cache_evict(const EvictParams& p, hipStream_t stream);
 
 }  // namespace wtc

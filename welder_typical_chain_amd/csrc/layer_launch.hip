@@ -201,6 +201,136 @@ AttnParams decode_params(const wtc_attention_args& p) {
   return q;
 }
 
+// Every query sees every key: it stands behind the last one, at up to lq + lk - 1.
+int check_positions(int64_t lq, int64_t lk) {
+  return lq + lk > kMost ? report(WTC_ERR_UNSUPPORTED, "more than 2^30 queries and keys") : WTC_OK;
+}
+AttnParams cross_params(const wtc_attention_args& p) {
+  AttnParams q = attention_params(p);
+  q.window = INT32_MAX;
+  q.sinks = 0;
+  q.full = 1;
+  return q;
+}
+int check_cross(const wtc_attention_args& p) {
+  if (p.window || p.sinks) return bad("cross attention has no window and no sinks");
+  return check_positions(p.lq, p.lk);
+}
+
+// ---- a prefix that a batch shares ------------------------------------------------
+// Two launches into slots of the same rows, joined by a third: the batch's queries as one
+// sequence that sees every prefix key, and each sequence's own keys.
+int check_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bool decode) {
+  if (int rc = check_attention(p, decode)) return rc;
+  if (p.window || p.sinks) return bad("attention with a shared prefix has no window and no sinks");
+  if (x.prefix < 0) return bad("negative extent");
+  if (x.prefix > kMost / p.kv_heads) return report(WTC_ERR_UNSUPPORTED, "extent above 2^30");
+  if (int rc = check_positions(p.batch * p.lq, x.prefix)) return rc;
+  if (int rc = check_positions(p.lk, x.prefix)) return rc;
+  const int64_t group = p.heads / p.kv_heads;
+  if (p.kv_heads * ((p.batch * p.lq * group + 127) / 128) >= kThreads / 512) return too_many();
+  for (const int64_t* s : {x.kp_stride, x.vp_stride}) {
+    const int64_t as3[3] = {0, s[0], s[1]};
+    if (int rc = check_strides(as3, 3, x.prefix, s == x.kp_stride ? "k_prefix" : "v_prefix")) return rc;
+  }
+  return WTC_OK;
+}
+struct PrefixPlan {
+  AttnParams common, own;
+  AttnPlan common_plan, own_plan;
+  int own_splits;
+  int64_t bytes;
+};
+PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bool decode, int cus) {
+  PrefixPlan q{};
+  q.own = decode ? decode_params(p) : attention_params(p);
+  if (decode) q.own.q_lens = q.own.k_lens;  // (an idle sequence has no query)
+  q.own.prefix = (int)x.prefix;
+  for (int i = 0; i < 2; ++i) {
+    q.own.kp_stride[i] = x.kp_stride[i];
+    q.own.vp_stride[i] = x.vp_stride[i];
+  }
+  AttnParams& c = q.common = q.own;
+  c.seq_rows = c.lq;
+  c.lq = (int)(p.batch * p.lq);
+  c.lk = c.prefix;
+  c.batch = 1;
+  c.q_lens = c.k_lens = nullptr;
+  c.window = INT32_MAX;
+  c.full = 1;
+  c.k_stride[1] = c.prefix <= 1 ? c.dim : x.kp_stride[0];
+  c.v_stride[1] = c.prefix <= 1 ? c.dim : x.vp_stride[0];
+  c.k_stride[2] = x.kp_stride[1];
+  c.v_stride[2] = x.vp_stride[1];
+  c.prefix = 0;
+  q.common_plan = plan_attention(c, cus);
+  if (decode) q.own_splits = plan_decode(q.own, cus);
+  else q.own_plan = plan_attention(q.own, cus), q.own_splits = q.own_plan.splits;
+  const int first = x.prefix ? q.common_plan.splits : 0;
+  c.slots = q.own.slots = first + (p.lk ? q.own_splits : 0);
+  q.own.slot0 = first;
+  q.bytes = align256(p.batch * p.lq * p.heads * c.slots * 4 * (p.dim + 1));
+  return q;
+}
+int launch_prefix(PrefixPlan& plan, bool decode, int dt, const void* q, const void* kp, const void* vp, const void* k,
+                  const void* v, const void* k_new, const void* v_new, void* out, float* lse, void* workspace,
+                  hipStream_t stream) {
+  const int64_t rows = (int64_t)plan.own.batch * plan.own.lq * plan.own.heads;
+  for (AttnParams* a : {&plan.common, &plan.own}) {
+    a->q = static_cast<const uint8_t*>(q);
+    a->part_out = static_cast<float*>(workspace);
+    a->part_lse = a->part_out + rows * a->slots * a->dim;
+  }
+  AttnParams& own = plan.own;
+  own.k = static_cast<const uint8_t*>(k);
+  own.v = static_cast<const uint8_t*>(v);
+  own.kp = static_cast<const uint8_t*>(kp);
+  own.vp = static_cast<const uint8_t*>(vp);
+  own.k_new = static_cast<const uint8_t*>(k_new);
+  own.v_new = static_cast<const uint8_t*>(v_new);
+  own.out = static_cast<uint8_t*>(out);
+  own.lse = lse;
+  plan.common.k = own.kp;
+  plan.common.v = own.vp;
+  if (plan.common.lk)
+    if (int rc = launched(launch_attention(plan.common, plan.common_plan, dt, stream), "prefix_attention")) return rc;
+  if (own.lk) {
+    const hipError_t e = decode ? launch_attention_decode(own, plan.own_splits, dt, stream)
+                                : launch_attention(own, plan.own_plan, dt, stream);
+    if (int rc = launched(e, "prefix_attention")) return rc;
+  }
+  return launched(launch_attention_join(own, dt, stream), "prefix_attention");
+}
+
+// Scores of a decode step go through memory: [batch][heads][lk + 2 tiles].
+int check_decode_weights(const wtc_attention_args& p) {
+  const int64_t rows = (p.lk + 31) / 32 * 32 + 64;
+  if (p.batch * p.heads > (1ll << 38) / rows || p.batch * p.kv_heads * ((rows + 255) / 256) + p.batch * p.heads >= kThreads / 256)
+    return too_many();
+  return WTC_OK;
+}
+
+int check_evict(const wtc_evict_args& p) {
+  if (p.dtype != WTC_DTYPE_F16 && p.dtype != WTC_DTYPE_BF16) return bad("dtype must be f16 or bf16");
+  if (p.batch < 0 || p.rows < 0) return bad("negative extent");
+  if (p.kv_heads <= 0) return bad("kv_heads must be positive");
+  if (p.dim < 8 || p.dim > kMaxDim || p.dim % 8) return bad("dim must be a multiple of 8 up to 128");
+  if (p.keep < 1 || p.recent < 0 || p.sinks < 0 || p.recent > p.keep || p.sinks > p.keep - p.recent)
+    return bad("keep must be at least 1, and hold recent + sinks rows");
+  if (p.out_rows < p.keep) return bad("the new cache must have at least keep rows");
+  if (p.batch > kMost || p.kv_heads > kMost || p.rows > kMost || p.out_rows > kMost ||
+      p.batch * p.kv_heads > kMost / std::max<int64_t>(1, std::max(p.rows, p.out_rows)))
+    return report(WTC_ERR_UNSUPPORTED, "extent above 2^30");
+  if (p.batch * p.kv_heads >= kThreads / 1024 || p.batch * p.kv_heads * p.keep >= kThreads / 16) return too_many();
+  int rc;
+  if ((rc = check_strides(p.k_stride, 3, 0, "k"))) return rc;
+  if ((rc = check_strides(p.v_stride, 3, 0, "v"))) return rc;
+  if ((rc = check_strides(p.ko_stride, 3, 0, "k_out"))) return rc;
+  if ((rc = check_strides(p.vo_stride, 3, 0, "v_out"))) return rc;
+  if ((rc = check_distinct(p.ko_stride, p.batch, p.out_rows, p.kv_heads, p.dim, "k_out"))) return rc;
+  return check_distinct(p.vo_stride, p.batch, p.out_rows, p.kv_heads, p.dim, "v_out");
+}
+
 // The gradient addresses a tile's query rows (64 positions or one group of query
 // heads) with 32-bit offsets.
 int check_group_span(const wtc_attention_args& p, const int64_t* s, const char* what) {
@@ -210,16 +340,26 @@ int check_group_span(const wtc_attention_args& p, const int64_t* s, const char* 
     return report(WTC_ERR_UNSUPPORTED, std::string(what) + ": a tile of query rows spans more than 2 GiB");
   return WTC_OK;
 }
-int check_attention_backward(const wtc_attention_args& p) {
+int check_attention_backward(const wtc_attention_args& p, bool cross = false) {
   if (int rc = check_attention(p, false)) return rc;
+  if (cross)
+    if (int rc = check_cross(p)) return rc;
   if (int rc = check_strides(p.do_stride, 3, p.lq, "dout")) return rc;
   if (int rc = check_group_span(p, p.q_stride, "q")) return rc;
   if (int rc = check_group_span(p, p.do_stride, "dout")) return rc;
-  const AttnParams a = attention_params(p);
+  const AttnParams a = cross ? cross_params(p) : attention_params(p);
   const AttnBackwardPlan plan = plan_attention_backward(a, cu_count());
   const int64_t seqs = p.batch * p.kv_heads;
   const int64_t groups = seqs * ((int64_t)plan.key_blocks * plan.near_chunks + (int64_t)plan.far_blocks * plan.far_chunks);
   if (groups >= kThreads / 512 || (plan.far_blocks && seqs * a.sinks >= kThreads / 64)) return too_many();
+  return WTC_OK;
+}
+int check_key_weights(const wtc_attention_args& p) {
+  if (int rc = check_attention(p, false)) return rc;
+  if (int rc = check_group_span(p, p.q_stride, "q")) return rc;
+  if (std::min<int64_t>(p.heads / p.kv_heads, 64) * p.lq > kSpan / 8) return report(WTC_ERR_UNSUPPORTED, "lse: a key head's rows span more than 2 GiB");
+  const KeyWeightsPlan plan = plan_key_weights(attention_params(p), cu_count());
+  if (p.batch * p.kv_heads * plan.key_blocks >= kThreads / 256 / plan.chunks) return too_many();
   return WTC_OK;
 }
 
@@ -362,23 +502,28 @@ int wtc_matmul_epilogue_plan(const wtc_matmul_args* p, int part, int cus, int64_
   });
 }
 
-int64_t wtc_window_attention_workspace_size(const wtc_attention_args* p) {
+static int64_t attention_workspace_size(const wtc_attention_args* p, bool cross) {
   if (!p) return bad("NULL arguments"), -1;
   if (guarded([&] { return check_attention(*p, false); })) return -1;
-  const AttnParams a = attention_params(*p);
+  if (cross && check_cross(*p)) return -1;
+  const AttnParams a = cross ? cross_params(*p) : attention_params(*p);
   return align256(attention_workspace(a, plan_attention(a, cu_count())));
 }
+int64_t wtc_window_attention_workspace_size(const wtc_attention_args* p) { return attention_workspace_size(p, false); }
+int64_t wtc_cross_attention_workspace_size(const wtc_attention_args* p) { return attention_workspace_size(p, true); }
 
-int wtc_window_attention(const wtc_attention_args* p, const void* q, const void* k, const void* v, void* out,
-                         float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+static int attention(bool cross, const wtc_attention_args* p, const void* q, const void* k, const void* v, void* out,
+                     float* lse, void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&]() -> int {
     if (!p) return bad("NULL arguments");
     if (int rc = check_attention(*p, false)) return rc;
+    if (cross)
+      if (int rc = check_cross(*p)) return rc;
     if (int rc = check_distinct(p->o_stride, p->batch, p->lq, p->heads, p->dim, "out")) return rc;
     if (p->batch == 0 || p->lq == 0) return WTC_OK;
     if (!q || !out || (p->lk && (!k || !v))) return bad("NULL operand");
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return bad("pointers must be 16-byte aligned");
-    AttnParams a = attention_params(*p);
+    AttnParams a = cross ? cross_params(*p) : attention_params(*p);
     a.q = static_cast<const uint8_t*>(q);
     a.k = static_cast<const uint8_t*>(k);
     a.v = static_cast<const uint8_t*>(v);
@@ -387,29 +532,44 @@ int wtc_window_attention(const wtc_attention_args* p, const void* q, const void*
     const AttnPlan plan = plan_attention(a, cu_count());
     if (int rc = check_workspace(workspace, workspace_bytes, align256(attention_workspace(a, plan)))) return rc;
     a.part_out = static_cast<float*>(workspace);
-    return launched(launch_attention(a, plan, (int)p->dtype, static_cast<hipStream_t>(stream)), "window_attention");
+    return launched(launch_attention(a, plan, (int)p->dtype, static_cast<hipStream_t>(stream)),
+                    cross ? "cross_attention" : "window_attention");
   });
 }
-
-int64_t wtc_window_attention_backward_workspace_size(const wtc_attention_args* p) {
-  if (!p) return bad("NULL arguments"), -1;
-  if (guarded([&] { return check_attention_backward(*p); })) return -1;
-  return plan_attention_backward(attention_params(*p), cu_count()).workspace;
+int wtc_window_attention(const wtc_attention_args* p, const void* q, const void* k, const void* v, void* out,
+                         float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  return attention(false, p, q, k, v, out, lse, workspace, workspace_bytes, stream);
+}
+int wtc_cross_attention(const wtc_attention_args* p, const void* q, const void* k, const void* v, void* out,
+                        float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  return attention(true, p, q, k, v, out, lse, workspace, workspace_bytes, stream);
 }
 
-int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout, const void* q, const void* k,
-                                  const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
-                                  void* workspace, size_t workspace_bytes, void* stream) {
+static int64_t attention_backward_workspace_size(const wtc_attention_args* p, bool cross) {
+  if (!p) return bad("NULL arguments"), -1;
+  if (guarded([&] { return check_attention_backward(*p, cross); })) return -1;
+  return plan_attention_backward(cross ? cross_params(*p) : attention_params(*p), cu_count()).workspace;
+}
+int64_t wtc_window_attention_backward_workspace_size(const wtc_attention_args* p) {
+  return attention_backward_workspace_size(p, false);
+}
+int64_t wtc_cross_attention_backward_workspace_size(const wtc_attention_args* p) {
+  return attention_backward_workspace_size(p, true);
+}
+
+static int attention_backward(bool cross, const wtc_attention_args* p, const void* dout, const void* q, const void* k,
+                              const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                              void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&]() -> int {
     if (!p) return bad("NULL arguments");
-    if (int rc = check_attention_backward(*p)) return rc;
+    if (int rc = check_attention_backward(*p, cross)) return rc;
     if (p->batch == 0) return WTC_OK;
     if ((p->lq && (!dout || !q || !out || !lse || !dq)) || (p->lk && (!k || !v || !dk || !dv)))
       return bad("NULL operand");
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(dout) || !aligned16(dq) ||
         !aligned16(dk) || !aligned16(dv))
       return bad("pointers must be 16-byte aligned");
-    AttnParams a = attention_params(*p);
+    AttnParams a = cross ? cross_params(*p) : attention_params(*p);
     const AttnBackwardPlan plan = plan_attention_backward(a, cu_count());
     if (int rc = check_workspace(workspace, workspace_bytes, plan.workspace)) return rc;
     a.q = static_cast<const uint8_t*>(q);
@@ -423,8 +583,18 @@ int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout,
     a.dk = static_cast<uint8_t*>(dk);
     a.dv = static_cast<uint8_t*>(dv);
     return launched(launch_attention_backward(a, plan, (int)p->dtype, static_cast<hipStream_t>(stream)),
-                    "window_attention_backward");
+                    cross ? "cross_attention_backward" : "window_attention_backward");
   });
+}
+int wtc_window_attention_backward(const wtc_attention_args* p, const void* dout, const void* q, const void* k,
+                                  const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  return attention_backward(false, p, dout, q, k, v, out, lse, dq, dk, dv, workspace, workspace_bytes, stream);
+}
+int wtc_cross_attention_backward(const wtc_attention_args* p, const void* dout, const void* q, const void* k,
+                                 const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  return attention_backward(true, p, dout, q, k, v, out, lse, dq, dk, dv, workspace, workspace_bytes, stream);
 }
 
 int wtc_window_attention_plan(const wtc_attention_args* p, int cus, int64_t* plan) {
@@ -444,33 +614,46 @@ int wtc_window_attention_plan(const wtc_attention_args* p, int cus, int64_t* pla
   });
 }
 
-int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p) {
+static int64_t decode_workspace_size(const wtc_attention_args* p, bool weights) {
   if (!p) return bad("NULL arguments"), -1;
   if (guarded([&] { return check_attention(*p, true); })) return -1;
+  if (weights && check_decode_weights(*p)) return -1;
   const AttnParams a = decode_params(*p);
-  return align256(decode_workspace(a, plan_decode(a, cu_count())));
+  const int splits = plan_decode(a, cu_count());
+  return align256(weights ? decode_weights_workspace(a, splits) : decode_workspace(a, splits));
+}
+int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p) { return decode_workspace_size(p, false); }
+int64_t wtc_window_attention_decode_weights_workspace_size(const wtc_attention_args* p) {
+  return decode_workspace_size(p, true);
 }
 
-int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void* k, void* v, const void* k_new,
-                                const void* v_new, void* out, void* workspace, size_t workspace_bytes,
-                                void* stream) {
+// What every call that may append a token to its caches asks of them.
+static int check_append(const wtc_attention_args* p, const void* k, const void* v, const void* k_new, const void* v_new) {
+  if (!k_new != !v_new) return bad("k_new and v_new go together");
+  if (!k_new) return WTC_OK;
+  if (k && k == v) return bad("k and v are the same cache: it cannot take both k_new and v_new");
+  if (int rc = check_distinct(p->k_stride, p->batch, p->lk, p->kv_heads, p->dim, "k")) return rc;
+  return check_distinct(p->v_stride, p->batch, p->lk, p->kv_heads, p->dim, "v");
+}
+
+// `weights`: set where has_weights
+static int decode(bool has_weights, const wtc_attention_args* p, const void* q, void* k, void* v, const void* k_new,
+                  const void* v_new, void* out, float* weights, void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&]() -> int {
     if (!p) return bad("NULL arguments");
     if (int rc = check_attention(*p, true)) return rc;
     if (int rc = check_distinct(p->o_stride, p->batch, 1, p->heads, p->dim, "out")) return rc;
-    if (!k_new != !v_new) return bad("k_new and v_new go together");
-    if (k_new) {
-      if (k && k == v) return bad("k and v are the same cache: it cannot take both k_new and v_new");
-      if (int rc = check_distinct(p->k_stride, p->batch, p->lk, p->kv_heads, p->dim, "k")) return rc;
-      if (int rc = check_distinct(p->v_stride, p->batch, p->lk, p->kv_heads, p->dim, "v")) return rc;
-    }
+    if (has_weights)
+      if (int rc = check_decode_weights(*p)) return rc;
+    if (int rc = check_append(p, k, v, k_new, v_new)) return rc;
     if (p->batch == 0) return WTC_OK;
-    if (!q || !k || !v || !out) return bad("NULL operand");
+    if (!q || !k || !v || !out || (has_weights && !weights)) return bad("NULL operand");
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(k_new) || !aligned16(v_new))
       return bad("pointers must be 16-byte aligned");
     AttnParams a = decode_params(*p);
     const int splits = plan_decode(a, cu_count());
-    if (int rc = check_workspace(workspace, workspace_bytes, align256(decode_workspace(a, splits)))) return rc;
+    const int64_t need = align256(has_weights ? decode_weights_workspace(a, splits) : decode_workspace(a, splits));
+    if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
     a.part_out = static_cast<float*>(workspace);
     a.q = static_cast<const uint8_t*>(q);
     a.k = static_cast<const uint8_t*>(k);
@@ -478,8 +661,137 @@ int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void
     a.k_new = static_cast<const uint8_t*>(k_new);
     a.v_new = static_cast<const uint8_t*>(v_new);
     a.out = static_cast<uint8_t*>(out);
-    return launched(launch_attention_decode(a, splits, (int)p->dtype, static_cast<hipStream_t>(stream)),
+    a.weights = weights;
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    return launched(has_weights ? launch_attention_decode_weights(a, splits, (int)p->dtype, on)
+                                : launch_attention_decode(a, splits, (int)p->dtype, on),
                     "window_attention_decode");
+  });
+}
+int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void* k, void* v, const void* k_new,
+                                const void* v_new, void* out, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  return decode(false, p, q, k, v, k_new, v_new, out, nullptr, workspace, workspace_bytes, stream);
+}
+int wtc_window_attention_decode_weights(const wtc_attention_args* p, const void* q, void* k, void* v,
+                                        const void* k_new, const void* v_new, void* out, float* weights,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+  return decode(true, p, q, k, v, k_new, v_new, out, weights, workspace, workspace_bytes, stream);
+}
+
+static int64_t prefix_workspace_size(const wtc_attention_args* p, const wtc_prefix_args* x, bool decode) {
+  if (!p || !x) return bad("NULL arguments"), -1;
+  if (guarded([&] { return check_prefix(*p, *x, decode); })) return -1;
+  return plan_prefix(*p, *x, decode, cu_count()).bytes;
+}
+int64_t wtc_prefix_attention_workspace_size(const wtc_attention_args* p, const wtc_prefix_args* x) {
+  return prefix_workspace_size(p, x, false);
+}
+int64_t wtc_prefix_attention_decode_workspace_size(const wtc_attention_args* p, const wtc_prefix_args* x) {
+  return prefix_workspace_size(p, x, true);
+}
+
+int wtc_prefix_attention(const wtc_attention_args* p, const wtc_prefix_args* x, const void* q, const void* k_prefix,
+                         const void* v_prefix, const void* k, const void* v, void* out, float* lse, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int {
+    if (!p || !x) return bad("NULL arguments");
+    if (int rc = check_prefix(*p, *x, false)) return rc;
+    if (int rc = check_distinct(p->o_stride, p->batch, p->lq, p->heads, p->dim, "out")) return rc;
+    if (p->batch == 0 || p->lq == 0) return WTC_OK;
+    if (!q || !out || (p->lk && (!k || !v)) || (x->prefix && (!k_prefix || !v_prefix))) return bad("NULL operand");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(out))
+      return bad("pointers must be 16-byte aligned");
+    PrefixPlan plan = plan_prefix(*p, *x, false, cu_count());
+    if (int rc = check_workspace(workspace, workspace_bytes, plan.bytes)) return rc;
+    return launch_prefix(plan, false, (int)p->dtype, q, k_prefix, v_prefix, k, v, nullptr, nullptr, out, lse, workspace,
+                         static_cast<hipStream_t>(stream));
+  });
+}
+
+int wtc_prefix_attention_decode(const wtc_attention_args* p, const wtc_prefix_args* x, const void* q,
+                                const void* k_prefix, const void* v_prefix, void* k, void* v, const void* k_new,
+                                const void* v_new, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int {
+    if (!p || !x) return bad("NULL arguments");
+    if (int rc = check_prefix(*p, *x, true)) return rc;
+    if (int rc = check_distinct(p->o_stride, p->batch, 1, p->heads, p->dim, "out")) return rc;
+    if (int rc = check_append(p, k, v, k_new, v_new)) return rc;
+    if (p->batch == 0) return WTC_OK;
+    if (!q || !k || !v || !out || (x->prefix && (!k_prefix || !v_prefix))) return bad("NULL operand");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(k_prefix) || !aligned16(v_prefix) ||
+        !aligned16(out) || !aligned16(k_new) || !aligned16(v_new))
+      return bad("pointers must be 16-byte aligned");
+    PrefixPlan plan = plan_prefix(*p, *x, true, cu_count());
+    if (int rc = check_workspace(workspace, workspace_bytes, plan.bytes)) return rc;
+    return launch_prefix(plan, true, (int)p->dtype, q, k_prefix, v_prefix, k, v, k_new, v_new, out, nullptr, workspace,
+                         static_cast<hipStream_t>(stream));
+  });
+}
+
+int64_t wtc_window_attention_weights_workspace_size(const wtc_attention_args* p) {
+  if (!p) return bad("NULL arguments"), -1;
+  if (guarded([&] { return check_key_weights(*p); })) return -1;
+  return align256(plan_key_weights(attention_params(*p), cu_count()).workspace);
+}
+
+int wtc_window_attention_weights(const wtc_attention_args* p, const void* q, const void* k, const float* lse,
+                                 float* weights, int add, void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int {
+    if (!p) return bad("NULL arguments");
+    if (int rc = check_key_weights(*p)) return rc;
+    if (p->batch == 0 || p->lk == 0) return WTC_OK;
+    if (!weights || !k || (p->lq && (!q || !lse))) return bad("NULL operand");
+    if (!aligned16(q) || !aligned16(k)) return bad("pointers must be 16-byte aligned");
+    AttnParams a = attention_params(*p);
+    const KeyWeightsPlan plan = plan_key_weights(a, cu_count());
+    if (int rc = check_workspace(workspace, workspace_bytes, align256(plan.workspace))) return rc;
+    a.q = static_cast<const uint8_t*>(q);
+    a.k = static_cast<const uint8_t*>(k);
+    a.lse_in = lse;
+    a.weights = weights;
+    a.add = add != 0;
+    a.part_out = static_cast<float*>(workspace);
+    return launched(launch_key_weights(a, plan, (int)p->dtype, static_cast<hipStream_t>(stream)),
+                    "window_attention_weights");
+  });
+}
+
+int wtc_cache_evict(const wtc_evict_args* p, const void* k, const void* v, const float* weights,
+                    const int32_t* lengths, void* k_out, void* v_out, float* weights_out, int32_t* rows,
+                    int32_t* lengths_out, void* stream) {
+  return guarded([&]() -> int {
+    if (!p) return bad("NULL arguments");
+    if (int rc = check_evict(*p)) return rc;
+    if (p->batch == 0) return WTC_OK;
+    if ((p->rows && (!k || !v || !weights)) || !lengths || !k_out || !v_out || !weights_out || !rows || !lengths_out)
+      return bad("NULL operand");
+    if (!aligned16(k) || !aligned16(v) || !aligned16(k_out) || !aligned16(v_out)) return bad("pointers must be 16-byte aligned");
+    EvictParams q{};
+    q.k = static_cast<const uint8_t*>(k);
+    q.v = static_cast<const uint8_t*>(v);
+    q.k_out = static_cast<uint8_t*>(k_out);
+    q.v_out = static_cast<uint8_t*>(v_out);
+    q.weights = weights;
+    q.weights_out = weights_out;
+    q.lengths = lengths;
+    q.kept = rows;
+    q.lengths_out = lengths_out;
+    for (int i = 0; i < 3; ++i) {
+      q.k_stride[i] = 2 * p->k_stride[i];
+      q.v_stride[i] = 2 * p->v_stride[i];
+      q.ko_stride[i] = 2 * p->ko_stride[i];
+      q.vo_stride[i] = 2 * p->vo_stride[i];
+    }
+    q.batch = (int)p->batch;
+    q.kv_heads = (int)p->kv_heads;
+    q.rows = (int)p->rows;
+    q.out_rows = (int)p->out_rows;
+    q.keep = (int)p->keep;
+    q.recent = (int)p->recent;
+    q.sinks = (int)p->sinks;
+    q.row_bytes = (int)p->dim * 2;
+    return launched(launch_cache_evict(q, static_cast<hipStream_t>(stream)), "cache_evict");
   });
 }
 

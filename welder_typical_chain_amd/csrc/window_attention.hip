@@ -43,26 +43,36 @@ template <int DT> struct Redo {
   }
 };
 
+// The last key that query i of sequence b sees.
+__device__ inline int last_seen(const AttnParams& p, int b, int i) {
+  const int nq = seq_queries(p, b), nk = seq_keys(p, b);
+  return min(i + first_position(p, nq, nk), nk - 1);
+}
+
 template <int DT> __device__ inline void attention_row(const AttnParams& p, int b, int h, int i) {
   using T = typename Elem<DT>::type;
   const int lane = threadIdx.x & 63;
-  const int pos = i + seq_keys(p, b) - seq_queries(p, b);
   const T* q = (const T*)p.q + b * p.q_stride[0] + i * p.q_stride[1] + h * p.q_stride[2];
   const T* k = (const T*)p.k + b * p.k_stride[0] + h / p.group * p.k_stride[2];
   const T* v = (const T*)p.v + b * p.v_stride[0] + h / p.group * p.v_stride[2];
-  const Seen seen(p.window, p.sinks, pos);
+  const T* kp = (const T*)p.kp + h / p.group * p.kp_stride[1];
+  const T* vp = (const T*)p.vp + h / p.group * p.vp_stride[1];
+  const Seen seen(p.window, p.sinks, last_seen(p, b, i));
+  const int count = p.prefix + seen.count;
+  auto key = [&](int t) { return t < p.prefix ? kp + t * p.kp_stride[0] : k + seen.key(t - p.prefix) * p.k_stride[1]; };
+  auto value = [&](int t) { return t < p.prefix ? vp + t * p.vp_stride[0] : v + seen.key(t - p.prefix) * p.v_stride[1]; };
   Redo<DT> out(p.out, b * p.o_stride[0] + i * p.o_stride[1] + h * p.o_stride[2], p.dim, lane);
   float top = -INFINITY, total = 0.0f;
-  for (int t0 = 0; t0 < seen.count && !out.settled(); t0 += 64) {
-    const bool in = t0 + lane < seen.count;
-    const float s = in ? p.scale * dot_rows<DT>(q, k + seen.key(t0 + lane) * p.k_stride[1], p.dim) : -INFINITY;
+  for (int t0 = 0; t0 < count && !out.settled(); t0 += 64) {
+    const bool in = t0 + lane < count;
+    const float s = in ? p.scale * dot_rows<DT>(q, key(t0 + lane), p.dim) : -INFINITY;
     const float next = fmaxf(top, wave_max(s));
     const float keep = next == -INFINITY ? 1.0f : __expf(top - next);
     const float e = in ? (next == -INFINITY ? (s != s ? s : 0.0f) : __expf(s - next)) : 0.0f;
     total = total * keep + wave_sum(e);
     for (int c = 0; c < kCols; ++c) out.acc[c] *= keep;
     top = next;
-    for (int t = 0; t < min(64, seen.count - t0); ++t) out.add(__shfl(e, t), v + seen.key(t0 + t) * p.v_stride[1], lane);
+    for (int t = 0; t < min(64, count - t0); ++t) out.add(__shfl(e, t), value(t0 + t), lane);
   }
   out.store(total == 0.0f ? 0.0f : 1.0f / total, lane);
 }
@@ -116,7 +126,7 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
   const uint32_t rest = id / p.splits;
   const int blk = p.row_blocks - 1 - (int)(rest % p.row_blocks);  // the longest rows first
   const int hk = (int)(rest / p.row_blocks % p.kv_heads), b = (int)(rest / p.row_blocks / p.kv_heads);
-  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
+  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = first_position(p, nq, nk);
   const int r0 = blk * ROWS;
 
   // this lane's row
@@ -128,7 +138,7 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
   const int i_last = min((r0 + ROWS - 1) / p.group, nq - 1);
   const int p_lo = r0 / p.group + shift, p_hi = i_last + shift;
   const int lo = (int)max((int64_t)0, (int64_t)p_lo - p.window + 1);
-  const int end = r0 / p.group < nq ? max(p_hi + 1, 0) : 0;
+  const int end = r0 / p.group < nq ? min(max(p_hi + 1, 0), nk) : 0;
   const int s_end = end ? min(p.sinks, lo) : 0;
   const int t_sink = (s_end + kKeys - 1) / kKeys, t_all = end > lo ? t_sink + (end - lo + kKeys - 1) / kKeys : 0;
   const int t0 = (int)((int64_t)t_all * split / p.splits), t1 = (int)((int64_t)t_all * (split + 1) / p.splits);
@@ -138,7 +148,8 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
   const bool w_any = (r0 + wave * 32) / p.group < nq && w_hi >= 0;
 
   u32x4 qf[NS];
-  load_row<NS>(p.q + 2 * (b * p.q_stride[0] + (int64_t)i * p.q_stride[1] + h * p.q_stride[2]), valid, p.dim, half, qf);
+  const int q_seq = p.seq_rows ? i / p.seq_rows : b, q_row = p.seq_rows ? i % p.seq_rows : i;
+  load_row<NS>(p.q + 2 * (q_seq * p.q_stride[0] + (int64_t)q_row * p.q_stride[1] + h * p.q_stride[2]), valid, p.dim, half, qf);
   const float c2 = positive_scale<NS>(p.scale, qf);
 
   f32x16 o[ND];
@@ -298,8 +309,8 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   const float lse = (top + __builtin_amdgcn_logf(total)) * kLn2;  // (v_log_f32: log2)
-  if (p.splits > 1) {
-    const int64_t row = (((int64_t)b * p.lq + i) * p.heads + h) * p.splits + split;
+  if (p.slots) {
+    const int64_t row = (((int64_t)b * p.lq + i) * p.heads + h) * p.slots + p.slot0 + split;
     if (valid) {
       if (half == 0) p.part_lse[row] = total == 0.0f ? -INFINITY : top + __builtin_amdgcn_logf(total);
 #pragma unroll
@@ -363,7 +374,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
   if (c < p.dim) {
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     float lse = -INFINITY;
-    if (valid) lse = join_splits(p.part_out + row * p.splits * p.dim, p.part_lse + row * p.splits, p.splits, p.dim, c, &x);
+    if (valid) lse = join_splits(p.part_out + row * p.slots * p.dim, p.part_lse + row * p.slots, p.slots, p.dim, c, &x);
 #pragma unroll
     for (int v = 0; v < 4; ++v) nan |= x[v] != x[v];
     if (at < rows) {
@@ -457,7 +468,6 @@ template <int DT> struct DsRange {
 template <int DT> __device__ inline void dq_row(const AttnParams& p, int b, int h, int i) {
   using T = typename Elem<DT>::type;
   const int lane = threadIdx.x & 63;
-  const int pos = i + seq_keys(p, b) - seq_queries(p, b);
   const T* q = (const T*)p.q + b * p.q_stride[0] + i * p.q_stride[1] + h * p.q_stride[2];
   const T* k = (const T*)p.k + b * p.k_stride[0] + h / p.group * p.k_stride[2];
   const T* v = (const T*)p.v + b * p.v_stride[0] + h / p.group * p.v_stride[2];
@@ -465,7 +475,7 @@ template <int DT> __device__ inline void dq_row(const AttnParams& p, int b, int 
   const T* o = (const T*)p.o + b * p.o_stride[0] + i * p.o_stride[1] + h * p.o_stride[2];
   const float delta = dot_rows<DT>(g, o, p.dim);
   const float lse = p.lse_in[((int64_t)b * p.heads + h) * p.lq + i];
-  const Seen seen(p.window, p.sinks, pos);
+  const Seen seen(p.window, p.sinks, last_seen(p, b, i));
   Redo<DT> dq(p.dq, (((int64_t)b * p.lq + i) * p.heads + h) * p.dim, p.dim, lane);
   for (int t0 = 0; t0 < seen.count && !dq.settled(); t0 += 64) {
     float ds = 0.0f;
@@ -483,7 +493,7 @@ template <int DT> __device__ inline void dq_row(const AttnParams& p, int b, int 
 template <int DT> __device__ inline void dkv_row(const AttnParams& p, int b, int hk, int j) {
   using T = typename Elem<DT>::type;
   const int lane = threadIdx.x & 63;
-  const int nq = seq_queries(p, b), shift = seq_keys(p, b) - nq;
+  const int nq = seq_queries(p, b), shift = first_position(p, nq, seq_keys(p, b));
   const T* k = (const T*)p.k + b * p.k_stride[0] + j * p.k_stride[1] + hk * p.k_stride[2];
   const T* v = (const T*)p.v + b * p.v_stride[0] + j * p.v_stride[1] + hk * p.v_stride[2];
   // queries of positions j .. j + window - 1 (a first token: all from j on)
@@ -540,7 +550,7 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
   const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
   const int blk = p.row_blocks - 1 - (int)(id % p.row_blocks);
   const int hk = (int)(id / p.row_blocks % p.kv_heads), b = (int)(id / p.row_blocks / p.kv_heads);
-  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
+  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = first_position(p, nq, nk);
   const int r0 = blk * NW * 32;
   const int r = r0 + wave * 32 + (lane & 31), i = r / p.group, x_head = r - i * p.group, h = hk * p.group + x_head;
   const bool valid = i < nq;
@@ -548,7 +558,7 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
   const int i_last = min((r0 + NW * 32 - 1) / p.group, nq - 1);
   const int p_lo = r0 / p.group + shift, p_hi = i_last + shift;
   const int lo = (int)max((int64_t)0, (int64_t)p_lo - p.window + 1);
-  const int end = r0 / p.group < nq ? max(p_hi + 1, 0) : 0;
+  const int end = r0 / p.group < nq ? min(max(p_hi + 1, 0), nk) : 0;
   const int s_end = end ? min(p.sinks, lo) : 0;
   const int t_sink = (s_end + kKeys - 1) / kKeys, t_all = end > lo ? t_sink + (end - lo + kKeys - 1) / kKeys : 0;
   const int w_lo = (r0 + wave * 32) / p.group + shift;
@@ -835,7 +845,7 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
   const bool far = w >= near;
   const int parts_of = far ? p.far_chunks : p.near_chunks;
   const int kb = (far ? w - near : w) / parts_of, chunk = (far ? w - near : w) % parts_of;
-  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
+  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = first_position(p, nq, nk);
   const int sub = wave >> 2;  // rows of a tile
   const int j_first = kb * kDkvKeys, j_wave = j_first + (wave & 3) * 32, j = j_wave + (lane & 31);
   const bool valid = j < nk;
@@ -1170,14 +1180,22 @@ int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan) {
 hipError_t launch_attention(const AttnParams& params, const AttnPlan& plan, int dt, hipStream_t stream) {
   AttnParams p = params;
   const int64_t rows = (int64_t)p.lq * p.group;
+  const bool joined = p.slots;  // by the caller, with the results of other launches
   p.splits = plan.splits;
+  if (!joined) {
+    p.slots = plan.splits > 1 ? plan.splits : 0;
+    p.part_lse = p.part_out + (int64_t)p.batch * p.lq * p.heads * p.splits * p.dim;
+  }
   p.row_blocks = (int)((rows * plan.key_groups + 255) / 256);
-  p.part_lse = p.part_out + (int64_t)p.batch * p.lq * p.heads * p.splits * p.dim;
   const int nd = (p.dim + 31) / 32;
   const void* fn = plan.key_groups == 2 ? (dt == DT_F16 ? tile_kernel<DT_F16, 2>(nd) : tile_kernel<DT_BF16, 2>(nd))
                                         : (dt == DT_F16 ? tile_kernel<DT_F16, 1>(nd) : tile_kernel<DT_BF16, 1>(nd));
   const hipError_t e = launch(fn, (int64_t)p.batch * p.kv_heads * p.row_blocks * p.splits, 512, p, stream);
-  if (e != hipSuccess || p.splits == 1) return e;
+  if (e != hipSuccess || p.splits == 1 || joined) return e;
+  return launch_attention_join(p, dt, stream);
+}
+
+hipError_t launch_attention_join(const AttnParams& p, int dt, hipStream_t stream) {
   return launch(WTC_BY_TYPE(attention_join_kernel, dt), ((int64_t)p.batch * p.lq * p.heads + 7) / 8, 256, p, stream);
 }
 

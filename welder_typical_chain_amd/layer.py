@@ -1,6 +1,8 @@
 """PyTorch-facing entry points of the operators around the fused chain that a
-transformer layer needs: matrix products with an epilogue, and attention with
-a sliding window whose first tokens stay visible.
+transformer layer needs: matrix products with an epilogue, attention with a
+sliding window whose first tokens stay visible, attention to another sequence
+and behind a prefix that a batch shares, and a cache cut to the rows that
+attention has weighed most.
 
 As in ``chain.py``, PyTorch supplies device memory and the current HIP stream
 and every byte is computed by the HIP kernels behind ``include/wtc/wtc_layer.h``.
@@ -29,6 +31,8 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 # The C structs are eight-byte fields throughout, packed here into bytes.
 _pack_matmul = struct.Struct("13q").pack
 _pack_attention = struct.Struct("28q2qd").pack
+_pack_prefix = struct.Struct("5q").pack
+_pack_evict = struct.Struct("21q").pack
 _SIZES_END = 28 * 8  # where sizes and strides end: addresses and the scale follow
 
 
@@ -77,13 +81,13 @@ def _launch(device, fn, *args):
 _sizes: dict = {}  # (function, arguments without addresses) -> bytes
 
 
-def _scratch(name, args, device, keyed=None):
+def _scratch(name, args, device, keyed=None, *more):
     """(tensor, pointer, bytes) of a call's workspace; none for size 0."""
-    key = (name, device, args if keyed is None else args[:keyed])
+    key = (name, device, args if keyed is None else args[:keyed], *more)
     size = _sizes.get(key)
     if size is None:
         with torch.cuda.device(device):  # the plan goes by its compute units
-            size = getattr(_lib.lib(), name)(args)
+            size = getattr(_lib.lib(), name)(args, *more)
         if size < 0:
             _lib.check(_lib.WTC_ERR_ARG)
         if len(_sizes) >= 4096:
@@ -95,8 +99,8 @@ def _scratch(name, args, device, keyed=None):
     return t, t.data_ptr(), size
 
 
-def _check_out(out, *named):
-    """Refuses an `out` that starts where an input does, or lies over one: of tensors
+def _check_out(out, *named, what="out"):
+    """Refuses an `out` (called `what`) that starts where an input does, or lies over one: of tensors
     without gaps that is known, of others only the start (columns side by side in one
     buffer share no element, but their ranges meet)."""
     size = out.numel() * out.element_size()
@@ -110,7 +114,7 @@ def _check_out(out, *named):
         first = t.data_ptr()
         if first == at or (end > at and t.is_contiguous() and first < end and
                            at < first + t.numel() * t.element_size()):
-            raise ValueError(f"out may not be or lie over {name}")
+            raise ValueError(f"{what} may not be or lie over {name}")
 
 
 def _ptr(t):
@@ -365,6 +369,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     type before the product with v.  With return_lse=True the result is
     (out, lse), lse the rows' log-sum-exp, float32 [B, H, Lq].
     """
+    return _attention("wtc_window_attention", q, k, v, window, sinks, scale, q_lens, k_lens, out, return_lse)
+
+
+def _attention(name, q, k, v, window, sinks, scale, q_lens, k_lens, out, return_lse):
     device = _check_inputs(q.dtype, ("q", q), ("k", k), ("v", v), ("out", out))
     head, tail = _attention_args(q, k, v, window, sinks, scale, q_lens, k_lens, device)
     if out is None:
@@ -376,9 +384,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     b, lq, h, _ = q.shape
     lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if return_lse else None
     args = _pack_attention(*head, *_strides(out, "out"), 0, 0, 0, 0, 0, 0, 0, *tail)
-    lib = _lib.lib()
-    ws, ws_ptr, ws_bytes = _scratch("wtc_window_attention_workspace_size", args, device, _SIZES_END)
-    _launch(device, lib.wtc_window_attention, args, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+    ws, ws_ptr, ws_bytes = _scratch(name + "_workspace_size", args, device, _SIZES_END)
+    _launch(device, getattr(_lib.lib(), name), args, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
             _ptr(lse), ws_ptr, ws_bytes)
     return (out, lse) if return_lse else out
 
@@ -395,22 +402,30 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     gradient may have any size that its results have).  Two calls give the same
     bits.
     """
+    return _attention_backward("wtc_window_attention_backward", dout, q, k, v, out, lse, window, sinks, scale,
+                               q_lens, k_lens)
+
+
+def _check_lse(lse, b, h, lq, device):
+    if lse.shape != (b, h, lq) or lse.dtype != torch.float32 or not lse.is_contiguous() or \
+            not lse.is_cuda or lse.get_device() != device:
+        raise ValueError("lse must be the forward call's: float32, contiguous, [B, H, Lq]")
+    _check_inputs(None, ("lse", lse))
+
+
+def _attention_backward(name, dout, q, k, v, out, lse, window, sinks, scale, q_lens, k_lens):
     device = _check_inputs(q.dtype, ("dout", dout), ("q", q), ("k", k), ("v", v), ("out", out))
     head, tail = _attention_args(q, k, v, window, sinks, scale, q_lens, k_lens, device)
     b, lq, h, _ = q.shape
     if dout.shape != q.shape or out.shape != q.shape:
         raise ValueError("dout and out must have q's shape")
-    if lse.shape != (b, h, lq) or lse.dtype != torch.float32 or not lse.is_contiguous() or \
-            not lse.is_cuda or lse.get_device() != device:
-        raise ValueError("lse must be window_attention's: float32, contiguous, [B, H, Lq]")
-    _check_inputs(None, ("lse", lse))
+    _check_lse(lse, b, h, lq, device)
     if dout.stride(3) != 1 or 0 in dout.stride():  # a gradient that autograd broadcast
         dout = dout.contiguous()
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    lib = _lib.lib()
     args = _pack_attention(*head, *_strides(out, "out"), *_strides(dout, "dout"), 0, 0, 0, 0, *tail)
-    ws, ws_ptr, ws_bytes = _scratch("wtc_window_attention_backward_workspace_size", args, device, _SIZES_END)
-    _launch(device, lib.wtc_window_attention_backward, args, dout.data_ptr(), q.data_ptr(), k.data_ptr(),
+    ws, ws_ptr, ws_bytes = _scratch(name + "_workspace_size", args, device, _SIZES_END)
+    _launch(device, getattr(_lib.lib(), name), args, dout.data_ptr(), q.data_ptr(), k.data_ptr(),
             v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws_ptr,
             ws_bytes)
     return dq, dk, dv
@@ -419,7 +434,8 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
 def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                             lengths: torch.Tensor, *, k_new: torch.Tensor | None = None,
                             v_new: torch.Tensor | None = None, window: int | None = None, sinks: int = 0,
-                            scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                            scale: float | None = None, out: torch.Tensor | None = None,
+                            weights: torch.Tensor | None = None) -> torch.Tensor:
     """window_attention for one token of each sequence, against a cache of fixed size.
 
     q: [B, H, D]; k_cache, v_cache: [B, C, Hkv, D], C > sinks.  Token j of a
@@ -430,12 +446,26 @@ def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     number; 0 is an idle sequence (its out is 0, its cache is left alone).
     k_new, v_new: [B, Hkv, D], the new token's key and value, written to the
     caches in the same pass; without them the caches hold it already.
+    weights: float32 [B, Hkv, C], contiguous: every visible row's softmax weight,
+    summed over the query heads of its key head, is added to it; the newest
+    token's row is set to it (what that row held was another token's).
     """
+    return _decode(q, k_cache, v_cache, lengths, k_new, v_new, window, sinks, scale, out, weights, None)
+
+
+def _key_weights(weights, b, kv, n, device):
+    if weights.shape != (b, kv, n) or weights.dtype != torch.float32 or not weights.is_contiguous() or \
+            weights.get_device() != device:
+        raise ValueError(f"weights must be float32, contiguous, {(b, kv, n)}, on the tensors' device")
+    _check_inputs(None, ("weights", weights))
+
+
+def _decode(q, k_cache, v_cache, lengths, k_new, v_new, window, sinks, scale, out, weights, prefix):
     shape, cache = q.shape, k_cache.shape
     if len(shape) != 3 or len(cache) != 4 or v_cache.shape != cache:
         raise ValueError("q must be [B, H, D], the caches [B, C, Hkv, D]")
     device = _check_inputs(q.dtype, ("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("k_new", k_new),
-                           ("v_new", v_new), ("out", out))
+                           ("v_new", v_new), ("out", out), *(prefix or ()))
     if lengths is None:
         raise ValueError("lengths must be given")
     b, h, d = shape
@@ -448,7 +478,8 @@ def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     elif out.shape != shape:
         raise ValueError("out must have q's shape")
     else:
-        _check_out(out, ("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("k_new", k_new), ("v_new", v_new))
+        _check_out(out, ("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("k_new", k_new), ("v_new", v_new),
+                   ("weights", weights), *(prefix or ()))
     kn = vn = (0, 0, 0)
     if k_new is not None and v_new is not None:
         if k_new.shape != (b, kv, d) or v_new.shape != (b, kv, d):
@@ -460,7 +491,179 @@ def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                            *_strides(k_cache, "k_cache"), *_strides(v_cache, "v_cache"), *_row_strides(out, "out"),
                            0, 0, 0, kn[0], kn[2], vn[0], vn[2], 0, _lens(lengths, b, "lengths", device),
                            d ** -0.5 if scale is None else float(scale))
-    ws, ws_ptr, ws_bytes = _scratch("wtc_window_attention_decode_workspace_size", args, device, _SIZES_END)
-    _launch(device, _lib.lib().wtc_window_attention_decode, args, q.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), _ptr(k_new), _ptr(v_new), out.data_ptr(), ws_ptr, ws_bytes)
+    tensors = k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_new), _ptr(v_new), out.data_ptr()
+    if prefix is not None:
+        (_, kp), (_, vp) = prefix
+        common = _prefix_args(kp, vp, kv, d)
+        ws, ws_ptr, ws_bytes = _scratch("wtc_prefix_attention_decode_workspace_size", args, device, _SIZES_END, common)
+        _launch(device, _lib.lib().wtc_prefix_attention_decode, args, common, q.data_ptr(), kp.data_ptr(),
+                vp.data_ptr(), *tensors, ws_ptr, ws_bytes)
+    elif weights is not None:
+        _key_weights(weights, b, kv, cap, device)
+        _check_out(weights, ("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("k_new", k_new), ("v_new", v_new),
+                   what="weights")
+        ws, ws_ptr, ws_bytes = _scratch("wtc_window_attention_decode_weights_workspace_size", args, device, _SIZES_END)
+        _launch(device, _lib.lib().wtc_window_attention_decode_weights, args, q.data_ptr(), *tensors,
+                weights.data_ptr(), ws_ptr, ws_bytes)
+    else:
+        ws, ws_ptr, ws_bytes = _scratch("wtc_window_attention_decode_workspace_size", args, device, _SIZES_END)
+        _launch(device, _lib.lib().wtc_window_attention_decode, args, q.data_ptr(), *tensors, ws_ptr, ws_bytes)
     return out
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None,
+                    q_lens: torch.Tensor | None = None, k_lens: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None, return_lse: bool = False):
+    """Softmax attention to another sequence, softmax_row(scale * q . k) . v: every query
+    of a sequence sees every key of it.
+
+    q: [B, Lq, H, D]; k, v: [B, Lk, Hkv, D]; types, strides, heads, dimensions,
+    lengths, scale and results are window_attention's.  Lq and Lk have nothing
+    to do with each other (Lq + Lk up to 2^30); one token a sequence is Lq = 1.
+    A query of a sequence without keys, and one behind its sequence's end, gives zeros.
+    """
+    return _attention("wtc_cross_attention", q, k, v, None, 0, scale, q_lens, k_lens, out, return_lse)
+
+
+def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                             out: torch.Tensor, lse: torch.Tensor, *, scale: float | None = None,
+                             q_lens: torch.Tensor | None = None, k_lens: torch.Tensor | None = None):
+    """(dq, dk, dv) of cross_attention called with the same arguments, which gave `out`
+    and `lse`; otherwise as window_attention_backward."""
+    return _attention_backward("wtc_cross_attention_backward", dout, q, k, v, out, lse, None, 0, scale, q_lens, k_lens)
+
+
+def _prefix_args(kp, vp, kv, d):
+    if kp.dim() != 3 or kp.shape[1:] != (kv, d) or vp.shape != kp.shape:
+        raise ValueError(f"k_prefix and v_prefix must be [P, {kv}, {d}]")
+    (k0, _, k1), (v0, _, v1) = _row_strides(kp, "k_prefix"), _row_strides(vp, "v_prefix")
+    return _pack_prefix(kp.shape[0], k0, k1, v0, v1)
+
+
+def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor,
+                     v: torch.Tensor, *, scale: float | None = None, q_lens: torch.Tensor | None = None,
+                     k_lens: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                     return_lse: bool = False):
+    """Causal attention of a batch whose sequences go on from one prefix: each query sees
+    the whole prefix and, as in window_attention, its own sequence up to itself.
+
+    k_prefix, v_prefix: [P, Hkv, D], one for the batch; q: [B, Lq, H, D]; k, v:
+    [B, Lk, Hkv, D], each sequence's own tokens, whose last ones the queries are.
+    P and Lk may be 0.  Everything else is window_attention's.  The prefix is
+    read for the queries of all sequences together.
+    """
+    common = ("k_prefix", k_prefix), ("v_prefix", v_prefix)
+    device = _check_inputs(q.dtype, ("q", q), ("k", k), ("v", v), ("out", out), *common)
+    head, tail = _attention_args(q, k, v, None, 0, scale, q_lens, k_lens, device)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    else:
+        _check_out(out, ("q", q), ("k", k), ("v", v), *common)
+    b, lq, h, d = q.shape
+    lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if return_lse else None
+    args = _pack_attention(*head, *_strides(out, "out"), 0, 0, 0, 0, 0, 0, 0, *tail)
+    shared = _prefix_args(k_prefix, v_prefix, k.shape[2], d)
+    ws, ws_ptr, ws_bytes = _scratch("wtc_prefix_attention_workspace_size", args, device, _SIZES_END, shared)
+    _launch(device, _lib.lib().wtc_prefix_attention, args, shared, q.data_ptr(), k_prefix.data_ptr(),
+            v_prefix.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), ws_ptr, ws_bytes)
+    return (out, lse) if return_lse else out
+
+
+def prefix_attention_decode(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
+                            k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, *,
+                            k_new: torch.Tensor | None = None, v_new: torch.Tensor | None = None,
+                            scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """prefix_attention for one token of each sequence, against caches of the own tokens.
+
+    q: [B, H, D]; k_prefix, v_prefix: [P, Hkv, D]; k_cache, v_cache: [B, C, Hkv, D],
+    C at least 1; lengths: int32 [B] on the GPU, tokens of each sequence behind
+    the prefix with the new one (0: an idle sequence, its out is 0).  Token j of
+    them stands in row j % C.  k_new, v_new: as in window_attention_decode.
+    """
+    return _decode(q, k_cache, v_cache, lengths, k_new, v_new, None, 0, scale, out, None,
+                   (("k_prefix", k_prefix), ("v_prefix", v_prefix)))
+
+
+def window_attention_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, window: int | None = None,
+                             sinks: int = 0, scale: float | None = None, q_lens: torch.Tensor | None = None,
+                             k_lens: torch.Tensor | None = None, weights: torch.Tensor | None = None):
+    """What each key has received in window_attention called with the same arguments, which
+    gave `lse`: float32 [B, Hkv, Lk], the softmax weights of the queries that see it, summed
+    over them and over the query heads of its key head (0 behind a sequence's end).
+
+    weights: float32 [B, Hkv, Lk], contiguous: they are added to it, and it is the result.
+    """
+    device = _check_inputs(q.dtype, ("q", q), ("k", k))
+    head, tail = _attention_args(q, k, k, window, sinks, scale, q_lens, k_lens, device)
+    b, lq, h, d = q.shape
+    _, lk, kv, _ = k.shape
+    _check_lse(lse, b, h, lq, device)
+    add = weights is not None
+    if add:
+        _key_weights(weights, b, kv, lk, device)
+        _check_out(weights, ("q", q), ("k", k), ("lse", lse), what="weights")
+    else:
+        weights = torch.empty((b, kv, lk), dtype=torch.float32, device=q.device)
+    args = _pack_attention(*head, lq * h * d, h * d, d, 0, 0, 0, 0, 0, 0, 0, *tail)
+    ws, ws_ptr, ws_bytes = _scratch("wtc_window_attention_weights_workspace_size", args, device, _SIZES_END)
+    _launch(device, _lib.lib().wtc_window_attention_weights, args, q.data_ptr(), k.data_ptr(), lse.data_ptr(),
+            weights.data_ptr(), add, ws_ptr, ws_bytes)
+    return weights
+
+
+def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, lengths: torch.Tensor,
+                keep: int, *, recent: int = 0, sinks: int = 0, k_out: torch.Tensor | None = None,
+                v_out: torch.Tensor | None = None, weights_out: torch.Tensor | None = None):
+    """(k, v, weights, rows, lengths) of a smaller cache that holds the rows of most weight.
+
+    k_cache, v_cache: [B, C, Hkv, D] (float16 or bfloat16, D contiguous), token j of a
+    sequence in row j; weights: float32 [B, Hkv, C], contiguous, what each row has
+    received (window_attention_weights, window_attention_decode); lengths: int32 [B]
+    on the GPU.  A sequence of at most `keep` rows keeps them all.  Of a longer one
+    each key head keeps its first `sinks` rows, its last `recent` ones and, of those
+    between, the ones of greatest weight (of equal ones the lowest; a NaN is
+    greater than any number), in their order.  recent + sinks <= keep.
+
+    The results: k, v [B, keep, Hkv, D], zeros behind a sequence's end; weights
+    [B, Hkv, keep], zeros there; rows, int32 [B, Hkv, keep]: which they were, -1
+    behind the end; lengths, int32 [B], min(lengths, keep).  k_out, v_out
+    [B, C', Hkv, D] and weights_out [B, Hkv, C'], C' >= keep, given together, take them
+    instead, with room for new tokens: rows of k_out and v_out from `keep` on stay as
+    they are, those of weights_out are 0.  They lie over no input.
+    """
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError("the caches must be [B, C, Hkv, D]")
+    given = k_out is not None
+    if given != (v_out is not None) or given != (weights_out is not None):
+        raise ValueError("k_out, v_out and weights_out go together")
+    device = _check_inputs(k_cache.dtype, ("k_cache", k_cache), ("v_cache", v_cache), ("k_out", k_out), ("v_out", v_out))
+    b, cap, kv, d = shape
+    code = _code_of(k_cache, "k_cache")
+    _key_weights(weights, b, kv, cap, device)
+    if lengths is None:
+        raise ValueError("lengths must be given")
+    lens = _lens(lengths, b, "lengths", device)
+    if not 0 < keep or recent < 0 or sinks < 0 or recent + sinks > keep:
+        raise ValueError("keep must be at least 1, and hold recent + sinks rows")
+    if given:
+        if k_out.dim() != 4 or v_out.shape != k_out.shape or k_out.shape[0] != b or k_out.shape[2:] != shape[2:] or \
+                k_out.shape[1] < keep:
+            raise ValueError(f"k_out and v_out must be [{b}, C, {kv}, {d}], C at least {keep}")
+        _key_weights(weights_out, b, kv, k_out.shape[1], device)
+        inputs = ("k_cache", k_cache), ("v_cache", v_cache), ("weights", weights), ("lengths", lengths)
+        _check_out(k_out, *inputs, what="k_out")
+        _check_out(v_out, *inputs, ("k_out", k_out), what="v_out")
+        _check_out(weights_out, *inputs, ("k_out", k_out), ("v_out", v_out), what="weights_out")
+    else:
+        k_out, v_out = (torch.empty((b, keep, kv, d), dtype=k_cache.dtype, device=k_cache.device) for _ in range(2))
+        weights_out = torch.empty((b, kv, keep), dtype=torch.float32, device=k_cache.device)
+    rows = torch.empty((b, kv, keep), dtype=torch.int32, device=k_cache.device)
+    kept = torch.empty(b, dtype=torch.int32, device=k_cache.device)
+    args = _pack_evict(b, kv, cap, k_out.shape[1], d, code, keep, recent, sinks, *_strides(k_cache, "k_cache"),
+                       *_strides(v_cache, "v_cache"), *_strides(k_out, "k_out"), *_strides(v_out, "v_out"))
+    _launch(device, _lib.lib().wtc_cache_evict, args, k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), lens,
+            k_out.data_ptr(), v_out.data_ptr(), weights_out.data_ptr(), rows.data_ptr(), kept.data_ptr())
+    return k_out, v_out, weights_out, rows, kept
