@@ -53,7 +53,7 @@ ARCH = "gfx950"
 HIP_SOURCES = ["fused_matmul_softmax.hip", "wide_tile.hip", "rowblock_softmax.hip", "fewrows_softmax.hip",
                "unfused_chain.hip",
                "matmul_epilogue.hip", "window_attention.hip", "window_decode.hip",
-               "key_weights.hip", "cache_evict.hip",
+               "cross_attention.hip", "key_weights.hip", "cache_evict.hip",
                "launch.hip", "layer_launch.hip"]
 HOST_SOURCES = ["launch.hip", "layer_launch.hip"]  # no kernels to report on
 CXX_SOURCES = ["chain_recognizer.cpp", "variants.cpp", "tile_solver.cpp", "compile_capi.cpp"]
@@ -71,7 +71,8 @@ HIP_FLAGS = [
 ]
 # Per-source extra flags.  The tile kernels take their first-load scalars as
 # leading arguments; gfx950 preloads those into SGPRs.
-HIP_EXTRA = {"fused_matmul_softmax.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
+HIP_EXTRA = {"cross_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+             "fused_matmul_softmax.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
              "wide_tile.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"]}
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra",
              f"-I{ROOT / 'include'}", f"-I{CSRC}"]

@@ -38,11 +38,17 @@ hipError_t launch_act_backward(const ActBackwardParams& p, int dt, hipStream_t s
 
 struct AttnPlan {
   int key_groups, splits;
+  bool rows64;  // launch_attention_rows
 };
 AttnPlan plan_attention(const AttnParams& p, int cu_count);
 int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);
 // p.part_out: attention_workspace() bytes
 hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, hipStream_t stream);
+// Many rows that see nearly all of their keys (p.full, or behind p.prefix).
+// Splits (0: attention_tile_kernel is faster) and an estimate; p.part_out of launch_attention_rows:
+// attention_workspace() bytes.
+int plan_attention_rows(const AttnParams& p, int cu_count, double* us);
+hipError_t launch_attention_rows(const AttnParams& p, int splits, int dt, hipStream_t stream);
 // Results of the rows from p.slots partial ones, p.part_out [batch][lq][heads][slots][dim] and p.part_lse without dim.
 hipError_t launch_attention_join(const AttnParams& p, int dt, hipStream_t stream);
 struct AttnBackwardPlan {

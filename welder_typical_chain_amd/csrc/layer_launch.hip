@@ -239,6 +239,7 @@ struct PrefixPlan {
   AttnParams common, own;
   AttnPlan common_plan, own_plan;
   int own_splits;
+  bool single;  // one launch: each sequence's rows against the prefix and its own keys
   int64_t bytes;
 };
 PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bool decode, int cus) {
@@ -264,8 +265,21 @@ PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bo
   c.v_stride[2] = x.vp_stride[1];
   c.prefix = 0;
   q.common_plan = plan_attention(c, cus);
-  if (decode) q.own_splits = plan_decode(q.own, cus);
-  else q.own_plan = plan_attention(q.own, cus), q.own_splits = q.own_plan.splits;
+  if (decode) {
+    q.own_splits = plan_decode(q.own, cus);
+  } else {
+    if (x.prefix) {
+      double us;
+      q.own_splits = plan_attention_rows(q.own, cus, &us);
+      q.single = q.own_splits && q.own.lq * q.own.group >= 128;
+    }
+    if (q.single) {
+      q.bytes = align256(attention_workspace(q.own, AttnPlan{1, q.own_splits, true}));
+      return q;
+    }
+    q.own_plan = plan_attention(q.own, cus);
+    q.own_splits = q.own_plan.splits;
+  }
   const int first = x.prefix ? q.common_plan.splits : 0;
   c.slots = q.own.slots = first + (p.lk ? q.own_splits : 0);
   q.own.slot0 = first;
@@ -276,7 +290,7 @@ int launch_prefix(PrefixPlan& plan, bool decode, int dt, const void* q, const vo
                   const void* v, const void* k_new, const void* v_new, void* out, float* lse, void* workspace,
                   hipStream_t stream) {
   const int64_t rows = (int64_t)plan.own.batch * plan.own.lq * plan.own.heads;
-  for (AttnParams* a : {&plan.common, &plan.own}) {
+  for (AttnParams* a : {&plan.common, &plan.own}) {  // (part_lse: of two launches)
     a->q = static_cast<const uint8_t*>(q);
     a->part_out = static_cast<float*>(workspace);
     a->part_lse = a->part_out + rows * a->slots * a->dim;
@@ -290,13 +304,16 @@ int launch_prefix(PrefixPlan& plan, bool decode, int dt, const void* q, const vo
   own.v_new = static_cast<const uint8_t*>(v_new);
   own.out = static_cast<uint8_t*>(out);
   own.lse = lse;
+  if (plan.single) return launched(launch_attention_rows(own, plan.own_splits, dt, stream), "prefix_attention");
   plan.common.k = own.kp;
   plan.common.v = own.vp;
   if (plan.common.lk)
     if (int rc = launched(launch_attention(plan.common, plan.common_plan, dt, stream), "prefix_attention")) return rc;
   if (own.lk) {
-    const hipError_t e = decode ? launch_attention_decode(own, plan.own_splits, dt, stream)
-                                : launch_attention(own, plan.own_plan, dt, stream);
+    AttnParams a = own;
+    a.prefix = 0;
+    const hipError_t e = decode ? launch_attention_decode(a, plan.own_splits, dt, stream)
+                                : launch_attention(a, plan.own_plan, dt, stream);
     if (int rc = launched(e, "prefix_attention")) return rc;
   }
   return launched(launch_attention_join(own, dt, stream), "prefix_attention");

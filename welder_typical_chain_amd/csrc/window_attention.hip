@@ -9,74 +9,6 @@ namespace {
 
 using namespace attn;
 
-// Where the mask hides a NaN or an infinity.  The tiles' products meet it as 0 * NaN,
-// so an output element that comes out as NaN is computed again by a whole wave
-// from the keys (queries) that it sees, 64 at a time.  Only those elements are,
-// and only until each of them is NaN again, which an element that sees the bad
-// value is as soon as it is met: an input full of NaN costs one step a row.
-constexpr int kCols = 2;  // columns a lane: lane, lane + 64
-template <int DT> struct Redo {
-  using T = typename Elem<DT>::type;
-  T* row;
-  bool bad[kCols];
-  float acc[kCols];
-  __device__ inline Redo(void* base, int64_t at, int dim, int lane) : row(static_cast<T*>(base) + at) {
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      const float x = lane + 64 * c < dim ? (float)row[lane + 64 * c] : 0.0f;
-      bad[c] = x != x;
-      acc[c] = 0.0f;
-    }
-  }
-  __device__ inline void add(float w, const T* x, int lane) {
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-      if (bad[c]) acc[c] = __builtin_fmaf(w, (float)x[lane + 64 * c], acc[c]);
-  }
-  __device__ inline bool settled() const {  // every one of them is NaN for good
-    return __all((!bad[0] || acc[0] != acc[0]) && (!bad[1] || acc[1] != acc[1]));
-  }
-  __device__ inline void store(float by, int lane) {
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-      if (bad[c]) row[lane + 64 * c] = (T)(acc[c] * by);
-  }
-};
-
-// The last key that query i of sequence b sees.
-__device__ inline int last_seen(const AttnParams& p, int b, int i) {
-  const int nq = seq_queries(p, b), nk = seq_keys(p, b);
-  return min(i + first_position(p, nq, nk), nk - 1);
-}
-
-template <int DT> __device__ inline void attention_row(const AttnParams& p, int b, int h, int i) {
-  using T = typename Elem<DT>::type;
-  const int lane = threadIdx.x & 63;
-  const T* q = (const T*)p.q + b * p.q_stride[0] + i * p.q_stride[1] + h * p.q_stride[2];
-  const T* k = (const T*)p.k + b * p.k_stride[0] + h / p.group * p.k_stride[2];
-  const T* v = (const T*)p.v + b * p.v_stride[0] + h / p.group * p.v_stride[2];
-  const T* kp = (const T*)p.kp + h / p.group * p.kp_stride[1];
-  const T* vp = (const T*)p.vp + h / p.group * p.vp_stride[1];
-  const Seen seen(p.window, p.sinks, last_seen(p, b, i));
-  const int count = p.prefix + seen.count;
-  auto key = [&](int t) { return t < p.prefix ? kp + t * p.kp_stride[0] : k + seen.key(t - p.prefix) * p.k_stride[1]; };
-  auto value = [&](int t) { return t < p.prefix ? vp + t * p.vp_stride[0] : v + seen.key(t - p.prefix) * p.v_stride[1]; };
-  Redo<DT> out(p.out, b * p.o_stride[0] + i * p.o_stride[1] + h * p.o_stride[2], p.dim, lane);
-  float top = -INFINITY, total = 0.0f;
-  for (int t0 = 0; t0 < count && !out.settled(); t0 += 64) {
-    const bool in = t0 + lane < count;
-    const float s = in ? p.scale * dot_rows<DT>(q, key(t0 + lane), p.dim) : -INFINITY;
-    const float next = fmaxf(top, wave_max(s));
-    const float keep = next == -INFINITY ? 1.0f : __expf(top - next);
-    const float e = in ? (next == -INFINITY ? (s != s ? s : 0.0f) : __expf(s - next)) : 0.0f;
-    total = total * keep + wave_sum(e);
-    for (int c = 0; c < kCols; ++c) out.acc[c] *= keep;
-    top = next;
-    for (int t = 0; t < min(64, count - t0); ++t) out.add(__shfl(e, t), value(t0 + t), lane);
-  }
-  out.store(total == 0.0f ? 0.0f : 1.0f / total, lane);
-}
-
 // ---- forward -----------------------------------------------------------------
 // A workgroup takes 256 / KG query rows of one sequence and key head.  The rows
 // of the query heads that share the key head are packed (row r = query r / G,
@@ -1162,7 +1094,12 @@ template <int DT, int KG> const void* tile_kernel(int nd) {
 // Rows a workgroup (256 / key_groups) and splits of the keys, from the sizes alone:
 // splits while CUs are idle and a wave keeps 4 tiles.
 AttnPlan plan_attention(const AttnParams& p, int cu_count) {
-  AttnPlan plan{1, 1};
+  AttnPlan plan{1, 1, false};
+  if (p.full) {
+    double us;
+    const int splits = plan_attention_rows(p, cu_count, &us);
+    if (splits) return AttnPlan{1, splits, true};
+  }
   const int64_t rows = (int64_t)p.lq * p.group, seqs = (int64_t)p.batch * p.kv_heads;
   if (seqs * ((rows + 255) / 256) < cu_count) plan.key_groups = 2;
   const int64_t block = 256 / plan.key_groups, grid = seqs * ((rows + block - 1) / block);
@@ -1178,6 +1115,7 @@ int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan) {
 }
 
 hipError_t launch_attention(const AttnParams& params, const AttnPlan& plan, int dt, hipStream_t stream) {
+  if (plan.rows64) return launch_attention_rows(params, plan.splits, dt, stream);
   AttnParams p = params;
   const int64_t rows = (int64_t)p.lq * p.group;
   const bool joined = p.slots;  // by the caller, with the results of other launches
