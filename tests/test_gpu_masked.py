@@ -384,9 +384,7 @@ def check_decode_weights(W, b, cap, lengths, h, kv, d, dtype, window=None, sinks
     w = rand(seed + 5, b, kv, cap).abs()
     ref = M.decode(q, kc, vc, lengths, window=window, sinks=sinks, k_new=kn, v_new=vn, weights=w)
     kw = dict(k_new=kn, v_new=vn, window=window, sinks=sinks)
-    plain = W.window_attention_decode(q, kc.clone(), vc.clone(), lengths, **kw)
     out = W.window_attention_decode(q, kc, vc, lengths, weights=w, **kw)
-    assert torch.equal(out, plain)
     within(out, ref["out"], "out")
     within(w, ref["weights"], "weights")
     assert torch.equal(kc, ref["k_cache"]) and torch.equal(vc, ref["v_cache"])

@@ -266,7 +266,7 @@ PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bo
   c.prefix = 0;
   q.common_plan = plan_attention(c, cus);
   if (decode) {
-    q.own_splits = plan_decode(q.own, cus);
+    q.own_splits = plan_decode_joined(q.own, cus);
   } else {
     if (x.prefix) {
       double us;
@@ -636,7 +636,7 @@ static int64_t decode_workspace_size(const wtc_attention_args* p, bool weights) 
   if (guarded([&] { return check_attention(*p, true); })) return -1;
   if (weights && check_decode_weights(*p)) return -1;
   const AttnParams a = decode_params(*p);
-  const int splits = plan_decode(a, cu_count());
+  const int splits = weights ? plan_decode_joined(a, cu_count()) : plan_decode(a, cu_count());
   return align256(weights ? decode_weights_workspace(a, splits) : decode_workspace(a, splits));
 }
 int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p) { return decode_workspace_size(p, false); }
@@ -668,7 +668,7 @@ static int decode(bool has_weights, const wtc_attention_args* p, const void* q, 
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(k_new) || !aligned16(v_new))
       return bad("pointers must be 16-byte aligned");
     AttnParams a = decode_params(*p);
-    const int splits = plan_decode(a, cu_count());
+    const int splits = has_weights ? plan_decode_joined(a, cu_count()) : plan_decode(a, cu_count());
     const int64_t need = align256(has_weights ? decode_weights_workspace(a, splits) : decode_workspace(a, splits));
     if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
     a.part_out = static_cast<float*>(workspace);

@@ -335,6 +335,15 @@ int plan_decode(const AttnParams& p, int cu_count) {
   while (splits < 64 && grid * splits * 2 <= cu_count && tiles / (2 * splits) >= 4 * kWaves) splits *= 2;
   return splits;
 }
+// Sequences of unequal length leave CUs idle at the end: splits until the chip has two
+// workgroups a CU, one after another, while a wave keeps at least 4 tiles.
+int plan_decode_joined(const AttnParams& p, int cu_count) {
+  const int64_t grid = (int64_t)p.batch * p.kv_heads * ((p.group + kHeads - 1) / kHeads);
+  const int64_t tiles = (std::min<int64_t>(p.lk, p.window + p.sinks) + kRows - 1) / kRows;
+  int splits = 1;
+  while (splits < 64 && grid * splits < 2 * cu_count && tiles / (2 * splits) >= 4 * kWaves) splits *= 2;
+  return splits;
+}
 int64_t decode_workspace(const AttnParams& p, int splits) {
   return splits > 1 ? (int64_t)p.batch * p.heads * splits * (p.dim + 1) * 4 : 0;
 }
