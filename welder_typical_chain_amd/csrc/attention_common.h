@@ -99,6 +99,14 @@ template <int NS> __device__ inline void load_row(const uint8_t* row, bool valid
   }
 }
 
+// Has the loads of f arrive here.  The compiler waits for a load where its result is first
+// used; in a loop it would do so in every turn, for all loads in flight, the
+// direct-to-LDS ones (which it does not know of) too.
+template <int NS> __device__ inline void landed(u32x4 (&f)[NS]) {
+#pragma unroll
+  for (int s = 0; s < NS; ++s) asm volatile("" : "+v"(f[s]));
+}
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Scores in the log2 domain are c2 times the products, c2 > 0: with a negative scale

@@ -95,9 +95,11 @@ __global__ void __launch_bounds__(kWaves * 64, ND <= 2 ? 2 : 1) attention_rows_k
     const int q_seq = p.seq_rows ? i[a] / p.seq_rows : b, q_row = p.seq_rows ? i[a] % p.seq_rows : i[a];
     load_row<NS>(p.q + 2 * (q_seq * p.q_stride[0] + (int64_t)q_row * p.q_stride[1] + h[a] * p.q_stride[2]), valid[a], p.dim, half, qf[a]);
     c2 = positive_scale<NS>(p.scale, qf[a]);
-    if constexpr (ND >= 3) {
+    if constexpr (ND >= 3) {  // Q's place is the accumulation registers: the products read it there
 #pragma unroll
       for (int st = 0; st < NS; ++st) asm volatile("" : "+a"(qf[a][st]));
+    } else {
+      landed(qf[a]);
     }
   }
   // units: the prefix's, then the own keys' up to the last one that a row of the block sees

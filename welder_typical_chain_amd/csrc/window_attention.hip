@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
 #pragma unroll
   for (int x = 0; x < L::STAGES - 1; ++x) issue(x);
 
+  landed(qf);
   const uint32_t k_at = row_addr<RB>(lane) + group * 2 * L::TILE, v_at = L::TILE + col_addr<RB>(lane) + group * 2 * L::TILE;
   for (int x = 0; x < steps; ++x) {
     wait_loads_barrier<LOADS*(L::STAGES - 2)>();  // the step's tiles landed; every wave is done with the last one's
@@ -625,6 +626,8 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
     p.row_delta[stats_row(p, b, hk, i) + x_head] = -delta;
   }
 
+  landed(qf);
+  landed(gf);
   f32x16 dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -853,6 +856,8 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
   };
 #pragma unroll
   for (int t = 0; t < L::STAGES - 1; ++t) issue(t);
+  landed(kf);
+  landed(vf);
   const uint32_t r_at = row_addr<RB>(lane) + (uint32_t)row0 * RB, c_at = col_addr<RB>(lane) + (uint32_t)row0 * RB;
   for (int t = 0; t < t_all; ++t) {
     // tile t landed; every wave is done with tile t - 1 (wave 0 has two more loads a tile)

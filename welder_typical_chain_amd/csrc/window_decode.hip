@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) decode_kernel(const AttnParams
 #pragma unroll
   for (int x = 0; x < L::STAGES; ++x) issue(x);
 
+  landed(qf);
   for (int x = 0; t0 + wave + x * kWaves < t1; ++x) {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS * (L::STAGES - 1)) : "memory");
     int row, rows;
