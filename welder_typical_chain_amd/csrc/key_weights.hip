@@ -55,16 +55,19 @@ template <int N> __device__ inline void column_sums(float (&x)[N], int lane) {
   }
 }
 
-// Queries i0 .. i1 - 1 of a chunk that may see a key of block kb.
+// Queries i0 .. i1 - 1 of a chunk that may see a key of block kb: the block's queries in as
+// many equal chunks as keep within chunk_rows.
 struct Chunk {
   int i0, i1;
-  __device__ inline Chunk(const AttnParams& p, int nq, int nk, int kb, int chunk, int chunk_rows) {
+  __device__ inline Chunk(const AttnParams& p, int nq, int nk, int kb, int chunk, int chunk_rows, int tile_rows) {
     const int shift = first_position(p, nq, nk), j_first = kb * kKeys;
-    i0 = min(max(0, j_first - shift), nq);
-    i1 = j_first < p.sinks ? nq : (int)max((int64_t)i0, min((int64_t)nq, (int64_t)min(j_first + kKeys, nk) - 1 + p.window - shift));
-    if (j_first >= nk) i1 = i0;
-    i0 = (int)min((int64_t)i1, max((int64_t)i0, (int64_t)chunk * chunk_rows));
-    i1 = (int)max((int64_t)i0, min((int64_t)i1, (int64_t)(chunk + 1) * chunk_rows));
+    const int lo = min(max(0, j_first - shift), nq);
+    int hi = j_first < p.sinks ? nq : (int)max((int64_t)lo, min((int64_t)nq, (int64_t)min(j_first + kKeys, nk) - 1 + p.window - shift));
+    if (j_first >= nk) hi = lo;
+    const int chunks = (hi - lo + chunk_rows - 1) / chunk_rows, tiles = (hi - lo + tile_rows - 1) / tile_rows;
+    const int share = chunks ? (tiles + chunks - 1) / chunks * tile_rows : 0;
+    i0 = (int)min((int64_t)hi, lo + (int64_t)chunk * share);
+    i1 = min(hi, i0 + share);
   }
 };
 __device__ inline int clamp32(int64_t x) { return (int)min((int64_t)INT32_MAX, max((int64_t)INT32_MIN, x)); }
@@ -77,13 +80,14 @@ __global__ void __launch_bounds__(kWaves * 64, 2) key_weights_kernel(const AttnP
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
-  const int chunk = (int)(id % p.splits), kb = (int)(id / p.splits % p.key_blocks);
+  // (the chunks that a causal sequence's last blocks do not have come last)
+  const int kb = (int)(id % p.key_blocks), chunk = (int)(id / p.key_blocks % p.splits);
   const int hk = (int)(id / p.splits / p.key_blocks % p.kv_heads), b = (int)(id / p.splits / p.key_blocks / p.kv_heads);
   const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = first_position(p, nq, nk);
   const int j_wave = kb * kKeys + wave * 64;
-  const auto [i0, i1] = Chunk(p, nq, nk, kb, chunk, chunk_rows);
-  if (p.splits > 1 && i0 == i1) return;  // (nothing to add: the second kernel knows)
   const int hg = min(p.group, kRows), groups = (p.group + hg - 1) / hg, tp = kRows / hg;  // heads, parts, positions of a tile
+  const auto [i0, i1] = Chunk(p, nq, nk, kb, chunk, chunk_rows, tp);
+  if (p.splits > 1 && i0 == i1) return;  // (nothing to add: the second kernel knows)
 
   const uint8_t* q_base = p.q + 2 * (b * p.q_stride[0] + (int64_t)hk * p.group * p.q_stride[2]);
   uint32_t q_off[NB], at_row[NB];  // at_row: position and head (high half)
@@ -273,7 +277,7 @@ __global__ void __launch_bounds__(256) key_weights_sum_kernel(const AttnParams p
       for (int c = 0; c < 8; ++c) {
         x[c] = 0.0f;
         if (c0 + c >= p.splits) continue;
-        const Chunk of(p, nq, nk, kb, c0 + c, chunk_rows);
+        const Chunk of(p, nq, nk, kb, c0 + c, chunk_rows, kRows / min(p.group, kRows));
         if (of.i0 < of.i1) x[c] = p.part_out[(seq * p.splits + c0 + c) * p.lk + j];
       }
 #pragma unroll
@@ -297,7 +301,7 @@ template <int DT> const void* kernel_for(int nd) {
 }  // namespace
 
 // Chunks of the queries, so that the rounds of workgroups (two a CU) times what each
-// takes are least: its tiles and about four tiles' time for its start and end.
+// takes are least: its tiles and about eight tiles' time for its start and end.
 KeyWeightsPlan plan_key_weights(const AttnParams& p, int cu_count) {
   KeyWeightsPlan plan{};
   plan.key_blocks = (p.lk + kKeys - 1) / kKeys;
@@ -312,12 +316,12 @@ KeyWeightsPlan plan_key_weights(const AttnParams& p, int cu_count) {
     seen[i] = std::max<int64_t>(0, hi - lo);
   }
   double least = 1e30;
-  for (int64_t tiles = 4, end = (p.lq + tp - 1) / tp;; tiles += std::max<int64_t>(1, tiles / 4)) {  // positions' tiles a chunk
+  for (int64_t tiles = 4, end = (p.lq + tp - 1) / tp;; tiles += std::max<int64_t>(1, tiles / 16)) {  // positions' tiles a chunk
     tiles = std::min(tiles, std::max<int64_t>(1, end));
     int64_t chunks = 0;
     for (int i = 0; i < SAMPLES; ++i) chunks += std::max<int64_t>(1, (seen[i] + tiles * tp - 1) / (tiles * tp));
-    const double groups = (double)seqs * plan.key_blocks * chunks / SAMPLES, rounds = std::ceil(groups / (2 * cu_count));
-    const double us = std::max(rounds, groups / (2 * cu_count) + 0.5) * (tiles * parts + 4) + (tiles < end ? 6 : 0);
+    const double groups = (double)seqs * plan.key_blocks * chunks / SAMPLES;
+    const double us = std::ceil(groups / (2 * cu_count)) * (tiles * parts + 8) + (tiles < end ? 4 : 0);
     if (us < least) {
       least = us;
       plan.chunk_rows = (int)(tiles * tp);
