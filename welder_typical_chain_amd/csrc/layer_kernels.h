@@ -38,7 +38,7 @@ hipError_t launch_act_backward(const ActBackwardParams& p, int dt, hipStream_t s
 
 struct AttnPlan {
   int key_groups, splits;
-  bool rows64;  // launch_attention_rows
+  enum { TILE, ROWS, FEW } kernel;  // attention_tile_kernel, launch_attention_rows, launch_few_rows
 };
 AttnPlan plan_attention(const AttnParams& p, int cu_count);
 int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);
@@ -49,6 +49,17 @@ hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, h
 // attention_workspace() bytes.
 int plan_attention_rows(const AttnParams& p, int cu_count, double* us);
 hipError_t launch_attention_rows(const AttnParams& p, int splits, int dt, hipStream_t stream);
+// Few rows (p.full) against many keys; splits, 0: too many rows.  p.part_out: as above.
+int plan_few_rows(const AttnParams& p, int cu_count);
+hipError_t launch_few_rows(const AttnParams& p, int splits, int dt, hipStream_t stream);
+// One token a sequence: the batch's queries as one sequence's against a prefix, and own caches,
+// into p.slots partial results, and their join; splits of both.
+struct PrefixTokenPlan {
+  int common, own;
+  bool many;  // attention_rows for the prefix
+};
+PrefixTokenPlan plan_prefix_token(const AttnParams& common, const AttnParams& own, int cu_count);
+hipError_t launch_prefix_token(const AttnParams& common, const AttnParams& own, const PrefixTokenPlan& plan, int dt, hipStream_t stream);
 // Results of the rows from p.slots partial ones, p.part_out [batch][lq][heads][slots][dim] and p.part_lse without dim.
 hipError_t launch_attention_join(const AttnParams& p, int dt, hipStream_t stream);
 struct AttnBackwardPlan {

@@ -238,6 +238,7 @@ int check_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bool dec
 struct PrefixPlan {
   AttnParams common, own;
   AttnPlan common_plan, own_plan;
+  PrefixTokenPlan token;  // decode
   int own_splits;
   bool single;  // one launch: each sequence's rows against the prefix and its own keys
   int64_t bytes;
@@ -264,23 +265,26 @@ PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bo
   c.k_stride[2] = x.kp_stride[1];
   c.v_stride[2] = x.vp_stride[1];
   c.prefix = 0;
-  q.common_plan = plan_attention(c, cus);
+  int first = 0;
   if (decode) {
-    q.own_splits = plan_decode_joined(q.own, cus);
+    q.token = plan_prefix_token(c, q.own, cus);
+    first = q.token.common;
+    q.own_splits = q.token.own;
   } else {
+    q.common_plan = plan_attention(c, cus);
+    first = x.prefix ? q.common_plan.splits : 0;
     if (x.prefix) {
       double us;
       q.own_splits = plan_attention_rows(q.own, cus, &us);
       q.single = q.own_splits && q.own.lq * q.own.group >= 128;
     }
     if (q.single) {
-      q.bytes = align256(attention_workspace(q.own, AttnPlan{1, q.own_splits, true}));
+      q.bytes = align256(attention_workspace(q.own, AttnPlan{1, q.own_splits, AttnPlan::ROWS}));
       return q;
     }
     q.own_plan = plan_attention(q.own, cus);
     q.own_splits = q.own_plan.splits;
   }
-  const int first = x.prefix ? q.common_plan.splits : 0;
   c.slots = q.own.slots = first + (p.lk ? q.own_splits : 0);
   q.own.slot0 = first;
   q.bytes = align256(p.batch * p.lq * p.heads * c.slots * 4 * (p.dim + 1));
@@ -307,14 +311,13 @@ int launch_prefix(PrefixPlan& plan, bool decode, int dt, const void* q, const vo
   if (plan.single) return launched(launch_attention_rows(own, plan.own_splits, dt, stream), "prefix_attention");
   plan.common.k = own.kp;
   plan.common.v = own.vp;
+  if (decode) return launched(launch_prefix_token(plan.common, own, plan.token, dt, stream), "prefix_attention_decode");
   if (plan.common.lk)
     if (int rc = launched(launch_attention(plan.common, plan.common_plan, dt, stream), "prefix_attention")) return rc;
   if (own.lk) {
     AttnParams a = own;
     a.prefix = 0;
-    const hipError_t e = decode ? launch_attention_decode(a, plan.own_splits, dt, stream)
-                                : launch_attention(a, plan.own_plan, dt, stream);
-    if (int rc = launched(e, "prefix_attention")) return rc;
+    if (int rc = launched(launch_attention(a, plan.own_plan, dt, stream), "prefix_attention")) return rc;
   }
   return launched(launch_attention_join(own, dt, stream), "prefix_attention");
 }
