@@ -13,19 +13,25 @@ using namespace attn;
 
 using namespace rows;
 
-template <int DT, int ND, bool PREFIX>
-__global__ void __launch_bounds__(kWaves * 64, ND <= 2 ? 2 : 1) attention_rows_kernel(const AttnParams p) {
-  __shared__ __attribute__((aligned(256))) uint8_t smem[RowsLds<ND>::TOTAL];
-  attention_rows<DT, ND, PREFIX>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
+// A row block of 32 or two a wave (up to dim 64: two, and two workgroups a CU).  One a wave
+// makes two waves a SIMD, between which issue slots and the two pipes are shared, but
+// reads each key fragment twice as often.  On a full chip the clock then falls from 1.89
+// to 1.65 GHz and two a wave are faster (4 x 2048 x 4096, 32 / 8 heads of 128: 465 us
+// against 488); where workgroups are few, one (8 x 200 behind 4096: 121 against 126).
+template <int DT, int ND, bool PREFIX, int A>
+__global__ void __launch_bounds__(waves(A) * 64, A == 1 || ND <= 2 ? 2 : 1) attention_rows_kernel(const AttnParams p) {
+  __shared__ __attribute__((aligned(256))) uint8_t smem[RowsLds<ND, A>::TOTAL];
+  attention_rows<DT, ND, PREFIX, A>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
 }
 
-template <int DT, bool PREFIX> const void* kernel_for(int nd) {
+template <int DT, bool PREFIX> const void* kernel_for(int nd, int a) {
+  if (a == 1) return nd == 3 ? (const void*)&attention_rows_kernel<DT, 3, PREFIX, 1> : (const void*)&attention_rows_kernel<DT, 4, PREFIX, 1>;
   switch (nd) {
-    case 1: return (const void*)&attention_rows_kernel<DT, 1, PREFIX>;
-    case 2: return (const void*)&attention_rows_kernel<DT, 2, PREFIX>;
-    case 3: return (const void*)&attention_rows_kernel<DT, 3, PREFIX>;
+    case 1: return (const void*)&attention_rows_kernel<DT, 1, PREFIX, 2>;
+    case 2: return (const void*)&attention_rows_kernel<DT, 2, PREFIX, 2>;
+    case 3: return (const void*)&attention_rows_kernel<DT, 3, PREFIX, 2>;
   }
-  return (const void*)&attention_rows_kernel<DT, 4, PREFIX>;
+  return (const void*)&attention_rows_kernel<DT, 4, PREFIX, 2>;
 }
 
 }  // namespace
@@ -46,7 +52,7 @@ int plan_attention_rows(const AttnParams& p, int cu_count, double* us_out) {
   return best;
 }
 
-hipError_t launch_attention_rows(const AttnParams& params, int splits, int dt, hipStream_t stream) {
+hipError_t launch_attention_rows(const AttnParams& params, int splits, int cu_count, int dt, hipStream_t stream) {
   AttnParams p = params;
   const bool joined = p.slots;  // by the caller, with the results of other launches
   p.splits = splits;
@@ -56,11 +62,12 @@ hipError_t launch_attention_rows(const AttnParams& params, int splits, int dt, h
   }
   p.row_blocks = (int)(((int64_t)p.lq * p.group + kRows - 1) / kRows);
   const int nd = (p.dim + 31) / 32;
-  const void* fn = p.prefix ? (dt == DT_F16 ? kernel_for<DT_F16, true>(nd) : kernel_for<DT_BF16, true>(nd))
-                            : (dt == DT_F16 ? kernel_for<DT_F16, false>(nd) : kernel_for<DT_BF16, false>(nd));
-  void* args[] = {&p};
   const int64_t grid = (int64_t)p.batch * p.kv_heads * p.row_blocks * splits;
-  const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)grid), dim3(kWaves * 64), args, 0, stream);
+  const int a = nd >= 3 && grid <= cu_count ? 1 : 2;
+  const void* fn = p.prefix ? (dt == DT_F16 ? kernel_for<DT_F16, true>(nd, a) : kernel_for<DT_BF16, true>(nd, a))
+                            : (dt == DT_F16 ? kernel_for<DT_F16, false>(nd, a) : kernel_for<DT_BF16, false>(nd, a));
+  void* args[] = {&p};
+  const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)grid), dim3(waves(a) * 64), args, 0, stream);
   if (e != hipSuccess || splits == 1 || joined) return e;
   return launch_attention_join(p, dt, stream);
 }
@@ -73,10 +80,10 @@ namespace {
 
 template <int DT, int ND, bool MANY>
 __global__ void __launch_bounds__(256, 1) prefix_token_kernel(const AttnParams common, const AttnParams own, int common_blocks) {
-  constexpr int MOST = decode::DecodeLds<ND>::TOTAL > RowsLds<ND>::TOTAL ? decode::DecodeLds<ND>::TOTAL : RowsLds<ND>::TOTAL;
+  constexpr int MOST = decode::DecodeLds<ND>::TOTAL > RowsLds<ND, 2>::TOTAL ? decode::DecodeLds<ND>::TOTAL : RowsLds<ND, 2>::TOTAL;
   __shared__ __attribute__((aligned(256))) uint8_t smem[MOST];
   if ((int)blockIdx.x >= common_blocks) decode::decode_tile<DT, ND, false, false>(own, smem, (int)blockIdx.x - common_blocks);
-  else if constexpr (MANY) attention_rows<DT, ND, false>(common, smem, xcd_remap(blockIdx.x, (uint32_t)common_blocks));
+  else if constexpr (MANY) attention_rows<DT, ND, false, 2>(common, smem, xcd_remap(blockIdx.x, (uint32_t)common_blocks));
   else decode::decode_tile<DT, ND, false, true>(common, smem, (int)blockIdx.x);
 }
 template <int DT, bool MANY> const void* token_kernel_for(int nd) {

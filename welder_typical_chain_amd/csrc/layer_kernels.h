@@ -39,6 +39,7 @@ hipError_t launch_act_backward(const ActBackwardParams& p, int dt, hipStream_t s
 struct AttnPlan {
   int key_groups, splits;
   enum { TILE, ROWS, FEW } kernel;  // attention_tile_kernel, launch_attention_rows, launch_few_rows
+  int cu_count;
 };
 AttnPlan plan_attention(const AttnParams& p, int cu_count);
 int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);
@@ -48,7 +49,7 @@ hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, h
 // Splits (0: attention_tile_kernel is faster) and an estimate; p.part_out of launch_attention_rows:
 // attention_workspace() bytes.
 int plan_attention_rows(const AttnParams& p, int cu_count, double* us);
-hipError_t launch_attention_rows(const AttnParams& p, int splits, int dt, hipStream_t stream);
+hipError_t launch_attention_rows(const AttnParams& p, int splits, int cu_count, int dt, hipStream_t stream);
 // Few rows (p.full) against many keys; splits, 0: too many rows.  p.part_out: as above.
 int plan_few_rows(const AttnParams& p, int cu_count);
 hipError_t launch_few_rows(const AttnParams& p, int splits, int dt, hipStream_t stream);

@@ -279,7 +279,7 @@ PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bo
       q.single = q.own_splits && q.own.lq * q.own.group >= 128;
     }
     if (q.single) {
-      q.bytes = align256(attention_workspace(q.own, AttnPlan{1, q.own_splits, AttnPlan::ROWS}));
+      q.bytes = align256(attention_workspace(q.own, AttnPlan{1, q.own_splits, AttnPlan::ROWS, cus}));
       return q;
     }
     q.own_plan = plan_attention(q.own, cus);
@@ -308,7 +308,7 @@ int launch_prefix(PrefixPlan& plan, bool decode, int dt, const void* q, const vo
   own.v_new = static_cast<const uint8_t*>(v_new);
   own.out = static_cast<uint8_t*>(out);
   own.lse = lse;
-  if (plan.single) return launched(launch_attention_rows(own, plan.own_splits, dt, stream), "prefix_attention");
+  if (plan.single) return launched(launch_attention_rows(own, plan.own_splits, cu_count(), dt, stream), "prefix_attention");
   plan.common.k = own.kp;
   plan.common.v = own.vp;
   if (decode) return launched(launch_prefix_token(plan.common, own, plan.token, dt, stream), "prefix_attention_decode");

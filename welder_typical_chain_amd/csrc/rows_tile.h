@@ -8,26 +8,28 @@ namespace rows {
 
 using namespace attn;
 
-constexpr int kWaves = 4;
-constexpr int kRows = 64 * kWaves;  // query rows a workgroup
+constexpr int kRows = 256;  // query rows a workgroup
+// A: the row blocks of 32 that a wave owns.
+constexpr int waves(int a) { return kRows / 32 / a; }
 constexpr int kUnit = 32;           // keys
 // The reference that a row's exponentials are taken against is only moved when 16 of
 // them pass this in sum (weights then stay below it, and sums far from f16's and f32's
 // ends): no maximum is taken of the other scores.
 constexpr float kMostSum = 1024.0f;
 
-template <int ND> struct RowsLds {
+template <int ND, int A> struct RowsLds {
   static constexpr int RB = row_bytes(ND), STAGES = 3;
   static constexpr int HALF = kUnit * RB, STAGE = 4 * HALF;
   static constexpr int PITCH = ND * 64 + 16;  // bytes of a row staged for the output
-  static constexpr int RING = STAGES * STAGE, OUT = kWaves * 32 * PITCH;
+  static constexpr int RING = STAGES * STAGE, OUT = waves(A) * 32 * PITCH;
   static constexpr int TOTAL = RING > OUT ? RING : OUT;
   static_assert(TOTAL <= 160 * 1024, "LDS");
 };
 
 // Loads of two units, by all waves, of which each loads part of both.
-template <int RB> struct UnitLoader {
-  static constexpr int NB = kUnit * RB / 1024 / kWaves;
+template <int RB, int NW> struct UnitLoader {
+  static constexpr int NB = kUnit * RB / 1024 / NW;
+  static_assert(NB * 1024 * NW == kUnit * RB, "blocks over waves");
   const uint8_t* base;
   uint32_t stride;  // bytes
   uint32_t off[2 * NB];
@@ -64,10 +66,11 @@ template <int DT> __device__ inline uint32_t pack2(float a, float b) {
 }
 
 // PREFIX: p.prefix keys before the own ones, of which a row sees those up to its own position.
-template <int DT, int ND, bool PREFIX>
+template <int DT, int ND, bool PREFIX, int A>
 __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32_t id) {
-  using L = RowsLds<ND>;
+  using L = RowsLds<ND, A>;
   constexpr int RB = L::RB, NS = 2 * ND;
+  using Loader = UnitLoader<RB, waves(A)>;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = (int)(id % p.splits);
@@ -78,13 +81,13 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
   const int r0 = blk * kRows;
 
   // this lane's rows; `sees`: own keys that a row sees
-  int i[2], h[2], sees[2];
-  bool valid[2];
-  u32x4 qf[2][NS];
+  int i[A], h[A], sees[A];
+  bool valid[A];
+  u32x4 qf[A][NS];
   float c2 = 0.0f;
 #pragma unroll
-  for (int a = 0; a < 2; ++a) {
-    const int r = r0 + wave * 64 + 32 * a + (lane & 31);
+  for (int a = 0; a < A; ++a) {
+    const int r = r0 + wave * 32 * A + 32 * a + (lane & 31);
     i[a] = r / p.group;
     h[a] = hk * p.group + r - i[a] * p.group;
     valid[a] = i[a] < nq;
@@ -92,7 +95,7 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
     const int q_seq = p.seq_rows ? i[a] / p.seq_rows : b, q_row = p.seq_rows ? i[a] % p.seq_rows : i[a];
     load_row<NS>(p.q + 2 * (q_seq * p.q_stride[0] + (int64_t)q_row * p.q_stride[1] + h[a] * p.q_stride[2]), valid[a], p.dim, half, qf[a]);
     c2 = positive_scale<NS>(p.scale, qf[a]);
-    if constexpr (ND >= 3) {  // Q's place is the accumulation registers: the products read it there
+    if constexpr (A == 2 && ND >= 3) {  // (one wave a SIMD) the products read them in the accumulation registers
 #pragma unroll
       for (int st = 0; st < NS; ++st) asm volatile("" : "+a"(qf[a][st]));
     } else {
@@ -109,17 +112,17 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
   const int n0 = (int)((int64_t)all * split / p.splits), n1 = (int)((int64_t)all * (split + 1) / p.splits);
   const int steps = (n1 - n0 + 1) / 2, plain = max(0, min(whole, n1) - n0) / 2;
 
-  UnitLoader<RB> own_k, own_v, pre_k, pre_v;
+  Loader own_k, own_v, pre_k, pre_v;
   own_k.init(p.k + 2 * (b * p.k_stride[0] + hk * p.k_stride[2]), 2 * p.k_stride[1], p.dim, wave, lane);
   own_v.init(p.v + 2 * (b * p.v_stride[0] + hk * p.v_stride[2]), 2 * p.v_stride[1], p.dim, wave, lane);
   if constexpr (PREFIX) {
     pre_k.init(p.kp + 2 * hk * p.kp_stride[1], 2 * p.kp_stride[0], p.dim, wave, lane);
     pre_v.init(p.vp + 2 * hk * p.vp_stride[1], 2 * p.vp_stride[0], p.dim, wave, lane);
   }
-  constexpr int LOADS = 4 * UnitLoader<RB>::NB;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem + (uint32_t)(wave * UnitLoader<RB>::NB * 1024);
+  constexpr int LOADS = 4 * Loader::NB;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem + (uint32_t)(wave * Loader::NB * 1024);
   const uint32_t dim_bytes = (uint32_t)p.dim * 2u;
-  auto load = [&](const UnitLoader<RB>& of_own, const UnitLoader<RB>& of_prefix, int n, uint32_t to) __attribute__((always_inline)) {
+  auto load = [&](const Loader& of_own, const Loader& of_prefix, int n, uint32_t to) __attribute__((always_inline)) {
     const int g = n0 + n;
     const bool in = n >= 0 && g < n1;
     if (PREFIX && g < prefix_units) of_prefix.issue(to, in ? g * kUnit : 0, in ? min(kUnit, prefix - g * kUnit) : 0, dim_bytes);
@@ -148,23 +151,27 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
     left -= 2 * kUnit;
   };
 
-  f32x16 o[2][ND], s[2][2];  // s: of two units in turn
+  f32x16 o[A][ND], s[2][A];  // s: of two units in turn
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int a = 0; a < A; ++a)
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int v = 0; v < 16; ++v) o[a][d][v] = 0.0f;
-  u32x4 pf[2][2];
+  u32x4 pf[A][2];
   // ref: minus the reference (log2 domain); +inf where there is none yet, which makes any
   // exponential pass kMostSum or be NaN.  total: this lane's half of the keys.
-  float ref[2] = {INFINITY, INFINITY}, total[2] = {0.0f, 0.0f};
+  float ref[A], total[A];
 #pragma unroll
-  for (int a = 0; a < 2; ++a) pf[a][0] = pf[a][1] = u32x4{0, 0, 0, 0};
+  for (int a = 0; a < A; ++a) {
+    ref[a] = INFINITY;
+    total[a] = 0.0f;
+    pf[a][0] = pf[a][1] = u32x4{0, 0, 0, 0};
+  }
 
   const uint32_t k_at = row_addr<RB>(lane), v_at = 2 * L::HALF + col_addr<RB>(lane);
   // Fragment y of half x of a stage: NS of keys, then NS of values.
-  constexpr int STEPS = 2 * NS, AHEAD = 3;
+  constexpr int STEPS = 2 * NS, AHEAD = A == 1 ? 4 : 3;
   auto read = [&](uint32_t stage, int x, int y) __attribute__((always_inline)) {
     if (y < NS) return row_frag<RB>(smem, k_at + stage, kUnit * x, y);
     return col_frag<RB>(smem, v_at + stage, kUnit * x + 16 * ((y - NS) / ND), (y - NS) % ND);
@@ -174,15 +181,17 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
   // (into next) and unit n - 1's values.  In steps of one fragment, two products and a
   // share of the weights, each fragment read AHEAD steps before its products; the
   // compiler moves nothing from one step to another.
-  auto phase = [&](auto masked, int t, int x, uint32_t& stage, uint32_t fill, f32x16 (&cur)[2], f32x16 (&next)[2]) __attribute__((always_inline)) {
-    u32x4 w[2][2];
-    float sum[2] = {0.0f, 0.0f};
+  auto phase = [&](auto masked, int t, int x, uint32_t& stage, uint32_t fill, f32x16 (&cur)[A], f32x16 (&next)[A]) __attribute__((always_inline)) {
+    u32x4 w[A][2];
+    float sum[A];
+#pragma unroll
+    for (int a = 0; a < A; ++a) sum[a] = 0.0f;
     if constexpr (decltype(masked)::value) {
       const int g = n0 + 2 * t + x;
       const bool common = PREFIX && g < prefix_units;
       const int j0 = (common ? g : g - prefix_units) * kUnit + 4 * half;
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
+      for (int a = 0; a < A; ++a) {
         const uint64_t seen = g < n1 ? bits_below((common ? prefix : sees[a]) - j0) : 0;
 #pragma unroll
         for (int v = 0; v < 16; ++v) cur[a][v] = keep_bit(cur[a][v], seen, 8 * (v >> 2) + (v & 3));
@@ -201,7 +210,7 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
       }
       frag[y + AHEAD] = y + AHEAD < STEPS ? read(from, x, y + AHEAD) : read(from, x ^ 1, y + AHEAD - STEPS);
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
+      for (int a = 0; a < A; ++a) {
         if (y < NS) {
           const f32x16 zero = {};
           next[a] = mfma32<DT>(frag[y], qf[a][y], y == 0 ? zero : next[a]);
@@ -219,8 +228,8 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
         else issue_values(fill);
       }
 #pragma unroll
-      for (int z = 0; z < 16; ++z) {  // pairs of scores
-        if (z * STEPS / 16 != y) continue;
+      for (int z = 0; z < 8 * A; ++z) {  // pairs of scores
+        if (z * STEPS / (8 * A) != y) continue;
         const int a = z / 8, v = z % 8 * 2;
         const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[a][v], c2, ref[a]));
         const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[a][v + 1], c2, ref[a]));
@@ -230,9 +239,9 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (__any(!(sum[0] < kMostSum && sum[1] < kMostSum))) {
+    if (__any(!(sum[0] < kMostSum && sum[A - 1] < kMostSum))) {
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
+      for (int a = 0; a < A; ++a) {
         float m = cur[a][0];
 #pragma unroll
         for (int v = 1; v < 16; ++v) m = fmaxf(m, cur[a][v]);
@@ -261,7 +270,7 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
 #pragma unroll
     for (int y = 0; y < AHEAD; ++y) frag[y] = frag[STEPS + y];
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < A; ++a) {
       total[a] += sum[a];
       pf[a][0] = w[a][0];
       pf[a][1] = w[a][1];
@@ -276,14 +285,14 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
     for (int part = 0; part < 4; ++part) issue(x - 1, x * L::STAGE, part);
   }
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int a = 0; a < A; ++a)
 #pragma unroll
     for (int v = 0; v < 16; ++v) s[0][a][v] = 0.0f;
 #pragma unroll
   for (int st = 0; st < NS; ++st) {
     const u32x4 k = read(0, 1, st);
 #pragma unroll
-    for (int a = 0; a < 2; ++a) s[0][a] = mfma32<DT>(k, qf[a][st], s[0][a]);
+    for (int a = 0; a < A; ++a) s[0][a] = mfma32<DT>(k, qf[a][st], s[0][a]);
   }
   uint32_t stage = L::STAGE, fill = 0;  // read, and left by every wave
   wait_loads_barrier<LOADS*(L::STAGES - 2)>();
@@ -302,13 +311,13 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
   for (int y = NS; y < STEPS; ++y) {
     const u32x4 v = read(stage, 0, y);
 #pragma unroll
-    for (int a = 0; a < 2; ++a) o[a][(y - NS) % ND] = mfma32<DT>(v, pf[a][(y - NS) / ND], o[a][(y - NS) % ND]);
+    for (int a = 0; a < A; ++a) o[a][(y - NS) % ND] = mfma32<DT>(v, pf[a][(y - NS) / ND], o[a][(y - NS) % ND]);
   }
   wait_loads_barrier<0>();
 
   // ---- the rows' results
 #pragma unroll
-  for (int a = 0; a < 2; ++a) {
+  for (int a = 0; a < A; ++a) {
     total[a] = valid[a] ? xor32_sum(total[a]) : 0.0f;
     const float inv = total[a] == 0.0f ? 0.0f : 1.0f / total[a];
     const float lse = total[a] == 0.0f ? -INFINITY : __builtin_amdgcn_logf(total[a]) - ref[a];
@@ -347,7 +356,7 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
     if (p.lse && half == 0 && i[a] < p.lq) p.lse[((int64_t)b * p.heads + h[a]) * p.lq + i[a]] = lse * kLn2;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     constexpr int CPR = ND * 4;  // chunks a row
-    const int first = r0 + wave * 64 + 32 * a;
+    const int first = r0 + wave * 32 * A + 32 * a;
 #pragma unroll 4
     for (int x = lane; x < 32 * CPR; x += 64) {
       const int row = x / CPR, c = x % CPR;

@@ -1099,11 +1099,11 @@ template <int DT, int KG> const void* tile_kernel(int nd) {
 // Rows a workgroup (256 / key_groups) and splits of the keys, from the sizes alone:
 // splits while CUs are idle and a wave keeps 4 tiles.
 AttnPlan plan_attention(const AttnParams& p, int cu_count) {
-  AttnPlan plan{1, 1, AttnPlan::TILE};
+  AttnPlan plan{1, 1, AttnPlan::TILE, cu_count};
   if (p.full && p.lk) {
     double us;
-    if (const int splits = plan_few_rows(p, cu_count)) return AttnPlan{1, splits, AttnPlan::FEW};
-    if (const int splits = plan_attention_rows(p, cu_count, &us)) return AttnPlan{1, splits, AttnPlan::ROWS};
+    if (const int splits = plan_few_rows(p, cu_count)) return AttnPlan{1, splits, AttnPlan::FEW, cu_count};
+    if (const int splits = plan_attention_rows(p, cu_count, &us)) return AttnPlan{1, splits, AttnPlan::ROWS, cu_count};
   }
   const int64_t rows = (int64_t)p.lq * p.group, seqs = (int64_t)p.batch * p.kv_heads;
   if (seqs * ((rows + 255) / 256) < cu_count) plan.key_groups = 2;
@@ -1121,7 +1121,7 @@ int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan) {
 
 hipError_t launch_attention(const AttnParams& params, const AttnPlan& plan, int dt, hipStream_t stream) {
   if (plan.kernel == AttnPlan::FEW) return launch_few_rows(params, plan.splits, dt, stream);
-  if (plan.kernel == AttnPlan::ROWS) return launch_attention_rows(params, plan.splits, dt, stream);
+  if (plan.kernel == AttnPlan::ROWS) return launch_attention_rows(params, plan.splits, plan.cu_count, dt, stream);
   AttnParams p = params;
   const int64_t rows = (int64_t)p.lq * p.group;
   const bool joined = p.slots;  // by the caller, with the results of other launches
