@@ -25,7 +25,14 @@ __global__ void __launch_bounds__(waves(A) * 64, A == 1 || ND <= 2 ? 2 : 1) atte
 }
 
 template <int DT, bool PREFIX> const void* kernel_for(int nd, int a) {
-  if (a == 1) return nd == 3 ? (const void*)&attention_rows_kernel<DT, 3, PREFIX, 1> : (const void*)&attention_rows_kernel<DT, 4, PREFIX, 1>;
+  if (a == 1) {
+    switch (nd) {
+      case 1: return (const void*)&attention_rows_kernel<DT, 1, PREFIX, 1>;
+      case 2: return (const void*)&attention_rows_kernel<DT, 2, PREFIX, 1>;
+      case 3: return (const void*)&attention_rows_kernel<DT, 3, PREFIX, 1>;
+    }
+    return (const void*)&attention_rows_kernel<DT, 4, PREFIX, 1>;
+  }
   switch (nd) {
     case 1: return (const void*)&attention_rows_kernel<DT, 1, PREFIX, 2>;
     case 2: return (const void*)&attention_rows_kernel<DT, 2, PREFIX, 2>;
@@ -63,7 +70,7 @@ hipError_t launch_attention_rows(const AttnParams& params, int splits, int cu_co
   p.row_blocks = (int)(((int64_t)p.lq * p.group + kRows - 1) / kRows);
   const int nd = (p.dim + 31) / 32;
   const int64_t grid = (int64_t)p.batch * p.kv_heads * p.row_blocks * splits;
-  const int a = nd >= 3 && grid <= cu_count ? 1 : 2;
+  const int a = grid <= cu_count ? 1 : 2;
   const void* fn = p.prefix ? (dt == DT_F16 ? kernel_for<DT_F16, true>(nd, a) : kernel_for<DT_BF16, true>(nd, a))
                             : (dt == DT_F16 ? kernel_for<DT_F16, false>(nd, a) : kernel_for<DT_BF16, false>(nd, a));
   void* args[] = {&p};

@@ -26,10 +26,9 @@ template <int ND, int A> struct RowsLds {
   static_assert(TOTAL <= 160 * 1024, "LDS");
 };
 
-// Loads of two units, by all waves, of which each loads part of both.
-template <int RB, int NW> struct UnitLoader {
-  static constexpr int NB = kUnit * RB / 1024 / NW;
-  static_assert(NB * 1024 * NW == kUnit * RB, "blocks over waves");
+// Loads of two units by four waves, of which each loads part of both.
+template <int RB> struct UnitLoader {
+  static constexpr int NB = kUnit * RB / 1024 / 4;
   const uint8_t* base;
   uint32_t stride;  // bytes
   uint32_t off[2 * NB];
@@ -70,7 +69,7 @@ template <int DT, int ND, bool PREFIX, int A>
 __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32_t id) {
   using L = RowsLds<ND, A>;
   constexpr int RB = L::RB, NS = 2 * ND;
-  using Loader = UnitLoader<RB, waves(A)>;
+  using Loader = UnitLoader<RB>;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = (int)(id % p.splits);
@@ -112,43 +111,46 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
   const int n0 = (int)((int64_t)all * split / p.splits), n1 = (int)((int64_t)all * (split + 1) / p.splits);
   const int steps = (n1 - n0 + 1) / 2, plain = max(0, min(whole, n1) - n0) / 2;
 
-  Loader own_k, own_v, pre_k, pre_v;
-  own_k.init(p.k + 2 * (b * p.k_stride[0] + hk * p.k_stride[2]), 2 * p.k_stride[1], p.dim, wave, lane);
-  own_v.init(p.v + 2 * (b * p.v_stride[0] + hk * p.v_stride[2]), 2 * p.v_stride[1], p.dim, wave, lane);
-  if constexpr (PREFIX) {
-    pre_k.init(p.kp + 2 * hk * p.kp_stride[1], 2 * p.kp_stride[0], p.dim, wave, lane);
-    pre_v.init(p.vp + 2 * hk * p.vp_stride[1], 2 * p.vp_stride[0], p.dim, wave, lane);
-  }
-  constexpr int LOADS = 4 * Loader::NB;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem + (uint32_t)(wave * Loader::NB * 1024);
+  // Of eight waves the first four load keys, the others values; four load both.
+  constexpr int TENSORS = A == 2 ? 2 : 1, LOADS = TENSORS * 2 * Loader::NB;
+  const int loader = wave & 3, other = A == 2 ? 0 : wave >> 2;  // other: 1 for values
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem + (uint32_t)(loader * Loader::NB * 1024);
   const uint32_t dim_bytes = (uint32_t)p.dim * 2u;
+  Loader own[TENSORS], pre[TENSORS];
+#pragma unroll
+  for (int y = 0; y < TENSORS; ++y) {
+    const bool values = y + other;
+    own[y].init(values ? p.v + 2 * (b * p.v_stride[0] + hk * p.v_stride[2]) : p.k + 2 * (b * p.k_stride[0] + hk * p.k_stride[2]),
+                2 * (values ? p.v_stride[1] : p.k_stride[1]), p.dim, loader, lane);
+    if constexpr (PREFIX)
+      pre[y].init(values ? p.vp + 2 * hk * p.vp_stride[1] : p.kp + 2 * hk * p.kp_stride[1],
+                  2 * (values ? p.vp_stride[0] : p.kp_stride[0]), p.dim, loader, lane);
+  }
   auto load = [&](const Loader& of_own, const Loader& of_prefix, int n, uint32_t to) __attribute__((always_inline)) {
     const int g = n0 + n;
     const bool in = n >= 0 && g < n1;
     if (PREFIX && g < prefix_units) of_prefix.issue(to, in ? g * kUnit : 0, in ? min(kUnit, prefix - g * kUnit) : 0, dim_bytes);
     else of_own.issue(to, in ? (g - prefix_units) * kUnit : 0, in ? min(kUnit, end - (g - prefix_units) * kUnit) : 0, dim_bytes);
   };
-  // stage s: keys of units 2 s + 1 and 2 s + 2, values of units 2 s - 1 and 2 s, in four parts
+  // stage s: keys of units 2 s + 1 and 2 s + 2, values of units 2 s - 1 and 2 s, in parts of one
   auto issue = [&](int s, uint32_t at, int part) __attribute__((always_inline)) {
-    const int x = part & 1;
-    if (part < 2) load(own_k, pre_k, 2 * s + 1 + x, lds0 + at + x * L::HALF);
-    else load(own_v, pre_v, 2 * s - 1 + x, lds0 + at + (2 + x) * L::HALF);
+    const int x = part & 1, y = part >> 1, values = y + other;
+    if (y < TENSORS) load(own[y], pre[y], 2 * s + 1 - 2 * values + x, lds0 + at + (2 * values + x) * L::HALF);
   };
   auto after = [&](uint32_t at) { return at + L::STAGE == L::RING ? 0u : at + L::STAGE; };
-  // The same in two parts from stage STAGES - 1 on, one after another, where there is one
+  // The same in parts of two from stage STAGES - 1 on, one after another, where there is one
   // kind of keys: pointers go on by 64 rows, and the rows that are left count down.
   const int first = L::STAGES - 1, limit = min(end, n1 * kUnit);
-  const uint8_t* next_k = own_k.base + (uint64_t)(uint32_t)((n0 + 2 * first + 1) * kUnit) * own_k.stride;
-  const uint8_t* next_v = own_v.base + (uint64_t)(uint32_t)((n0 + 2 * first - 1) * kUnit) * own_v.stride;
-  int left = limit - (n0 + 2 * first + 1) * kUnit;
-  auto issue_keys = [&](uint32_t at) __attribute__((always_inline)) {
-    own_k.issue2(lds0 + at, next_k, left, dim_bytes);
-    next_k += (uint64_t)(2 * kUnit) * own_k.stride;
-  };
-  auto issue_values = [&](uint32_t at) __attribute__((always_inline)) {
-    own_v.issue2(lds0 + at + 2 * L::HALF, next_v, left + 2 * kUnit, dim_bytes);
-    next_v += (uint64_t)(2 * kUnit) * own_v.stride;
-    left -= 2 * kUnit;
+  const uint8_t* next_rows[TENSORS];
+#pragma unroll
+  for (int y = 0; y < TENSORS; ++y)
+    next_rows[y] = own[y].base + (uint64_t)(uint32_t)((n0 + 2 * first + 1 - 2 * (y + other)) * kUnit) * own[y].stride;
+  int left = limit - (n0 + 2 * first + 1) * kUnit;  // of the keys
+  auto issue_pair = [&](uint32_t at, int y) __attribute__((always_inline)) {
+    const int values = y + other;
+    own[y].issue2(lds0 + at + 2 * values * L::HALF, next_rows[y], left + 2 * values * kUnit, dim_bytes);
+    next_rows[y] += (uint64_t)(2 * kUnit) * own[y].stride;
+    if (y == TENSORS - 1) left -= 2 * kUnit;
   };
 
   f32x16 o[A][ND], s[2][A];  // s: of two units in turn
@@ -223,9 +225,8 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
       if constexpr (PREFIX) {
         if (STEPS > AHEAD + 2 ? y == 1 : y == 0) issue(t + L::STAGES - 1, fill, x);
         if (STEPS > AHEAD + 2 ? y == 2 : y == 0) issue(t + L::STAGES - 1, fill, 2 + x);
-      } else if (y == 0) {
-        if (x == 0) issue_keys(fill);
-        else issue_values(fill);
+      } else if (y == 0 && x < TENSORS) {
+        issue_pair(fill, x);
       }
 #pragma unroll
       for (int z = 0; z < 8 * A; ++z) {  // pairs of scores
