@@ -809,9 +809,10 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
   for (int q = 0; q < NB; ++q) {
     const int row = (int)block_row<RB>(wave * NB + q, lane);
     const uint32_t c = block_chunk<RB>(wave * NB + q, lane) * 16u;
-    at_row[q] = c < (uint32_t)p.dim * 2u ? (uint32_t)(row / hg | row % hg << 16) : 0xFFFFu;
-    q_off[q] = (uint32_t)(2 * (row / hg * p.q_stride[1] + row % hg * p.q_stride[2])) + c;
-    g_off[q] = (uint32_t)(2 * (row / hg * p.do_stride[1] + row % hg * p.do_stride[2])) + c;
+    const bool in = c < (uint32_t)p.dim * 2u && row < tp * hg;
+    at_row[q] = (uint32_t)(row / hg | row % hg << 16);
+    q_off[q] = in ? (uint32_t)(2 * (row / hg * p.q_stride[1] + row % hg * p.q_stride[2])) + c : kOutOfRange;
+    g_off[q] = in ? (uint32_t)(2 * (row / hg * p.do_stride[1] + row % hg * p.do_stride[2])) + c : kOutOfRange;
   }
   const int64_t st_row = stats_row(p, b, hk, 0);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
@@ -833,46 +834,69 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
     for (int v = 0; v < 16; ++v) dk[d][v] = dv[d][v] = 0.0f;
   DsRange<DT> range{DT == DT_F16 ? 60 : 0};  // (2^14 P (dP - D) is below 2^56 for f16 inputs)
 
+  // The next tile to load: positions from i, heads of part hc.
+  struct {
+    const uint8_t *q, *g;
+    int64_t row;
+    int i, hc;
+  } next = {q_base + 2 * i0 * p.q_stride[1], g_base + 2 * i0 * p.do_stride[1], st_row + (int64_t)i0 * p.group, i0, 0};
+  const int64_t q_part = 2 * hg * p.q_stride[2], q_step = 2 * tp * p.q_stride[1] - (chunks - 1) * q_part;
+  const int64_t g_part = 2 * hg * p.do_stride[2], g_step = 2 * tp * p.do_stride[1] - (chunks - 1) * g_part;
+  const int row_step = tp * p.group - (chunks - 1) * hg;
   auto issue = [&](int t) {
-    const int step = t / chunks, hc = t - step * chunks, i = i0 + step * tp;
-    const int npos = t < t_all ? min(tp, i1 - i) : 0, nhead = p.group - hc * hg;
+    const int npos = t < t_all ? min(tp, i1 - next.i) : 0, nhead = p.group - next.hc * hg;
     const uint32_t st = lds0 + (uint32_t)t % L::STAGES * L::STAGE + (uint32_t)(wave * NB * 1024);
     // what is in range is said by the offsets alone
-    const i32x4 rq = raw_rsrc(q_base + 2 * (i * p.q_stride[1] + hc * hg * p.q_stride[2]), 0x7FFFFFFFu);
-    const i32x4 rg = raw_rsrc(g_base + 2 * (i * p.do_stride[1] + hc * hg * p.do_stride[2]), 0x7FFFFFFFu);
+    const i32x4 rq = raw_rsrc(next.q, 0x7FFFFFFFu), rg = raw_rsrc(next.g, 0x7FFFFFFFu);
+    if (npos == tp && nhead >= hg) {
 #pragma unroll
-    for (int q = 0; q < NB; ++q) {
-      const bool in = (int)(at_row[q] & 0xFFFFu) < npos && (int)(at_row[q] >> 16) < nhead;
-      dma16(rq, in ? q_off[q] : kOutOfRange, st + q * 1024);
-      dma16(rg, in ? g_off[q] : kOutOfRange, st + L::TILE + q * 1024);
+      for (int q = 0; q < NB; ++q) {
+        dma16(rq, q_off[q], st + q * 1024);
+        dma16(rg, g_off[q], st + L::TILE + q * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < NB; ++q) {
+        const bool in = (int)(at_row[q] & 0xFFFFu) < npos && (int)(at_row[q] >> 16) < nhead;
+        dma16(rq, in ? q_off[q] : kOutOfRange, st + q * 1024);
+        dma16(rg, in ? g_off[q] : kOutOfRange, st + L::TILE + q * 1024);
+      }
     }
     if (wave == 0) {  // the rows' lse and D: contiguous
       const int rows = min(npos * hg, hg == p.group ? kQueries : nhead);
-      const int64_t row = st_row + (int64_t)i * p.group + hc * hg;
       const uint32_t bytes = rows > 0 ? (uint32_t)rows * 4u : 0u, at = lds0 + (uint32_t)t % L::STAGES * L::STAGE + L::STATS;
-      dma16(raw_rsrc(p.row_lse + row, bytes), lane * 16, at);
-      dma16(raw_rsrc(p.row_delta + row, bytes), lane * 16, at + 1024);
+      dma16(raw_rsrc(p.row_lse + next.row, bytes), lane * 16, at);
+      dma16(raw_rsrc(p.row_delta + next.row, bytes), lane * 16, at + 1024);
     }
+    const bool last = next.hc + 1 == chunks;
+    next.q += last ? q_step : q_part;
+    next.g += last ? g_step : g_part;
+    next.row += last ? row_step : hg;
+    next.i += last ? tp : 0;
+    next.hc = last ? 0 : next.hc + 1;
   };
 #pragma unroll
   for (int t = 0; t < L::STAGES - 1; ++t) issue(t);
   landed(kf);
   landed(vf);
   const uint32_t r_at = row_addr<RB>(lane) + (uint32_t)row0 * RB, c_at = col_addr<RB>(lane) + (uint32_t)row0 * RB;
-  for (int t = 0; t < t_all; ++t) {
+  int i = i0, hc = 0;  // the tile's
+  for (int t = 0; t < t_all; ++t, hc = hc + 1 == chunks ? 0 : hc + 1, i += hc ? 0 : tp) {
     // tile t landed; every wave is done with tile t - 1 (wave 0 has two more loads a tile)
     if (wave == 0) wait_loads_barrier<(2 * NB + 2) * (L::STAGES - 2)>();
     else wait_loads_barrier<2 * NB * (L::STAGES - 2)>();
     issue(t + L::STAGES - 1);
-    const int step = t / chunks, hc = t - step * chunks, i = i0 + step * tp;
     const uint32_t stage = (uint32_t)t % L::STAGES * L::STAGE;
     const uint8_t* stt = smem + stage + L::STATS;
     // tile row x is a query that sees this lane's key if t_lo <= x < t_hi
     const int rows = min(min(tp, i1 - i) * hg, hg == p.group ? kQueries : p.group - hc * hg);
-    const int64_t back = (int64_t)j - shift - i;
-    const int t_lo = (int)min((int64_t)1 << 20, max((int64_t)0, back)) * hg;
-    const int64_t reach = j < p.sinks ? 1 << 20 : max((int64_t)0, min((int64_t)1 << 20, back + p.window)) * hg;
-    const int t_hi = valid ? (int)min((int64_t)rows, reach) : 0;
+    int t_lo = 0, t_hi = valid ? rows : 0;
+    if (!p.full) {
+      const int64_t back = (int64_t)j - shift - i;
+      t_lo = (int)min((int64_t)1 << 20, max((int64_t)0, back)) * hg;
+      const int64_t reach = j < p.sinks ? 1 << 20 : max((int64_t)0, min((int64_t)1 << 20, back + p.window)) * hg;
+      t_hi = valid ? (int)min((int64_t)rows, reach) : 0;
+    }
     const bool all = __all(t_lo <= row0 && t_hi >= row0 + 32);
     if (!all && !__any(max(t_lo, row0) < min(t_hi, row0 + 32))) continue;
     uint32_t ra = r_at + stage, ca = c_at + stage;
