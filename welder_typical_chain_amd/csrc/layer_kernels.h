@@ -65,6 +65,7 @@ hipError_t launch_prefix_token(const AttnParams& common, const AttnParams& own, 
 hipError_t launch_attention_join(const AttnParams& p, int dt, hipStream_t stream);
 struct AttnBackwardPlan {
   int dq_groups;  // waves that share a query row
+  bool together;  // dq and dk / dv in one launch
   int key_blocks, near_blocks, near_chunks, far_blocks, far_chunks, far_keys;
   int64_t part_at, far_at, workspace;  // bytes
 };

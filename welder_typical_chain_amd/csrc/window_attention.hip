@@ -471,16 +471,15 @@ template <int ND, int KG> struct DqLds {
   static constexpr int TOTAL = RING > OUT ? RING : OUT;
   static_assert(TOTAL <= 160 * 1024, "LDS");
 };
-template <int DT, int ND, int KG>
-__global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnParams p) {
+// STATS: the rows' statistics for dk / dv are written (otherwise attention_stats_kernel did).
+template <int DT, int ND, int KG, bool STATS>
+__device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t id) {
   using L = DqLds<ND, KG>;
   constexpr int NW = 4;
   constexpr int RB = L::RB, NS = 2 * ND;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = wave_id % 4, group = wave_id / 4;  // rows, tiles
-  const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
   const int blk = p.row_blocks - 1 - (int)(id % p.row_blocks);
   const int hk = (int)(id / p.row_blocks % p.kv_heads), b = (int)(id / p.row_blocks / p.kv_heads);
   const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = first_position(p, nq, nk);
@@ -621,7 +620,7 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
     }
     delta = delta != delta ? delta : sum;  // (a NaN value that is seen, be its weight 0, is in out)
   }
-  if (half == 0 && group == 0 && i < p.lq) {
+  if (STATS && half == 0 && group == 0 && i < p.lq) {
     p.row_lse[stats_row(p, b, hk, i) + x_head] = lse2 - kWeightBits<DT>;
     p.row_delta[stats_row(p, b, hk, i) + x_head] = -delta;
   }
@@ -715,6 +714,11 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
     redo &= redo - 1;
   }
 }
+template <int DT, int ND, int KG>
+__global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnParams p) {
+  __shared__ __attribute__((aligned(256))) uint8_t smem[DqLds<ND, KG>::TOTAL];
+  attention_dq<DT, ND, KG, true>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
+}
 
 // A workgroup takes kDkvKeys keys of one (sequence, key head) and streams the
 // queries that see them in tiles of 64 packed rows: whole positions of up to 64
@@ -767,15 +771,13 @@ __device__ inline float* far_part(const AttnParams& p, int b, int hk, int kb, in
 }
 
 template <int DT, int ND>
-__global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const AttnParams p) {
+__device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_t id) {
   using L = DkvLds<ND>;
   constexpr int RB = L::RB, NS = 2 * ND, NB = kQueries * RB / 1024 / kDkvWaves;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[L::TOTAL];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // workgroups of a (sequence, key head): the key blocks' near chunks, then the far ones
   const int near = p.key_blocks * p.near_chunks, per = near + p.far_blocks * p.far_chunks;
-  const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
   const int w = (int)(id % per), hk = (int)(id / per % p.kv_heads), b = (int)(id / per / p.kv_heads);
   const bool far = w >= near;
   const int parts_of = far ? p.far_chunks : p.near_chunks;
@@ -1053,6 +1055,48 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const 
     redo &= redo - 1;
   }
 }
+template <int DT, int ND>
+__global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const AttnParams p) {
+  __shared__ __attribute__((aligned(256))) uint8_t smem[DkvLds<ND>::TOTAL];
+  attention_dkv<DT, ND>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
+}
+
+// Both at once, where their workgroups together leave each a CU of its own: the rows'
+// statistics come from a kernel before (3 x 333 on 1000 states, 6 / 3 heads of 80 in f16:
+// 28 us and 21 one after the other, TOGETHER at once).
+template <int DT, int ND>
+__global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_gradients_kernel(const AttnParams p, int dq_blocks) {
+  static_assert(kDkvWaves * 64 == 2 * 256, "threads of attention_dq with KG 2");
+  constexpr int MOST = DqLds<ND, 2>::TOTAL > DkvLds<ND>::TOTAL ? DqLds<ND, 2>::TOTAL : DkvLds<ND>::TOTAL;
+  __shared__ __attribute__((aligned(256))) uint8_t smem[MOST];
+  if ((int)blockIdx.x < dq_blocks) attention_dq<DT, ND, 2, false>(p, smem, blockIdx.x);
+  else attention_dkv<DT, ND>(p, smem, blockIdx.x - (uint32_t)dq_blocks);
+}
+// lse in the log2 domain and -D = -sum of dout out of the rows: 16 lanes a row.
+template <int DT>
+__global__ void __launch_bounds__(256) attention_stats_kernel(const AttnParams p) {
+  const int64_t rows = (int64_t)p.batch * p.heads * p.lq, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int c = (threadIdx.x & 15) * 8;
+  const int64_t at = min(row, rows - 1);
+  const int h = (int)(at % p.heads), i = (int)(at / p.heads % p.lq), b = (int)(at / p.heads / p.lq);
+  const bool valid = i < seq_queries(p, b);
+  float delta = 0.0f;
+  if (valid && c < p.dim) {
+    using V = typename Elem<DT>::vec8;
+    const V g = *reinterpret_cast<const V*>(p.dout + 2 * (b * p.do_stride[0] + (int64_t)i * p.do_stride[1] + h * p.do_stride[2] + c));
+    const V o = *reinterpret_cast<const V*>(p.o + 2 * (b * p.o_stride[0] + (int64_t)i * p.o_stride[1] + h * p.o_stride[2] + c));
+#pragma unroll
+    for (int v = 0; v < 8; ++v) delta = __builtin_fmaf((float)g[v], (float)o[v], delta);
+  }
+#pragma unroll
+  for (int x = 8; x; x >>= 1) delta += __shfl_xor(delta, x);
+  if (row >= rows || c) return;
+  const float lse = valid ? p.lse_in[((int64_t)b * p.heads + h) * p.lq + i] : -INFINITY;
+  const int hk = h / p.group;
+  const int64_t to = stats_row(p, b, hk, i) + h - hk * p.group;
+  p.row_lse[to] = (lse == -INFINITY ? INFINITY : lse * kLog2e) - kWeightBits<DT>;
+  p.row_delta[to] = lse == -INFINITY ? 0.0f : -delta;
+}
 
 // dk and dv of the keys whose sums came in parts, the parts in order.  One wave a
 // key, four elements a lane.
@@ -1176,6 +1220,14 @@ template <int DT, int KG> const void* dq_kernel(int nd) {
   }
   return (const void*)&attention_dq_kernel<DT, 4, KG>;
 }
+template <int DT> const void* gradients_kernel(int nd) {
+  switch (nd) {
+    case 1: return (const void*)&attention_gradients_kernel<DT, 1>;
+    case 2: return (const void*)&attention_gradients_kernel<DT, 2>;
+    case 3: return (const void*)&attention_gradients_kernel<DT, 3>;
+  }
+  return (const void*)&attention_gradients_kernel<DT, 4>;
+}
 template <int DT> const void* dkv_kernel(int nd) {
   switch (nd) {
     case 1: return (const void*)&attention_dkv_kernel<DT, 1>;
@@ -1205,6 +1257,8 @@ AttnBackwardPlan plan_attention_backward(const AttnParams& p, int cu_count) {
   const int64_t tiles = std::min<int64_t>(p.lq, p.window + kDkvKeys) * p.group / kQueries;
   plan.near_chunks = 1;
   while (plan.near_chunks < 16 && seqs * plan.key_blocks * plan.near_chunks * 2 <= cu_count && tiles / (2 * plan.near_chunks) >= 4) plan.near_chunks *= 2;
+  // (blocks of at most two key tiles sum D themselves, and hand it on)
+  plan.together = p.full && p.lq && p.lk > 2 * kKeys && seqs * (row_blocks + (int64_t)plan.key_blocks * plan.near_chunks) <= cu_count;
   plan.near_blocks = plan.near_chunks > 1 ? plan.key_blocks : plan.far_blocks;
   const int64_t rows = (int64_t)p.batch * p.lq * p.heads;
   plan.part_at = (rows * 8 + 255) / 256 * 256;
@@ -1226,6 +1280,17 @@ hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwar
   p.far_chunks = plan.far_chunks;
   const int nd = (p.dim + 31) / 32;
   const int64_t seqs = (int64_t)p.batch * p.kv_heads;
+  if (plan.together) {
+    p.row_blocks = (int)(((int64_t)p.lq * p.group + kDqRows - 1) / kDqRows);
+    hipError_t e = launch(WTC_BY_TYPE(attention_stats_kernel, dt), ((int64_t)p.batch * p.lq * p.heads + 15) / 16, 256, p, stream);
+    if (e != hipSuccess) return e;
+    int dq_blocks = (int)(seqs * p.row_blocks);
+    void* args[] = {&p, &dq_blocks};
+    e = hipLaunchKernel(dt == DT_F16 ? gradients_kernel<DT_F16>(nd) : gradients_kernel<DT_BF16>(nd),
+                        dim3((unsigned)(dq_blocks + seqs * p.key_blocks * p.near_chunks)), dim3(kDkvWaves * 64), args, 0, stream);
+    if (e != hipSuccess || p.near_chunks == 1) return e;
+    return launch(WTC_BY_TYPE(attention_sum_kernel, dt), (seqs * p.lk + 3) / 4, 256, p, stream);
+  }
   if (p.lq) {
     p.row_blocks = (int)(((int64_t)p.lq * p.group + kDqRows - 1) / kDqRows);
     const bool pairs = plan.dq_groups == 2;
