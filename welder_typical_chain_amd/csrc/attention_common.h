@@ -36,24 +36,24 @@ template <int RB, int ROWS, int NW> struct TileLoader {
   static constexpr int NB = BLOCKS / NW;
   static_assert(NB * NW == BLOCKS, "blocks over waves");
   const uint8_t* base;  // row 0 of the (sequence, head)
-  int64_t stride;       // bytes
+  uint32_t stride;      // bytes
   uint32_t dim_bytes;
   uint32_t off[NB];
   uint32_t lds;
   __device__ inline void init(const uint8_t* base_, int64_t stride_bytes, int dim, int wave, int lane) {
     base = base_;
-    stride = stride_bytes;
+    stride = (uint32_t)stride_bytes;
     dim_bytes = (uint32_t)dim * 2u;
     lds = (uint32_t)(wave * NB * 1024);
 #pragma unroll
     for (int q = 0; q < NB; ++q) {
       const uint32_t c = block_chunk<RB>(wave * NB + q, lane) * 16u;
-      off[q] = c < dim_bytes ? block_row<RB>(wave * NB + q, lane) * (uint32_t)stride + c : kOutOfRange;
+      off[q] = c < dim_bytes ? block_row<RB>(wave * NB + q, lane) * stride + c : kOutOfRange;
     }
   }
   // rows row0 .. row0 + rows - 1 (rows <= ROWS; none: zeros)
   __device__ inline void issue(uint32_t stage, int row0, int rows) const {
-    const i32x4 r = raw_rsrc(base + (rows > 0 ? (int64_t)row0 * stride : 0), rows > 0 ? (uint32_t)(rows - 1) * (uint32_t)stride + dim_bytes : 0u);
+    const i32x4 r = raw_rsrc(base + (uint64_t)(uint32_t)max(rows > 0 ? row0 : 0, 0) * stride, rows > 0 ? (uint32_t)(rows - 1) * stride + dim_bytes : 0u);
 #pragma unroll
     for (int q = 0; q < NB; ++q) dma16(r, off[q], stage + lds + q * 1024);
   }
