@@ -87,11 +87,11 @@ namespace {
 
 template <int DT, int ND, bool MANY>
 __global__ void __launch_bounds__(256, 1) prefix_token_kernel(const AttnParams common, const AttnParams own, int common_blocks) {
-  constexpr int MOST = decode::DecodeLds<ND>::TOTAL > RowsLds<ND, 2>::TOTAL ? decode::DecodeLds<ND>::TOTAL : RowsLds<ND, 2>::TOTAL;
+  constexpr int MOST = decode::DecodeLds<ND, 1>::TOTAL > RowsLds<ND, 2>::TOTAL ? decode::DecodeLds<ND, 1>::TOTAL : RowsLds<ND, 2>::TOTAL;
   __shared__ __attribute__((aligned(256))) uint8_t smem[MOST];
-  if ((int)blockIdx.x >= common_blocks) decode::decode_tile<DT, ND, false, false>(own, smem, (int)blockIdx.x - common_blocks);
+  if ((int)blockIdx.x >= common_blocks) decode::decode_tile<DT, ND, false, false, 1>(own, smem, (int)blockIdx.x - common_blocks);
   else if constexpr (MANY) attention_rows<DT, ND, false, 2>(common, smem, xcd_remap(blockIdx.x, (uint32_t)common_blocks));
-  else decode::decode_tile<DT, ND, false, true>(common, smem, (int)blockIdx.x);
+  else decode::decode_tile<DT, ND, false, true, 1>(common, smem, (int)blockIdx.x);
 }
 template <int DT, bool MANY> const void* token_kernel_for(int nd) {
   switch (nd) {

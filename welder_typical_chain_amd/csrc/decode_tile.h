@@ -12,15 +12,16 @@ constexpr int kRows = 32;   // cache rows a tile
 constexpr int kWaves = 4;
 constexpr int kHeads = 32;  // query heads a workgroup
 
-template <int ND> struct DecodeLds {
+// GROUPS: workgroups a CU.
+template <int ND, int GROUPS> struct DecodeLds {
   static constexpr int RB = row_bytes(ND);
   static constexpr int TILE = kRows * RB, STAGE = 2 * TILE;
-  static constexpr int STAGES = RB == 256 ? 2 : 4;  // 128 KiB over the waves
+  static constexpr int STAGES = (RB == 256 ? 2 : 4) / GROUPS;  // 128 KiB a CU
   static constexpr int RING = kWaves * STAGES * STAGE;
   static constexpr int PITCH = ND * 32 + 4;          // floats of a head's result
   static constexpr int JOIN = kWaves * kHeads * PITCH * 4;
   static constexpr int TOTAL = (RING > JOIN ? RING : JOIN) + kWaves * kHeads * 8;
-  static_assert(TOTAL <= 160 * 1024, "LDS");
+  static_assert(TOTAL * GROUPS <= 160 * 1024, "LDS");
 };
 
 // The visible rows of a sequence's cache as tiles.
@@ -61,9 +62,9 @@ __host__ __device__ inline int most_tiles(int lk) { return (lk + kRows - 1) / kR
 // ROWS: the rows are those of p.lq queries, each of which sees every key, instead of one
 // query's heads; a batch's queries may be one sequence's (p.seq_rows).
 // SCORES: the scores go to p.scores as well, in the log2 domain, [batch][heads][most_tiles][kRows].
-template <int DT, int ND, bool SCORES, bool ROWS>
+template <int DT, int ND, bool SCORES, bool ROWS, int GROUPS>
 __device__ inline void decode_tile(const AttnParams& p, uint8_t* smem, int id) {
-  using L = DecodeLds<ND>;
+  using L = DecodeLds<ND, GROUPS>;
   constexpr int RB = L::RB, NS = 2 * ND;
   using T = typename Elem<DT>::type;
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -102,30 +103,38 @@ __device__ inline void decode_tile(const AttnParams& p, uint8_t* smem, int id) {
   TileLoader<RB, kRows, 1> lk, lv;
   lk.init(p.k + 2 * (b * p.k_stride[0] + hk * p.k_stride[2]), 2 * p.k_stride[1], p.dim, 0, lane);
   lv.init(p.v + 2 * (b * p.v_stride[0] + hk * p.v_stride[2]), 2 * p.v_stride[1], p.dim, 0, lane);
-  constexpr int LOADS = 2 * TileLoader<RB, kRows, 1>::NB;
+  // The loads, stores too, count in their order: those that may be in flight when a tile's keys,
+  // or its values, have landed (of each tensor STAGES tiles are under way, and from the
+  // second tile on the scores of the one before).
+  constexpr int BEHIND = TileLoader<RB, kRows, 1>::NB * (2 * L::STAGES - 1), STORES = SCORES ? 4 : 0;
+  auto wait = [](bool first) __attribute__((always_inline)) {
+    if (first) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(BEHIND) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" : : "n"(BEHIND + STORES) : "memory");
+  };
   uint8_t* ring = smem + wave * L::STAGES * L::STAGE;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)ring;
-  auto issue = [&](int x) {  // this wave's x-th tile
+  auto issue = [&](auto& of, int x, int at) __attribute__((always_inline)) {  // this wave's x-th tile
     int row, rows;
     const int t = t0 + wave + x * kWaves;
     runs.tile(t, &row, &rows);
-    if (t >= t1) rows = 0;
-    const uint32_t st = lds0 + (uint32_t)x % L::STAGES * L::STAGE;
-    lk.issue(st, row, rows);
-    lv.issue(st + L::TILE, row, rows);
+    of.issue(lds0 + (uint32_t)x % L::STAGES * L::STAGE + at, row, t < t1 ? rows : 0);
   };
 #pragma unroll
-  for (int x = 0; x < L::STAGES; ++x) issue(x);
+  for (int x = 0; x < L::STAGES; ++x) {
+    issue(lk, x, 0);
+    issue(lv, x, L::TILE);
+  }
 
   landed(qf);
   for (int x = 0; t0 + wave + x * kWaves < t1; ++x) {
-    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS * (L::STAGES - 1)) : "memory");
     int row, rows;
     const int t = t0 + wave + x * kWaves;
     runs.tile(t, &row, &rows);
+    wait(x == 0);
     uint8_t* kt = ring + x % L::STAGES * L::STAGE;
     uint8_t* vt = kt + L::TILE;
     if (!ROWS && t == t_all - 1 && p.k_new && lane * 8 < p.dim) {  // the new token: over what the cache held in its row
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       const u32x4 kn = *reinterpret_cast<const u32x4*>(p.k_new + 2 * (b * p.kn_stride[0] + hk * p.kn_stride[1]) + lane * 16);
       const u32x4 vn = *reinterpret_cast<const u32x4*>(p.v_new + 2 * (b * p.vn_stride[0] + hk * p.vn_stride[1]) + lane * 16);
       *reinterpret_cast<u32x4*>(kt + tile_offset<RB>(rows - 1, lane)) = kn;
@@ -145,19 +154,13 @@ __device__ inline void decode_tile(const AttnParams& p, uint8_t* smem, int id) {
     for (int v = 0; v < 16; ++v) s[v] = 0.0f;
 #pragma unroll
     for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ka, 0, st), qf[st], s);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys are read: their place may be filled again
+    issue(lk, x + L::STAGES, 0);
     float m = -INFINITY;
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
       if (8 * (v >> 2) + (v & 3) + 4 * half >= rows) s[v] = -INFINITY;
       m = fmaxf(m, s[v]);
-    }
-    if constexpr (SCORES) {
-      if (hq < heads) {
-        float* dst = p.scores + (((int64_t)b * p.heads + h0 + hq) * most_tiles(p.lk) + t) * kRows + 4 * half;
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(dst + 8 * g) = f32x4{s[4 * g] * c2, s[4 * g + 1] * c2, s[4 * g + 2] * c2, s[4 * g + 3] * c2};
-      }
     }
     m = xor32_max(m) * c2;
     const float next = fmaxf(top, m);
@@ -186,12 +189,21 @@ __device__ inline void decode_tile(const AttnParams& p, uint8_t* smem, int id) {
       pf[g >> 1][2 * (g & 1) + 1] = w1;
     }
     total = __builtin_fmaf(total, keep, sum);
+    wait(x == 0);
 #pragma unroll
     for (int st = 0; st < 2; ++st)
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] = mfma32<DT>(col_frag<RB>(smem, va, 16 * st, d), pf[st], o[d]);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its stage may be filled again
-    issue(x + L::STAGES);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    issue(lv, x + L::STAGES, L::TILE);
+    if constexpr (SCORES) {
+      if (hq < heads) {
+        float* dst = p.scores + (((int64_t)b * p.heads + h0 + hq) * most_tiles(p.lk) + t) * kRows + 4 * half;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(dst + 8 * g) = f32x4{s[4 * g] * c2, s[4 * g + 1] * c2, s[4 * g + 2] * c2, s[4 * g + 3] * c2};
+      }
+    }
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();

@@ -27,15 +27,17 @@ using namespace attn;
 
 using namespace decode;
 
+constexpr int kGroups = 2;
+
 template <int DT, int ND, bool SCORES>
-__global__ void __launch_bounds__(kWaves * 64, 1) decode_kernel(const AttnParams p) {
-  __shared__ __attribute__((aligned(256))) uint8_t smem[DecodeLds<ND>::TOTAL];
-  decode_tile<DT, ND, SCORES, false>(p, smem, (int)blockIdx.x);
+__global__ void __launch_bounds__(kWaves * 64, kGroups) decode_kernel(const AttnParams p) {
+  __shared__ __attribute__((aligned(256))) uint8_t smem[DecodeLds<ND, kGroups>::TOTAL];
+  decode_tile<DT, ND, SCORES, false, kGroups>(p, smem, (int)blockIdx.x);
 }
 template <int DT, int ND>
-__global__ void __launch_bounds__(kWaves * 64, 1) few_rows_kernel(const AttnParams p) {
-  __shared__ __attribute__((aligned(256))) uint8_t smem[DecodeLds<ND>::TOTAL];
-  decode_tile<DT, ND, false, true>(p, smem, (int)blockIdx.x);
+__global__ void __launch_bounds__(kWaves * 64, kGroups) few_rows_kernel(const AttnParams p) {
+  __shared__ __attribute__((aligned(256))) uint8_t smem[DecodeLds<ND, kGroups>::TOTAL];
+  decode_tile<DT, ND, false, true, kGroups>(p, smem, (int)blockIdx.x);
 }
 
 // The splits of a head's row: half a wave a row.
