@@ -114,7 +114,7 @@ PrefixTokenPlan plan_prefix_token(const AttnParams& common, const AttnParams& ow
   const int64_t units = ((int64_t)common.lk + kUnit - 1) / kUnit;
   plan.common = common.lk ? 1 : 0;
   while (plan.common && plan.common < 64 && grid * plan.common * 2 <= cu_count / 4 && units / (2 * plan.common) >= 8) plan.common *= 2;
-  plan.own = plan_decode_joined(own, cu_count);
+  plan.own = plan_decode_joined(own, 2, cu_count);
   return plan;
 }
 

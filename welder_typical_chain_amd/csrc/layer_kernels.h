@@ -73,7 +73,7 @@ AttnBackwardPlan plan_attention_backward(const AttnParams& p, int cu_count);
 // p.row_lse: plan.workspace bytes
 hipError_t launch_attention_backward(const AttnParams& p, const AttnBackwardPlan& plan, int dt, hipStream_t stream);
 int plan_decode(const AttnParams& p, int cu_count);  // splits
-int plan_decode_joined(const AttnParams& p, int cu_count);  // the same where a second launch is there anyway
+int plan_decode_joined(const AttnParams& p, int rounds, int cu_count);  // the same where a second launch is there anyway
 int64_t decode_workspace(const AttnParams& p, int splits);
 // p.part_out: decode_workspace() bytes; p.window: at most p.lk - p.sinks
 hipError_t launch_attention_decode(const AttnParams& p, int splits, int dt, hipStream_t stream);

@@ -17,6 +17,7 @@ constexpr int64_t kSpan = 0x7FFFFFFFll;       // bytes of an operand of a produc
 constexpr int64_t kTokenStride = 1ll << 23;   // elements: a tile's rows stay within 32-bit offsets
 constexpr int64_t kMaxDim = 128;
 constexpr int64_t kThreads = 1ll << 32;       // a launch takes fewer
+constexpr int kWeightRounds = 8;              // workgroups a CU of a decode step that counts weights
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -639,7 +640,7 @@ static int64_t decode_workspace_size(const wtc_attention_args* p, bool weights) 
   if (guarded([&] { return check_attention(*p, true); })) return -1;
   if (weights && check_decode_weights(*p)) return -1;
   const AttnParams a = decode_params(*p);
-  const int splits = weights ? plan_decode_joined(a, cu_count()) : plan_decode(a, cu_count());
+  const int splits = weights ? plan_decode_joined(a, kWeightRounds, cu_count()) : plan_decode(a, cu_count());
   return align256(weights ? decode_weights_workspace(a, splits) : decode_workspace(a, splits));
 }
 int64_t wtc_window_attention_decode_workspace_size(const wtc_attention_args* p) { return decode_workspace_size(p, false); }
@@ -671,7 +672,7 @@ static int decode(bool has_weights, const wtc_attention_args* p, const void* q, 
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(k_new) || !aligned16(v_new))
       return bad("pointers must be 16-byte aligned");
     AttnParams a = decode_params(*p);
-    const int splits = has_weights ? plan_decode_joined(a, cu_count()) : plan_decode(a, cu_count());
+    const int splits = has_weights ? plan_decode_joined(a, kWeightRounds, cu_count()) : plan_decode(a, cu_count());
     const int64_t need = align256(has_weights ? decode_weights_workspace(a, splits) : decode_workspace(a, splits));
     if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
     a.part_out = static_cast<float*>(workspace);

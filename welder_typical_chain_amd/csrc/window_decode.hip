@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const AttnParams p) {
 // What the rows of a cache received from the token: p.weights [batch][kv_heads][lk] +=
 // the sum over the key head's query heads of exp2(score - log2-sum-exp).  The newest
 // token's row is set instead: nobody weighed it before.  Workgroups [0, weight_blocks)
-// take 256 tile rows of a (sequence, key head), those behind them join the splits
+// take 1024 tile rows of a (sequence, key head), four a thread, those behind them join the splits
 // as decode_join_kernel does.
 constexpr int kHeadsAtOnce = 64;
 template <int DT>
@@ -71,15 +71,26 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(const AttnParams p,
   __shared__ float lse[kHeadsAtOnce];
   const int chunk = (int)blockIdx.x % chunks, seq = (int)blockIdx.x / chunks, b = seq / p.kv_heads, hk = seq % p.kv_heads;
   const Runs runs(p, max(p.k_lens[b], 0));
-  const int x = chunk * 256 + threadIdx.x, t = x / kRows;
-  if (chunk * 256 / kRows >= runs.t_all) return;  // (the whole workgroup)
+  const int x = (chunk * 256 + (int)threadIdx.x) * 4, t = x / kRows;
+  if (chunk * 1024 / kRows >= runs.t_all) return;  // (the whole workgroup)
   int row = 0, rows = 0;
   if (t < runs.t_all) runs.tile(t, &row, &rows);
-  const bool in = x % kRows < rows;
-  float sum = 0.0f;
+  const int in = min(4, rows - x % kRows);  // rows of this thread
+  float* w = p.weights + (int64_t)seq * p.lk + row + x % kRows;
+  float sum[4] = {}, before[4] = {};
+#pragma unroll
+  for (int v = 0; v < 4; ++v)
+    if (v < in) before[v] = w[v];
+  if (t == runs.t_all - 1 && in > 0 && x % kRows + in == rows) before[in - 1] = 0.0f;
+  const int64_t pitch = (int64_t)most_tiles(p.lk) * kRows;
   for (int g0 = 0; g0 < p.group; g0 += kHeadsAtOnce) {
     const int heads = min(kHeadsAtOnce, p.group - g0);
     const int64_t h0 = (int64_t)b * p.heads + hk * p.group + g0;
+    const float* score = p.scores + h0 * pitch + x;
+    f32x4 y[4];  // of four heads, on their way while the log-sum-exps come
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      if (in > 0 && g < heads) y[g] = *reinterpret_cast<const f32x4*>(score + g * pitch);
     __syncthreads();
     if ((int)threadIdx.x < heads) {
       const float* part = p.part_lse + (h0 + threadIdx.x) * p.slots;
@@ -91,14 +102,20 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(const AttnParams p,
       lse[threadIdx.x] = total == 0.0f ? INFINITY : ref + __builtin_amdgcn_logf(total);
     }
     __syncthreads();
-    if (in) {
-      const float* score = p.scores + h0 * most_tiles(p.lk) * kRows + x;
-      for (int g = 0; g < heads; ++g) sum += __builtin_amdgcn_exp2f(score[(int64_t)g * most_tiles(p.lk) * kRows] - lse[g]);
+    if (in <= 0) continue;
+    for (int g4 = 0; g4 < heads; g4 += 4) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (g4 + g >= heads) continue;
+        if (g4) y[g] = *reinterpret_cast<const f32x4*>(score + (g4 + g) * pitch);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) sum[v] += __builtin_amdgcn_exp2f(y[g][v] - lse[g4 + g]);
+      }
     }
   }
-  if (!in) return;
-  float* w = p.weights + (int64_t)seq * p.lk + row + x % kRows;
-  *w = t == runs.t_all - 1 && x % kRows == rows - 1 ? sum : *w + sum;
+#pragma unroll
+  for (int v = 0; v < 4; ++v)
+    if (v < in) w[v] = before[v] + sum[v];
 }
 
 template <int DT> const void* few_rows_for(int nd) {
@@ -128,13 +145,13 @@ int plan_decode(const AttnParams& p, int cu_count) {
   while (splits < 64 && grid * splits * 2 <= cu_count && tiles / (2 * splits) >= 4 * kWaves) splits *= 2;
   return splits;
 }
-// Sequences of unequal length leave CUs idle at the end: splits until the chip has two
-// workgroups a CU, one after another, while a wave keeps at least 4 tiles.
-int plan_decode_joined(const AttnParams& p, int cu_count) {
+// Sequences of unequal length leave CUs idle at the end: splits until there are `rounds`
+// workgroups a CU, while a wave keeps at least 4 tiles.
+int plan_decode_joined(const AttnParams& p, int rounds, int cu_count) {
   const int64_t grid = (int64_t)p.batch * p.kv_heads * ((p.group + kHeads - 1) / kHeads);
   const int64_t tiles = (std::min<int64_t>(p.lk, p.window + p.sinks) + kRows - 1) / kRows;
   int splits = 1;
-  while (splits < 64 && grid * splits < 2 * cu_count && tiles / (2 * splits) >= 4 * kWaves) splits *= 2;
+  while (splits < 64 && grid * splits < (int64_t)rounds * cu_count && tiles / (2 * splits) >= 4 * kWaves) splits *= 2;
   return splits;
 }
 int64_t decode_workspace(const AttnParams& p, int splits) {
@@ -198,7 +215,7 @@ hipError_t launch_attention_decode_weights(const AttnParams& params, int splits,
   const int64_t rows = (int64_t)p.batch * p.heads;
   p.scores = p.part_out + rows * splits * p.dim;  // (both multiples of 8 elements)
   p.part_lse = p.scores + rows * most_tiles(p.lk) * kRows;
-  int chunks = (most_tiles(p.lk) * kRows + 255) / 256, weight_blocks = p.batch * p.kv_heads * chunks;
+  int chunks = (most_tiles(p.lk) * kRows + 1023) / 1024, weight_blocks = p.batch * p.kv_heads * chunks;
   void* args[] = {&p, &weight_blocks, &chunks};
   const int nd = (p.dim + 31) / 32;
   const hipError_t e = launch(dt == DT_F16 ? kernel_for<DT_F16, true>(nd) : kernel_for<DT_BF16, true>(nd), decode_grid(p), args, stream);
