@@ -472,7 +472,8 @@ template <int ND, int KG> struct DqLds {
   static_assert(TOTAL <= 160 * 1024, "LDS");
 };
 // STATS: the rows' statistics for dk / dv are written (otherwise attention_stats_kernel did).
-template <int DT, int ND, int KG, bool STATS>
+// FULL: every query sees every key.
+template <int DT, int ND, int KG, bool STATS, bool FULL>
 __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t id) {
   using L = DqLds<ND, KG>;
   constexpr int NW = 4;
@@ -482,16 +483,16 @@ __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t
   const int wave = wave_id % 4, group = wave_id / 4;  // rows, tiles
   const int blk = p.row_blocks - 1 - (int)(id % p.row_blocks);
   const int hk = (int)(id / p.row_blocks % p.kv_heads), b = (int)(id / p.row_blocks / p.kv_heads);
-  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = first_position(p, nq, nk);
+  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = FULL ? nk - 1 : nk - nq;
   const int r0 = blk * NW * 32;
   const int r = r0 + wave * 32 + (lane & 31), i = r / p.group, x_head = r - i * p.group, h = hk * p.group + x_head;
   const bool valid = i < nq;
   const int pos = valid ? i + shift : -1;
   const int i_last = min((r0 + NW * 32 - 1) / p.group, nq - 1);
   const int p_lo = r0 / p.group + shift, p_hi = i_last + shift;
-  const int lo = (int)max((int64_t)0, (int64_t)p_lo - p.window + 1);
+  const int lo = FULL ? 0 : (int)max((int64_t)0, (int64_t)p_lo - p.window + 1);
   const int end = r0 / p.group < nq ? min(max(p_hi + 1, 0), nk) : 0;
-  const int s_end = end ? min(p.sinks, lo) : 0;
+  const int s_end = !FULL && end ? min(p.sinks, lo) : 0;
   const int t_sink = (s_end + kKeys - 1) / kKeys, t_all = end > lo ? t_sink + (end - lo + kKeys - 1) / kKeys : 0;
   const int w_lo = (r0 + wave * 32) / p.group + shift;
   const int w_hi = min((r0 + wave * 32 + 31) / p.group, nq - 1) + shift;
@@ -557,14 +558,14 @@ __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t
     const int t = x * KG + group;
     const int j0 = tile_base(t), j1 = tile_end(t);
     const int k0 = j0 + 32 * u;
-    const bool below = t >= t_sink && (int64_t)k0 + 31 + p.window <= w_lo && k0 >= p.sinks;
-    if (t >= t_all || !w_any || k0 > w_hi || k0 >= j1 || below) return false;
+    const bool below = !FULL && t >= t_sink && (int64_t)k0 + 31 + p.window <= w_lo && k0 >= p.sinks;
+    if (t >= t_all || !w_any || (!FULL && k0 > w_hi) || k0 >= j1 || below) return false;
 #pragma unroll
     for (int v = 0; v < 16; ++v) s[v] = g[v] = 0.0f;
 #pragma unroll
     for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ka, 32 * u, st), qf[st], s);
-    if (k0 + 32 > j1 || k0 + 31 > w_lo || (t >= t_sink && (int64_t)k0 + p.window <= w_hi)) {
-      const uint64_t seen = seen_bits(k0 + 4 * half, j1, pos, p.window, p.sinks);
+    if (k0 + 32 > j1 || (!FULL && (k0 + 31 > w_lo || (t >= t_sink && (int64_t)k0 + p.window <= w_hi)))) {
+      const uint64_t seen = FULL ? bits_below(j1 - k0 - 4 * half) : seen_bits(k0 + 4 * half, j1, pos, p.window, p.sinks);
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[v] = keep_bit(s[v], seen, 8 * (v >> 2) + (v & 3));
     }
@@ -714,10 +715,10 @@ __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t
     redo &= redo - 1;
   }
 }
-template <int DT, int ND, int KG>
+template <int DT, int ND, int KG, bool FULL>
 __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnParams p) {
   __shared__ __attribute__((aligned(256))) uint8_t smem[DqLds<ND, KG>::TOTAL];
-  attention_dq<DT, ND, KG, true>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
+  attention_dq<DT, ND, KG, true, FULL>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
 }
 
 // A workgroup takes kDkvKeys keys of one (sequence, key head) and streams the
@@ -770,7 +771,7 @@ __device__ inline float* far_part(const AttnParams& p, int b, int hk, int kb, in
   return p.part_far + (((((int64_t)b * p.kv_heads + hk) * p.far_blocks + kb) * p.far_chunks + slot) * p.far_keys + key) * 2 * p.dim;
 }
 
-template <int DT, int ND>
+template <int DT, int ND, bool FULL>
 __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_t id) {
   using L = DkvLds<ND>;
   constexpr int RB = L::RB, NS = 2 * ND, NB = kQueries * RB / 1024 / kDkvWaves;
@@ -779,16 +780,16 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
   // workgroups of a (sequence, key head): the key blocks' near chunks, then the far ones
   const int near = p.key_blocks * p.near_chunks, per = near + p.far_blocks * p.far_chunks;
   const int w = (int)(id % per), hk = (int)(id / per % p.kv_heads), b = (int)(id / per / p.kv_heads);
-  const bool far = w >= near;
+  const bool far = !FULL && w >= near;
   const int parts_of = far ? p.far_chunks : p.near_chunks;
   const int kb = (far ? w - near : w) / parts_of, chunk = (far ? w - near : w) % parts_of;
-  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = first_position(p, nq, nk);
+  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = FULL ? nk - 1 : nk - nq;
   const int sub = wave >> 2;  // rows of a tile
   const int j_first = kb * kDkvKeys, j_wave = j_first + (wave & 3) * 32, j = j_wave + (lane & 31);
   const bool valid = j < nk;
   // queries: the near ones are those whose window may reach a key of the block
-  int i0 = min(max(0, j_first - shift), nq);
-  int i1 = (int)max((int64_t)i0, min((int64_t)nq, (int64_t)min(j_first + kDkvKeys, nk) - 1 + p.window - shift));
+  int i0 = FULL ? 0 : min(max(0, j_first - shift), nq);
+  int i1 = FULL ? nq : (int)max((int64_t)i0, min((int64_t)nq, (int64_t)min(j_first + kDkvKeys, nk) - 1 + p.window - shift));
   if (far) {
     i0 = i1;
     i1 = nq;
@@ -892,8 +893,8 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
     const uint8_t* stt = smem + stage + L::STATS;
     // tile row x is a query that sees this lane's key if t_lo <= x < t_hi
     const int rows = min(min(tp, i1 - i) * hg, hg == p.group ? kQueries : p.group - hc * hg);
-    int t_lo = 0, t_hi = valid ? rows : 0;
-    if (!p.full) {
+    int t_lo = 0, t_hi = rows;  // (of a key behind the end nothing is kept)
+    if constexpr (!FULL) {
       const int64_t back = (int64_t)j - shift - i;
       t_lo = (int)min((int64_t)1 << 20, max((int64_t)0, back)) * hg;
       const int64_t reach = j < p.sinks ? 1 << 20 : max((int64_t)0, min((int64_t)1 << 20, back + p.window)) * hg;
@@ -1000,7 +1001,7 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
     }
   }
   // keys whose sums the last kernel adds up: all, or the first tokens'
-  const int summed = p.near_chunks > 1 ? p.lk : kb < p.far_blocks ? p.sinks : 0;
+  const int summed = p.near_chunks > 1 ? p.lk : !FULL && kb < p.far_blocks ? p.sinks : 0;
   if (summed > j_first) {
     if (j < (far ? p.sinks : summed)) {
       float* dst = (far ? far_part(p, b, hk, kb, chunk, j - j_first) : near_part(p, b, hk, kb, chunk, j - j_first)) + sub * p.dim;
@@ -1055,10 +1056,10 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
     redo &= redo - 1;
   }
 }
-template <int DT, int ND>
+template <int DT, int ND, bool FULL>
 __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const AttnParams p) {
   __shared__ __attribute__((aligned(256))) uint8_t smem[DkvLds<ND>::TOTAL];
-  attention_dkv<DT, ND>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
+  attention_dkv<DT, ND, FULL>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
 }
 
 // Both at once, where their workgroups together leave each a CU of its own: the rows'
@@ -1069,8 +1070,8 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_gradients_kernel(
   static_assert(kDkvWaves * 64 == 2 * 256, "threads of attention_dq with KG 2");
   constexpr int MOST = DqLds<ND, 2>::TOTAL > DkvLds<ND>::TOTAL ? DqLds<ND, 2>::TOTAL : DkvLds<ND>::TOTAL;
   __shared__ __attribute__((aligned(256))) uint8_t smem[MOST];
-  if ((int)blockIdx.x < dq_blocks) attention_dq<DT, ND, 2, false>(p, smem, blockIdx.x);
-  else attention_dkv<DT, ND>(p, smem, blockIdx.x - (uint32_t)dq_blocks);
+  if ((int)blockIdx.x < dq_blocks) attention_dq<DT, ND, 2, false, true>(p, smem, blockIdx.x);
+  else attention_dkv<DT, ND, true>(p, smem, blockIdx.x - (uint32_t)dq_blocks);
 }
 // lse in the log2 domain and -D = -sum of dout out of the rows: 16 lanes a row.
 template <int DT>
@@ -1212,13 +1213,16 @@ hipError_t launch_attention_join(const AttnParams& p, int dt, hipStream_t stream
 }
 
 namespace {
-template <int DT, int KG> const void* dq_kernel(int nd) {
+template <int DT, int KG, bool FULL> const void* dq_kernel(int nd) {
   switch (nd) {
-    case 1: return (const void*)&attention_dq_kernel<DT, 1, KG>;
-    case 2: return (const void*)&attention_dq_kernel<DT, 2, KG>;
-    case 3: return (const void*)&attention_dq_kernel<DT, 3, KG>;
+    case 1: return (const void*)&attention_dq_kernel<DT, 1, KG, FULL>;
+    case 2: return (const void*)&attention_dq_kernel<DT, 2, KG, FULL>;
+    case 3: return (const void*)&attention_dq_kernel<DT, 3, KG, FULL>;
   }
-  return (const void*)&attention_dq_kernel<DT, 4, KG>;
+  return (const void*)&attention_dq_kernel<DT, 4, KG, FULL>;
+}
+template <int DT, bool FULL> const void* dq_kernel(int nd, bool pairs) {
+  return pairs ? dq_kernel<DT, 2, FULL>(nd) : dq_kernel<DT, 1, FULL>(nd);
 }
 template <int DT> const void* gradients_kernel(int nd) {
   switch (nd) {
@@ -1228,13 +1232,13 @@ template <int DT> const void* gradients_kernel(int nd) {
   }
   return (const void*)&attention_gradients_kernel<DT, 4>;
 }
-template <int DT> const void* dkv_kernel(int nd) {
+template <int DT, bool FULL> const void* dkv_kernel(int nd) {
   switch (nd) {
-    case 1: return (const void*)&attention_dkv_kernel<DT, 1>;
-    case 2: return (const void*)&attention_dkv_kernel<DT, 2>;
-    case 3: return (const void*)&attention_dkv_kernel<DT, 3>;
+    case 1: return (const void*)&attention_dkv_kernel<DT, 1, FULL>;
+    case 2: return (const void*)&attention_dkv_kernel<DT, 2, FULL>;
+    case 3: return (const void*)&attention_dkv_kernel<DT, 3, FULL>;
   }
-  return (const void*)&attention_dkv_kernel<DT, 4>;
+  return (const void*)&attention_dkv_kernel<DT, 4, FULL>;
 }
 }  // namespace
 
@@ -1294,13 +1298,15 @@ hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwar
   if (p.lq) {
     p.row_blocks = (int)(((int64_t)p.lq * p.group + kDqRows - 1) / kDqRows);
     const bool pairs = plan.dq_groups == 2;
-    const void* fn = pairs ? (dt == DT_F16 ? dq_kernel<DT_F16, 2>(nd) : dq_kernel<DT_BF16, 2>(nd))
-                           : (dt == DT_F16 ? dq_kernel<DT_F16, 1>(nd) : dq_kernel<DT_BF16, 1>(nd));
+    const void* fn = p.full ? (dt == DT_F16 ? dq_kernel<DT_F16, true>(nd, pairs) : dq_kernel<DT_BF16, true>(nd, pairs))
+                            : (dt == DT_F16 ? dq_kernel<DT_F16, false>(nd, pairs) : dq_kernel<DT_BF16, false>(nd, pairs));
     const hipError_t e = launch(fn, seqs * p.row_blocks, pairs ? 512 : 256, p, stream);
     if (e != hipSuccess) return e;
   }
   if (!p.lk) return hipSuccess;
-  const hipError_t e = launch(dt == DT_F16 ? dkv_kernel<DT_F16>(nd) : dkv_kernel<DT_BF16>(nd),
+  const void* dkv = p.full ? (dt == DT_F16 ? dkv_kernel<DT_F16, true>(nd) : dkv_kernel<DT_BF16, true>(nd))
+                           : (dt == DT_F16 ? dkv_kernel<DT_F16, false>(nd) : dkv_kernel<DT_BF16, false>(nd));
+  const hipError_t e = launch(dkv,
                               seqs * (p.key_blocks * p.near_chunks + p.far_blocks * p.far_chunks), kDkvWaves * 64, p, stream);
   if (e != hipSuccess || (p.near_chunks == 1 && !p.far_blocks)) return e;
   return launch(WTC_BY_TYPE(attention_sum_kernel, dt), (seqs * (p.near_chunks > 1 ? p.lk : p.sinks) + 3) / 4, 256, p, stream);
