@@ -12,7 +12,7 @@
 // in LDS; a second launch copies them, 16 bytes a thread, neighbours in the new cache
 // by neighbours, which bounds the call.  (In one launch, with as many workgroups a
 // sequence as fill the chip, each finding all rows for itself: 72 us for 16 caches of
-// 8192 rows of 8 heads of 128 cut to 2048, against TWO.)
+// 8192 rows of 8 heads of 128 cut to 2048, against 57.)
 #include "layer_kernels.h"
 
 namespace wtc {

@@ -352,12 +352,12 @@ int check_evict(const wtc_evict_args& p) {
   return check_distinct(p.vo_stride, p.batch, p.out_rows, p.kv_heads, p.dim, "v_out");
 }
 
-// The gradient addresses a tile's query rows (64 positions or one group of query
-// heads) with 32-bit offsets.
-int check_group_span(const wtc_attention_args& p, const int64_t* s, const char* what) {
-  const int64_t heads = std::min<int64_t>(p.heads / p.kv_heads, 64), most = kSpan / 2;
+// A tile of query rows (`rows` positions, or fewer of a group of query heads) is addressed
+// with 32-bit offsets.
+int check_group_span(const wtc_attention_args& p, const int64_t* s, int64_t rows, const char* what) {
+  const int64_t heads = std::min<int64_t>(p.heads / p.kv_heads, rows), most = kSpan / 2;
   if (p.heads > 1 && s[2] > most / heads) return report(WTC_ERR_UNSUPPORTED, std::string(what) + ": a key head's query heads span more than 2 GiB");
-  if (p.lq > 1 && (heads - 1) * s[2] + 64 / heads * s[1] + p.dim > most)
+  if (p.lq > 1 && (heads - 1) * s[2] + rows / heads * s[1] + p.dim > most)
     return report(WTC_ERR_UNSUPPORTED, std::string(what) + ": a tile of query rows spans more than 2 GiB");
   return WTC_OK;
 }
@@ -366,8 +366,9 @@ int check_attention_backward(const wtc_attention_args& p, bool cross = false) {
   if (cross)
     if (int rc = check_cross(p)) return rc;
   if (int rc = check_strides(p.do_stride, 3, p.lq, "dout")) return rc;
-  if (int rc = check_group_span(p, p.q_stride, "q")) return rc;
-  if (int rc = check_group_span(p, p.do_stride, "dout")) return rc;
+  const int64_t tile = cross ? 128 : 64;
+  if (int rc = check_group_span(p, p.q_stride, tile, "q")) return rc;
+  if (int rc = check_group_span(p, p.do_stride, tile, "dout")) return rc;
   const AttnParams a = cross ? cross_params(p) : attention_params(p);
   const AttnBackwardPlan plan = plan_attention_backward(a, cu_count());
   const int64_t seqs = p.batch * p.kv_heads;
@@ -377,7 +378,7 @@ int check_attention_backward(const wtc_attention_args& p, bool cross = false) {
 }
 int check_key_weights(const wtc_attention_args& p) {
   if (int rc = check_attention(p, false)) return rc;
-  if (int rc = check_group_span(p, p.q_stride, "q")) return rc;
+  if (int rc = check_group_span(p, p.q_stride, 64, "q")) return rc;
   if (std::min<int64_t>(p.heads / p.kv_heads, 64) * p.lq > kSpan / 8) return report(WTC_ERR_UNSUPPORTED, "lse: a key head's rows span more than 2 GiB");
   const KeyWeightsPlan plan = plan_key_weights(attention_params(p), cu_count());
   if (p.batch * p.kv_heads * plan.key_blocks >= kThreads / 256 / plan.chunks) return too_many();

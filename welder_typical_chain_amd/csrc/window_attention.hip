@@ -748,10 +748,13 @@ __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnPar
 constexpr int kDkvWaves = 8;
 constexpr int kDkvKeys = 128;
 constexpr int kQueries = 64;
+// Rows of a tile where every query sees every key (FULL): twice as many while LDS holds them, so
+// that a wave does two blocks a barrier (4 x 1024 on 1500 states, 16 heads of 64: 83 -> 77 us).
+constexpr int tile_queries(int nd, bool full) { return full && nd <= 2 ? 2 * kQueries : kQueries; }
 
-template <int ND> struct DkvLds {
+template <int ND, bool FULL> struct DkvLds {
   static constexpr int RB = row_bytes(ND), STAGES = 2;
-  static constexpr int TILE = kQueries * RB, STATS = 2 * TILE, STAGE = 2 * TILE + 2048;
+  static constexpr int Q = tile_queries(ND, FULL), TILE = Q * RB, STATS = 2 * TILE, STAGE = 2 * TILE + 2048;
   // At dim 128 the registers do not hold all of K's and V's fragments beside the
   // sums (a spilled one is loaded through vmcnt, behind the next tile's loads):
   // the last KEPT of the k-steps of V are read from LDS, 1 KiB a wave and step.
@@ -773,8 +776,8 @@ __device__ inline float* far_part(const AttnParams& p, int b, int hk, int kb, in
 
 template <int DT, int ND, bool FULL>
 __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_t id) {
-  using L = DkvLds<ND>;
-  constexpr int RB = L::RB, NS = 2 * ND, NB = kQueries * RB / 1024 / kDkvWaves;
+  using L = DkvLds<ND, FULL>;
+  constexpr int Q = L::Q, RB = L::RB, NS = 2 * ND, NB = Q * RB / 1024 / kDkvWaves;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // workgroups of a (sequence, key head): the key blocks' near chunks, then the far ones
@@ -800,8 +803,8 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
     i0 = (int)min((int64_t)last, first + (int64_t)chunk * share);
     i1 = min(last, i0 + share);
   }
-  const int hg = min(p.group, kQueries), chunks = (p.group + hg - 1) / hg;  // query heads a tile, tiles a position
-  const int tp = kQueries / hg;                                             // positions a tile
+  const int hg = min(p.group, Q), chunks = (p.group + hg - 1) / hg;  // query heads a tile, tiles a position
+  const int tp = Q / hg;                                             // positions a tile
 
   // loads of a tile: block q of this wave holds tile row `row[q]`, position row / hg, head row % hg
   const uint8_t* q_base = p.q + 2 * (b * p.q_stride[0] + (int64_t)hk * p.group * p.q_stride[2]);
@@ -819,7 +822,6 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
   }
   const int64_t st_row = stats_row(p, b, hk, 0);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
-  const int row0 = 32 * sub;
   const int steps = (i1 - i0 + tp - 1) / tp, t_all = steps * chunks;
   u32x4 kf[NS], vf[NS];
   load_row<NS>(p.k + 2 * (b * p.k_stride[0] + (int64_t)j * p.k_stride[1] + hk * p.k_stride[2]), valid, p.dim, half, kf);
@@ -866,7 +868,7 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
       }
     }
     if (wave == 0) {  // the rows' lse and D: contiguous
-      const int rows = min(npos * hg, hg == p.group ? kQueries : nhead);
+      const int rows = min(npos * hg, hg == p.group ? Q : nhead);
       const uint32_t bytes = rows > 0 ? (uint32_t)rows * 4u : 0u, at = lds0 + (uint32_t)t % L::STAGES * L::STAGE + L::STATS;
       dma16(raw_rsrc(p.row_lse + next.row, bytes), lane * 16, at);
       dma16(raw_rsrc(p.row_delta + next.row, bytes), lane * 16, at + 1024);
@@ -882,7 +884,7 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
   for (int t = 0; t < L::STAGES - 1; ++t) issue(t);
   landed(kf);
   landed(vf);
-  const uint32_t r_at = row_addr<RB>(lane) + (uint32_t)row0 * RB, c_at = col_addr<RB>(lane) + (uint32_t)row0 * RB;
+  const uint32_t r_at = row_addr<RB>(lane) + (uint32_t)(32 * sub) * RB, c_at = col_addr<RB>(lane) + (uint32_t)(32 * sub) * RB;
   int i = i0, hc = 0;  // the tile's
   for (int t = 0; t < t_all; ++t, hc = hc + 1 == chunks ? 0 : hc + 1, i += hc ? 0 : tp) {
     // tile t landed; every wave is done with tile t - 1 (wave 0 has two more loads a tile)
@@ -892,7 +894,7 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
     const uint32_t stage = (uint32_t)t % L::STAGES * L::STAGE;
     const uint8_t* stt = smem + stage + L::STATS;
     // tile row x is a query that sees this lane's key if t_lo <= x < t_hi
-    const int rows = min(min(tp, i1 - i) * hg, hg == p.group ? kQueries : p.group - hc * hg);
+    const int rows = min(min(tp, i1 - i) * hg, hg == p.group ? Q : p.group - hc * hg);
     int t_lo = 0, t_hi = rows;  // (of a key behind the end nothing is kept)
     if constexpr (!FULL) {
       const int64_t back = (int64_t)j - shift - i;
@@ -900,74 +902,78 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
       const int64_t reach = j < p.sinks ? 1 << 20 : max((int64_t)0, min((int64_t)1 << 20, back + p.window)) * hg;
       t_hi = valid ? (int)min((int64_t)rows, reach) : 0;
     }
-    const bool all = __all(t_lo <= row0 && t_hi >= row0 + 32);
-    if (!all && !__any(max(t_lo, row0) < min(t_hi, row0 + 32))) continue;
-    uint32_t ra = r_at + stage, ca = c_at + stage;
-    fresh(ra);
-    fresh(ca);
-    f32x16 s, g;
 #pragma unroll
-    for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+    for (int part = 0; part < Q / 64; ++part) {
+      const int row0 = 32 * sub + 64 * part;
+      const bool all = __all(t_lo <= row0 && t_hi >= row0 + 32);
+      if (!all && !__any(max(t_lo, row0) < min(t_hi, row0 + 32))) continue;
+      uint32_t ra = r_at + stage + 64 * part * RB, ca = c_at + stage + 64 * part * RB;
+      fresh(ra);
+      fresh(ca);
+      f32x16 s, g;
 #pragma unroll
-    for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ra, 0, st), kf[st], s);
-    if (!all) {
-      const int at = row0 + 4 * half;
-      const uint64_t in = bits_below(t_hi - at) & ~bits_below(t_lo - at);
+      for (int v = 0; v < 16; ++v) s[v] = 0.0f;
 #pragma unroll
-      for (int v = 0; v < 16; ++v) s[v] = keep_bit(s[v], in, 8 * (v >> 2) + (v & 3));
+      for (int st = 0; st < NS; ++st) s = mfma32<DT>(row_frag<RB>(smem, ra, 0, st), kf[st], s);
+      if (!all) {
+        const int at = row0 + 4 * half;
+        const uint64_t in = bits_below(t_hi - at) & ~bits_below(t_lo - at);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] = keep_bit(s[v], in, 8 * (v >> 2) + (v & 3));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // the exponentials among the products of dP - D, which start from -D
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 del = *reinterpret_cast<const f32x4*>(stt + 1024 + (row0 + 8 * q + 4 * half) * 4);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) g[4 * q + v] = del[v];
+      }
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
+        const int x = st - (NS - L::KEPT);
+        g = mfma32<DT>(row_frag<RB>(smem, ra, Q, st), x < 0 ? vf[st] : *reinterpret_cast<const u32x4*>(smem + kept_at + x * 1024), g);
+      }
+      u32x4 pf[2], df[2];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(stt + (row0 + 8 * q + 4 * half) * 4);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[4 * q + v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + v], c2, -lse[v]));
+        uint32_t w0, w1;
+        pack4<DT>(f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]}, &w0, &w1);
+        pf[q >> 1][2 * (q & 1)] = w0;
+        pf[q >> 1][2 * (q & 1) + 1] = w1;
+      }
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 40 / NS, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // dS among the products of dv
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dv[d] = mfma32<DT>(col_frag<RB>(smem, ca, Q + 16 * st, d), pf[st], dv[d]);
+      const float by = power_of_2(range.ex);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[v] = DT == DT_F16 ? s[v] * by * g[v] : s[v] * g[v];
+      const float most = range.pack(s, df);
+#pragma unroll
+      for (int x = 0; x < 2 * ND; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, (DT == DT_F16 ? 48 : 24) / (2 * ND), 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      range.fit(most, s, dk, df);
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dk[d] = mfma32<DT>(col_frag<RB>(smem, ca, 16 * st, d), df[st], dk[d]);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    // the exponentials among the products of dP - D, which start from -D
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 del = *reinterpret_cast<const f32x4*>(stt + 1024 + (row0 + 8 * q + 4 * half) * 4);
-#pragma unroll
-      for (int v = 0; v < 4; ++v) g[4 * q + v] = del[v];
-    }
-#pragma unroll
-    for (int st = 0; st < NS; ++st) {
-      const int x = st - (NS - L::KEPT);
-      g = mfma32<DT>(row_frag<RB>(smem, ra, kQueries, st), x < 0 ? vf[st] : *reinterpret_cast<const u32x4*>(smem + kept_at + x * 1024), g);
-    }
-    u32x4 pf[2], df[2];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(stt + (row0 + 8 * q + 4 * half) * 4);
-#pragma unroll
-      for (int v = 0; v < 4; ++v) s[4 * q + v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + v], c2, -lse[v]));
-      uint32_t w0, w1;
-      pack4<DT>(f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]}, &w0, &w1);
-      pf[q >> 1][2 * (q & 1)] = w0;
-      pf[q >> 1][2 * (q & 1) + 1] = w1;
-    }
-#pragma unroll
-    for (int x = 0; x < NS; ++x) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 40 / NS, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    // dS among the products of dv
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) dv[d] = mfma32<DT>(col_frag<RB>(smem, ca, kQueries + 16 * st, d), pf[st], dv[d]);
-    const float by = power_of_2(range.ex);
-#pragma unroll
-    for (int v = 0; v < 16; ++v) s[v] = DT == DT_F16 ? s[v] * by * g[v] : s[v] * g[v];
-    const float most = range.pack(s, df);
-#pragma unroll
-    for (int x = 0; x < 2 * ND; ++x) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, (DT == DT_F16 ? 48 : 24) / (2 * ND), 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    range.fit(most, s, dk, df);
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) dk[d] = mfma32<DT>(col_frag<RB>(smem, ca, 16 * st, d), df[st], dk[d]);
   }
   wait_loads_barrier<0>();
   range.undo(dk, kWeightBits<DT>);
@@ -1058,17 +1064,17 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
 }
 template <int DT, int ND, bool FULL>
 __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_dkv_kernel(const AttnParams p) {
-  __shared__ __attribute__((aligned(256))) uint8_t smem[DkvLds<ND>::TOTAL];
+  __shared__ __attribute__((aligned(256))) uint8_t smem[DkvLds<ND, FULL>::TOTAL];
   attention_dkv<DT, ND, FULL>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
 }
 
 // Both at once, where their workgroups together leave each a CU of its own: the rows'
 // statistics come from a kernel before (3 x 333 on 1000 states, 6 / 3 heads of 80 in f16:
-// 28 us and 21 one after the other, TOGETHER at once).
+// 28 us and 21 one after the other, 4 and 31 so).
 template <int DT, int ND>
 __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_gradients_kernel(const AttnParams p, int dq_blocks) {
   static_assert(kDkvWaves * 64 == 2 * 256, "threads of attention_dq with KG 2");
-  constexpr int MOST = DqLds<ND, 2>::TOTAL > DkvLds<ND>::TOTAL ? DqLds<ND, 2>::TOTAL : DkvLds<ND>::TOTAL;
+  constexpr int MOST = DqLds<ND, 2>::TOTAL > DkvLds<ND, true>::TOTAL ? DqLds<ND, 2>::TOTAL : DkvLds<ND, true>::TOTAL;
   __shared__ __attribute__((aligned(256))) uint8_t smem[MOST];
   if ((int)blockIdx.x < dq_blocks) attention_dq<DT, ND, 2, false, true>(p, smem, blockIdx.x);
   else attention_dkv<DT, ND, true>(p, smem, blockIdx.x - (uint32_t)dq_blocks);
