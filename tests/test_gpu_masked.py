@@ -164,7 +164,14 @@ def test_cross_empty(W):
 
 
 @pytest.mark.parametrize("b,lq,lk,h,kv,d", [(40, 130, 150, 8, 8, 64), (30, 1, 300, 32, 8, 128), (3, 1000, 700, 6, 3, 80),
-                                            (1, 2100, 90, 8, 2, 128), (1, 64, 5000, 4, 4, 64), (200, 2, 65, 4, 2, 96)])
+                                            (1, 2100, 90, 8, 2, 128), (1, 64, 5000, 4, 4, 64), (200, 2, 65, 4, 2, 96),
+                                            # more workgroups than CUs: two row blocks a wave, at every width
+                                            (70, 150, 200, 8, 4, 128), (90, 100, 130, 6, 3, 96), (130, 140, 100, 4, 4, 40),
+                                            (300, 70, 33, 1, 1, 16),
+                                            # few workgroups: keys split, gradients in one launch or in two
+                                            (1, 300, 3000, 2, 2, 128), (1, 90, 2500, 5, 5, 24), (2, 400, 129, 4, 4, 96), (2, 600, 900, 12, 4, 64),
+                                            # a group of over 64 heads in tiles of 128 rows
+                                            (1, 30, 300, 100, 1, 64), (1, 9, 200, 260, 2, 32)])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_cross_large(W, b, lq, lk, h, kv, d, dtype):
     check_cross(W, *cross_inputs(43, b, lq, lk, h, kv, d, dtype))
@@ -201,6 +208,15 @@ def test_prefix_sizes(W, n, lq, lk, dtype, h, kv, d):
 @pytest.mark.parametrize("lq", [1, 6])
 def test_prefix_batches(W, b, lq):
     check_prefix(W, *prefix_inputs(55, b, 1000, lq, 20, 8, 2, 64, BF16))
+
+
+@pytest.mark.parametrize("b,n,lq,lk,h,kv,d", [
+    (70, 90, 100, 100, 4, 4, 128), (90, 65, 90, 130, 6, 3, 96), (300, 40, 130, 130, 2, 2, 64), (300, 33, 140, 140, 1, 1, 24),  # full chips
+    (1, 5000, 150, 300, 2, 2, 128), (2, 3000, 64, 64, 8, 2, 80), (1, 4001, 500, 500, 1, 1, 64),  # keys split
+    (2, 31, 200, 200, 2, 1, 128), (2, 32, 200, 231, 2, 1, 96), (2, 95, 130, 130, 1, 1, 64), (2, 96, 257, 300, 1, 1, 32)])  # units' ends
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_prefix_large(W, b, n, lq, lk, h, kv, d, dtype):
+    check_prefix(W, *prefix_inputs(57, b, n, lq, lk, h, kv, d, dtype))
 
 
 @pytest.mark.parametrize("d", [8, 24, 40, 96, 120])
@@ -500,6 +516,29 @@ def test_evict_past_32_bits(W):
     at = [*range(16), *range(rows - 40, rows - 30), *range(rows - 4, rows)]
     assert got[3].flatten().tolist() == at
     assert torch.equal(got[0][0], k[0, torch.tensor(at, device="cuda")]) and torch.equal(got[0], got[1])
+
+
+def test_offsets_past_32_bits(W):
+    """Sequences, and tokens of one sequence, more than 2^32 bytes apart."""
+    far = torch.zeros(5 << 29, dtype=F16, device="cuda")  # 5.4 GB
+    apart = far.as_strided((2, 200, 1, 64), ((1 << 31) + 4096, 64, 64, 1))
+    strided = far.as_strided((1, 300, 1, 64), (0, 1 << 23, 64, 1))  # 300 tokens over 5 GB
+    for k, lq in ((apart, 1), (apart, 90), (strided, 1), (strided, 300)):
+        b, n = k.shape[:2]
+        k.copy_(rand(153, *k.shape, dtype=F16))
+        q, g = rand(154, b, lq, 1, 64, dtype=F16), rand(155, b, lq, 1, 64, dtype=F16)
+        check_cross(W, q, k, k, g)
+        check_prefix(W, q, k[0], k[0], k, k)
+        check_weights(W, q, k)
+        w = torch.ones(b, 1, n, device="cuda")
+        ref = M.decode(q[:, 0], k.contiguous(), k.contiguous(), lens(*[n] * b), kp=k[0].contiguous(), vp=k[0].contiguous())
+        within(W.prefix_attention_decode(q[:, 0], k[0], k[0], k, k, lens(*[n] * b)), ref["out"], "decode")
+        ref = M.decode(q[:, 0], k.contiguous(), k.contiguous(), lens(*[n] * b), weights=w.clone())
+        W.window_attention_decode(q[:, 0], k, k, lens(*[n] * b), weights=w)
+        within(w, ref["weights"], "weights")
+        check_evict(W, k.contiguous(), k.contiguous(), w, lens(*[n] * b), 50)
+        got = W.cache_evict(k, k, w, lens(*[n] * b), 50, recent=3)
+        assert all(torch.equal(x, y) for x, y in zip(got, W.cache_evict(k.contiguous(), k.contiguous(), w, lens(*[n] * b), 50, recent=3)))
 
 
 # ---------------------------------------------------------------------------

@@ -43,17 +43,19 @@ template <int DT, bool PREFIX> const void* kernel_for(int nd, int a) {
 
 }  // namespace
 
-int plan_attention_rows(const AttnParams& p, int cu_count, double* us_out) {
+// The splits of the keys for which the rounds of workgroups (two a CU up to dim 64), each of
+// some six units' time for its start and end, and the join take least.
+int plan_attention_rows(const AttnParams& p, int cu_count) {
+  constexpr double kUnitUs = 0.6, kJoinUs = 4, kJoinBytesUs = 4e6;
   const int64_t rows = (int64_t)p.lq * p.group, blocks = (rows + kRows - 1) / kRows;
-  if (rows <= 64) return 0;
   const int64_t grid = (int64_t)p.batch * p.kv_heads * blocks, at_once = (int64_t)cu_count * (p.dim <= 64 ? 2 : 1);
   const int64_t units = ((int64_t)p.prefix + kUnit - 1) / kUnit + (p.lk + kUnit - 1) / kUnit;
-  const double unit_us = p.dim <= 64 ? 0.6 : 0.6, row_bytes = 8.0 * p.dim * p.batch * p.lq * p.heads;
+  const double row_bytes = 8.0 * p.dim * p.batch * p.lq * p.heads;  // written and read a split
   int best = 1;
-  double& least = *us_out = 1e30;
+  double least = 1e30;
   for (int s = 1; s <= 32 && (s == 1 || units / s >= 4); ++s) {
     const int64_t rounds = (grid * s + at_once - 1) / at_once;
-    const double us = rounds * ((units + s - 1) / s + 6) * unit_us + (s > 1 ? 4 + row_bytes * s / 4e6 : 0);
+    const double us = rounds * ((units + s - 1) / s + 6) * kUnitUs + (s > 1 ? kJoinUs + row_bytes * s / kJoinBytesUs : 0);
     if (us < least) least = us, best = s;
   }
   return best;

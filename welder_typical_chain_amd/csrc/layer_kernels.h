@@ -46,9 +46,8 @@ int64_t attention_workspace(const AttnParams& p, const AttnPlan& plan);
 // p.part_out: attention_workspace() bytes
 hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, hipStream_t stream);
 // Many rows that see nearly all of their keys (p.full, or behind p.prefix).
-// Splits (0: attention_tile_kernel is faster) and an estimate; p.part_out of launch_attention_rows:
-// attention_workspace() bytes.
-int plan_attention_rows(const AttnParams& p, int cu_count, double* us);
+// Splits; p.part_out of launch_attention_rows: attention_workspace() bytes.
+int plan_attention_rows(const AttnParams& p, int cu_count);
 hipError_t launch_attention_rows(const AttnParams& p, int splits, int cu_count, int dt, hipStream_t stream);
 // Few rows (p.full) against many keys; splits, 0: too many rows.  p.part_out: as above.
 int plan_few_rows(const AttnParams& p, int cu_count);

@@ -228,8 +228,10 @@ int check_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bool dec
   if (x.prefix > kMost / p.kv_heads) return report(WTC_ERR_UNSUPPORTED, "extent above 2^30");
   if (int rc = check_positions(p.batch * p.lq, x.prefix)) return rc;
   if (int rc = check_positions(p.lk, x.prefix)) return rc;
-  const int64_t group = p.heads / p.kv_heads;
-  if (p.kv_heads * ((p.batch * p.lq * group + 127) / 128) >= kThreads / 512) return too_many();
+  // (the join takes half a wave a row; a token's launch has workgroups for both parts)
+  const int64_t group = p.heads / p.kv_heads, common = p.kv_heads * ((p.batch * p.lq * group + 31) / 32);
+  if (common >= kThreads / 512 || p.batch * p.lq * p.heads >= kThreads / 32) return too_many();
+  if (decode && common + p.batch * p.kv_heads * ((group + 31) / 32) >= kThreads / 256) return too_many();
   for (const int64_t* s : {x.kp_stride, x.vp_stride}) {
     const int64_t as3[3] = {0, s[0], s[1]};
     if (int rc = check_strides(as3, 3, x.prefix, s == x.kp_stride ? "k_prefix" : "v_prefix")) return rc;
@@ -274,12 +276,10 @@ PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bo
   } else {
     q.common_plan = plan_attention(c, cus);
     first = x.prefix ? q.common_plan.splits : 0;
-    if (x.prefix) {
-      double us;
-      q.own_splits = plan_attention_rows(q.own, cus, &us);
-      q.single = q.own_splits && q.own.lq * q.own.group >= 128;
-    }
+    // from half a workgroup's rows a sequence on, each takes the prefix by itself
+    q.single = x.prefix && (int64_t)q.own.lq * q.own.group >= 128;
     if (q.single) {
+      q.own_splits = plan_attention_rows(q.own, cus);
       q.bytes = align256(attention_workspace(q.own, AttnPlan{1, q.own_splits, AttnPlan::ROWS, cus}));
       return q;
     }

@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
   const uint32_t rest = id / p.splits;
   const int blk = p.row_blocks - 1 - (int)(rest % p.row_blocks);  // the longest rows first
   const int hk = (int)(rest / p.row_blocks % p.kv_heads), b = (int)(rest / p.row_blocks / p.kv_heads);
-  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = first_position(p, nq, nk);
+  const int nk = seq_keys(p, b), nq = seq_queries(p, b), shift = nk - nq;
   const int r0 = blk * ROWS;
 
   // this lane's row
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
   const int i_last = min((r0 + ROWS - 1) / p.group, nq - 1);
   const int p_lo = r0 / p.group + shift, p_hi = i_last + shift;
   const int lo = (int)max((int64_t)0, (int64_t)p_lo - p.window + 1);
-  const int end = r0 / p.group < nq ? min(max(p_hi + 1, 0), nk) : 0;
+  const int end = r0 / p.group < nq ? max(p_hi + 1, 0) : 0;
   const int s_end = end ? min(p.sinks, lo) : 0;
   const int t_sink = (s_end + kKeys - 1) / kKeys, t_all = end > lo ? t_sink + (end - lo + kKeys - 1) / kKeys : 0;
   const int t0 = (int)((int64_t)t_all * split / p.splits), t1 = (int)((int64_t)t_all * (split + 1) / p.splits);
@@ -80,8 +80,7 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
   const bool w_any = (r0 + wave * 32) / p.group < nq && w_hi >= 0;
 
   u32x4 qf[NS];
-  const int q_seq = p.seq_rows ? i / p.seq_rows : b, q_row = p.seq_rows ? i % p.seq_rows : i;
-  load_row<NS>(p.q + 2 * (q_seq * p.q_stride[0] + (int64_t)q_row * p.q_stride[1] + h * p.q_stride[2]), valid, p.dim, half, qf);
+  load_row<NS>(p.q + 2 * (b * p.q_stride[0] + (int64_t)i * p.q_stride[1] + h * p.q_stride[2]), valid, p.dim, half, qf);
   const float c2 = positive_scale<NS>(p.scale, qf);
 
   f32x16 o[ND];
@@ -1176,9 +1175,8 @@ template <int DT, int KG> const void* tile_kernel(int nd) {
 AttnPlan plan_attention(const AttnParams& p, int cu_count) {
   AttnPlan plan{1, 1, AttnPlan::TILE, cu_count};
   if (p.full && p.lk) {
-    double us;
     if (const int splits = plan_few_rows(p, cu_count)) return AttnPlan{1, splits, AttnPlan::FEW, cu_count};
-    if (const int splits = plan_attention_rows(p, cu_count, &us)) return AttnPlan{1, splits, AttnPlan::ROWS, cu_count};
+    return AttnPlan{1, plan_attention_rows(p, cu_count), AttnPlan::ROWS, cu_count};
   }
   const int64_t rows = (int64_t)p.lq * p.group, seqs = (int64_t)p.batch * p.kv_heads;
   if (seqs * ((rows + 255) / 256) < cu_count) plan.key_groups = 2;

@@ -495,6 +495,9 @@ def _decode(q, k_cache, v_cache, lengths, k_new, v_new, window, sinks, scale, ou
     if prefix is not None:
         (_, kp), (_, vp) = prefix
         common = _prefix_args(kp, vp, kv, d)
+        if k_new is not None:
+            _check_out(k_cache, *prefix, what="k_cache")
+            _check_out(v_cache, *prefix, what="v_cache")
         ws, ws_ptr, ws_bytes = _scratch("wtc_prefix_attention_decode_workspace_size", args, device, _SIZES_END, common)
         _launch(device, _lib.lib().wtc_prefix_attention_decode, args, common, q.data_ptr(), kp.data_ptr(),
                 vp.data_ptr(), *tensors, ws_ptr, ws_bytes)
@@ -549,8 +552,8 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
 
     k_prefix, v_prefix: [P, Hkv, D], one for the batch; q: [B, Lq, H, D]; k, v:
     [B, Lk, Hkv, D], each sequence's own tokens, whose last ones the queries are.
-    P and Lk may be 0.  Everything else is window_attention's.  The prefix is
-    read for the queries of all sequences together.
+    P and Lk may be 0.  Everything else is window_attention's.  Where sequences
+    have few query rows, the prefix is read once for all of them together.
     """
     common = ("k_prefix", k_prefix), ("v_prefix", v_prefix)
     device = _check_inputs(q.dtype, ("q", q), ("k", k), ("v", v), ("out", out), *common)
