@@ -70,7 +70,9 @@ HIP_FLAGS = [
     f"-I{CSRC}",
 ]
 # Per-source extra flags.  The tile kernels take their first-load scalars as
-# leading arguments; gfx950 preloads those into SGPRs.
+# leading arguments; gfx950 preloads those into SGPRs.  Attention's scores are
+# wanted in the vector registers, where the exponentials take them, not in the
+# accumulation registers, which would have to be copied first.
 HIP_EXTRA = {"cross_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
              "fused_matmul_softmax.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
              "wide_tile.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"]}

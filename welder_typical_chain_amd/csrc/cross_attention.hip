@@ -43,19 +43,27 @@ template <int DT, bool PREFIX> const void* kernel_for(int nd, int a) {
 
 }  // namespace
 
-// The splits of the keys for which the rounds of workgroups (two a CU up to dim 64), each of
-// some six units' time for its start and end, and the join take least.
-int plan_attention_rows(const AttnParams& p, int cu_count) {
+// What a launch of so many splits takes about, with the join of `slots` partial results a row
+// (0: none): the rounds of workgroups (two a CU up to dim 64), each of some six units' time
+// for its start and end.  (A unit takes a CU 0.9 us on a full chip, less where the clock is
+// not held down.)
+double attention_rows_us(const AttnParams& p, int splits, int slots, int cu_count) {
   constexpr double kUnitUs = 0.6, kJoinUs = 4, kJoinBytesUs = 4e6;
   const int64_t rows = (int64_t)p.lq * p.group, blocks = (rows + kRows - 1) / kRows;
-  const int64_t grid = (int64_t)p.batch * p.kv_heads * blocks, at_once = (int64_t)cu_count * (p.dim <= 64 ? 2 : 1);
+  const int64_t grid = (int64_t)p.batch * p.kv_heads * blocks * splits, at_once = (int64_t)cu_count * (p.dim <= 64 ? 2 : 1);
   const int64_t units = ((int64_t)p.prefix + kUnit - 1) / kUnit + (p.lk + kUnit - 1) / kUnit;
-  const double row_bytes = 8.0 * p.dim * p.batch * p.lq * p.heads;  // written and read a split
+  const double row_bytes = 8.0 * p.dim * p.batch * p.lq * p.heads;  // written and read a partial result
+  const int64_t rounds = (grid + at_once - 1) / at_once;
+  return rounds * ((units + splits - 1) / splits + 6) * kUnitUs + (slots ? kJoinUs + row_bytes * slots / kJoinBytesUs : 0);
+}
+
+// The splits of the keys for which that is least, while each keeps four units.
+int plan_attention_rows(const AttnParams& p, int cu_count) {
+  const int64_t units = ((int64_t)p.prefix + kUnit - 1) / kUnit + (p.lk + kUnit - 1) / kUnit;
   int best = 1;
   double least = 1e30;
   for (int s = 1; s <= 32 && (s == 1 || units / s >= 4); ++s) {
-    const int64_t rounds = (grid * s + at_once - 1) / at_once;
-    const double us = rounds * ((units + s - 1) / s + 6) * kUnitUs + (s > 1 ? kJoinUs + row_bytes * s / kJoinBytesUs : 0);
+    const double us = attention_rows_us(p, s, s > 1 ? s : 0, cu_count);
     if (us < least) least = us, best = s;
   }
   return best;
@@ -84,7 +92,11 @@ hipError_t launch_attention_rows(const AttnParams& params, int splits, int cu_co
 // ---- one token a sequence behind a shared prefix ------------------------------------
 // Workgroups [0, common_blocks) take the batch's queries as one sequence's against the
 // prefix, the others each sequence's own cache, in one launch: the first are bound by the
-// matrix cores (from some 100 rows a key head on), the second by memory.
+// matrix cores (from some 100 rows a key head on), the second by memory.  A prefix is read
+// once for all sequences (MANY: over 64 rows a key head; fewer take the memory-bound tiles of
+// decode_tile.h).  64 tokens behind 8192, own caches of up to 1024, 32 / 8 heads of 128, bf16:
+// 53 us with the caches cold (44 warm), of which the join takes 5; the prefix and the caches
+// in two launches one after another took 63 warm.
 namespace {
 
 template <int DT, int ND, bool MANY>
@@ -106,8 +118,9 @@ template <int DT, bool MANY> const void* token_kernel_for(int nd) {
 
 }  // namespace
 
-// Splits of the prefix: half of the CUs' worth of workgroups (the own caches have the
-// others' time), while each keeps 8 units, or a wave two tiles.
+// Splits of the prefix: a quarter of the CUs' worth of workgroups (the own caches have the
+// others' time; half of them: 48 us for the above against 44, each split more to join), while
+// each keeps 8 units.
 PrefixTokenPlan plan_prefix_token(const AttnParams& common, const AttnParams& own, int cu_count) {
   PrefixTokenPlan plan{};
   const int64_t rows = (int64_t)common.lq * common.group;

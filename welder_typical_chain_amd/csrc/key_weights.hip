@@ -10,9 +10,11 @@
 // The sums stay in the lanes, a query column each, until the end, where 31 exchanges
 // add the 32 columns.  A score costs a lane 24 cycles of its SIMD (16 of them the
 // exponential) and 16 of the matrix cores: so 32 rows' exponentials against 32
-// keys run among the products of the next ones, and the loop is kept short of scalar work, which a wave
-// issues one instruction in four cycles like any other.
+// keys run among the products of the next ones, and the loop is kept short of scalar work,
+// which a wave issues like any other instruction.
 // Long sequences go in chunks of queries, whose sums a second kernel adds in their order.
+// 4096 causal tokens, 32 / 8 heads of 128, bf16: 101 us, 680 TFLOP/s of the visible half;
+// exponentials after their products instead of among the next ones: 127.
 #include <algorithm>
 #include <cmath>
 
@@ -41,8 +43,8 @@ __device__ inline float zero_bit(float x, uint64_t bits, int c) {
   return __builtin_bit_cast(float, in & __builtin_bit_cast(uint32_t, x));
 }
 
-// x[0 .. N): the sums over the lanes whose numbers agree but for the bits below BIT * 2;
-// afterwards x[0] of a lane is that of x[lane % N].
+// x[0 .. N) of the 2 N lanes whose numbers agree above bit log2(N) are summed over the lanes
+// of each half of 32; a lane's x[0] is then the sum of x[lane % N].
 template <int N> __device__ inline void column_sums(float (&x)[N], int lane) {
   if constexpr (N > 1) {
     constexpr int H = N / 2;

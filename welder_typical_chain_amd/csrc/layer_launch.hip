@@ -276,14 +276,23 @@ PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bo
   } else {
     q.common_plan = plan_attention(c, cus);
     first = x.prefix ? q.common_plan.splits : 0;
-    // from half a workgroup's rows a sequence on, each takes the prefix by itself
-    q.single = x.prefix && (int64_t)q.own.lq * q.own.group >= 128;
+    q.own_plan = plan_attention(q.own, cus);
+    // In one launch each sequence takes the prefix by itself, in workgroups that its rows may
+    // not fill; in two launches and a join all rows take it together.  (Behind 4096, 32 / 8
+    // heads of 128: 8 x 200 rows 135 us against 143, 2 x 32 25 against 40, but 64 x 32 243
+    // against 164.)  Rows for the tiles of few rows do not come here.
+    const int single_splits = plan_attention_rows(q.own, cus);
+    AttnParams alone = q.own;
+    alone.prefix = 0;
+    const int slots = first + (p.lk ? q.own_plan.splits : 0);
+    q.single = x.prefix && (int64_t)q.own.lq * q.own.group > 64 &&
+               attention_rows_us(q.own, single_splits, single_splits > 1 ? single_splits : 0, cus) <=
+                   attention_rows_us(c, first, 0, cus) + attention_rows_us(alone, q.own_plan.splits, slots, cus);
     if (q.single) {
-      q.own_splits = plan_attention_rows(q.own, cus);
+      q.own_splits = single_splits;
       q.bytes = align256(attention_workspace(q.own, AttnPlan{1, q.own_splits, AttnPlan::ROWS, cus}));
       return q;
     }
-    q.own_plan = plan_attention(q.own, cus);
     q.own_splits = q.own_plan.splits;
   }
   c.slots = q.own.slots = first + (p.lk ? q.own_splits : 0);
@@ -295,7 +304,7 @@ int launch_prefix(PrefixPlan& plan, bool decode, int dt, const void* q, const vo
                   const void* v, const void* k_new, const void* v_new, void* out, float* lse, void* workspace,
                   hipStream_t stream) {
   const int64_t rows = (int64_t)plan.own.batch * plan.own.lq * plan.own.heads;
-  for (AttnParams* a : {&plan.common, &plan.own}) {  // (part_lse: of two launches)
+  for (AttnParams* a : {&plan.common, &plan.own}) {
     a->q = static_cast<const uint8_t*>(q);
     a->part_out = static_cast<float*>(workspace);
     a->part_lse = a->part_out + rows * a->slots * a->dim;

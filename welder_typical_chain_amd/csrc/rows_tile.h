@@ -1,5 +1,24 @@
 // rows_tile.h -- a workgroup's part of forward attention of many query rows that see
-// (nearly) all of their keys.
+// (nearly) all of their keys:
+//   S^T = K . Q^T,  W = exp2(c S - ref),  O^T += V^T . W^T,  total += sum W,
+// and at the end O / total and ref + log2 total.
+//
+// What bounds it: a unit of 32 keys against 32 rows is 8 ND products of 8 passes (at
+// ND = 4, 256 cycles of a SIMD's matrix core) beside 16 exponentials, 16 multiply-adds,
+// 16 additions and 8 conversions a lane, about 300 cycles of its vector unit, and a
+// fragment read from LDS feeds one product a row block.  So
+// - a wave owns two row blocks (64 rows, whose queries stay in registers) and reads each
+//   key and value fragment once for both: one a wave needs the whole of LDS's bandwidth;
+// - unit n's weights are taken among the products of unit n + 1's scores and n - 1's
+//   values, in steps of one fragment each: the two pipes work at once, and no
+//   product waits for a weight;
+// - no running maximum is kept.  The weights' own sum, needed anyway, says whether a row
+//   has outgrown its reference (kMostSum), which happens once or twice a row;
+// - keys and values go straight to LDS through a ring of three stages of two units, one
+//   barrier a stage.
+// 4 x 2048 rows on 4096 keys, 32 / 8 heads of 128, bf16: 475 us, 1160 TFLOP/s, of which the
+// matrix cores are busy 57 % of the cycles; the clock is held at 1.89 GHz by the power
+// that this takes.  Tiles of 32 rows a wave with a maximum a tile: 680 us.
 #pragma once
 #include "attention_common.h"
 
