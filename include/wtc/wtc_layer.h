@@ -160,6 +160,7 @@ int wtc_window_attention_decode(const wtc_attention_args* p, const void* q, void
 /*
  * Attention to another sequence: as wtc_window_attention, but query i < q_len sees
  * every key j < k_len.  window and sinks are 0; lq + lk is at most 2^30.
+ * The rows of a sequence of k, and of v, do not overlap.
  */
 int64_t wtc_cross_attention_workspace_size(const wtc_attention_args* p);
 int wtc_cross_attention(const wtc_attention_args* p, const void* q, const void* k, const void* v, void* out,
@@ -173,7 +174,7 @@ int wtc_cross_attention_backward(const wtc_attention_args* p, const void* dout, 
  * A prefix that all sequences of a batch share, [prefix][kv_heads][dim], strides of
  * token and head.  A query i < q_len sees every prefix key and, of its sequence's
  * own keys, those that it sees in wtc_window_attention without a window (window and
- * sinks are 0).  prefix and lk may be 0.
+ * sinks are 0).  prefix and lk may be 0; the prefix's rows do not overlap.
  */
 typedef struct wtc_prefix_args {
   int64_t prefix;

@@ -40,13 +40,14 @@ def evict_args(**kw):
 
 
 @pytest.mark.parametrize("kw,code", BAD_ATTENTION + [
-    *NONE, (dict(o=(2048, 0, 64)), ERR_ARG), (dict(o=(0, 256, 64)), ERR_ARG), (dict(batch=1, kv_heads=1, heads=1, lq=1 << 29, lk=(1 << 29) + 1), ERR_UNSUPPORTED)])
+    *NONE, (dict(o=(2048, 0, 64)), ERR_ARG), (dict(o=(0, 256, 64)), ERR_ARG), (dict(batch=1, kv_heads=1, heads=1, lq=1 << 29, lk=(1 << 29) + 1), ERR_UNSUPPORTED),
+    (dict(k=(2048, 56, 64)), ERR_ARG), (dict(v=(2048, 0, 64)), ERR_ARG)])
 def test_cross_refusals(L, kw, code):
     assert L.wtc_cross_attention(attention_args(**kw), A, A, A, A, None, A, BIG, None) == code
     assert L.wtc_last_error()
 
 
-@pytest.mark.parametrize("kw,code", BAD_ATTENTION + [*NONE, (dict(do=(2048, 250, 64)), ERR_ARG)])
+@pytest.mark.parametrize("kw,code", BAD_ATTENTION + [*NONE, (dict(do=(2048, 250, 64)), ERR_ARG), (dict(k=(2048, 0, 64)), ERR_ARG)])
 def test_cross_backward_refusals(L, kw, code):
     args = attention_args(**kw)
     assert L.wtc_cross_attention_backward(args, A, A, A, A, A, A, A, A, A, A, BIG, None) == code
@@ -74,7 +75,7 @@ def test_cross_pointer_and_workspace_refusals(L):
     assert need > 0 and L.wtc_cross_attention(many, A, A, A, A, None, A, need - 1, None) == ERR_WS
 
 
-BAD_PREFIX = [(dict(prefix=-1), ERR_ARG), (dict(kp=(120, 60)), ERR_ARG), (dict(vp=(-128, 64)), ERR_ARG),
+BAD_PREFIX = [(dict(prefix=-1), ERR_ARG), (dict(kp=(120, 60)), ERR_ARG), (dict(vp=(-128, 64)), ERR_ARG), (dict(vp=(0, 64)), ERR_ARG), (dict(kp=(56, 64)), ERR_ARG),
               (dict(kp=(1 << 24, 64)), ERR_UNSUPPORTED), (dict(prefix=1 << 30), ERR_UNSUPPORTED), (dict(prefix=1 << 40), ERR_UNSUPPORTED)]
 
 

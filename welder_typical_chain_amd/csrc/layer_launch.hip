@@ -213,14 +213,21 @@ AttnParams cross_params(const wtc_attention_args& p) {
   q.full = 1;
   return q;
 }
+// Keys that no mask hides: a tile's rows behind the last one have to be zeros, which loads
+// give outside a tensor's range only (a weight of 0 times an infinite value is NaN).
+int check_apart(int64_t stride, int64_t tokens, int64_t dim, const char* what) {
+  return tokens > 1 && stride < dim ? bad(std::string(what) + ": a sequence's rows overlap") : WTC_OK;
+}
 int check_cross(const wtc_attention_args& p) {
   if (p.window || p.sinks) return bad("cross attention has no window and no sinks");
+  if (int rc = check_apart(p.k_stride[1], p.lk, p.dim, "k")) return rc;
+  if (int rc = check_apart(p.v_stride[1], p.lk, p.dim, "v")) return rc;
   return check_positions(p.lq, p.lk);
 }
 
 // ---- a prefix that a batch shares ------------------------------------------------
-// Two launches into slots of the same rows, joined by a third: the batch's queries as one
-// sequence that sees every prefix key, and each sequence's own keys.
+// One launch, or two into slots of the same rows, joined by a third: the batch's queries as
+// one sequence that sees every prefix key, and each sequence's own keys.
 int check_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bool decode) {
   if (int rc = check_attention(p, decode)) return rc;
   if (p.window || p.sinks) return bad("attention with a shared prefix has no window and no sinks");
@@ -234,7 +241,9 @@ int check_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bool dec
   if (decode && common + p.batch * p.kv_heads * ((group + 31) / 32) >= kThreads / 256) return too_many();
   for (const int64_t* s : {x.kp_stride, x.vp_stride}) {
     const int64_t as3[3] = {0, s[0], s[1]};
-    if (int rc = check_strides(as3, 3, x.prefix, s == x.kp_stride ? "k_prefix" : "v_prefix")) return rc;
+    const char* what = s == x.kp_stride ? "k_prefix" : "v_prefix";
+    if (int rc = check_strides(as3, 3, x.prefix, what)) return rc;
+    if (int rc = check_apart(s[0], x.prefix, p.dim, what)) return rc;
   }
   return WTC_OK;
 }
@@ -252,8 +261,8 @@ PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bo
   if (decode) q.own.q_lens = q.own.k_lens;  // (an idle sequence has no query)
   q.own.prefix = (int)x.prefix;
   for (int i = 0; i < 2; ++i) {
-    q.own.kp_stride[i] = x.kp_stride[i];
-    q.own.vp_stride[i] = x.vp_stride[i];
+    q.own.kp_stride[i] = x.prefix <= 1 && i == 0 ? p.dim : x.kp_stride[i];
+    q.own.vp_stride[i] = x.prefix <= 1 && i == 0 ? p.dim : x.vp_stride[i];
   }
   AttnParams& c = q.common = q.own;
   c.seq_rows = c.lq;
@@ -263,10 +272,10 @@ PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bo
   c.q_lens = c.k_lens = nullptr;
   c.window = INT32_MAX;
   c.full = 1;
-  c.k_stride[1] = c.prefix <= 1 ? c.dim : x.kp_stride[0];
-  c.v_stride[1] = c.prefix <= 1 ? c.dim : x.vp_stride[0];
-  c.k_stride[2] = x.kp_stride[1];
-  c.v_stride[2] = x.vp_stride[1];
+  for (int i = 0; i < 2; ++i) {
+    c.k_stride[1 + i] = c.kp_stride[i];
+    c.v_stride[1 + i] = c.vp_stride[i];
+  }
   c.prefix = 0;
   int first = 0;
   if (decode) {

@@ -523,6 +523,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale:
     q: [B, Lq, H, D]; k, v: [B, Lk, Hkv, D]; types, strides, heads, dimensions,
     lengths, scale and results are window_attention's.  Lq and Lk have nothing
     to do with each other (Lq + Lk up to 2^30); one token a sequence is Lq = 1.
+    The rows of a sequence of k, and of v, may not overlap.
     A query of a sequence without keys, and one behind its sequence's end, gives zeros.
     """
     return _attention("wtc_cross_attention", q, k, v, None, 0, scale, q_lens, k_lens, out, return_lse)
@@ -552,7 +553,7 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
 
     k_prefix, v_prefix: [P, Hkv, D], one for the batch; q: [B, Lq, H, D]; k, v:
     [B, Lk, Hkv, D], each sequence's own tokens, whose last ones the queries are.
-    P and Lk may be 0.  Everything else is window_attention's.  Where sequences
+    P and Lk may be 0; the prefix's rows may not overlap.  Everything else is window_attention's.  Where sequences
     have few query rows, the prefix is read once for all of them together.
     """
     common = ("k_prefix", k_prefix), ("v_prefix", v_prefix)
