@@ -213,7 +213,8 @@ def test_prefix_batches(W, b, lq):
 @pytest.mark.parametrize("b,n,lq,lk,h,kv,d", [
     (70, 90, 100, 100, 4, 4, 128), (90, 65, 90, 130, 6, 3, 96), (300, 40, 130, 130, 2, 2, 64), (300, 33, 140, 140, 1, 1, 24),  # full chips
     (1, 5000, 150, 300, 2, 2, 128), (2, 3000, 64, 64, 8, 2, 80), (1, 4001, 500, 500, 1, 1, 64),  # keys split
-    (2, 31, 200, 200, 2, 1, 128), (2, 32, 200, 231, 2, 1, 96), (2, 95, 130, 130, 1, 1, 64), (2, 96, 257, 300, 1, 1, 32)])  # units' ends
+    (2, 31, 200, 200, 2, 1, 128), (2, 32, 200, 231, 2, 1, 96), (2, 95, 130, 130, 1, 1, 64), (2, 96, 257, 300, 1, 1, 32),  # units' ends
+    (130, 5000, 32, 40, 8, 2, 128), (70, 4000, 20, 20, 16, 4, 96)])  # over 64 rows a sequence, in two launches
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_prefix_large(W, b, n, lq, lk, h, kv, d, dtype):
     check_prefix(W, *prefix_inputs(57, b, n, lq, lk, h, kv, d, dtype))

@@ -525,6 +525,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale:
     to do with each other (Lq + Lk up to 2^30); one token a sequence is Lq = 1.
     The rows of a sequence of k, and of v, may not overlap.
     A query of a sequence without keys, and one behind its sequence's end, gives zeros.
+    An infinite value of v makes what its sequence's queries get of it infinite or NaN
+    (where its weight is rounded to 0).
     """
     return _attention("wtc_cross_attention", q, k, v, None, 0, scale, q_lens, k_lens, out, return_lse)
 
