@@ -21,6 +21,7 @@
 // that this takes.  Tiles of 32 rows a wave with a maximum a tile: 680 us.
 #pragma once
 #include "attention_common.h"
+#include "rows_schedule.h"
 
 namespace wtc {
 namespace rows {
@@ -37,7 +38,7 @@ constexpr int kUnit = 32;           // keys
 constexpr float kMostSum = 1024.0f;
 
 template <int ND, int A> struct RowsLds {
-  static constexpr int RB = row_bytes(ND), STAGES = 3;
+  static constexpr int RB = row_bytes(ND), STAGES = RowsSchedule<ND, false, A>::STAGES;
   static constexpr int HALF = kUnit * RB, STAGE = 4 * HALF;
   static constexpr int PITCH = ND * 64 + 16;  // bytes of a row staged for the output
   static constexpr int RING = STAGES * STAGE, OUT = waves(A) * 32 * PITCH;
@@ -87,7 +88,8 @@ template <int DT> __device__ inline uint32_t pack2(float a, float b) {
 template <int DT, int ND, bool PREFIX, int A>
 __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32_t id) {
   using L = RowsLds<ND, A>;
-  constexpr int RB = L::RB, NS = 2 * ND;
+  using Order = RowsSchedule<ND, PREFIX, A>;
+  constexpr int RB = L::RB, NS = Order::FRAGS;
   using Loader = UnitLoader<RB>;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -131,7 +133,7 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
   const int steps = (n1 - n0 + 1) / 2, plain = max(0, min(whole, n1) - n0) / 2;
 
   // Of eight waves the first four load keys, the others values; four load both.
-  constexpr int TENSORS = A == 2 ? 2 : 1, LOADS = TENSORS * 2 * Loader::NB;
+  constexpr int TENSORS = Order::TENSORS, LOADS = TENSORS * 2 * Loader::NB;
   const int loader = wave & 3, other = A == 2 ? 0 : wave >> 2;  // other: 1 for values
   const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem + (uint32_t)(loader * Loader::NB * 1024);
   const uint32_t dim_bytes = (uint32_t)p.dim * 2u;
@@ -192,7 +194,7 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
 
   const uint32_t k_at = row_addr<RB>(lane), v_at = 2 * L::HALF + col_addr<RB>(lane);
   // Fragment y of half x of a stage: NS of keys, then NS of values.
-  constexpr int STEPS = 2 * NS, AHEAD = A == 1 ? 4 : 3;
+  constexpr int STEPS = Order::STEPS, AHEAD = Order::AHEAD;
   auto read = [&](uint32_t stage, int x, int y) __attribute__((always_inline)) {
     if (y < NS) return row_frag<RB>(smem, k_at + stage, kUnit * x, y);
     return col_frag<RB>(smem, v_at + stage, kUnit * x + 16 * ((y - NS) / ND), (y - NS) % ND);
@@ -223,9 +225,9 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int y = 0; y < STEPS; ++y) {
-      if (x == 1 && y == STEPS - AHEAD) {
+      if (x == 1 && y == Order::BARRIER) {
         // all of the stage is read: the next one landed, every wave is done with this one
-        wait_loads_barrier<LOADS*(L::STAGES - 2)>();
+        wait_loads_barrier<LOADS*Order::LOADING>();
         stage = from = after(stage);
         fresh(from);
       }
@@ -242,9 +244,9 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
       // the stage that every wave has left takes units of the iteration after the next
       // (all of them before the barrier, which counts loads)
       if constexpr (PREFIX) {
-        if (STEPS > AHEAD + 2 ? y == 1 : y == 0) issue(t + L::STAGES - 1, fill, x);
-        if (STEPS > AHEAD + 2 ? y == 2 : y == 0) issue(t + L::STAGES - 1, fill, 2 + x);
-      } else if (y == 0 && x < TENSORS) {
+        if (y == Order::FIRST) issue(t + L::STAGES - 1, fill, x);
+        if (y == Order::SECOND) issue(t + L::STAGES - 1, fill, 2 + x);
+      } else if (y == (x ? Order::SECOND : Order::FIRST) && x < TENSORS) {
         issue_pair(fill, x);
       }
 #pragma unroll
@@ -300,7 +302,7 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
   // stages -1 and up; unit 0's scores
 #pragma unroll
   for (int x = 0; x < L::STAGES; ++x) {
-    if (x == L::STAGES - 1) wait_loads_barrier<LOADS*(L::STAGES - 2)>();
+    if (x == L::STAGES - 1) wait_loads_barrier<LOADS*Order::LOADING>();
 #pragma unroll
     for (int part = 0; part < 4; ++part) issue(x - 1, x * L::STAGE, part);
   }
@@ -315,7 +317,7 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
     for (int a = 0; a < A; ++a) s[0][a] = mfma32<DT>(k, qf[a][st], s[0][a]);
   }
   uint32_t stage = L::STAGE, fill = 0;  // read, and left by every wave
-  wait_loads_barrier<LOADS*(L::STAGES - 2)>();
+  wait_loads_barrier<LOADS*Order::LOADING>();
 #pragma unroll
   for (int y = 0; y < AHEAD; ++y) frag[y] = read(stage, 0, y);
   auto step = [&](auto masked, int t) __attribute__((always_inline)) {
