@@ -470,9 +470,13 @@ template <int ND, int KG> struct DqLds {
   static constexpr int TOTAL = RING > OUT ? RING : OUT;
   static_assert(TOTAL <= 160 * 1024, "LDS");
 };
-// STATS: the rows' statistics for dk / dv are written (otherwise attention_stats_kernel did).
+// What becomes of the rows' statistics: taken and written for dk / dv; no more than that, for
+// sequences of few keys (FULL); or taken as they were written before.
+enum class Rows { ALL, STATS, GIVEN };
+constexpr int kFewTiles = 2;
+__host__ __device__ inline bool few_keys(int nk) { return nk > 0 && nk <= kFewTiles * kKeys; }
 // FULL: every query sees every key.
-template <int DT, int ND, int KG, bool STATS, bool FULL>
+template <int DT, int ND, int KG, Rows ROWS, bool FULL>
 __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t id) {
   using L = DqLds<ND, KG>;
   constexpr int NW = 4;
@@ -496,12 +500,13 @@ __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t
   const int w_lo = (r0 + wave * 32) / p.group + shift;
   const int w_hi = min((r0 + wave * 32 + 31) / p.group, nq - 1) + shift;
   const bool w_any = (r0 + wave * 32) / p.group < nq && w_hi >= 0;
+  if (ROWS == Rows::STATS && (!end || !few_keys(nk))) return;
 
   u32x4 qf[NS], gf[NS];
   load_row<NS>(p.q + 2 * (b * p.q_stride[0] + (int64_t)i * p.q_stride[1] + h * p.q_stride[2]), valid, p.dim, half, qf);
   load_row<NS>(p.dout + 2 * (b * p.do_stride[0] + (int64_t)i * p.do_stride[1] + h * p.do_stride[2]), valid, p.dim, half, gf);
   float delta = 0.0f, lse2 = INFINITY;  // no keys: every weight 0
-  {
+  if constexpr (ROWS != Rows::GIVEN) {
     const uint8_t* orow = p.o + 2 * (b * p.o_stride[0] + (int64_t)i * p.o_stride[1] + h * p.o_stride[2]);
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -514,11 +519,13 @@ __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t
       }
     }
     delta = xor32_sum(delta);
-    if (valid) {
-      const float lse = p.lse_in[((int64_t)b * p.heads + h) * p.lq + i];
-      if (lse == -INFINITY) delta = 0.0f;
-      else lse2 = lse * kLog2e;
-    }
+  } else if (valid) {
+    delta = -p.row_delta[stats_row(p, b, hk, i) + x_head];
+  }
+  if (valid) {
+    const float lse = p.lse_in[((int64_t)b * p.heads + h) * p.lq + i];
+    if (lse == -INFINITY) delta = 0.0f;
+    else lse2 = lse * kLog2e;
   }
   const float c2 = positive_scale<NS>(p.scale, qf);
   // |P (dP - D)| is at most 2 dim max|dout| max|v|, 2^24 max|dout| for any f16 v
@@ -591,10 +598,10 @@ __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t
   };
 
   // D from the rounded `out` is off by that rounding times |dout|, which shows where
-  // weights are large: in rows of few keys.  Blocks of at most two tiles sum it
+  // weights are large: in rows of few keys.  Blocks of at most kFewTiles tiles sum it
   // themselves first, D = sum_j P dP (dq of causal rows in f16 1.48 -> 1.42
   // roundings off 64 bits; the D of later rows changes nothing there).
-  if (t_all <= 2) {
+  if (ROWS != Rows::GIVEN && t_all <= kFewTiles) {
 #pragma unroll
     for (int x = 0; x < L::STAGES - 1; ++x) issue(x);
     float sum = 0.0f;
@@ -620,10 +627,11 @@ __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t
     }
     delta = delta != delta ? delta : sum;  // (a NaN value that is seen, be its weight 0, is in out)
   }
-  if (STATS && half == 0 && group == 0 && i < p.lq) {
+  if (ROWS != Rows::GIVEN && half == 0 && group == 0 && i < (ROWS == Rows::STATS ? nq : p.lq)) {
     p.row_lse[stats_row(p, b, hk, i) + x_head] = lse2 - kWeightBits<DT>;
     p.row_delta[stats_row(p, b, hk, i) + x_head] = -delta;
   }
+  if constexpr (ROWS == Rows::STATS) return;
 
   landed(qf);
   landed(gf);
@@ -717,7 +725,7 @@ __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t
 template <int DT, int ND, int KG, bool FULL>
 __global__ void __launch_bounds__(KG * 256, 2) attention_dq_kernel(const AttnParams p) {
   __shared__ __attribute__((aligned(256))) uint8_t smem[DqLds<ND, KG>::TOTAL];
-  attention_dq<DT, ND, KG, true, FULL>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
+  attention_dq<DT, ND, KG, Rows::ALL, FULL>(p, smem, xcd_remap(blockIdx.x, gridDim.x));
 }
 
 // A workgroup takes kDkvKeys keys of one (sequence, key head) and streams the
@@ -1075,13 +1083,14 @@ __global__ void __launch_bounds__(kDkvWaves * 64, 2) attention_gradients_kernel(
   static_assert(kDkvWaves * 64 == 2 * 256, "threads of attention_dq with KG 2");
   constexpr int MOST = DqLds<ND, 2>::TOTAL > DkvLds<ND, true>::TOTAL ? DqLds<ND, 2>::TOTAL : DkvLds<ND, true>::TOTAL;
   __shared__ __attribute__((aligned(256))) uint8_t smem[MOST];
-  if ((int)blockIdx.x < dq_blocks) attention_dq<DT, ND, 2, false, true>(p, smem, blockIdx.x);
+  if ((int)blockIdx.x < dq_blocks) attention_dq<DT, ND, 2, Rows::GIVEN, true>(p, smem, blockIdx.x);
   else attention_dkv<DT, ND, true>(p, smem, blockIdx.x - (uint32_t)dq_blocks);
 }
-// lse in the log2 domain and -D = -sum of dout out of the rows: 16 lanes a row.
-template <int DT>
-__global__ void __launch_bounds__(256) attention_stats_kernel(const AttnParams p) {
-  const int64_t rows = (int64_t)p.batch * p.heads * p.lq, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+// lse in the log2 domain and -D = -sum of dout out of 16 rows, 16 lanes a row.  FEW: but
+// for rows of attention_dq's Rows::STATS.
+template <int DT, bool FEW>
+__device__ inline void attention_stats(const AttnParams& p, int64_t block) {
+  const int64_t rows = (int64_t)p.batch * p.heads * p.lq, row = block * 16 + (threadIdx.x >> 4);
   const int c = (threadIdx.x & 15) * 8;
   const int64_t at = min(row, rows - 1);
   const int h = (int)(at % p.heads), i = (int)(at / p.heads % p.lq), b = (int)(at / p.heads / p.lq);
@@ -1096,12 +1105,24 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(const AttnParams p
   }
 #pragma unroll
   for (int x = 8; x; x >>= 1) delta += __shfl_xor(delta, x);
-  if (row >= rows || c) return;
+  if (row >= rows || c || (FEW && valid && few_keys(seq_keys(p, b)))) return;
   const float lse = valid ? p.lse_in[((int64_t)b * p.heads + h) * p.lq + i] : -INFINITY;
   const int hk = h / p.group;
   const int64_t to = stats_row(p, b, hk, i) + h - hk * p.group;
   p.row_lse[to] = (lse == -INFINITY ? INFINITY : lse * kLog2e) - kWeightBits<DT>;
   p.row_delta[to] = lse == -INFINITY ? 0.0f : -delta;
+}
+template <int DT> __global__ void __launch_bounds__(256) attention_stats_kernel(const AttnParams p) {
+  attention_stats<DT, false>(p, blockIdx.x);
+}
+// The same where a padded batch may have sequences of few keys: dq and dk / dv then take
+// the D that separate launches give them (3 x 333 on 1000, 128 and 40 states, 6 / 3 heads of
+// 80 in f16, both gradients: 42 us, 38 with D from the rounded `out` in all).
+template <int DT, int ND>
+__global__ void __launch_bounds__(256, 2) attention_padded_stats_kernel(const AttnParams p, int dq_blocks) {
+  __shared__ __attribute__((aligned(256))) uint8_t smem[DqLds<ND, 1>::TOTAL];
+  if ((int)blockIdx.x < dq_blocks) attention_dq<DT, ND, 1, Rows::STATS, true>(p, smem, blockIdx.x);
+  else attention_stats<DT, true>(p, (int64_t)blockIdx.x - dq_blocks);
 }
 
 // dk and dv of the keys whose sums came in parts, the parts in order.  One wave a
@@ -1236,6 +1257,14 @@ template <int DT> const void* gradients_kernel(int nd) {
   }
   return (const void*)&attention_gradients_kernel<DT, 4>;
 }
+template <int DT> const void* padded_stats_kernel(int nd) {
+  switch (nd) {
+    case 1: return (const void*)&attention_padded_stats_kernel<DT, 1>;
+    case 2: return (const void*)&attention_padded_stats_kernel<DT, 2>;
+    case 3: return (const void*)&attention_padded_stats_kernel<DT, 3>;
+  }
+  return (const void*)&attention_padded_stats_kernel<DT, 4>;
+}
 template <int DT, bool FULL> const void* dkv_kernel(int nd) {
   switch (nd) {
     case 1: return (const void*)&attention_dkv_kernel<DT, 1, FULL>;
@@ -1265,8 +1294,8 @@ AttnBackwardPlan plan_attention_backward(const AttnParams& p, int cu_count) {
   const int64_t tiles = std::min<int64_t>(p.lq, p.window + kDkvKeys) * p.group / kQueries;
   plan.near_chunks = 1;
   while (plan.near_chunks < 16 && seqs * plan.key_blocks * plan.near_chunks * 2 <= cu_count && tiles / (2 * plan.near_chunks) >= 4) plan.near_chunks *= 2;
-  // (blocks of at most two key tiles sum D themselves, and hand it on)
-  plan.together = p.full && p.lq && p.lk > 2 * kKeys && seqs * (row_blocks + (int64_t)plan.key_blocks * plan.near_chunks) <= cu_count;
+  // (where all sequences have few keys the statistics would take a launch like dq's own)
+  plan.together = p.full && p.lq && p.lk > kFewTiles * kKeys && seqs * (row_blocks + (int64_t)plan.key_blocks * plan.near_chunks) <= cu_count;
   plan.near_blocks = plan.near_chunks > 1 ? plan.key_blocks : plan.far_blocks;
   const int64_t rows = (int64_t)p.batch * p.lq * p.heads;
   plan.part_at = (rows * 8 + 255) / 256 * 256;
@@ -1290,10 +1319,13 @@ hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwar
   const int64_t seqs = (int64_t)p.batch * p.kv_heads;
   if (plan.together) {
     p.row_blocks = (int)(((int64_t)p.lq * p.group + kDqRows - 1) / kDqRows);
-    hipError_t e = launch(WTC_BY_TYPE(attention_stats_kernel, dt), ((int64_t)p.batch * p.lq * p.heads + 15) / 16, 256, p, stream);
-    if (e != hipSuccess) return e;
+    const int64_t stats_blocks = ((int64_t)p.batch * p.lq * p.heads + 15) / 16;
     int dq_blocks = (int)(seqs * p.row_blocks);
     void* args[] = {&p, &dq_blocks};
+    hipError_t e = p.k_lens ? hipLaunchKernel(dt == DT_F16 ? padded_stats_kernel<DT_F16>(nd) : padded_stats_kernel<DT_BF16>(nd),
+                                              dim3((unsigned)(dq_blocks + stats_blocks)), dim3(256), args, 0, stream)
+                            : launch(WTC_BY_TYPE(attention_stats_kernel, dt), stats_blocks, 256, p, stream);
+    if (e != hipSuccess) return e;
     e = hipLaunchKernel(dt == DT_F16 ? gradients_kernel<DT_F16>(nd) : gradients_kernel<DT_BF16>(nd),
                         dim3((unsigned)(dq_blocks + seqs * p.key_blocks * p.near_chunks)), dim3(kDkvWaves * 64), args, 0, stream);
     if (e != hipSuccess || p.near_chunks == 1) return e;
