@@ -77,3 +77,26 @@ def test_cross_gradients_of_few_keys_in_a_padded_batch(W, lq, h, kv, d, lk, n, d
             U.assert_within(dk[i, :y], *refs[1], f"dk of {y} keys")
         assert not dq[i, x:].any() and not dk[i, y:].any() and not dv[i, y:].any() and not out[i, x:].any()
         assert bool(torch.isneginf(lse[i, :, x:]).all()) and bool(torch.isfinite(lse[i, :, :x]).all())
+
+
+def test_heads_over_2_gib_apart(W):  # noqa: F811
+    """Each key head has one query head, and the heads of q and dout are further apart than 32-bit offsets reach."""
+    b, lq, lk, h, d = 2, 70, 150, 2, 64
+    q, k, v, g = cross_inputs(321, b, lq, lk, h, h, d, BF16)
+    strides = (lq * d, d, (1 << 30) + 64, 1)
+    far = []
+    for x in (q, g):
+        buffer = torch.empty(strides[2] + b * lq * d, dtype=BF16, device="cuda")
+        far.append(buffer.as_strided(x.shape, strides).copy_(x))
+    nk = lens(150, 90)
+    out, lse = W.cross_attention(q, k, v, k_lens=nk, return_lse=True)
+    assert torch.equal(out, W.cross_attention(far[0], k, v, k_lens=nk))
+    for x, y in zip(W.cross_attention_backward(g, q, k, v, out, lse, k_lens=nk),
+                    W.cross_attention_backward(far[1], far[0], k, v, out, lse, k_lens=nk)):
+        assert torch.equal(x, y)
+    out, lse = W.window_attention(q, k, v, window=40, k_lens=nk, return_lse=True)
+    for x, y in zip(W.window_attention_backward(g, q, k, v, out, lse, window=40, k_lens=nk),
+                    W.window_attention_backward(far[1], far[0], k, v, out, lse, window=40, k_lens=nk)):
+        assert torch.equal(x, y)
+    assert torch.equal(W.window_attention_weights(q, k, lse, window=40, k_lens=nk),
+                       W.window_attention_weights(far[0], k, lse, window=40, k_lens=nk))

@@ -374,7 +374,7 @@ int check_evict(const wtc_evict_args& p) {
 // with 32-bit offsets.
 int check_group_span(const wtc_attention_args& p, const int64_t* s, int64_t rows, const char* what) {
   const int64_t heads = std::min<int64_t>(p.heads / p.kv_heads, rows), most = kSpan / 2;
-  if (p.heads > 1 && s[2] > most / heads) return report(WTC_ERR_UNSUPPORTED, std::string(what) + ": a key head's query heads span more than 2 GiB");
+  if (heads > 1 && s[2] > most / heads) return report(WTC_ERR_UNSUPPORTED, std::string(what) + ": a key head's query heads span more than 2 GiB");
   if (p.lq > 1 && (heads - 1) * s[2] + rows / heads * s[1] + p.dim > most)
     return report(WTC_ERR_UNSUPPORTED, std::string(what) + ": a tile of query rows spans more than 2 GiB");
   return WTC_OK;
