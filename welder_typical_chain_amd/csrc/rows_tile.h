@@ -393,7 +393,7 @@ __device__ inline void attention_rows(const AttnParams& p, uint8_t* smem, uint32
       if (redo) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the rows are read back
       while (redo) {
         const int rr = first + __builtin_ctz(redo);
-        attention_row<DT>(p, b, hk * p.group + rr % p.group, rr / p.group);
+        attention_row<DT, false, true>(p, b, hk * p.group + rr % p.group, rr / p.group);
         redo &= redo - 1;
       }
     }

@@ -289,13 +289,13 @@ __global__ void __launch_bounds__(512, 2) attention_tile_kernel(const AttnParams
   if (redo) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the rows are read back
   while (redo) {
     const int rr = r0 + wave * 32 + __builtin_ctz(redo);
-    attention_row<DT>(p, b, hk * p.group + rr % p.group, rr / p.group);
+    attention_row<DT, false, false>(p, b, hk * p.group + rr % p.group, rr / p.group);
     redo &= redo - 1;
   }
 }
 
 // Joins the splits of a row: half a wave a row.
-template <int DT>
+template <int DT, bool FULL, bool PREFIX>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p) {
   const int lane = threadIdx.x & 63, c = (lane & 31) * 4;
   const int64_t rows = (int64_t)p.batch * p.lq * p.heads, at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
   if (redo) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   for (int half = 0; half < 2; ++half) {
     const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 6) * 2 + half;
-    if (redo >> (32 * half) & 0xFFFFFFFFu) attention_row<DT>(p, (int)(r / p.heads / p.lq), (int)(r % p.heads), (int)(r / p.heads % p.lq));
+    if (redo >> (32 * half) & 0xFFFFFFFFu) attention_row<DT, FULL, PREFIX>(p, (int)(r / p.heads / p.lq), (int)(r % p.heads), (int)(r / p.heads % p.lq));
   }
 }
 
@@ -397,7 +397,7 @@ template <int DT> struct DsRange {
   }
 };
 
-template <int DT> __device__ inline void dq_row(const AttnParams& p, int b, int h, int i) {
+template <int DT, bool FULL> __device__ inline void dq_row(const AttnParams& p, int b, int h, int i) {
   using T = typename Elem<DT>::type;
   const int lane = threadIdx.x & 63;
   const T* q = (const T*)p.q + b * p.q_stride[0] + i * p.q_stride[1] + h * p.q_stride[2];
@@ -407,7 +407,7 @@ template <int DT> __device__ inline void dq_row(const AttnParams& p, int b, int 
   const T* o = (const T*)p.o + b * p.o_stride[0] + i * p.o_stride[1] + h * p.o_stride[2];
   const float delta = dot_rows<DT>(g, o, p.dim);
   const float lse = p.lse_in[((int64_t)b * p.heads + h) * p.lq + i];
-  const Seen seen(p.window, p.sinks, last_seen(p, b, i));
+  const Seen seen(p.window, p.sinks, last_seen<FULL>(p, b, i));
   Redo<DT> dq(p.dq, (((int64_t)b * p.lq + i) * p.heads + h) * p.dim, p.dim, lane);
   for (int t0 = 0; t0 < seen.count && !dq.settled(); t0 += 64) {
     float ds = 0.0f;
@@ -422,10 +422,10 @@ template <int DT> __device__ inline void dq_row(const AttnParams& p, int b, int 
 }
 
 // dk and dv of one key.
-template <int DT> __device__ inline void dkv_row(const AttnParams& p, int b, int hk, int j) {
+template <int DT, bool FULL> __device__ inline void dkv_row(const AttnParams& p, int b, int hk, int j) {
   using T = typename Elem<DT>::type;
   const int lane = threadIdx.x & 63;
-  const int nq = seq_queries(p, b), shift = first_position(p, nq, seq_keys(p, b));
+  const int nq = seq_queries(p, b), shift = seq_keys(p, b) - (FULL ? 1 : nq);
   const T* k = (const T*)p.k + b * p.k_stride[0] + j * p.k_stride[1] + hk * p.k_stride[2];
   const T* v = (const T*)p.v + b * p.v_stride[0] + j * p.v_stride[1] + hk * p.v_stride[2];
   // queries of positions j .. j + window - 1 (a first token: all from j on)
@@ -718,7 +718,7 @@ __device__ inline void attention_dq(const AttnParams& p, uint8_t* smem, uint32_t
   if (redo) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   while (redo) {
     const int rr = r0 + wave * 32 + __builtin_ctz(redo);
-    dq_row<DT>(p, b, hk * p.group + rr % p.group, rr / p.group);
+    dq_row<DT, FULL>(p, b, hk * p.group + rr % p.group, rr / p.group);
     redo &= redo - 1;
   }
 }
@@ -1065,7 +1065,7 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
   if (sub) return;
   uint32_t redo = __builtin_amdgcn_readfirstlane(marks[wave] | marks[wave + 4]);
   while (redo) {
-    dkv_row<DT>(p, b, hk, j_wave + __builtin_ctz(redo));
+    dkv_row<DT, FULL>(p, b, hk, j_wave + __builtin_ctz(redo));
     redo &= redo - 1;
   }
 }
@@ -1127,7 +1127,7 @@ __global__ void __launch_bounds__(256, 2) attention_padded_stats_kernel(const At
 
 // dk and dv of the keys whose sums came in parts, the parts in order.  One wave a
 // key, four elements a lane.
-template <int DT>
+template <int DT, bool FULL>
 __global__ void __launch_bounds__(256) attention_sum_kernel(const AttnParams p) {
   const int lane = threadIdx.x & 63;
   const int keys = p.near_chunks > 1 ? p.lk : p.sinks;
@@ -1167,7 +1167,7 @@ __global__ void __launch_bounds__(256) attention_sum_kernel(const AttnParams p) 
   }
   if (!__any(nan)) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  dkv_row<DT>(p, b, hk, j);
+  dkv_row<DT, FULL>(p, b, hk, j);
 }
 
 hipError_t launch(const void* fn, int64_t grid, int threads, const AttnParams& p, hipStream_t stream) {
@@ -1233,8 +1233,16 @@ hipError_t launch_attention(const AttnParams& params, const AttnPlan& plan, int 
   return launch_attention_join(p, dt, stream);
 }
 
+namespace {
+template <int DT> const void* join_kernel(const AttnParams& p) {
+  if (p.full) return (const void*)&attention_join_kernel<DT, true, false>;
+  return p.prefix ? (const void*)&attention_join_kernel<DT, false, true> : (const void*)&attention_join_kernel<DT, false, false>;
+}
+}  // namespace
+
 hipError_t launch_attention_join(const AttnParams& p, int dt, hipStream_t stream) {
-  return launch(WTC_BY_TYPE(attention_join_kernel, dt), ((int64_t)p.batch * p.lq * p.heads + 7) / 8, 256, p, stream);
+  const void* fn = dt == DT_F16 ? join_kernel<DT_F16>(p) : join_kernel<DT_BF16>(p);
+  return launch(fn, ((int64_t)p.batch * p.lq * p.heads + 7) / 8, 256, p, stream);
 }
 
 namespace {
@@ -1256,6 +1264,10 @@ template <int DT> const void* gradients_kernel(int nd) {
     case 3: return (const void*)&attention_gradients_kernel<DT, 3>;
   }
   return (const void*)&attention_gradients_kernel<DT, 4>;
+}
+const void* sum_kernel(bool full, int dt) {
+  if (full) return dt == DT_F16 ? (const void*)&attention_sum_kernel<DT_F16, true> : (const void*)&attention_sum_kernel<DT_BF16, true>;
+  return dt == DT_F16 ? (const void*)&attention_sum_kernel<DT_F16, false> : (const void*)&attention_sum_kernel<DT_BF16, false>;
 }
 template <int DT> const void* padded_stats_kernel(int nd) {
   switch (nd) {
@@ -1329,7 +1341,7 @@ hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwar
     e = hipLaunchKernel(dt == DT_F16 ? gradients_kernel<DT_F16>(nd) : gradients_kernel<DT_BF16>(nd),
                         dim3((unsigned)(dq_blocks + seqs * p.key_blocks * p.near_chunks)), dim3(kDkvWaves * 64), args, 0, stream);
     if (e != hipSuccess || p.near_chunks == 1) return e;
-    return launch(WTC_BY_TYPE(attention_sum_kernel, dt), (seqs * p.lk + 3) / 4, 256, p, stream);
+    return launch(sum_kernel(true, dt), (seqs * p.lk + 3) / 4, 256, p, stream);
   }
   if (p.lq) {
     p.row_blocks = (int)(((int64_t)p.lq * p.group + kDqRows - 1) / kDqRows);
@@ -1345,7 +1357,7 @@ hipError_t launch_attention_backward(const AttnParams& params, const AttnBackwar
   const hipError_t e = launch(dkv,
                               seqs * (p.key_blocks * p.near_chunks + p.far_blocks * p.far_chunks), kDkvWaves * 64, p, stream);
   if (e != hipSuccess || (p.near_chunks == 1 && !p.far_blocks)) return e;
-  return launch(WTC_BY_TYPE(attention_sum_kernel, dt), (seqs * (p.near_chunks > 1 ? p.lk : p.sinks) + 3) / 4, 256, p, stream);
+  return launch(sum_kernel(p.full, dt), (seqs * (p.near_chunks > 1 ? p.lk : p.sinks) + 3) / 4, 256, p, stream);
 }
 
 }  // namespace wtc
