@@ -830,9 +830,9 @@ __device__ inline void attention_dkv(const AttnParams& p, uint8_t* smem, uint32_
   const int64_t st_row = stats_row(p, b, hk, 0);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(WTC_LDS uint8_t*)smem;
   const int steps = (i1 - i0 + tp - 1) / tp, t_all = steps * chunks;
-  u32x4 kf[NS], vf[NS];
-  load_row<NS>(p.k + 2 * (b * p.k_stride[0] + (int64_t)j * p.k_stride[1] + hk * p.k_stride[2]), valid, p.dim, half, kf);
-  load_row<NS>(p.v + 2 * (b * p.v_stride[0] + (int64_t)j * p.v_stride[1] + hk * p.v_stride[2]), valid, p.dim, half, vf);
+  u32x4 kf[NS], vf[NS];  // (not read where no query sees the block)
+  load_row<NS>(p.k + 2 * (b * p.k_stride[0] + (int64_t)j * p.k_stride[1] + hk * p.k_stride[2]), valid && t_all, p.dim, half, kf);
+  load_row<NS>(p.v + 2 * (b * p.v_stride[0] + (int64_t)j * p.v_stride[1] + hk * p.v_stride[2]), valid && t_all, p.dim, half, vf);
   const float c2 = positive_scale<NS>(p.scale, kf);
   const uint32_t kept_at = (uint32_t)(L::KEPT_AT + (wave & 3) * L::KEPT * 1024 + lane * 16);
   if (!sub) {
