@@ -170,6 +170,12 @@ int wtc_cross_attention_backward(const wtc_attention_args* p, const void* dout, 
                                  const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
                                  void* workspace, size_t workspace_bytes, void* stream);
 
+/* What the two calls above run on a device of `cu_count` compute units (0: the
+ * current one's), five numbers: whether the kernel for few rows takes the forward
+ * pass; row blocks of 32 that a wave holds; key splits; whether the gradients are
+ * one launch behind the rows' statistics; parts of a key block's queries in dk / dv. */
+int wtc_cross_attention_plan(const wtc_attention_args* p, int cu_count, int64_t* plan);
+
 /*
  * A prefix that all sequences of a batch share, [prefix][kv_heads][dim], strides of
  * token and head.  A query i < q_len sees every prefix key and, of its sequence's
@@ -186,6 +192,12 @@ int64_t wtc_prefix_attention_workspace_size(const wtc_attention_args* p, const w
 int wtc_prefix_attention(const wtc_attention_args* p, const wtc_prefix_args* x, const void* q, const void* k_prefix,
                          const void* v_prefix, const void* k, const void* v, void* out, float* lse, void* workspace,
                          size_t workspace_bytes, void* stream);
+
+/* What it runs on a device of `cu_count` compute units (0: the current one's), four
+ * numbers: whether one launch takes prefix and own keys; key splits of the prefix's
+ * own launch (0: there is none) and of the launch for the own keys or for both (0:
+ * none); row blocks of 32 that a wave holds where the prefix is read. */
+int wtc_prefix_attention_plan(const wtc_attention_args* p, const wtc_prefix_args* x, int cu_count, int64_t* plan);
 
 int64_t wtc_prefix_attention_decode_workspace_size(const wtc_attention_args* p, const wtc_prefix_args* x);
 /* One token a sequence.  The own caches, their lengths (without the prefix) and the

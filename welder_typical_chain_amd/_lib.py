@@ -95,6 +95,8 @@ SIGNATURES = {
     "wtc_window_attention_decode": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 7 + [ctypes.c_size_t, _c_p]),
     "wtc_cross_attention_workspace_size": (_c_i64, [ctypes.c_char_p]),
     "wtc_cross_attention": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 6 + [ctypes.c_size_t, _c_p]),
+    "wtc_cross_attention_plan": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(_c_i64)]),
+    "wtc_prefix_attention_plan": (ctypes.c_int, [ctypes.c_char_p] * 2 + [ctypes.c_int, ctypes.POINTER(_c_i64)]),
     "wtc_cross_attention_backward_workspace_size": (_c_i64, [ctypes.c_char_p]),
     "wtc_cross_attention_backward": (ctypes.c_int, [ctypes.c_char_p] + [_c_p] * 10 + [ctypes.c_size_t, _c_p]),
     "wtc_prefix_attention_workspace_size": (_c_i64, [ctypes.c_char_p] * 2),

@@ -43,10 +43,17 @@ template <int DT, bool PREFIX> const void* kernel_for(int nd, int a) {
 
 }  // namespace
 
+int attention_rows_blocks(const AttnParams& p, int splits, int cu_count) {
+  const int64_t blocks = ((int64_t)p.lq * p.group + kRows - 1) / kRows;
+  return (int64_t)p.batch * p.kv_heads * blocks * splits <= cu_count ? 1 : 2;
+}
+
 // What a launch of so many splits takes about, with the join of `slots` partial results a row
 // (0: none): the rounds of workgroups (two a CU up to dim 64), each of some six units' time
-// for its start and end.  (A unit takes a CU 0.9 us on a full chip, less where the clock is
-// not held down.)
+// for its start and end.  An estimate to choose by: a unit is given 0.6 us, what one takes
+// where a round does not fill the chip and splits are chosen (0.9 on a full chip, where the
+// clock is held down, which weighs on all choices alike); every unit counts as seen, and
+// a workgroup as full.
 double attention_rows_us(const AttnParams& p, int splits, int slots, int cu_count) {
   constexpr double kUnitUs = 0.6, kJoinUs = 4, kJoinBytesUs = 4e6;
   const int64_t rows = (int64_t)p.lq * p.group, blocks = (rows + kRows - 1) / kRows;
@@ -80,7 +87,7 @@ hipError_t launch_attention_rows(const AttnParams& params, int splits, int cu_co
   p.row_blocks = (int)(((int64_t)p.lq * p.group + kRows - 1) / kRows);
   const int nd = (p.dim + 31) / 32;
   const int64_t grid = (int64_t)p.batch * p.kv_heads * p.row_blocks * splits;
-  const int a = grid <= cu_count ? 1 : 2;
+  const int a = attention_rows_blocks(p, splits, cu_count);
   const void* fn = p.prefix ? (dt == DT_F16 ? kernel_for<DT_F16, true>(nd, a) : kernel_for<DT_BF16, true>(nd, a))
                             : (dt == DT_F16 ? kernel_for<DT_F16, false>(nd, a) : kernel_for<DT_BF16, false>(nd, a));
   void* args[] = {&p};

@@ -48,6 +48,7 @@ hipError_t launch_attention(const AttnParams& p, const AttnPlan& plan, int dt, h
 // Many rows that see nearly all of their keys (p.full, or behind p.prefix).
 // Splits; p.part_out of launch_attention_rows: attention_workspace() bytes.
 int plan_attention_rows(const AttnParams& p, int cu_count);
+int attention_rows_blocks(const AttnParams& p, int splits, int cu_count);  // of 32 rows a wave
 double attention_rows_us(const AttnParams& p, int splits, int slots, int cu_count);
 hipError_t launch_attention_rows(const AttnParams& p, int splits, int cu_count, int dt, hipStream_t stream);
 // Few rows (p.full) against many keys; splits, 0: too many rows.  p.part_out: as above.

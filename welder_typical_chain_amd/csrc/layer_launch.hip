@@ -288,8 +288,12 @@ PrefixPlan plan_prefix(const wtc_attention_args& p, const wtc_prefix_args& x, bo
     q.own_plan = plan_attention(q.own, cus);
     // In one launch each sequence takes the prefix by itself, in workgroups that its rows may
     // not fill; in two launches and a join all rows take it together.  (Behind 4096, 32 / 8
-    // heads of 128: 8 x 200 rows 135 us against 143, 2 x 32 25 against 40, but 64 x 32 243
-    // against 164.)  Rows for the tiles of few rows do not come here.
+    // heads of 128: 8 x 200 rows 132 us against 149, 2 x 32 24 against 39, but 64 x 32 243
+    // against 164.)  The estimates are rough: the own keys' launch is priced as if the rows'
+    // kernel took it, with all of its keys.  Of 70 sizes (2 to 64 sequences behind 16 to 8192
+    // keys, mostly drawn) they took the faster side or one within 4 % of it in 67; the
+    // others, of which two fill less than half of a workgroup's rows, lost 13, 23 and 28 %.
+    // Rows for the tiles of few rows do not come here.
     const int single_splits = plan_attention_rows(q.own, cus);
     AttnParams alone = q.own;
     alone.prefix = 0;
@@ -650,6 +654,38 @@ int wtc_window_attention_plan(const wtc_attention_args* p, int cus, int64_t* pla
     plan[2] = backward.dq_groups;
     plan[3] = backward.near_chunks;
     plan[4] = (int64_t)backward.far_blocks * backward.far_chunks;
+    return WTC_OK;
+  });
+}
+
+int wtc_cross_attention_plan(const wtc_attention_args* p, int cus, int64_t* plan) {
+  return guarded([&]() -> int {
+    if (!p || !plan) return bad("NULL argument");
+    if (int rc = check_attention_backward(*p, true)) return rc;
+    if (cus <= 0) cus = cu_count();
+    const AttnParams a = cross_params(*p);
+    const AttnPlan forward = plan_attention(a, cus);
+    const AttnBackwardPlan backward = plan_attention_backward(a, cus);
+    plan[0] = forward.kernel == AttnPlan::FEW;
+    plan[1] = forward.kernel == AttnPlan::ROWS ? attention_rows_blocks(a, forward.splits, cus) : 1;
+    plan[2] = forward.splits;
+    plan[3] = backward.together;
+    plan[4] = backward.near_chunks;
+    return WTC_OK;
+  });
+}
+
+int wtc_prefix_attention_plan(const wtc_attention_args* p, const wtc_prefix_args* x, int cus, int64_t* plan) {
+  return guarded([&]() -> int {
+    if (!p || !x || !plan) return bad("NULL argument");
+    if (int rc = check_prefix(*p, *x, false)) return rc;
+    if (cus <= 0) cus = cu_count();
+    const PrefixPlan q = plan_prefix(*p, *x, false, cus);
+    const bool rows = q.single || (x->prefix && q.common_plan.kernel == AttnPlan::ROWS);
+    plan[0] = q.single;
+    plan[1] = q.single || !x->prefix ? 0 : q.common_plan.splits;
+    plan[2] = p->lk || q.single ? q.own_splits : 0;
+    plan[3] = !rows ? 1 : q.single ? attention_rows_blocks(q.own, q.own_splits, cus) : attention_rows_blocks(q.common, q.common_plan.splits, cus);
     return WTC_OK;
   });
 }

@@ -293,12 +293,38 @@ def window_attention_plan(batch: int, heads: int, kv_heads: int, lq: int, lk: in
     """What window_attention and its gradients run for dense tensors of these sizes on a
     device of `cu_count` compute units (0: the current one): "row_waves" and "key_splits" of
     the forward pass, "dq_row_waves", "query_parts" and "far_parts" of the gradients."""
-    q, kv = (lq * heads * dim, heads * dim, dim), (lk * kv_heads * dim, kv_heads * dim, dim)
-    args = _pack_attention(batch, heads, kv_heads, lq, lk, dim, *_mask(window, sinks), _lib.DTYPE_BF16, *q, *kv, *kv,
-                           *q, *q, 0, 0, 0, 0, 0, 0, dim ** -0.5)
     got = (ctypes.c_int64 * 5)()
-    _lib.check(_lib.lib().wtc_window_attention_plan(args, cu_count, got))
+    _lib.check(_lib.lib().wtc_window_attention_plan(
+        _dense_attention(batch, heads, kv_heads, lq, lk, dim, *_mask(window, sinks)), cu_count, got))
     return dict(zip(("row_waves", "key_splits", "dq_row_waves", "query_parts", "far_parts"), got))
+
+
+def _dense_attention(batch, heads, kv_heads, lq, lk, dim, window=0, sinks=0):
+    q, kv = (lq * heads * dim, heads * dim, dim), (lk * kv_heads * dim, kv_heads * dim, dim)
+    return _pack_attention(batch, heads, kv_heads, lq, lk, dim, window, sinks, _lib.DTYPE_BF16, *q, *kv, *kv,
+                           *q, *q, 0, 0, 0, 0, 0, 0, dim ** -0.5)
+
+
+def cross_attention_plan(batch: int, heads: int, kv_heads: int, lq: int, lk: int, dim: int, *,
+                         cu_count: int = 0) -> dict:
+    """What cross_attention and its gradients run, as window_attention_plan: "few_rows"
+    (the kernel for few rows takes the forward pass), "wave_blocks" (row blocks of 32 that a
+    wave holds), "key_splits", "one_launch" (dq with dk and dv), "query_parts" of those."""
+    got = (ctypes.c_int64 * 5)()
+    _lib.check(_lib.lib().wtc_cross_attention_plan(_dense_attention(batch, heads, kv_heads, lq, lk, dim), cu_count, got))
+    return dict(zip(("few_rows", "wave_blocks", "key_splits", "one_launch", "query_parts"), got))
+
+
+def prefix_attention_plan(batch: int, heads: int, kv_heads: int, prefix: int, lq: int, lk: int, dim: int, *,
+                          cu_count: int = 0) -> dict:
+    """What prefix_attention runs, as window_attention_plan: "one_launch" (for prefix and own
+    keys), "prefix_splits" (of the prefix's own launch), "key_splits" (of the other launch),
+    "wave_blocks" (row blocks of 32 that a wave holds where the prefix is read)."""
+    got = (ctypes.c_int64 * 4)()
+    shared = _pack_prefix(prefix, kv_heads * dim, dim, kv_heads * dim, dim)
+    _lib.check(_lib.lib().wtc_prefix_attention_plan(_dense_attention(batch, heads, kv_heads, lq, lk, dim), shared,
+                                                    cu_count, got))
+    return dict(zip(("one_launch", "prefix_splits", "key_splits", "wave_blocks"), got))
 
 
 def _strides(t, name):
