@@ -10,9 +10,12 @@
 //
 // One workgroup finds the rows of a (sequence, key head), with up to kHeld weights kept
 // in LDS; a second launch copies them, 16 bytes a thread, neighbours in the new cache
-// by neighbours, which bounds the call.  (In one launch, with as many workgroups a
-// sequence as fill the chip, each finding all rows for itself: 72 us for 16 caches of
-// 8192 rows of 8 heads of 128 cut to 2048, against 57.)
+// by neighbours, which bounds the call while the weights fit.  (In one launch, with as many
+// workgroups a sequence as fill the chip, each finding all rows for itself: 72 us for 16
+// caches of 8192 rows of 8 heads of 128 cut to 2048, against 57.)  More weights than kHeld are
+// read from memory once a digit and once for the rows, which then bounds it: one cache of
+// 65536 rows, 8 heads of 128, cut to 4096 takes 98 us so and 8 for the copy; of 8200 rows 20,
+// of 8192 rows 14.
 #include "layer_kernels.h"
 
 namespace wtc {

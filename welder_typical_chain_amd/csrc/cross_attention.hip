@@ -103,7 +103,8 @@ hipError_t launch_attention_rows(const AttnParams& params, int splits, int cu_co
 // once for all sequences (MANY: over 64 rows a key head; fewer take the memory-bound tiles of
 // decode_tile.h).  64 tokens behind 8192, own caches of up to 1024, 32 / 8 heads of 128, bf16:
 // 53 us with the caches cold (44 warm), of which the join takes 5; the prefix and the caches
-// in two launches one after another took 63 warm.
+// in two launches one after another took 63 warm.  The prefix's 64 workgroups alone take 37 and
+// the caches' alone 33 (a CU holds one workgroup of either), both together 46.
 namespace {
 
 template <int DT, int ND, bool MANY>

@@ -16,7 +16,7 @@
 //   has outgrown its reference (kMostSum), which happens once or twice a row;
 // - keys and values go straight to LDS through a ring of three stages of two units, one
 //   barrier a stage.
-// 4 x 2048 rows on 4096 keys, 32 / 8 heads of 128, bf16: 475 us, 1160 TFLOP/s, of which the
+// 4 x 2048 rows on 4096 keys, 32 / 8 heads of 128, bf16: 475 us, 1160 TFLOP/s, in which the
 // matrix cores are busy 57 % of the cycles; the clock is held at 1.89 GHz by the power
 // that this takes.  Tiles of 32 rows a wave with a maximum a tile: 680 us.
 #pragma once
